@@ -353,6 +353,97 @@ int wh_whisper_retrieve(const wh_whisper_ids *ids, const uint32_t *generated, in
 int wh_whisper_decode(wh_model *m, const float *enc_dev, int frames, const uint32_t *prompt, int n_prompt,
                       uint32_t *out, int cap, float *no_speech, float *avg_logprob);
 
+/* ------------------------------------------------------------------- decoding with drafted tokens */
+
+/* A decoder step over drafted tokens (no counterpart in the reference, whose decoder takes one token
+ * per step, src/transformer.rs:254-290): every sequence has n[b] committed tokens, whose keys and
+ * values lie in caches of wh_pack's layout, and a tree of up to `rows` drafted ones, its nodes, the
+ * rows of this step.  Node 0 is the root (the token picked last, not yet in the cache); a node stands
+ * after its parent.  The arrays are in device memory and are read when the queued work runs, so a
+ * recorded pass follows them.  n[b] and count[b] are taken into 0 .. the cache's positions and
+ * 0 .. rows.  batch * rows <= 2^22, rows <= 1024. */
+typedef struct wh_tree {
+  int batch, rows;
+  const int32_t *n;       /* [batch] committed tokens */
+  const int32_t *count;   /* [batch] nodes that are there (NULL: rows); rows past them are not written */
+  const uint32_t *tokens; /* [batch][rows] the nodes' ids (not read by wh_tree_attend) */
+  /* [batch][rows][(rows + 31) / 32]: bit j of node i's words is 1 where i sees node j: itself and its
+   * ancestors.  wh_tree_attend and wh_logit_rules take any bits (bits past count[b] are not looked
+   * at); NULL there: no node is seen.  mask_stride: words between two sequences' masks (0: one tree
+   * for all). */
+  const uint32_t *mask;
+  size_t mask_stride;
+} wh_tree;
+
+/* Attention of every node over its sequence's committed keys and the nodes that it sees:
+ *   o[b][i] = sum_j softmax_j(q_i . k_j / sqrt(hd)) v_j per query head, over j < n[b] of the cache and
+ *   the nodes j with bit j of i's mask; a row that sees nothing gets zeros.
+ * q, k, v: row (b, i) at (b * rows + i) * stride elements, heads * hd values of q and kv_heads * hd of k
+ * and v, f32 or (in16) f16: parts of one projection's rows [q | k | v].  Query head x reads key head
+ * x / (heads / kv_heads).  k and v are taken as the cache will hold them (rounded to f16); with k and v
+ * NULL, or without a mask, the cache is all that is seen (cross attention).  kv: the caches, cols
+ * positions of kv_heads * hd values each, kv_stride words apart (0: one cache for all).  o:
+ * [batch * rows][heads * hd], f32 or (out16) f16.  Products of f32 queries and of the f32 softmax keep
+ * their precision (each is split into two f16 parts); f16 queries are exact, and with out16 the softmax
+ * weights are rounded to f16.  Masked keys and values may hold anything.  hd % 4 == 0, hd <= 128,
+ * heads % kv_heads == 0; f32 pointers and f16 rows 4-byte aligned (stride even for f16). */
+int wh_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void *k, const void *v, size_t stride,
+                   int in16, const uint32_t *kv, size_t kv_stride, int cols, void *o, int out16, int heads,
+                   int kv_heads, int hd);
+
+/* The rules of the requests' logits; every array may be NULL (no such rule) and is in device memory. */
+typedef struct wh_rules {
+  /* [batch][3] repetition r, frequency f and presence p penalties.  An id that stands c > 0 times in
+   * the sequence's text gets x = ((x > 0 ? x / r : x * r) - f * c) - p. */
+  const float *penalty;
+  /* [batch][history_cols]: the sequences' ids; the text of a node is ids from .. n[b] - 1 and the
+   * tokens of the nodes that it sees.  NULL: those tokens alone. */
+  const uint32_t *history;
+  int history_cols, from;
+  /* Biases added to single ids: entries bias_start[b] .. bias_start[b + 1] - 1 of bias_id and bias (of
+   * bias_len) are sequence b's; of several for one id the last one counts. */
+  const int32_t *bias_start;
+  const uint32_t *bias_id;
+  const float *bias;
+  int bias_len;
+  /* [batch * rows][(vocab + 31) / 32]: ids with a 0 bit get minus infinity (a grammar's or a
+   * suppression list's mask). */
+  const uint32_t *allow;
+} wh_rules;
+
+/* The rules applied to the rows of logits [batch * rows] (row r at r * ld values, f32 or, with f16 != 0,
+ * f16; vocab values each), in the order penalties, bias, mask, in f32: into out (the same layout;
+ * may be logits itself, or NULL: not written), with pick[r] the first maximum (0xffffffff where
+ * nothing is left; NaN is never picked) and logprob[r] its log-softmax over the row (minus infinity
+ * where nothing is left, NaN where the row holds one), either of which may be NULL.  Pick and log-probability are those of the f32
+ * values, before an f16 output is rounded.  Ids past vocab in history, tokens and bias_id are passed
+ * over.  search::decode's `pick` for rows of many requests (src/whisper/search.rs:46-59). */
+int wh_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *rules, const void *logits, void *out, int vocab,
+                   size_t ld, int f16, uint32_t *pick, float *logprob);
+
+/* Where wh_tree_accept puts the keys and values of the kept nodes: node (b, i)'s k and v of layer l are d
+ * values at (l * layer_stride + (b * rows + i) * stride) elements, f32 or (in16) f16; layer l's cache of
+ * sequence b is at kv + l * kv_layer_stride + b * kv_stride words, cols positions in wh_pack's layout. */
+typedef struct wh_kept {
+  const void *k, *v;
+  size_t stride, layer_stride;
+  int in16;
+  uint32_t *kv;
+  size_t kv_stride, kv_layer_stride;
+  int layers, d;
+} wh_kept;
+
+/* Keeps the drafted path that the model agrees with (greedy): from the root on, the first child whose
+ * token is the pick of its parent (picks[b][i], wh_logit_rules' pick of node i), as long as there is one
+ * and the sequence has room in its `cols` positions.  path[b]: the kept nodes, then -1; kept[b]: their
+ * number; next[b]: the token after them (the last kept node's pick; the root's token where there was no
+ * room for it; as it was where the sequence has no nodes); n_out[b] = n[b] + kept[b] (may be n itself).
+ * history [batch][history_cols] (or NULL) gets the kept tokens at n[b] .. (and then has to have room,
+ * too), and, with where != NULL, the caches get the kept nodes' keys and values there.  The masks are
+ * those of trees: bit j of i for j = i and all ancestors, so that i's parent is the highest one below i. */
+int wh_tree_accept(wh_ctx *ctx, const wh_tree *t, const uint32_t *picks, const wh_kept *where, int cols, int32_t *path,
+                   int32_t *kept, uint32_t *next, int32_t *n_out, uint32_t *history, int history_cols);
+
 #ifdef __cplusplus
 }
 #endif

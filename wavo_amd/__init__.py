@@ -70,6 +70,9 @@ SIGNATURES = {
     "wh_depthwise": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i]),
     "wh_flatten": (_i, [_vp, _vp, _vp, _i, _i, _i]),
     "wh_argmax": (_i, [_vp, _vp, _vp, _i]),
+    "wh_tree_attend": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _i, _vp, _sz, _i, _vp, _i, _i, _i, _i]),
+    "wh_logit_rules": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _sz, _i, _vp, _vp]),
+    "wh_tree_accept": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i]),
     "wh_model_load": (_i, [_vp, ctypes.c_char_p, ctypes.POINTER(_vp)]),
     "wh_model_free": (None, [_vp]),
     "wh_model_info": (_i, [_vp] + [ctypes.POINTER(_i)] * 5),
@@ -253,6 +256,33 @@ def _p(x):
     return int(x)
 
 
+class Tree(ctypes.Structure):
+    """wh_tree: a decoder step over drafted tokens (device pointers: Buffer, int or None)."""
+
+    _fields_ = [("batch", _i), ("rows", _i), ("n", _vp), ("count", _vp), ("tokens", _vp), ("mask", _vp),
+                ("mask_stride", _sz)]
+
+    def __init__(self, batch, rows, n, count=None, tokens=None, mask=None, mask_stride=0):
+        super().__init__(batch, rows, _p(n), _p(count), _p(tokens), _p(mask), mask_stride)
+
+
+class Rules(ctypes.Structure):
+    """wh_rules: the requests' penalties, biases and masks on their logits (device pointers)."""
+
+    _fields_ = [("penalty", _vp), ("history", _vp), ("history_cols", _i), ("from_", _i), ("bias_start", _vp),
+                ("bias_id", _vp), ("bias", _vp), ("bias_len", _i), ("allow", _vp)]
+
+    def __init__(self, penalty=None, history=None, history_cols=0, from_=0, bias_start=None, bias_id=None, bias=None,
+                 bias_len=0, allow=None):
+        super().__init__(_p(penalty), _p(history), history_cols, from_, _p(bias_start), _p(bias_id), _p(bias), bias_len,
+                         _p(allow))
+
+
+class _Kept(ctypes.Structure):
+    _fields_ = [("k", _vp), ("v", _vp), ("stride", _sz), ("layer_stride", _sz), ("in16", _i), ("kv", _vp),
+                ("kv_stride", _sz), ("kv_layer_stride", _sz), ("layers", _i), ("d", _i)]
+
+
 class Pass:
     """A recorded pass (wh_record_end): replay() queues it again on its context's stream."""
 
@@ -425,6 +455,26 @@ class Gpu:
 
     def pack(self, x, src, stride, y, rows, d, cols, col):
         self._check(lib().wh_pack(self.h, _p(x), src, stride, _p(y), rows, d, cols, col))
+
+    # -- decoding with drafted tokens
+    def tree_attend(self, tree, q, k, v, stride, kv, kv_stride, cols, o, heads, kv_heads, hd, in16=False, out16=False):
+        """Attention of every node of `tree` (Tree) over its sequence's cache and the nodes that it sees."""
+        self._check(lib().wh_tree_attend(self.h, ctypes.byref(tree), _p(q), _p(k), _p(v), stride, in16, _p(kv), kv_stride,
+                                         cols, _p(o), out16, heads, kv_heads, hd))
+
+    def logit_rules(self, tree, rules, logits, out, vocab, ld, half=False, pick=None, logprob=None):
+        """Penalties, biases and masks (Rules) on the nodes' logits; the first maxima and their log-softmax."""
+        self._check(lib().wh_logit_rules(self.h, ctypes.byref(tree), ctypes.byref(rules), _p(logits), _p(out), vocab, ld,
+                                         half, _p(pick), _p(logprob)))
+
+    def tree_accept(self, tree, picks, k, v, stride, layer_stride, kv, kv_stride, kv_layer_stride, layers, cols, d, path,
+                    kept, next, n_out, history=None, history_cols=0, in16=False):
+        """The drafted path that the picks agree with, its keys and values into the caches (kv None: decide only)."""
+        where = None
+        if kv is not None:
+            where = ctypes.byref(_Kept(_p(k), _p(v), stride, layer_stride, in16, _p(kv), kv_stride, kv_layer_stride, layers, d))
+        self._check(lib().wh_tree_accept(self.h, ctypes.byref(tree), _p(picks), where, cols, _p(path), _p(kept), _p(next),
+                                         _p(n_out), _p(history), history_cols))
 
     def im2col(self, x, col, t, ch, kernel, stride, pad):
         self._check(lib().wh_im2col(self.h, _p(x), _p(col), t, ch, kernel, stride, pad))

@@ -302,6 +302,18 @@ int launch_set_int(wh_ctx *ctx, int *dst, int v);
 int launch_copy(wh_ctx *ctx, void *dst, const void *src, size_t bytes);
 int launch_add_rows(wh_ctx *ctx, float *x, const float *add, size_t n);
 
+// ---- decoding with drafted tokens (tree.hip, rules.hip); nodes of one step and rows of one sequence, at most ----
+constexpr int TREE_ROWS = 1024;
+constexpr int TREE_NODES = 1 << 22;
+// Whether a call can run over `t` (its error set if not).
+int tree_check(wh_ctx *ctx, const char *what, const wh_tree *t);
+int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void *k, const void *v, size_t stride, int in16,
+                       const uint32_t *kv, size_t kv_stride, int cols, void *o, int out16, int heads, int kv_heads, int hd);
+int launch_tree_accept(wh_ctx *ctx, const wh_tree *t, const uint32_t *picks, const wh_kept *where, int cols, int32_t *path,
+                       int32_t *kept, uint32_t *next, int32_t *n_out, uint32_t *history, int history_cols);
+int launch_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *r, const void *logits, void *out, int vocab, size_t ld,
+                       int f16, uint32_t *pick, float *logprob);
+
 // ---- greedy decoding on the device (greedy.hip) ----
 // The TDT loop's state (src/parakeet/decoder.rs:158-191), in device memory: the call's encoder output
 // and (token, frame) list too, so a recorded decision serves every call.

@@ -806,4 +806,22 @@ int wh_argmax(wh_ctx *ctx, const float *x, uint32_t *out, int n) {
   return launch_argmax(ctx, x, out, n);
 }
 
+int wh_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void *k, const void *v, size_t stride, int in16,
+                   const uint32_t *kv, size_t kv_stride, int cols, void *o, int out16, int heads, int kv_heads, int hd) {
+  if (!ctx) return WH_EARG;
+  return launch_tree_attend(ctx, t, q, k, v, stride, in16, kv, kv_stride, cols, o, out16, heads, kv_heads, hd);
+}
+
+int wh_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *rules, const void *logits, void *out, int vocab, size_t ld,
+                   int f16, uint32_t *pick, float *logprob) {
+  if (!ctx) return WH_EARG;
+  return launch_logit_rules(ctx, t, rules, logits, out, vocab, ld, f16, pick, logprob);
+}
+
+int wh_tree_accept(wh_ctx *ctx, const wh_tree *t, const uint32_t *picks, const wh_kept *where, int cols, int32_t *path,
+                   int32_t *kept, uint32_t *next, int32_t *n_out, uint32_t *history, int history_cols) {
+  if (!ctx) return WH_EARG;
+  return launch_tree_accept(ctx, t, picks, where, cols, path, kept, next, n_out, history, history_cols);
+}
+
 }  // extern "C"
