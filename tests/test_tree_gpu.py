@@ -123,7 +123,8 @@ def check_attend(got, q, k, v, seen, n, count, kc, vc, heads, kv_heads, hd, in16
         src = b if len(kc) > 1 else 0
         want, tol = plain_attend(q[b][:c], kb, vb, s, nn, kc[src], vc[src], heads, kv_heads, hd)
         if out16:  # the weights are rounded to f16 (their largest is at least 2^-1 of the type's normal range), and the output
-            vmax = max(np.abs(vc[src][:nn]).max(initial=0), 0 if vb is None else np.abs(vb).max(initial=0))
+            finite = lambda x: np.abs(x[np.isfinite(x)]).max(initial=0).astype(np.float64)  # noqa: E731  (of what may be seen)
+            vmax = max(finite(vc[src][:nn]), 0 if vb is None else finite(vb))
             tol = tol + (EPS16 + (nn + rows) * 2.0**-25) * vmax + EPS16 * np.abs(want) + 2.0**-25
         err = np.abs(got[b][:c].astype(np.float64) - want)
         assert np.all(np.isfinite(got[b][:c])), f"sequence {b}"

@@ -8,9 +8,18 @@
 
 namespace {
 
-__device__ __forceinline__ float half_bits(uint32_t h) { return (float)__builtin_bit_cast(_Float16, (uint16_t)h); }
 __device__ __forceinline__ float number(const float *p, size_t i) { return p[i]; }
 __device__ __forceinline__ float number(const _Float16 *p, size_t i) { return (float)p[i]; }
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+// The same loaded from and stored to 4-byte aligned places (one wide access all the same).
+typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
+typedef u32x2 u32x2_a4 __attribute__((aligned(4)));
+typedef floatx4 floatx4_a4 __attribute__((aligned(4)));
 
 struct AttendArgs {
   const void *q, *k, *v;
@@ -21,76 +30,435 @@ struct AttendArgs {
   const int32_t *n, *count;
   const uint32_t *mask;
   size_t mask_stride;
-  int rows, words, cols, heads, group, hd;
+  int batch, rows, words, cols, heads, kv_heads, hd;
   float scale;
+  int qw, kw, splits, row_blocks;
+  // splits > 1: unnormalized outputs [split][batch * rows][heads][hd] and (maximum, sum) pairs
+  // [split][batch * rows][heads] of the splits that are used.
+  float *po, *pml;
 };
 
-constexpr int KEYS = 256;
+// The blocks of keys of a sequence (the cache's, then the nodes'), and how its `splits` workgroups share them:
+// runs of `per` blocks, at least one for each wavefront, so that a short sequence uses fewer of them.
+struct Share {
+  int n, count, cached, blocks, per, used;
+};
+template <int KB>
+__device__ __forceinline__ Share share_of(const AttendArgs &a, int b) {
+  Share s;
+  s.n = min(max(a.n[b], 0), a.cols);
+  s.count = a.count ? min(max(a.count[b], 0), a.rows) : a.rows;
+  s.cached = (s.n + KB - 1) / KB;
+  s.blocks = s.cached + (a.mask && a.k ? (s.count + KB - 1) / KB : 0);
+  s.per = max((s.blocks + a.splits - 1) / a.splits, a.kw);
+  s.used = max((s.blocks + s.per - 1) / s.per, 1);
+  return s;
+}
 
-// One workgroup per query head of a node: blocks of 256 keys, one per thread, with the running maximum and
-// sum of the softmax; then a thread per value.
-template <typename T, typename OT>
-__global__ __launch_bounds__(KEYS) void attend_kernel(AttendArgs a) {
-  __shared__ float qs[128], p[KEYS], red[8];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int head = blockIdx.x % a.heads, row = blockIdx.x / a.heads, b = row / a.rows, i = row % a.rows;
-  const int n = min(max(a.n[b], 0), a.cols), count = a.count ? min(max(a.count[b], 0), a.rows) : a.rows;
-  if (i >= count) return;
-  const int half = a.heads / a.group * a.hd / 2, pairs = a.hd / 2, kh = head / a.group;
-  const uint32_t *kc = a.kv + (size_t)b * a.kv_stride, *vc = kc + (size_t)half * a.cols;
-  const T *q = (const T *)a.q + (size_t)row * a.stride + head * a.hd;
-  const size_t node0 = (size_t)b * a.rows * a.stride + kh * a.hd;
-  if (tid < a.hd) qs[tid] = number(q, tid);
-  float m = -INFINITY, l = 0.0f, acc = 0.0f;
-  const int total = n + (a.mask && a.k ? count : 0);
-  bool any = false;
-  for (int j0 = 0; j0 < total; j0 += KEYS) {
-    const int j = j0 + tid, u = j - n;
-    bool see = j < n;
-    if (!see && j < total) see = a.mask[(size_t)b * a.mask_stride + (size_t)i * a.words + u / 32] >> (u % 32) & 1;
-    float s = -INFINITY;
-    __syncthreads();
-    if (see) {
-      s = 0.0f;
-      if (j < n) {
-        for (int c = 0; c < pairs; c++) {
-          const uint32_t w = kc[((size_t)kh * pairs + c) * a.cols + j];
-          s += qs[2 * c] * half_bits(w & 0xffffu) + qs[2 * c + 1] * half_bits(w >> 16);
-        }
-      } else {
-        const T *k = (const T *)a.k + node0 + (size_t)u * a.stride;
-        for (int c = 0; c < a.hd; c++) s += qs[c] * (float)(_Float16)number(k, c);
+// Whether node i of sequence b sees anything at all.
+__device__ bool sees_any(const AttendArgs &a, const Share &s, int b, int i) {
+  if (s.n > 0) return true;
+  if (!a.mask || !a.k) return false;
+  const uint32_t *w = a.mask + (size_t)b * a.mask_stride + (size_t)i * a.words;
+  for (int j = 0; j < s.count; j += 32)
+    if (w[j / 32] & (s.count - j >= 32 ? 0xffffffffu : (1u << (s.count - j)) - 1u)) return true;
+  return false;
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)lo) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)hi) << 16;
+}
+// Four values of a row as f16 pairs.
+__device__ __forceinline__ u32x2 four(const float *p) {
+  const floatx4 x = *(const floatx4_a4 *)p;
+  return u32x2{pack2(x[0], x[1]), pack2(x[2], x[3])};
+}
+__device__ __forceinline__ u32x2 four(const _Float16 *p) { return *(const u32x2_a4 *)p; }
+
+__device__ __forceinline__ floatx4 mfma(half8 a, half8 b, floatx4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Attention over a run of key blocks.  A workgroup takes one key head of a sequence, up to 16 * QT * qw of its
+// rows (the heads / kv_heads query heads of a node are rows next to each other) and one split of its key
+// blocks; its wavefronts are qw groups of 16 * QT rows by kw, each of which takes every kw-th block.  A
+// wavefront reads a block's K and V straight into the registers that the matrix cores take:
+//
+//   Scores transposed, S^T = K Q^T (v_mfma_f32_16x16x32_f16).  The cache holds K as pairs of values, position by
+//   position, so a lane reads KP = 4 or 2 positions of a pair at once: lane 16g + m holds positions KP m ..
+//   KP m + KP - 1 of the pairs of 8 values from 8g on, which are the operand rows of KP tiles, tile u with
+//   position KP m + u in row m.  In the products, lane 16g + i then holds row i's scores of the NP = 4 KP
+//   positions from NP g on.
+//   Outputs transposed, O^T = V^T P^T: those scores are the operand of P as they stand, for k = 8g + e of
+//   instruction kk meaning position NP g + 8kk + e.  A lane reads 4 values (from 4m on) of its NP positions of
+//   V, and v_perm pairs those of two positions.  A row's softmax state is one lane column's everywhere.
+//
+// Blocks are 64 positions for heads of up to 64 values and 32 for those of up to 128: a block's K and V take 64
+// registers a lane either way, all loaded before the first is used.
+//
+// Precision: f32 queries are scaled by a power of two per row and split into two f16 parts, as is every
+// softmax weight for f32 outputs (weights are exp2(s - max + 10), so that the second part is no subnormal):
+// two products each, with an error of 2^-22 against f32's own 2^-24 per sum.  K and V are f16 as stored.
+template <typename T, int HD, int QT, bool P16>
+__global__ __launch_bounds__(512) void attend_kernel(AttendArgs a) {
+  constexpr int C = HD / 32, Z = HD / 64, QP = sizeof(T) == 4 ? 2 : 1;
+  constexpr int KP = 4 / Z, NP = 4 * KP, KB = 16 * KP, KK = KP / 2;
+  typedef uint32_t Words __attribute__((ext_vector_type(KP), aligned(4)));  // a pair's KP positions
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int g = lane >> 4, m = lane & 15;
+  int at = blockIdx.x;
+  const int split = at % a.splits;
+  at /= a.splits;
+  const int kh = at % a.kv_heads;
+  at /= a.kv_heads;
+  const int rb = at % a.row_blocks, b = at / a.row_blocks;
+  const Share s = share_of<KB>(a, b);
+  const int group = a.heads / a.kv_heads, tiles = QT * a.qw, r0 = rb * 16 * tiles, total = s.count * group;
+  if (split >= s.used || r0 >= total) return;
+  const int qi = wave % a.qw, ki = wave / a.qw;
+  const size_t row0 = (size_t)b * a.rows;
+
+  // The queries into LDS, in the operand's order: [tile][chunk of 32 values][part][lane]; 16 threads per row.
+  half8 *qs = (half8 *)smem;
+  float *coef = (float *)(smem + (size_t)tiles * C * QP * 1024);  // per row: scale * log2(e) / the row's power of two
+  for (int x = tid; x < 16 * 16 * tiles; x += blockDim.x) {
+    const int r = x >> 4, l = x & 15, row = min(r0 + r, total - 1);
+    const T *q = (const T *)a.q + (row0 + row / group) * a.stride + (size_t)(kh * group + row % group) * a.hd;
+    float f[Z][4], top = 0.0f;
+#pragma unroll
+    for (int z = 0; z < Z; z++) {
+      const int d = 64 * z + 4 * l;
+      const bool in = d < a.hd;
+      const T *p = q + (in ? d : 0);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        f[z][e] = in ? number(p, e) : 0.0f;
+        top = fmaxf(top, fabsf(f[z][e]));
       }
-      s *= a.scale;
     }
-    float bm = xlane::wave_max(s);
-    if (lane == 0) red[wave] = bm;
-    any |= __syncthreads_or(see) != 0;
-    bm = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float mn = fmaxf(m, bm), m0 = mn == -INFINITY ? 0.0f : mn, old = __expf(m - m0);
-    const float e = see ? __expf(s - m0) : 0.0f;
-    p[tid] = see ? e : -1.0f;  // −1: not seen
-    const float bl = xlane::wave_sum(e);
-    if (lane == 0) red[4 + wave] = bl;
-    __syncthreads();
-    l = l * old + (red[4] + red[5] + red[6] + red[7]);
-    acc *= old;
-    m = mn;
-    if (tid < a.hd)
-      for (int x = 0; x < min(KEYS, total - j0); x++) {
-        const int y = j0 + x;
-        if (p[x] < 0.0f) continue;
-        float val;
-        if (y < n) {
-          const uint32_t w = vc[(size_t)y * half + kh * pairs + tid / 2];
-          val = half_bits(tid & 1 ? w >> 16 : w & 0xffffu);
-        } else {
-          val = (float)(_Float16)number((const T *)a.v + node0 + (size_t)(y - n) * a.stride, tid);
+    int k = 0;
+    if constexpr (QP == 2) {
+      top = fmaxf(top, xlane::dpp<xlane::XOR1>(top));
+      top = fmaxf(top, xlane::dpp<xlane::XOR2>(top));
+      top = fmaxf(top, xlane::dpp<xlane::HALF_MIRROR>(top));
+      top = fmaxf(top, xlane::dpp<xlane::MIRROR>(top));
+      // The row's largest value into [2^7, 2^8).
+      if (top > 0.0f && top < INFINITY) k = min(7 - ilogbf(top), 100);
+    }
+#pragma unroll
+    for (int z = 0; z < Z; z++) {
+      const int d = 64 * z + 4 * l;
+      uint32_t *w = (uint32_t *)(qs + ((size_t)(r / 16 * C + d / 32) * QP) * 64 + (d % 32) / 8 * 16 + r % 16) + (d % 8) / 2;
+      float y[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) y[e] = QP == 2 ? ldexpf(f[z][e], k) : f[z][e];
+      w[0] = pack2(y[0], y[1]), w[1] = pack2(y[2], y[3]);
+      if constexpr (QP == 2) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) y[e] -= (float)(_Float16)y[e];
+        w[256] = pack2(y[0], y[1]), w[257] = pack2(y[2], y[3]);
+      }
+    }
+    if (l == 0) coef[r] = ldexpf(a.scale * 1.44269504088896341f, -k);
+  }
+  __syncthreads();
+
+  const int half = a.kv_heads * a.hd / 2, pairs = a.hd / 2;
+  const uint32_t *kc = a.kv + (size_t)b * a.kv_stride + (size_t)kh * pairs * a.cols;
+  const uint32_t *vc = a.kv + (size_t)b * a.kv_stride + (size_t)half * a.cols + kh * pairs;
+  floatx4 acc[QT][4 * Z];
+  float mx[QT], sum[QT], cf[QT];
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    mx[t] = -INFINITY, sum[t] = 0.0f, cf[t] = coef[(qi * QT + t) * 16 + m];
+#pragma unroll
+    for (int x = 0; x < 4 * Z; x++) acc[t][x] = floatx4{};
+  }
+  const int end = min((split + 1) * s.per, s.blocks);
+  const bool busy = r0 + qi * QT * 16 < total;  // (a wavefront past the last row only meets the others)
+  for (int blk = split * s.per + ki; busy && blk < end; blk += a.kw) {
+    half8 kf[C][KP];
+    u32x2 vw[NP][Z];
+    uint32_t vis[QT];
+    const bool cache = blk < s.cached;
+    const int j0 = (cache ? blk : blk - s.cached) * KB, last = (cache ? s.n : s.count) - 1 - j0;  // the block's last position
+    const bool all = cache && last >= KB - 1;
+    const int left = last + 1 - NP * g;  // of this lane's positions
+    const uint32_t there = left >= NP ? (1u << NP) - 1u : left > 0 ? (1u << left) - 1u : 0u;
+    if (cache) {
+      Words kw[C][4];
+      const int jk = min(KP * m, last & ~(KP - 1));
+#pragma unroll
+      for (int c = 0; c < C; c++) {
+        const uint32_t *base = kc + (size_t)(16 * c) * a.cols + j0;
+        const int top = pairs - 1 - 16 * c;  // the last pair of this chunk, where it has not 16
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+          if (a.cols < KP) {
+#pragma unroll
+            for (int u = 0; u < KP; u++) kw[c][x][u] = top >= 4 * g + x ? base[(4 * g + x) * a.cols + min(jk + u, last)] : 0u;
+          } else if (top >= 15) {  // (past the row's end: the next row, or V)
+            kw[c][x] = *(const Words *)(base + (size_t)x * a.cols + (uint32_t)(4 * g * a.cols + jk));
+          } else {
+            kw[c][x] = *(const Words *)(base + (uint32_t)(max(min(4 * g + x, top), 0) * a.cols + jk));
+            if (top < 4 * g + x) kw[c][x] = Words{};
+          }
         }
-        acc += p[x] * val;
+      }
+      const uint32_t *base = vc + (size_t)j0 * half;
+#pragma unroll
+      for (int e = 0; e < NP; e++)
+#pragma unroll
+        for (int z = 0; z < Z; z++)
+          vw[e][z] = *(const u32x2_a4 *)(base + (uint32_t)(min(NP * g + e, last) * half + (64 * z + 4 * m < a.hd ? 32 * z + 2 * m : 0)));
+#pragma unroll
+      for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int u = 0; u < KP; u++)
+          kf[c][u] = __builtin_bit_cast(half8, u32x4{kw[c][0][u], kw[c][1][u], kw[c][2][u], kw[c][3][u]});
+#pragma unroll
+      for (int t = 0; t < QT; t++) vis[t] = there;
+    } else {
+      const T *k = (const T *)a.k + (row0 + j0) * a.stride + (size_t)kh * a.hd;
+      const T *v = (const T *)a.v + (row0 + j0) * a.stride + (size_t)kh * a.hd;
+      const uint32_t stride = (uint32_t)a.stride;
+#pragma unroll
+      for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int u = 0; u < KP; u++) {
+          const T *src = k + (uint32_t)min(KP * m + u, last) * stride;
+          const int d = 32 * c + 8 * g;
+          u32x2 lo = four(src + (d < a.hd ? d : 0)), hi = four(src + (d + 4 < a.hd ? d + 4 : 0));
+          if (d >= a.hd) lo = u32x2{};
+          if (d + 4 >= a.hd) hi = u32x2{};
+          kf[c][u] = __builtin_bit_cast(half8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+        }
+#pragma unroll
+      for (int e = 0; e < NP; e++)
+#pragma unroll
+        for (int z = 0; z < Z; z++)
+          vw[e][z] = four(v + (uint32_t)min(NP * g + e, last) * stride + (64 * z + 4 * m < a.hd ? 64 * z + 4 * m : 0));
+#pragma unroll
+      for (int t = 0; t < QT; t++) {
+        const int i = min(r0 + (qi * QT + t) * 16 + m, total - 1) / group, j = j0 + NP * g;
+        vis[t] = j < a.rows ? a.mask[(size_t)b * a.mask_stride + (size_t)i * a.words + j / 32] >> (j % 32) & there : 0u;
+      }
+    }
+
+    // (read again for every block: with the values in registers all along, a wavefront would spill)
+    uint32_t qat = (qi * QT * C * QP) * 64 + lane;
+    asm volatile("" : "+v"(qat));
+    floatx4 st[QT][KP];
+#pragma unroll
+    for (int t = 0; t < QT; t++)
+#pragma unroll
+      for (int u = 0; u < KP; u++) st[t][u] = floatx4{};
+#pragma unroll
+    for (int t = 0; t < QT; t++)
+#pragma unroll
+      for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int part = 0; part < QP; part++) {
+          const half8 q = qs[qat + ((t * C + c) * QP + part) * 64];
+#pragma unroll
+          for (int u = 0; u < KP; u++) st[t][u] = mfma(kf[c][u], q, st[t][u]);
+        }
+
+    // The softmax: element KP r + u of the lane's NP positions is st[u][r].
+    half8 ph[QT][KK], pl[QT][KK];
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+      if (!all)
+#pragma unroll
+        for (int e = 0; e < NP; e++)
+          if (!(vis[t] >> e & 1)) st[t][e % KP][e / KP] = -INFINITY;
+      float top = st[t][0][0];
+#pragma unroll
+      for (int e = 1; e < NP; e++) top = fmaxf(top, st[t][e % KP][e / KP]);
+      top = xlane::bit4(top, xlane::Max{});
+      top = xlane::bit5(top, xlane::Max{});
+      top = fmaxf(top, mx[t]);
+      const float base = top == -INFINITY ? 0.0f : top;
+      if (__any(top != mx[t])) {
+        const float old = mx[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mx[t] - top) * cf[t]);
+        sum[t] *= old;
+#pragma unroll
+        for (int x = 0; x < 4 * Z; x++) acc[t][x] *= old;
+        mx[t] = top;
+      }
+#pragma unroll
+      for (int e = 0; e < NP; e++) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(st[t][e % KP][e / KP] - base, cf[t], 10.0f));
+        sum[t] += p;
+        const _Float16 h = (_Float16)p;
+        ph[t][e >> 3][e & 7] = h;
+        if constexpr (!P16) pl[t][e >> 3][e & 7] = (_Float16)(p - (float)h);
+      }
+    }
+
+    if (!all) {
+      // Values of positions that are not there are zeroed; one that is no finite number (bad: its rows' outputs) must
+      // not meet the zero weights of the rows that do not see it.
+      u16x2 big{};
+#pragma unroll
+      for (int e = 0; e < NP; e++)
+#pragma unroll
+        for (int z = 0; z < Z; z++) {
+          if (e >= left) vw[e][z] = u32x2{};
+          big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2, vw[e][z][0] & 0x7fff7fffu));
+          big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2, vw[e][z][1] & 0x7fff7fffu));
+        }
+      if (!cache && __any(big[0] >= 0x7c00 || big[1] >= 0x7c00)) {
+        // Which rows see a NaN, an infinity or a negative one, value by value, and the rest as if it were zero.
+        for (int kind = 0; kind < 3; kind++)
+#pragma unroll
+          for (int x = 0; x < 4 * Z; x++)
+#pragma unroll
+            for (int kk = 0; kk < KK; kk++) {
+              half8 is;
+#pragma unroll
+              for (int e = 0; e < 8; e++) {
+                const uint32_t h = vw[8 * kk + e][x / 4][x % 4 / 2] >> (16 * (x & 1)) & 0xffffu;
+                is[e] = (_Float16)(kind == 0 ? (h & 0x7fffu) > 0x7c00u : kind == 1 ? h == 0x7c00u : h == 0xfc00u);
+              }
+#pragma unroll
+              for (int t = 0; t < QT; t++) {
+                half8 see;
+#pragma unroll
+                for (int e = 0; e < 8; e++) see[e] = (_Float16)(vis[t] >> (8 * kk + e) & 1);
+                const floatx4 seen = mfma(is, see, floatx4{});
+#pragma unroll
+                for (int r = 0; r < 4; r++)
+                  if (seen[r] > 0.0f) acc[t][x][r] += kind == 0 ? NAN : kind == 1 ? INFINITY : -INFINITY;
+              }
+            }
+#pragma unroll
+        for (int e = 0; e < NP; e++)
+#pragma unroll
+          for (int z = 0; z < Z; z++)
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+              if ((vw[e][z][w] & 0x7c00u) == 0x7c00u) vw[e][z][w] &= 0xffff0000u;
+              if ((vw[e][z][w] & 0x7c000000u) == 0x7c000000u) vw[e][z][w] &= 0xffffu;
+            }
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < 4 * Z; x++)
+#pragma unroll
+      for (int kk = 0; kk < KK; kk++) {
+        u32x4 w;
+#pragma unroll
+        for (int y = 0; y < 4; y++)
+          w[y] = __builtin_amdgcn_perm(vw[8 * kk + 2 * y + 1][x / 4][x % 4 / 2], vw[8 * kk + 2 * y][x / 4][x % 4 / 2],
+                                       x & 1 ? 0x07060302u : 0x05040100u);
+        const half8 vf = __builtin_bit_cast(half8, w);
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+          acc[t][x] = mfma(vf, ph[t][kk], acc[t][x]);
+          if constexpr (!P16) acc[t][x] = mfma(vf, pl[t][kk], acc[t][x]);
+        }
       }
   }
-  if (tid < a.hd) ((OT *)a.o)[((size_t)row * a.heads + head) * a.hd + tid] = (OT)(any ? acc / l : 0.0f);
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    sum[t] = xlane::bit4(sum[t], xlane::Add{});
+    sum[t] = xlane::bit5(sum[t], xlane::Add{});
+  }
+
+  // The key groups' results joined through LDS, half of them at a time into the other half.
+  floatx4 *merge = (floatx4 *)smem;
+  constexpr int SLOT = QT * (4 * Z * 64 + 32);  // 16-byte units of one wavefront's accumulators, then maxima and sums
+  for (int step = a.kw / 2; step; step /= 2) {
+    __syncthreads();
+    floatx4 *slot = merge + (size_t)((ki % step) * a.qw + qi) * SLOT;
+    float *ml = (float *)(slot + QT * 4 * Z * 64);
+    if (ki >= step && ki < 2 * step) {
+#pragma unroll
+      for (int t = 0; t < QT; t++) {
+#pragma unroll
+        for (int x = 0; x < 4 * Z; x++) slot[(t * 4 * Z + x) * 64 + lane] = acc[t][x];
+        ml[t * 128 + lane] = mx[t], ml[t * 128 + 64 + lane] = sum[t];
+      }
+    }
+    __syncthreads();
+    if (ki < step) {
+#pragma unroll
+      for (int t = 0; t < QT; t++) {
+        const float om = ml[t * 128 + lane], os = ml[t * 128 + 64 + lane], top = fmaxf(mx[t], om);
+        const float f = mx[t] == top ? 1.0f : __builtin_amdgcn_exp2f((mx[t] - top) * cf[t]);
+        const float of = om == top ? 1.0f : __builtin_amdgcn_exp2f((om - top) * cf[t]);
+        sum[t] = sum[t] * f + os * of, mx[t] = top;
+#pragma unroll
+        for (int x = 0; x < 4 * Z; x++) acc[t][x] = acc[t][x] * f + slot[(t * 4 * Z + x) * 64 + lane] * of;
+      }
+    }
+  }
+  if (ki || !busy) return;
+  // Lane 16g + i holds row i's values 16g + 4r + (x % 4) of the chunk of 64 x / 4.
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    const int r = r0 + (qi * QT + t) * 16 + m;
+    if (r >= total) continue;
+    const int i = r / group, head = kh * group + r % group;
+    const size_t out = ((row0 + i) * a.heads + head) * a.hd;
+    if (s.used > 1) {
+      const size_t part = (size_t)split * a.batch * a.rows * a.heads;
+      if (g == 0) {
+        float *ml = a.pml + 2 * (part + (row0 + i) * a.heads + head);
+        ml[0] = mx[t] * cf[t], ml[1] = sum[t];
+      }
+#pragma unroll
+      for (int z = 0; z < Z; z++)
+#pragma unroll
+        for (int y = 0; y < 4; y++) {
+          const int d = 64 * z + 16 * g + 4 * y;
+          if (d < a.hd)
+            *(floatx4 *)(a.po + part * a.hd + out + d) =
+                floatx4{acc[t][4 * z][y], acc[t][4 * z + 1][y], acc[t][4 * z + 2][y], acc[t][4 * z + 3][y]};
+        }
+      continue;
+    }
+    const float inv = sum[t] == 0.0f && !sees_any(a, s, b, i) ? 0.0f : 1.0f / sum[t];
+#pragma unroll
+    for (int z = 0; z < Z; z++)
+#pragma unroll
+      for (int y = 0; y < 4; y++) {
+        const int d = 64 * z + 16 * g + 4 * y;
+        if (d >= a.hd) continue;
+        const floatx4 f = floatx4{acc[t][4 * z][y], acc[t][4 * z + 1][y], acc[t][4 * z + 2][y], acc[t][4 * z + 3][y]} * inv;
+        if constexpr (P16) *(u32x2_a4 *)((_Float16 *)a.o + out + d) = u32x2{pack2(f[0], f[1]), pack2(f[2], f[3])};
+        else *(floatx4_a4 *)((float *)a.o + out + d) = f;
+      }
+  }
+}
+
+// The splits' outputs of one head of a node rescaled to their common maximum, summed and divided; one wavefront
+// each, two values a lane.
+template <int KB, bool P16>
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
+  const int lane = threadIdx.x & 63, at = blockIdx.x * 4 + (threadIdx.x >> 6), heads = a.batch * a.rows * a.heads;
+  if (at >= heads) return;
+  const int row = at / a.heads, b = row / a.rows, i = row % a.rows;
+  const Share s = share_of<KB>(a, b);
+  if (s.used == 1 || i >= s.count) return;
+  float top = -INFINITY;
+  for (int x = 0; x < s.used; x++) top = fmaxf(top, a.pml[2 * ((size_t)x * heads + at)]);
+  const int d = 2 * lane;
+  float sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
+  for (int x = 0; x < s.used; x++) {
+    const float mx = a.pml[2 * ((size_t)x * heads + at)], f = mx == top ? 1.0f : __builtin_amdgcn_exp2f(mx - top);
+    sum += f * a.pml[2 * ((size_t)x * heads + at) + 1];
+    if (d < a.hd) {
+      const float2 p = *(const float2 *)(a.po + ((size_t)x * heads + at) * a.hd + d);
+      o0 += f * p.x, o1 += f * p.y;
+    }
+  }
+  if (d >= a.hd) return;
+  const float inv = sum == 0.0f && !sees_any(a, s, b, i) ? 0.0f : 1.0f / sum;
+  if constexpr (P16) *(uint32_t *)((_Float16 *)a.o + (size_t)at * a.hd + d) = pack2(o0 * inv, o1 * inv);
+  else *(float *)((float *)a.o + (size_t)at * a.hd + d) = o0 * inv, *(float *)((float *)a.o + (size_t)at * a.hd + d + 1) = o1 * inv;
 }
 
 // ------------------------------------------------------------------------------------- the kept path
@@ -167,6 +535,31 @@ __global__ __launch_bounds__(256) void keep_kernel(KeepArgs a) {
   }
 }
 
+constexpr int key_block(int hd) { return hd <= 64 ? 64 : 32; }
+
+template <typename T, int HD, int QT, bool P16>
+int attend_launch(wh_ctx *ctx, const AttendArgs &a) {
+  const size_t tiles = QT * a.qw, queries = tiles * (HD / 32 * (sizeof(T) == 4 ? 2 : 1) * 1024 + 64);
+  const size_t merge = (size_t)(a.kw / 2) * a.qw * QT * (4 * HD / 64 * 64 + 32) * 16;
+  {
+    ProfScope prof(ctx, "tree_attend", 4.0 * a.batch * a.rows * a.heads * a.cols * a.hd, 4.0 * a.batch * a.cols * a.kv_heads * a.hd);
+    wh_launch(ctx, (attend_kernel<T, HD, QT, P16>), a.batch * a.row_blocks * a.kv_heads * a.splits, 64 * a.qw * a.kw,
+              std::max(queries, merge), a);
+    if (int rc = wh_launched(ctx, "tree attention")) return rc;
+  }
+  if (a.splits == 1) return WH_OK;
+  const double heads = (double)a.batch * a.rows * a.heads;
+  ProfScope prof(ctx, "tree_attend_join", 0.0, 4.0 * heads * a.splits * (a.hd + 2));
+  wh_launch(ctx, (attend_join_kernel<key_block(HD), P16>), (a.batch * a.rows * a.heads + 3) / 4, 256, 0, a);
+  return wh_launched(ctx, "tree attention's join");
+}
+
+template <typename T, bool P16>
+int attend_t(wh_ctx *ctx, const AttendArgs &a, int qt) {
+  if (a.hd <= 64) return qt == 1 ? attend_launch<T, 64, 1, P16>(ctx, a) : attend_launch<T, 64, 2, P16>(ctx, a);
+  return qt == 1 ? attend_launch<T, 128, 1, P16>(ctx, a) : attend_launch<T, 128, 2, P16>(ctx, a);
+}
+
 }  // namespace
 
 int tree_check(wh_ctx *ctx, const char *what, const wh_tree *t) {
@@ -184,27 +577,39 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
                        const uint32_t *kv, size_t kv_stride, int cols, void *o, int out16, int heads, int kv_heads, int hd) {
   if (int rc = tree_check(ctx, "tree attention", t)) return rc;
   if (!q || !kv || !o || !k != !v) return wh_fail(ctx, WH_EARG, "tree attention: q, the cache, o, and k with v are needed");
-  if (heads <= 0 || heads > ATTEND_HEADS || kv_heads <= 0 || heads % kv_heads || hd <= 0 || hd > 128 || hd % 4 || cols <= 0)
+  if (heads <= 0 || heads > ATTEND_HEADS || kv_heads <= 0 || heads % kv_heads || hd <= 0 || hd > 128 || hd % 4 || cols <= 0 || cols > 1 << 26)
     return wh_fail(ctx, WH_EARG, "tree attention: bad shape (heads %d, key heads %d, head_dim %d, cols %d)", heads, kv_heads, hd,
                    cols);
-  if (stride < (size_t)heads * hd || stride > (size_t)1 << 31)
+  if (stride < (size_t)heads * hd || stride > (size_t)1 << 23)
     return wh_fail(ctx, WH_EARG, "tree attention: rows of %d queries %zu apart", heads * hd, stride);
   if (kv_stride && kv_stride < (size_t)cols * kv_heads * hd)
     return wh_fail(ctx, WH_EARG, "tree attention: caches of %zu words %zu apart", (size_t)cols * kv_heads * hd, kv_stride);
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)kv | (uintptr_t)o) % 4 || (in16 && stride % 2))
     return wh_fail(ctx, WH_EARG, "tree attention: buffers and rows must be 4-byte aligned");
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "tree attention: %s", hipGetErrorString(e));
-  const AttendArgs a{q, k, v, stride, kv, kv_stride, o, t->n, t->count, t->mask, t->mask_stride, t->rows, (t->rows + 31) / 32,
-                     cols, heads, heads / kv_heads, hd, 1.0f / sqrtf((float)hd)};
-  if ((size_t)t->batch * t->rows * heads >= (size_t)1 << 24)  // (a launch's threads fit 32 bits)
-    return wh_fail(ctx, WH_EARG, "tree attention: %d heads of %d nodes in one call", heads, t->batch * t->rows);
-  const int grid = t->batch * t->rows * heads;
-  ProfScope prof(ctx, "tree_attend", 4.0 * grid * cols * hd, 4.0 * t->batch * cols * kv_heads * hd);
-  if (in16 && out16) wh_launch(ctx, (attend_kernel<_Float16, _Float16>), grid, KEYS, 0, a);
-  else if (in16) wh_launch(ctx, (attend_kernel<_Float16, float>), grid, KEYS, 0, a);
-  else if (out16) wh_launch(ctx, (attend_kernel<float, _Float16>), grid, KEYS, 0, a);
-  else wh_launch(ctx, (attend_kernel<float, float>), grid, KEYS, 0, a);
-  return wh_launched(ctx, "tree attention");
+  AttendArgs a{q, k, v, stride, kv, kv_stride, o, t->n, t->count, t->mask, t->mask_stride, t->batch, t->rows, (t->rows + 31) / 32,
+               cols, heads, kv_heads, hd, 1.0f / sqrtf((float)hd), 1, 1, 1, 1, nullptr, nullptr};
+  const int rows = t->rows * (heads / kv_heads), tiles = (rows + 15) / 16;
+  const int qt = tiles > 1 ? 2 : 1;
+  const int qwaves = (tiles + qt - 1) / qt;
+  constexpr int WAVES = 8;
+  while (a.qw < std::min(qwaves, WAVES)) a.qw *= 2;
+  a.kw = WAVES / a.qw;
+  a.row_blocks = (qwaves + a.qw - 1) / a.qw;
+  const size_t units = (size_t)t->batch * kv_heads * a.row_blocks;
+  const int kb = key_block(hd), blocks = (cols + kb - 1) / kb + (t->mask && k ? (t->rows + kb - 1) / kb : 0);
+  const size_t cus = ctx->cus > 0 ? ctx->cus : 256;
+  a.splits = (int)std::max<size_t>(1, std::min<size_t>((2 * cus + units - 1) / units, (blocks + a.kw - 1) / a.kw));
+  const size_t nodes = (size_t)t->batch * t->rows;
+  if (units * a.splits >= (size_t)1 << 22 || nodes * heads >= (size_t)1 << 25)  // (a launch's threads fit 32 bits)
+    return wh_fail(ctx, WH_EARG, "tree attention: %d heads of %zu nodes in one call", heads, nodes);
+  if (a.splits > 1) {
+    const size_t part = (size_t)a.splits * nodes * heads;
+    if (!(a.po = (float *)wh_scratch(ctx, part * (hd + 2) * sizeof(float)))) return WH_EOOM;
+    a.pml = a.po + part * hd;
+  }
+  return in16 ? out16 ? attend_t<_Float16, true>(ctx, a, qt) : attend_t<_Float16, false>(ctx, a, qt)
+              : out16 ? attend_t<float, true>(ctx, a, qt) : attend_t<float, false>(ctx, a, qt);
 }
 
 int launch_tree_accept(wh_ctx *ctx, const wh_tree *t, const uint32_t *picks, const wh_kept *w, int cols, int32_t *path,
