@@ -2,6 +2,7 @@
 // its sequence's f16 cache and the nodes that it sees, and the path of the tree that is kept.
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "internal.h"
 #include "xlane.h"
@@ -33,17 +34,21 @@ struct AttendArgs {
   int batch, rows, words, cols, heads, kv_heads, hd;
   float scale;
   int qw, kw, splits, row_blocks;
-  // splits > 1: unnormalized outputs [split][batch * rows][heads][hd] and (maximum, sum) pairs
-  // [split][batch * rows][heads] of the splits that are used.
+  // splits > 1: unnormalized outputs [split][batch * rows][heads][hd] and (maximum, sum, factor of the maximum's
+  // exponent, -) [split][batch * rows][heads] of the splits that are used.
   float *po, *pml;
 };
+
+constexpr int KB = 32;  // keys per block
+
+// Wavefronts of a workgroup, at most: 16 where one needs no more than 128 registers.
+constexpr int most_waves(int hd, int qt) { return hd == 64 && qt == 1 ? 16 : 8; }
 
 // The blocks of keys of a sequence (the cache's, then the nodes'), and how its `splits` workgroups share them:
 // runs of `per` blocks, at least one for each wavefront, so that a short sequence uses fewer of them.
 struct Share {
   int n, count, cached, blocks, per, used;
 };
-template <int KB>
 __device__ __forceinline__ Share share_of(const AttendArgs &a, int b) {
   Share s;
   s.n = min(max(a.n[b], 0), a.cols);
@@ -75,35 +80,37 @@ __device__ __forceinline__ u32x2 four(const float *p) {
 }
 __device__ __forceinline__ u32x2 four(const _Float16 *p) { return *(const u32x2_a4 *)p; }
 
+// The 8 mask bits of node i from node j on.
+__device__ __forceinline__ uint32_t node_mask(const AttendArgs &a, int b, int i, int j) {
+  return j < a.rows ? a.mask[(size_t)b * a.mask_stride + (size_t)i * a.words + j / 32] >> (j % 32) : 0u;
+}
+
 __device__ __forceinline__ floatx4 mfma(half8 a, half8 b, floatx4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
 // Attention over a run of key blocks.  A workgroup takes one key head of a sequence, up to 16 * QT * qw of its
 // rows (the heads / kv_heads query heads of a node are rows next to each other) and one split of its key
-// blocks; its wavefronts are qw groups of 16 * QT rows by kw, each of which takes every kw-th block.  A
+// blocks of 32; its wavefronts are qw groups of 16 * QT rows by kw, each of which takes every kw-th block.  A
 // wavefront reads a block's K and V straight into the registers that the matrix cores take:
 //
 //   Scores transposed, S^T = K Q^T (v_mfma_f32_16x16x32_f16).  The cache holds K as pairs of values, position by
-//   position, so a lane reads KP = 4 or 2 positions of a pair at once: lane 16g + m holds positions KP m ..
-//   KP m + KP - 1 of the pairs of 8 values from 8g on, which are the operand rows of KP tiles, tile u with
-//   position KP m + u in row m.  In the products, lane 16g + i then holds row i's scores of the NP = 4 KP
-//   positions from NP g on.
-//   Outputs transposed, O^T = V^T P^T: those scores are the operand of P as they stand, for k = 8g + e of
-//   instruction kk meaning position NP g + 8kk + e.  A lane reads 4 values (from 4m on) of its NP positions of
-//   V, and v_perm pairs those of two positions.  A row's softmax state is one lane column's everywhere.
+//   position, so a lane reads two positions of a pair at once: lane 16g + m holds positions 2m and 2m + 1 of the
+//   pairs of 8 values from 8g on, which are the operand rows of two tiles, tile u with position 2m + u in row m.
+//   In the products, lane 16g + i then holds row i's scores of the 8 positions from 8g on.
+//   Outputs transposed, O^T = V^T P^T: those scores are the operand of P as they stand, k = 8g + e meaning position
+//   8g + e.  A lane reads 4 values (from 4m on) of its 8 positions of V, and v_perm pairs those of two positions.
+//   A row's softmax state is one lane column's everywhere.
 //
-// Blocks are 64 positions for heads of up to 64 values and 32 for those of up to 128: a block's K and V take 64
-// registers a lane either way, all loaded before the first is used.
+// The next block's K is loaded as soon as this one's scores are done, and its V after this one's outputs, so that
+// a wavefront always has loads in flight; the first block's before the queries are staged.
 //
 // Precision: f32 queries are scaled by a power of two per row and split into two f16 parts, as is every
 // softmax weight for f32 outputs (weights are exp2(s - max + 10), so that the second part is no subnormal):
 // two products each, with an error of 2^-22 against f32's own 2^-24 per sum.  K and V are f16 as stored.
 template <typename T, int HD, int QT, bool P16>
-__global__ __launch_bounds__(512) void attend_kernel(AttendArgs a) {
+__global__ __launch_bounds__(64 * most_waves(HD, QT)) void attend_kernel(AttendArgs a) {
   constexpr int C = HD / 32, Z = HD / 64, QP = sizeof(T) == 4 ? 2 : 1;
-  constexpr int KP = 4 / Z, NP = 4 * KP, KB = 16 * KP, KK = KP / 2;
-  typedef uint32_t Words __attribute__((ext_vector_type(KP), aligned(4)));  // a pair's KP positions
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, m = lane & 15;
@@ -113,32 +120,119 @@ __global__ __launch_bounds__(512) void attend_kernel(AttendArgs a) {
   const int kh = at % a.kv_heads;
   at /= a.kv_heads;
   const int rb = at % a.row_blocks, b = at / a.row_blocks;
-  const Share s = share_of<KB>(a, b);
-  const int group = a.heads / a.kv_heads, tiles = QT * a.qw, r0 = rb * 16 * tiles, total = s.count * group;
-  if (split >= s.used || r0 >= total) return;
-  const int qi = wave % a.qw, ki = wave / a.qw;
+  const int group = a.heads / a.kv_heads, tiles = QT * a.qw, r0 = rb * 16 * tiles, all_rows = a.rows * group;
   const size_t row0 = (size_t)b * a.rows;
-
-  // The queries into LDS, in the operand's order: [tile][chunk of 32 values][part][lane]; 16 threads per row.
-  half8 *qs = (half8 *)smem;
-  float *coef = (float *)(smem + (size_t)tiles * C * QP * 1024);  // per row: scale * log2(e) / the row's power of two
-  for (int x = tid; x < 16 * 16 * tiles; x += blockDim.x) {
-    const int r = x >> 4, l = x & 15, row = min(r0 + r, total - 1);
+  // Four (or, z = 1 too, eight) values of a row's query: 16 threads per row.
+  auto query = [&](int x, float (&f)[Z][4]) {
+    const int row = min(r0 + (x >> 4), all_rows - 1);
     const T *q = (const T *)a.q + (row0 + row / group) * a.stride + (size_t)(kh * group + row % group) * a.hd;
-    float f[Z][4], top = 0.0f;
 #pragma unroll
     for (int z = 0; z < Z; z++) {
-      const int d = 64 * z + 4 * l;
-      const bool in = d < a.hd;
-      const T *p = q + (in ? d : 0);
+      const int d = 64 * z + 4 * (x & 15);
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        f[z][e] = in ? number(p, e) : 0.0f;
-        top = fmaxf(top, fabsf(f[z][e]));
+      for (int e = 0; e < 4; e++) f[z][e] = d < a.hd ? number(q + d, e) : 0.0f;
+    }
+  };
+  float first[Z][4];
+  query(tid, first);
+  const Share s = share_of(a, b);
+  const int total = s.count * group;
+  if (split >= s.used || r0 >= total) return;
+  const int qi = wave % a.qw, ki = wave / a.qw;
+  const int half = a.kv_heads * a.hd / 2, pairs = a.hd / 2;
+  const uint32_t *kc = a.kv + (size_t)b * a.kv_stride + (size_t)kh * pairs * a.cols;
+  const uint32_t *vc = a.kv + (size_t)b * a.kv_stride + (size_t)half * a.cols + kh * pairs;
+  const bool busy = r0 + qi * QT * 16 < total;  // (a wavefront past the last row only meets the others)
+
+  u32x2 kw[C][4], vw[8][Z];  // a block's K, pair by pair, and V, position by position
+  // The same loads on every way through, so that a wait for one block's does not have to be one for the next block's.
+  auto load_k = [&](int blk) {
+    // (made anew for every block: what follows from them would otherwise be kept in more registers than there are)
+    int hd = a.hd, cols = a.cols;
+    asm volatile("" : "+s"(hd), "+s"(cols));
+    const int j0 = blk * KB, last = s.n - 1 - j0, jk = min(2 * m, last & ~1);  // (a position past the row's end: the next row, or V)
+#pragma unroll
+    for (int c = 0; c < C; c++) {
+      const uint32_t *base = kc + (size_t)(16 * c) * cols + j0;
+      const int top = hd / 2 - 1 - 16 * c;  // the last pair of this chunk, where it has not 16
+      if (top >= 15) {
+#pragma unroll
+        for (int x = 0; x < 4; x++) kw[c][x] = *(const u32x2_a4 *)(base + (size_t)x * cols + (uint32_t)(4 * g * cols + jk));
+      } else {
+#pragma unroll
+        for (int x = 0; x < 4; x++) {
+          kw[c][x] = *(const u32x2_a4 *)(base + (int64_t)max(min(4 * g + x, top), -16 * c) * cols + jk);
+          if (top < 4 * g + x) kw[c][x] = u32x2{};
+        }
       }
     }
+  };
+  auto load_v = [&](int blk) {
+    const int j0 = blk * KB, last = s.n - 1 - j0;
+    const uint32_t *base = vc + (size_t)j0 * half;
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+#pragma unroll
+      for (int z = 0; z < Z; z++)
+        vw[e][z] = *(const u32x2_a4 *)(base + (uint32_t)(min(8 * g + e, last) * half + (64 * z + 4 * m < a.hd ? 32 * z + 2 * m : 0)));
+  };
+  auto load_nodes = [&](int blk) {
+    const int j0 = (blk - s.cached) * KB, last = s.count - 1 - j0;
+    const T *k = (const T *)a.k + (row0 + j0) * a.stride + (size_t)kh * a.hd;
+    const T *v = (const T *)a.v + (row0 + j0) * a.stride + (size_t)kh * a.hd;
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const T *src = k + (uint32_t)min(2 * m + u, last) * (uint32_t)a.stride;
+        const int d = 32 * c + 8 * g;
+        u32x2 lo = four(src + (d < a.hd ? d : 0)), hi = four(src + (d + 4 < a.hd ? d + 4 : 0));
+        if (d >= a.hd) lo = u32x2{};
+        if (d + 4 >= a.hd) hi = u32x2{};
+        kw[c][0][u] = lo[0], kw[c][1][u] = lo[1], kw[c][2][u] = hi[0], kw[c][3][u] = hi[1];
+      }
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+#pragma unroll
+      for (int z = 0; z < Z; z++)
+        vw[e][z] = four(v + (uint32_t)min(8 * g + e, last) * (uint32_t)a.stride + (64 * z + 4 * m < a.hd ? 64 * z + 4 * m : 0));
+  };
+  int blk = split * s.per + ki;
+  const int end = min((split + 1) * s.per, s.blocks), cached = min(end, s.cached);
+  if (busy && blk < cached) {
+    if (a.cols > 1) {
+      load_k(blk);
+    } else {  // (a cache of one position: nothing behind it)
+#pragma unroll
+      for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int x = 0; x < 4; x++) kw[c][x] = u32x2{16 * c + 4 * g + x < pairs ? kc[16 * c + 4 * g + x] : 0u, 0u};
+    }
+    load_v(blk);
+  } else if (busy && blk < end) {
+    load_nodes(blk);
+  }
+
+  // The queries into LDS, in the operand's order: [tile][chunk of 32 values][part][lane].
+  float *coef = (float *)smem;  // per row: scale * log2(e) / the row's power of two
+  half8 *qs = (half8 *)(smem + 64 * tiles);
+  for (int x = tid; x < 16 * 16 * tiles; x += blockDim.x) {
+    float f[Z][4], top = 0.0f;
+    if (x == tid) {
+#pragma unroll
+      for (int z = 0; z < Z; z++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) f[z][e] = first[z][e];
+    } else {
+      query(x, f);
+    }
+    const int r = x >> 4, l = x & 15;
     int k = 0;
     if constexpr (QP == 2) {
+#pragma unroll
+      for (int z = 0; z < Z; z++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(f[z][e]));
       top = fmaxf(top, xlane::dpp<xlane::XOR1>(top));
       top = fmaxf(top, xlane::dpp<xlane::XOR2>(top));
       top = fmaxf(top, xlane::dpp<xlane::HALF_MIRROR>(top));
@@ -164,9 +258,6 @@ __global__ __launch_bounds__(512) void attend_kernel(AttendArgs a) {
   }
   __syncthreads();
 
-  const int half = a.kv_heads * a.hd / 2, pairs = a.hd / 2;
-  const uint32_t *kc = a.kv + (size_t)b * a.kv_stride + (size_t)kh * pairs * a.cols;
-  const uint32_t *vc = a.kv + (size_t)b * a.kv_stride + (size_t)half * a.cols + kh * pairs;
   floatx4 acc[QT][4 * Z];
   float mx[QT], sum[QT], cf[QT];
 #pragma unroll
@@ -175,107 +266,50 @@ __global__ __launch_bounds__(512) void attend_kernel(AttendArgs a) {
 #pragma unroll
     for (int x = 0; x < 4 * Z; x++) acc[t][x] = floatx4{};
   }
-  const int end = min((split + 1) * s.per, s.blocks);
-  const bool busy = r0 + qi * QT * 16 < total;  // (a wavefront past the last row only meets the others)
-  for (int blk = split * s.per + ki; busy && blk < end; blk += a.kw) {
-    half8 kf[C][KP];
-    u32x2 vw[NP][Z];
-    uint32_t vis[QT];
-    const bool cache = blk < s.cached;
-    const int j0 = (cache ? blk : blk - s.cached) * KB, last = (cache ? s.n : s.count) - 1 - j0;  // the block's last position
-    const bool all = cache && last >= KB - 1;
-    const int left = last + 1 - NP * g;  // of this lane's positions
-    const uint32_t there = left >= NP ? (1u << NP) - 1u : left > 0 ? (1u << left) - 1u : 0u;
-    if (cache) {
-      Words kw[C][4];
-      const int jk = min(KP * m, last & ~(KP - 1));
-#pragma unroll
-      for (int c = 0; c < C; c++) {
-        const uint32_t *base = kc + (size_t)(16 * c) * a.cols + j0;
-        const int top = pairs - 1 - 16 * c;  // the last pair of this chunk, where it has not 16
-#pragma unroll
-        for (int x = 0; x < 4; x++) {
-          if (a.cols < KP) {
-#pragma unroll
-            for (int u = 0; u < KP; u++) kw[c][x][u] = top >= 4 * g + x ? base[(4 * g + x) * a.cols + min(jk + u, last)] : 0u;
-          } else if (top >= 15) {  // (past the row's end: the next row, or V)
-            kw[c][x] = *(const Words *)(base + (size_t)x * a.cols + (uint32_t)(4 * g * a.cols + jk));
-          } else {
-            kw[c][x] = *(const Words *)(base + (uint32_t)(max(min(4 * g + x, top), 0) * a.cols + jk));
-            if (top < 4 * g + x) kw[c][x] = Words{};
-          }
-        }
-      }
-      const uint32_t *base = vc + (size_t)j0 * half;
-#pragma unroll
-      for (int e = 0; e < NP; e++)
-#pragma unroll
-        for (int z = 0; z < Z; z++)
-          vw[e][z] = *(const u32x2_a4 *)(base + (uint32_t)(min(NP * g + e, last) * half + (64 * z + 4 * m < a.hd ? 32 * z + 2 * m : 0)));
-#pragma unroll
-      for (int c = 0; c < C; c++)
-#pragma unroll
-        for (int u = 0; u < KP; u++)
-          kf[c][u] = __builtin_bit_cast(half8, u32x4{kw[c][0][u], kw[c][1][u], kw[c][2][u], kw[c][3][u]});
-#pragma unroll
-      for (int t = 0; t < QT; t++) vis[t] = there;
-    } else {
-      const T *k = (const T *)a.k + (row0 + j0) * a.stride + (size_t)kh * a.hd;
-      const T *v = (const T *)a.v + (row0 + j0) * a.stride + (size_t)kh * a.hd;
-      const uint32_t stride = (uint32_t)a.stride;
-#pragma unroll
-      for (int c = 0; c < C; c++)
-#pragma unroll
-        for (int u = 0; u < KP; u++) {
-          const T *src = k + (uint32_t)min(KP * m + u, last) * stride;
-          const int d = 32 * c + 8 * g;
-          u32x2 lo = four(src + (d < a.hd ? d : 0)), hi = four(src + (d + 4 < a.hd ? d + 4 : 0));
-          if (d >= a.hd) lo = u32x2{};
-          if (d + 4 >= a.hd) hi = u32x2{};
-          kf[c][u] = __builtin_bit_cast(half8, u32x4{lo[0], lo[1], hi[0], hi[1]});
-        }
-#pragma unroll
-      for (int e = 0; e < NP; e++)
-#pragma unroll
-        for (int z = 0; z < Z; z++)
-          vw[e][z] = four(v + (uint32_t)min(NP * g + e, last) * stride + (64 * z + 4 * m < a.hd ? 64 * z + 4 * m : 0));
-#pragma unroll
-      for (int t = 0; t < QT; t++) {
-        const int i = min(r0 + (qi * QT + t) * 16 + m, total - 1) / group, j = j0 + NP * g;
-        vis[t] = j < a.rows ? a.mask[(size_t)b * a.mask_stride + (size_t)i * a.words + j / 32] >> (j % 32) & there : 0u;
-      }
-    }
-
+  // One block: 0 a whole one of the cache, with the next one's loads; 1 the last one of the cache; 2 one of nodes.
+  auto step = [&](auto which) {
+    constexpr int KIND = which;
+    constexpr bool all = KIND == 0;
+    const int j0 = (KIND == 2 ? blk - s.cached : blk) * KB, last = (KIND == 2 ? s.count : s.n) - 1 - j0;
+    const int left = last + 1 - 8 * g;  // of this lane's positions
     // (read again for every block: with the values in registers all along, a wavefront would spill)
     uint32_t qat = (qi * QT * C * QP) * 64 + lane;
     asm volatile("" : "+v"(qat));
-    floatx4 st[QT][KP];
+    floatx4 st[QT][2];
 #pragma unroll
-    for (int t = 0; t < QT; t++)
+    for (int t = 0; t < QT; t++) st[t][0] = st[t][1] = floatx4{};
 #pragma unroll
-      for (int u = 0; u < KP; u++) st[t][u] = floatx4{};
+    for (int c = 0; c < C; c++) {
+      const half8 k0 = __builtin_bit_cast(half8, u32x4{kw[c][0][0], kw[c][1][0], kw[c][2][0], kw[c][3][0]});
+      const half8 k1 = __builtin_bit_cast(half8, u32x4{kw[c][0][1], kw[c][1][1], kw[c][2][1], kw[c][3][1]});
 #pragma unroll
-    for (int t = 0; t < QT; t++)
-#pragma unroll
-      for (int c = 0; c < C; c++)
+      for (int t = 0; t < QT; t++)
 #pragma unroll
         for (int part = 0; part < QP; part++) {
           const half8 q = qs[qat + ((t * C + c) * QP + part) * 64];
-#pragma unroll
-          for (int u = 0; u < KP; u++) st[t][u] = mfma(kf[c][u], q, st[t][u]);
+          st[t][0] = mfma(k0, q, st[t][0]), st[t][1] = mfma(k1, q, st[t][1]);
         }
+    }
+    if constexpr (KIND == 0) load_k(blk + a.kw);
 
-    // The softmax: element KP r + u of the lane's NP positions is st[u][r].
-    half8 ph[QT][KK], pl[QT][KK];
+    // The softmax: element 2r + u of the lane's 8 positions is st[u][r].
+    if constexpr (!all) {
+      const uint32_t there = left >= 8 ? 0xffu : left > 0 ? (1u << left) - 1u : 0u;
+#pragma unroll
+      for (int t = 0; t < QT; t++) {
+        uint32_t vis = there;
+        if constexpr (KIND == 2) vis &= node_mask(a, b, min(r0 + (qi * QT + t) * 16 + m, total - 1) / group, j0 + 8 * g);
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+          if (!(vis >> e & 1)) st[t][e & 1][e >> 1] = -INFINITY;
+      }
+    }
+    half8 ph[QT], pl[QT];
 #pragma unroll
     for (int t = 0; t < QT; t++) {
-      if (!all)
-#pragma unroll
-        for (int e = 0; e < NP; e++)
-          if (!(vis[t] >> e & 1)) st[t][e % KP][e / KP] = -INFINITY;
       float top = st[t][0][0];
 #pragma unroll
-      for (int e = 1; e < NP; e++) top = fmaxf(top, st[t][e % KP][e / KP]);
+      for (int e = 1; e < 8; e++) top = fmaxf(top, st[t][e & 1][e >> 1]);
       top = xlane::bit4(top, xlane::Max{});
       top = xlane::bit5(top, xlane::Max{});
       top = fmaxf(top, mx[t]);
@@ -288,53 +322,57 @@ __global__ __launch_bounds__(512) void attend_kernel(AttendArgs a) {
         mx[t] = top;
       }
 #pragma unroll
-      for (int e = 0; e < NP; e++) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(st[t][e % KP][e / KP] - base, cf[t], 10.0f));
+      for (int e = 0; e < 8; e++) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(st[t][e & 1][e >> 1] - base, cf[t], 10.0f));
         sum[t] += p;
         const _Float16 h = (_Float16)p;
-        ph[t][e >> 3][e & 7] = h;
-        if constexpr (!P16) pl[t][e >> 3][e & 7] = (_Float16)(p - (float)h);
+        ph[t][e] = h;
+        if constexpr (!P16) pl[t][e] = (_Float16)(p - (float)h);
       }
     }
 
-    if (!all) {
+    if constexpr (!all) {
       // Values of positions that are not there are zeroed; one that is no finite number (bad: its rows' outputs) must
       // not meet the zero weights of the rows that do not see it.
       u16x2 big{};
 #pragma unroll
-      for (int e = 0; e < NP; e++)
+      for (int e = 0; e < 8; e++)
 #pragma unroll
         for (int z = 0; z < Z; z++) {
           if (e >= left) vw[e][z] = u32x2{};
+          if constexpr (KIND != 2) continue;
           big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2, vw[e][z][0] & 0x7fff7fffu));
           big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2, vw[e][z][1] & 0x7fff7fffu));
         }
-      if (!cache && __any(big[0] >= 0x7c00 || big[1] >= 0x7c00)) {
+      if (KIND == 2 && __any(big[0] >= 0x7c00 || big[1] >= 0x7c00)) {
         // Which rows see a NaN, an infinity or a negative one, value by value, and the rest as if it were zero.
+        half8 see[QT];
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+          const uint32_t vis = node_mask(a, b, min(r0 + (qi * QT + t) * 16 + m, total - 1) / group, j0 + 8 * g);
+#pragma unroll
+          for (int e = 0; e < 8; e++) see[t][e] = (_Float16)(e < left && (vis >> e & 1));
+        }
+#pragma unroll 1
         for (int kind = 0; kind < 3; kind++)
 #pragma unroll
-          for (int x = 0; x < 4 * Z; x++)
+          for (int x = 0; x < 4 * Z; x++) {
+            half8 is;
 #pragma unroll
-            for (int kk = 0; kk < KK; kk++) {
-              half8 is;
-#pragma unroll
-              for (int e = 0; e < 8; e++) {
-                const uint32_t h = vw[8 * kk + e][x / 4][x % 4 / 2] >> (16 * (x & 1)) & 0xffffu;
-                is[e] = (_Float16)(kind == 0 ? (h & 0x7fffu) > 0x7c00u : kind == 1 ? h == 0x7c00u : h == 0xfc00u);
-              }
-#pragma unroll
-              for (int t = 0; t < QT; t++) {
-                half8 see;
-#pragma unroll
-                for (int e = 0; e < 8; e++) see[e] = (_Float16)(vis[t] >> (8 * kk + e) & 1);
-                const floatx4 seen = mfma(is, see, floatx4{});
-#pragma unroll
-                for (int r = 0; r < 4; r++)
-                  if (seen[r] > 0.0f) acc[t][x][r] += kind == 0 ? NAN : kind == 1 ? INFINITY : -INFINITY;
-              }
+            for (int e = 0; e < 8; e++) {
+              const uint32_t h = vw[e][x / 4][x % 4 / 2] >> (16 * (x & 1)) & 0xffffu;
+              is[e] = (_Float16)(kind == 0 ? (h & 0x7fffu) > 0x7c00u : kind == 1 ? h == 0x7c00u : h == 0xfc00u);
             }
 #pragma unroll
-        for (int e = 0; e < NP; e++)
+            for (int t = 0; t < QT; t++) {
+              const floatx4 seen = mfma(is, see[t], floatx4{});
+#pragma unroll
+              for (int r = 0; r < 4; r++)
+                if (seen[r] > 0.0f) acc[t][x][r] += kind == 0 ? NAN : kind == 1 ? INFINITY : -INFINITY;
+            }
+          }
+#pragma unroll
+        for (int e = 0; e < 8; e++)
 #pragma unroll
           for (int z = 0; z < Z; z++)
 #pragma unroll
@@ -345,111 +383,94 @@ __global__ __launch_bounds__(512) void attend_kernel(AttendArgs a) {
       }
     }
 #pragma unroll
-    for (int x = 0; x < 4 * Z; x++)
+    for (int x = 0; x < 4 * Z; x++) {
+      u32x4 w;
 #pragma unroll
-      for (int kk = 0; kk < KK; kk++) {
-        u32x4 w;
+      for (int y = 0; y < 4; y++)
+        w[y] = __builtin_amdgcn_perm(vw[2 * y + 1][x / 4][x % 4 / 2], vw[2 * y][x / 4][x % 4 / 2], x & 1 ? 0x07060302u : 0x05040100u);
+      const half8 vf = __builtin_bit_cast(half8, w);
 #pragma unroll
-        for (int y = 0; y < 4; y++)
-          w[y] = __builtin_amdgcn_perm(vw[8 * kk + 2 * y + 1][x / 4][x % 4 / 2], vw[8 * kk + 2 * y][x / 4][x % 4 / 2],
-                                       x & 1 ? 0x07060302u : 0x05040100u);
-        const half8 vf = __builtin_bit_cast(half8, w);
-#pragma unroll
-        for (int t = 0; t < QT; t++) {
-          acc[t][x] = mfma(vf, ph[t][kk], acc[t][x]);
-          if constexpr (!P16) acc[t][x] = mfma(vf, pl[t][kk], acc[t][x]);
-        }
+      for (int t = 0; t < QT; t++) {
+        acc[t][x] = mfma(vf, ph[t], acc[t][x]);
+        if constexpr (!P16) acc[t][x] = mfma(vf, pl[t], acc[t][x]);
       }
-  }
-#pragma unroll
-  for (int t = 0; t < QT; t++) {
-    sum[t] = xlane::bit4(sum[t], xlane::Add{});
-    sum[t] = xlane::bit5(sum[t], xlane::Add{});
+    }
+    if constexpr (KIND == 0) load_v(blk + a.kw);
+  };
+  if (busy) {
+    bool loaded = true;
+    if (blk < cached) {
+      for (; blk + a.kw < cached; blk += a.kw) step(std::integral_constant<int, 0>{});
+      step(std::integral_constant<int, 1>{});
+      blk += a.kw, loaded = false;
+    }
+    for (; blk < end; blk += a.kw, loaded = false) {
+      if (!loaded) load_nodes(blk);
+      step(std::integral_constant<int, 2>{});
+    }
   }
 
-  // The key groups' results joined through LDS, half of them at a time into the other half.
-  floatx4 *merge = (floatx4 *)smem;
-  constexpr int SLOT = QT * (4 * Z * 64 + 32);  // 16-byte units of one wavefront's accumulators, then maxima and sums
-  for (int step = a.kw / 2; step; step /= 2) {
-    __syncthreads();
-    floatx4 *slot = merge + (size_t)((ki % step) * a.qw + qi) * SLOT;
-    float *ml = (float *)(slot + QT * 4 * Z * 64);
-    if (ki >= step && ki < 2 * step) {
-#pragma unroll
-      for (int t = 0; t < QT; t++) {
-#pragma unroll
-        for (int x = 0; x < 4 * Z; x++) slot[(t * 4 * Z + x) * 64 + lane] = acc[t][x];
-        ml[t * 128 + lane] = mx[t], ml[t * 128 + 64 + lane] = sum[t];
-      }
-    }
-    __syncthreads();
-    if (ki < step) {
-#pragma unroll
-      for (int t = 0; t < QT; t++) {
-        const float om = ml[t * 128 + lane], os = ml[t * 128 + 64 + lane], top = fmaxf(mx[t], om);
-        const float f = mx[t] == top ? 1.0f : __builtin_amdgcn_exp2f((mx[t] - top) * cf[t]);
-        const float of = om == top ? 1.0f : __builtin_amdgcn_exp2f((om - top) * cf[t]);
-        sum[t] = sum[t] * f + os * of, mx[t] = top;
-#pragma unroll
-        for (int x = 0; x < 4 * Z; x++) acc[t][x] = acc[t][x] * f + slot[(t * 4 * Z + x) * 64 + lane] * of;
-      }
-    }
-  }
-  if (ki || !busy) return;
-  // Lane 16g + i holds row i's values 16g + 4r + (x % 4) of the chunk of 64 x / 4.
+  // The key groups' results joined through LDS: every wavefront writes its own, then every thread adds up four values
+  // of a row.  Lane 16g + i holds row i's values 16g + 4r + (x % 4) of the chunk of 64 x / 4.
+  floatx4 *merge = (floatx4 *)(smem + 64 * tiles);               // [ki][tile][z][r][lane]
+  float *ml = (float *)(merge + (size_t)a.kw * tiles * Z * 256);  // [ki][tile][maxima, sums][row]
+  __syncthreads();
 #pragma unroll
   for (int t = 0; t < QT; t++) {
-    const int r = r0 + (qi * QT + t) * 16 + m;
-    if (r >= total) continue;
-    const int i = r / group, head = kh * group + r % group;
-    const size_t out = ((row0 + i) * a.heads + head) * a.hd;
-    if (s.used > 1) {
-      const size_t part = (size_t)split * a.batch * a.rows * a.heads;
-      if (g == 0) {
-        float *ml = a.pml + 2 * (part + (row0 + i) * a.heads + head);
-        ml[0] = mx[t] * cf[t], ml[1] = sum[t];
-      }
-#pragma unroll
-      for (int z = 0; z < Z; z++)
-#pragma unroll
-        for (int y = 0; y < 4; y++) {
-          const int d = 64 * z + 16 * g + 4 * y;
-          if (d < a.hd)
-            *(floatx4 *)(a.po + part * a.hd + out + d) =
-                floatx4{acc[t][4 * z][y], acc[t][4 * z + 1][y], acc[t][4 * z + 2][y], acc[t][4 * z + 3][y]};
-        }
-      continue;
-    }
-    const float inv = sum[t] == 0.0f && !sees_any(a, s, b, i) ? 0.0f : 1.0f / sum[t];
+    const int tile = ki * tiles + qi * QT + t;
+    sum[t] = xlane::bit4(sum[t], xlane::Add{});
+    sum[t] = xlane::bit5(sum[t], xlane::Add{});
+    if (g == 0) ml[32 * tile + m] = mx[t], ml[32 * tile + 16 + m] = sum[t];
 #pragma unroll
     for (int z = 0; z < Z; z++)
 #pragma unroll
-      for (int y = 0; y < 4; y++) {
-        const int d = 64 * z + 16 * g + 4 * y;
-        if (d >= a.hd) continue;
-        const floatx4 f = floatx4{acc[t][4 * z][y], acc[t][4 * z + 1][y], acc[t][4 * z + 2][y], acc[t][4 * z + 3][y]} * inv;
-        if constexpr (P16) *(u32x2_a4 *)((_Float16 *)a.o + out + d) = u32x2{pack2(f[0], f[1]), pack2(f[2], f[3])};
-        else *(floatx4_a4 *)((float *)a.o + out + d) = f;
-      }
+      for (int r = 0; r < 4; r++)
+        merge[((tile * Z + z) * 4 + r) * 64 + lane] = floatx4{acc[t][4 * z][r], acc[t][4 * z + 1][r], acc[t][4 * z + 2][r], acc[t][4 * z + 3][r]};
+  }
+  __syncthreads();
+  for (int x = wave; x < tiles * Z * 4; x += a.qw * a.kw) {
+    const int tile = x / (4 * Z), z = x / 4 % Z, d = 64 * z + 16 * g + 4 * (x % 4), r = r0 + 16 * tile + m;
+    if (r >= total || d >= a.hd) continue;
+    float top = -INFINITY, l = 0.0f;
+    for (int k = 0; k < a.kw; k++) top = fmaxf(top, ml[32 * (k * tiles + tile) + m]);
+    const float c = coef[16 * tile + m];
+    floatx4 f{};
+    for (int k = 0; k < a.kw; k++) {
+      const float km = ml[32 * (k * tiles + tile) + m], w = km == top ? 1.0f : __builtin_amdgcn_exp2f((km - top) * c);
+      l += w * ml[32 * (k * tiles + tile) + 16 + m];
+      f += w * merge[((k * tiles * Z * 4) + x) * 64 + lane];
+    }
+    const int i = r / group, head = kh * group + r % group;
+    const size_t out = ((row0 + i) * a.heads + head) * a.hd + d;
+    if (s.used > 1) {
+      const size_t part = (size_t)split * a.batch * a.rows * a.heads;
+      if (d == 0) *(floatx4 *)(a.pml + 4 * (part + (row0 + i) * a.heads + head)) = floatx4{top, l, c, 0.0f};
+      *(floatx4 *)(a.po + part * a.hd + out) = f;
+      continue;
+    }
+    f *= l == 0.0f && !sees_any(a, s, b, i) ? 0.0f : 1.0f / l;
+    if constexpr (P16) *(u32x2_a4 *)((_Float16 *)a.o + out) = u32x2{pack2(f[0], f[1]), pack2(f[2], f[3])};
+    else *(floatx4_a4 *)((float *)a.o + out) = f;
   }
 }
 
 // The splits' outputs of one head of a node rescaled to their common maximum, summed and divided; one wavefront
 // each, two values a lane.
-template <int KB, bool P16>
+template <bool P16>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
   const int lane = threadIdx.x & 63, at = blockIdx.x * 4 + (threadIdx.x >> 6), heads = a.batch * a.rows * a.heads;
   if (at >= heads) return;
   const int row = at / a.heads, b = row / a.rows, i = row % a.rows;
-  const Share s = share_of<KB>(a, b);
+  const Share s = share_of(a, b);
   if (s.used == 1 || i >= s.count) return;
   float top = -INFINITY;
-  for (int x = 0; x < s.used; x++) top = fmaxf(top, a.pml[2 * ((size_t)x * heads + at)]);
+  for (int x = 0; x < s.used; x++) top = fmaxf(top, a.pml[4 * ((size_t)x * heads + at)]);
   const int d = 2 * lane;
+  const float c = a.pml[4 * (size_t)at + 2];
   float sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
   for (int x = 0; x < s.used; x++) {
-    const float mx = a.pml[2 * ((size_t)x * heads + at)], f = mx == top ? 1.0f : __builtin_amdgcn_exp2f(mx - top);
-    sum += f * a.pml[2 * ((size_t)x * heads + at) + 1];
+    const float mx = a.pml[4 * ((size_t)x * heads + at)], f = mx == top ? 1.0f : __builtin_amdgcn_exp2f((mx - top) * c);
+    sum += f * a.pml[4 * ((size_t)x * heads + at) + 1];
     if (d < a.hd) {
       const float2 p = *(const float2 *)(a.po + ((size_t)x * heads + at) * a.hd + d);
       o0 += f * p.x, o1 += f * p.y;
@@ -535,28 +556,27 @@ __global__ __launch_bounds__(256) void keep_kernel(KeepArgs a) {
   }
 }
 
-constexpr int key_block(int hd) { return hd <= 64 ? 64 : 32; }
-
 template <typename T, int HD, int QT, bool P16>
 int attend_launch(wh_ctx *ctx, const AttendArgs &a) {
-  const size_t tiles = QT * a.qw, queries = tiles * (HD / 32 * (sizeof(T) == 4 ? 2 : 1) * 1024 + 64);
-  const size_t merge = (size_t)(a.kw / 2) * a.qw * QT * (4 * HD / 64 * 64 + 32) * 16;
+  const size_t tiles = QT * a.qw, queries = tiles * HD / 32 * (sizeof(T) == 4 ? 2 : 1) * 1024;
+  const size_t merge = a.kw * tiles * (HD / 64 * 4096 + 128);
   {
     ProfScope prof(ctx, "tree_attend", 4.0 * a.batch * a.rows * a.heads * a.cols * a.hd, 4.0 * a.batch * a.cols * a.kv_heads * a.hd);
     wh_launch(ctx, (attend_kernel<T, HD, QT, P16>), a.batch * a.row_blocks * a.kv_heads * a.splits, 64 * a.qw * a.kw,
-              std::max(queries, merge), a);
+              64 * tiles + std::max(queries, merge), a);
     if (int rc = wh_launched(ctx, "tree attention")) return rc;
   }
   if (a.splits == 1) return WH_OK;
   const double heads = (double)a.batch * a.rows * a.heads;
-  ProfScope prof(ctx, "tree_attend_join", 0.0, 4.0 * heads * a.splits * (a.hd + 2));
-  wh_launch(ctx, (attend_join_kernel<key_block(HD), P16>), (a.batch * a.rows * a.heads + 3) / 4, 256, 0, a);
+  ProfScope prof(ctx, "tree_attend_join", 0.0, 4.0 * heads * a.splits * (a.hd + 4));
+  wh_launch(ctx, attend_join_kernel<P16>, (a.batch * a.rows * a.heads + 3) / 4, 256, 0, a);
   return wh_launched(ctx, "tree attention's join");
 }
 
 template <typename T, bool P16>
 int attend_t(wh_ctx *ctx, const AttendArgs &a, int qt) {
-  if (a.hd <= 64) return qt == 1 ? attend_launch<T, 64, 1, P16>(ctx, a) : attend_launch<T, 64, 2, P16>(ctx, a);
+  if (a.hd <= 64)
+    return qt == 1 ? attend_launch<T, 64, 1, P16>(ctx, a) : qt == 2 ? attend_launch<T, 64, 2, P16>(ctx, a) : attend_launch<T, 64, 4, P16>(ctx, a);
   return qt == 1 ? attend_launch<T, 128, 1, P16>(ctx, a) : attend_launch<T, 128, 2, P16>(ctx, a);
 }
 
@@ -590,22 +610,20 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
   AttendArgs a{q, k, v, stride, kv, kv_stride, o, t->n, t->count, t->mask, t->mask_stride, t->batch, t->rows, (t->rows + 31) / 32,
                cols, heads, kv_heads, hd, 1.0f / sqrtf((float)hd), 1, 1, 1, 1, nullptr, nullptr};
   const int rows = t->rows * (heads / kv_heads), tiles = (rows + 15) / 16;
-  const int qt = tiles > 1 ? 2 : 1;
-  const int qwaves = (tiles + qt - 1) / qt;
-  constexpr int WAVES = 8;
-  while (a.qw < std::min(qwaves, WAVES)) a.qw *= 2;
-  a.kw = WAVES / a.qw;
+  const int hdp = hd <= 64 ? 64 : 128, qt = tiles == 1 ? 1 : tiles == 2 || hdp == 128 ? 2 : 4, waves = most_waves(hdp, qt);
+  const int qwaves = (tiles + qt - 1) / qt, blocks = (cols + KB - 1) / KB + (t->mask && k ? (t->rows + KB - 1) / KB : 0);
+  a.qw = std::min(qwaves, waves);
   a.row_blocks = (qwaves + a.qw - 1) / a.qw;
+  a.kw = std::max(1, std::min(waves / a.qw, blocks));
   const size_t units = (size_t)t->batch * kv_heads * a.row_blocks;
-  const int kb = key_block(hd), blocks = (cols + kb - 1) / kb + (t->mask && k ? (t->rows + kb - 1) / kb : 0);
   const size_t cus = ctx->cus > 0 ? ctx->cus : 256;
-  a.splits = (int)std::max<size_t>(1, std::min<size_t>((2 * cus + units - 1) / units, (blocks + a.kw - 1) / a.kw));
+  a.splits = (int)std::max<size_t>(1, std::min<size_t>((cus + units - 1) / units, (blocks + 2 * a.kw - 1) / (2 * a.kw)));
   const size_t nodes = (size_t)t->batch * t->rows;
   if (units * a.splits >= (size_t)1 << 22 || nodes * heads >= (size_t)1 << 25)  // (a launch's threads fit 32 bits)
     return wh_fail(ctx, WH_EARG, "tree attention: %d heads of %zu nodes in one call", heads, nodes);
   if (a.splits > 1) {
     const size_t part = (size_t)a.splits * nodes * heads;
-    if (!(a.po = (float *)wh_scratch(ctx, part * (hd + 2) * sizeof(float)))) return WH_EOOM;
+    if (!(a.po = (float *)wh_scratch(ctx, part * (hd + 4) * sizeof(float)))) return WH_EOOM;
     a.pml = a.po + part * hd;
   }
   return in16 ? out16 ? attend_t<_Float16, true>(ctx, a, qt) : attend_t<_Float16, false>(ctx, a, qt)
