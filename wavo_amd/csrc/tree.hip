@@ -33,16 +33,19 @@ struct AttendArgs {
   size_t mask_stride;
   int batch, rows, words, cols, heads, kv_heads, hd;
   float scale;
-  int qw, kw, splits, row_blocks;
+  int qw, kw, splits, row_blocks, block;  // (block: keys per block)
   // splits > 1: unnormalized outputs [split][batch * rows][heads][hd] and (maximum, sum, factor of the maximum's
   // exponent, -) [split][batch * rows][heads] of the splits that are used.
   float *po, *pml;
 };
 
-constexpr int KB = 32;  // keys per block
+constexpr int KB = 32;  // keys per block of attend_kernel
 
 // Wavefronts of a workgroup, at most: 16 where one needs no more than 128 registers.
 constexpr int most_waves(int hd, int qt) { return hd == 64 && qt == 1 ? 16 : 8; }
+
+// Positions of a block of attend_rows_kernel.
+constexpr int rows_block(int hd) { return hd <= 64 ? 64 : 32; }
 
 // The blocks of keys of a sequence (the cache's, then the nodes'), and how its `splits` workgroups share them:
 // runs of `per` blocks, at least one for each wavefront, so that a short sequence uses fewer of them.
@@ -53,8 +56,8 @@ __device__ __forceinline__ Share share_of(const AttendArgs &a, int b) {
   Share s;
   s.n = min(max(a.n[b], 0), a.cols);
   s.count = a.count ? min(max(a.count[b], 0), a.rows) : a.rows;
-  s.cached = (s.n + KB - 1) / KB;
-  s.blocks = s.cached + (a.mask && a.k ? (s.count + KB - 1) / KB : 0);
+  s.cached = (s.n + a.block - 1) / a.block;
+  s.blocks = s.cached + (a.mask && a.k ? (s.count + a.block - 1) / a.block : 0);
   s.per = max((s.blocks + a.splits - 1) / a.splits, a.kw);
   s.used = max((s.blocks + s.per - 1) / s.per, 1);
   return s;
@@ -83,6 +86,31 @@ __device__ __forceinline__ u32x2 four(const _Float16 *p) { return *(const u32x2_
 // The 8 mask bits of node i from node j on.
 __device__ __forceinline__ uint32_t node_mask(const AttendArgs &a, int b, int i, int j) {
   return j < a.rows ? a.mask[(size_t)b * a.mask_stride + (size_t)i * a.words + j / 32] >> (j % 32) : 0u;
+}
+
+// A pair of f16 values with zeros for those that are no finite numbers.
+__device__ __forceinline__ uint32_t finite2(uint32_t w) {
+  return ((w & 0x7c00u) == 0x7c00u ? 0u : w & 0xffffu) | ((w & 0x7c000000u) == 0x7c000000u ? 0u : w & 0xffff0000u);
+}
+// Value d of a row as f16 if it is no finite number, or zero.
+template <typename T>
+__device__ __forceinline__ float not_finite(const T *p, int d, int hd) {
+  const float x = d < hd ? (float)(_Float16)p[d] : 0.0f;
+  return isfinite(x) ? 0.0f : x;
+}
+
+// 4 f16 values of column m of the 16 lanes' 4 x 16 matrix, 4 values of a row at each of the lanes' addresses.
+__device__ __forceinline__ u32x2 read_tr(const uint32_t *p) {
+  typedef short s16x4 __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) s16x4 *)(__attribute__((address_space(3))) void *)p));
+}
+
+// A barrier for what is in LDS: loads from memory stay under way.
+__device__ __forceinline__ void meet() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
 __device__ __forceinline__ floatx4 mfma(half8 a, half8 b, floatx4 c) {
@@ -332,8 +360,8 @@ __global__ __launch_bounds__(64 * most_waves(HD, QT)) void attend_kernel(AttendA
     }
 
     if constexpr (!all) {
-      // Values of positions that are not there are zeroed; one that is no finite number (bad: its rows' outputs) must
-      // not meet the zero weights of the rows that do not see it.
+      // Values of positions that are not there are zeroed, and so are a node's that are no finite numbers: those must not
+      // meet the zero weights of the rows that do not see them, and are added to the others' outputs one by one.
       u16x2 big{};
 #pragma unroll
       for (int e = 0; e < 8; e++)
@@ -345,41 +373,25 @@ __global__ __launch_bounds__(64 * most_waves(HD, QT)) void attend_kernel(AttendA
           big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2, vw[e][z][1] & 0x7fff7fffu));
         }
       if (KIND == 2 && __any(big[0] >= 0x7c00 || big[1] >= 0x7c00)) {
-        // Which rows see a NaN, an infinity or a negative one, value by value, and the rest as if it were zero.
-        half8 see[QT];
-#pragma unroll
-        for (int t = 0; t < QT; t++) {
-          const uint32_t vis = node_mask(a, b, min(r0 + (qi * QT + t) * 16 + m, total - 1) / group, j0 + 8 * g);
-#pragma unroll
-          for (int e = 0; e < 8; e++) see[t][e] = (_Float16)(e < left && (vis >> e & 1));
-        }
-#pragma unroll 1
-        for (int kind = 0; kind < 3; kind++)
-#pragma unroll
-          for (int x = 0; x < 4 * Z; x++) {
-            half8 is;
-#pragma unroll
-            for (int e = 0; e < 8; e++) {
-              const uint32_t h = vw[e][x / 4][x % 4 / 2] >> (16 * (x & 1)) & 0xffffu;
-              is[e] = (_Float16)(kind == 0 ? (h & 0x7fffu) > 0x7c00u : kind == 1 ? h == 0x7c00u : h == 0xfc00u);
-            }
-#pragma unroll
-            for (int t = 0; t < QT; t++) {
-              const floatx4 seen = mfma(is, see[t], floatx4{});
-#pragma unroll
-              for (int r = 0; r < 4; r++)
-                if (seen[r] > 0.0f) acc[t][x][r] += kind == 0 ? NAN : kind == 1 ? INFINITY : -INFINITY;
-            }
-          }
 #pragma unroll
         for (int e = 0; e < 8; e++)
 #pragma unroll
-          for (int z = 0; z < Z; z++)
+          for (int z = 0; z < Z; z++) vw[e][z] = u32x2{finite2(vw[e][z][0]), finite2(vw[e][z][1])};
+#pragma unroll 1
+        for (int j = 0; j < min(KB, last + 1); j++) {
+          int hd = a.hd;
+          asm volatile("" : "+s"(hd));  // (nothing of this loop is worth a register outside)
+          const T *v = (const T *)a.v + (row0 + j0 + j) * a.stride + (size_t)kh * a.hd;
 #pragma unroll
-            for (int w = 0; w < 2; w++) {
-              if ((vw[e][z][w] & 0x7c00u) == 0x7c00u) vw[e][z][w] &= 0xffff0000u;
-              if ((vw[e][z][w] & 0x7c000000u) == 0x7c000000u) vw[e][z][w] &= 0xffffu;
-            }
+          for (int t = 0; t < QT; t++) {
+            const int i = min(r0 + (qi * QT + t) * 16 + m, total - 1) / group;
+            if (!(node_mask(a, b, i, j0 + j) & 1)) continue;
+#pragma unroll
+            for (int x = 0; x < 4 * Z; x++)
+#pragma unroll
+              for (int r = 0; r < 4; r++) acc[t][x][r] += not_finite(v, 64 * (x / 4) + 16 * g + 4 * r + x % 4, hd);
+          }
+        }
       }
     }
 #pragma unroll
@@ -451,6 +463,272 @@ __global__ __launch_bounds__(64 * most_waves(HD, QT)) void attend_kernel(AttendA
     f *= l == 0.0f && !sees_any(a, s, b, i) ? 0.0f : 1.0f / l;
     if constexpr (P16) *(u32x2_a4 *)((_Float16 *)a.o + out) = u32x2{pack2(f[0], f[1]), pack2(f[2], f[3])};
     else *(floatx4_a4 *)((float *)a.o + out) = f;
+  }
+}
+
+// The same for more rows than two tiles of one key head: every wavefront takes 16 * QT rows, and all of them go
+// through the same key blocks (64 positions for heads of up to 64 values, 32 for larger ones: 16 KiB) one after
+// the other.  The workgroup's threads load a block two blocks ahead, each its share of 16-byte pieces, and write
+// it to one of two LDS buffers, from which the wavefronts read operands as they stand: a pair's position from
+// each of 4 rows of K (rows 4 words longer than a block, so that the 4 lane groups hit distinct banks), and V
+// transposed by ds_read_b64_tr_b16 (rows 32 bytes longer, for the same reason).  Tile u's row r is position
+// 16u + r, so lane 16g + i's scores are those of positions 16u + 4g + 0 .. 3 of every u.
+template <typename T, int HD, int QT, int W, bool P16>
+__global__ __launch_bounds__(64 * W, W == 8 ? 4 : 3) void attend_rows_kernel(AttendArgs a) {
+  constexpr int C = HD / 32, X = HD / 16, QP = sizeof(T) == 4 ? 2 : 1, B = rows_block(HD), NT = B / 16, KK = B / 32;
+  constexpr int KS = B + 4, VS = HD / 2 + 8;  // words per row of K and of V in LDS
+  constexpr int KW = KS * HD / 2, BUF = KW + VS * B, U = 512;  // words of K and of a buffer; 16-byte pieces of K or V
+  extern __shared__ __attribute__((aligned(16))) uint32_t words[];
+  __shared__ int odd;  // set where a node's value is no finite number
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, m = lane & 15;
+  constexpr int threads = 64 * W, MOST = U / threads;  // MOST: pieces per thread
+  int at = blockIdx.x;
+  const int split = at % a.splits;
+  at /= a.splits;
+  const int kh = at % a.kv_heads;
+  at /= a.kv_heads;
+  const int rb = at % a.row_blocks, b = at / a.row_blocks;
+  const int group = a.heads / a.kv_heads, r0 = 16 * QT * (rb * W + wave);
+  const size_t row0 = (size_t)b * a.rows;
+  const Share s = share_of(a, b);
+  const int total = s.count * group;
+  if (split >= s.used || 16 * QT * W * rb >= total) return;
+  const int half = a.kv_heads * a.hd / 2, pairs = a.hd / 2;
+  const uint32_t *kc = a.kv + (size_t)b * a.kv_stride + (size_t)kh * pairs * a.cols;
+  const uint32_t *vc = a.kv + (size_t)b * a.kv_stride + (size_t)half * a.cols + kh * pairs;
+  const int begin = split * s.per, end = min(begin + s.per, s.blocks), cached = min(end, s.cached);
+
+  // A cached block's pieces into registers, then into LDS.
+  struct Pieces {
+    u32x4 k[MOST], v[MOST];
+  };
+  auto load = [&](Pieces &p, int blk) {
+    const int j0 = blk * B, last = s.n - 1 - j0;
+#pragma unroll
+    for (int i = 0; i < MOST; i++) {
+      const int u = tid + threads * i, pair = u / (B / 4), q = u % (B / 4), row = u / (HD / 8), d = u % (HD / 8) * 4;
+      p.k[i] = *(const u32x4_a4 *)(kc + (size_t)min(pair, pairs - 1) * a.cols + j0 + min(4 * q, last & ~3));
+      p.v[i] = *(const u32x4_a4 *)(vc + (size_t)j0 * half + (uint32_t)(min(row, last) * half + (d < pairs ? d : 0)));
+    }
+  };
+  auto store = [&](const Pieces &p, int blk, uint32_t *buf) {
+    const int last = s.n - 1 - blk * B;
+#pragma unroll
+    for (int i = 0; i < MOST; i++) {
+      const int u = tid + threads * i, pair = u / (B / 4), q = u % (B / 4), row = u / (HD / 8), d = u % (HD / 8) * 4;
+      *(u32x4 *)(buf + pair * KS + 4 * q) = pair < pairs ? p.k[i] : u32x4{};
+      *(u32x4 *)(buf + KW + row * VS + d) = row <= last ? p.v[i] : u32x4{};
+    }
+  };
+  Pieces p0, p1;
+  if (begin < cached) load(p0, begin);
+  if (begin + 1 < cached) load(p1, begin + 1);
+
+  // The queries, scaled as above, in registers.
+  half8 q[QT][C][QP];
+  float cf[QT];
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    const int row = min(r0 + 16 * t + m, total - 1);
+    const T *src = (const T *)a.q + (row0 + row / group) * a.stride + (size_t)(kh * group + row % group) * a.hd;
+    float f[C][8], top = 0.0f;
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const int d = 32 * c + 8 * g;
+        f[c][e] = d < a.hd ? number(src + d, e) : 0.0f;
+        top = fmaxf(top, fabsf(f[c][e]));
+      }
+    int k = 0;
+    if constexpr (QP == 2) {
+      top = xlane::bit4(top, xlane::Max{});
+      top = xlane::bit5(top, xlane::Max{});
+      if (top > 0.0f && top < INFINITY) k = min(7 - ilogbf(top), 100);
+    }
+    cf[t] = ldexpf(a.scale * 1.44269504088896341f, -k);
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const float y = QP == 2 ? ldexpf(f[c][e], k) : f[c][e];
+        q[t][c][0][e] = (_Float16)y;
+        if constexpr (QP == 2) q[t][c][1][e] = (_Float16)(y - (float)q[t][c][0][e]);
+      }
+  }
+  floatx4 acc[QT][X];
+  float mx[QT], sum[QT];
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    mx[t] = -INFINITY, sum[t] = 0.0f;
+#pragma unroll
+    for (int x = 0; x < X; x++) acc[t][x] = floatx4{};
+  }
+
+  // One block from LDS; nodes: a block of nodes, otherwise the cache's.
+  auto step = [&](auto nodes, int blk, const uint32_t *buf) {
+    constexpr bool NODES = nodes;
+    const int j0 = (NODES ? blk - s.cached : blk) * B, last = (NODES ? s.count : s.n) - 1 - j0;
+    floatx4 st[QT][NT];
+#pragma unroll
+    for (int t = 0; t < QT; t++)
+#pragma unroll
+      for (int u = 0; u < NT; u++) st[t][u] = floatx4{};
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+      for (int u = 0; u < NT; u++) {
+        const uint32_t *k = buf + (16 * c + 4 * g) * KS + 16 * u + m;
+        const half8 kf = __builtin_bit_cast(half8, u32x4{k[0], k[KS], k[2 * KS], k[3 * KS]});
+#pragma unroll
+        for (int t = 0; t < QT; t++)
+#pragma unroll
+          for (int part = 0; part < QP; part++) st[t][u] = mfma(kf, q[t][c][part], st[t][u]);
+      }
+    if (NODES || last < B - 1) {
+#pragma unroll
+      for (int t = 0; t < QT; t++)
+#pragma unroll
+        for (int kk = 0; kk < KK; kk++) {
+          const int left = last + 1 - 32 * kk;
+          uint32_t vis = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u;
+          if constexpr (NODES) vis &= node_mask(a, b, min(r0 + 16 * t + m, total - 1) / group, j0 + 32 * kk);
+#pragma unroll
+          for (int e = 0; e < 8; e++)
+            if (!(vis >> (16 * (e >> 2) + 4 * g + (e & 3)) & 1)) st[t][2 * kk + (e >> 2)][e & 3] = -INFINITY;
+        }
+    }
+    half8 ph[QT][KK], pl[QT][KK];
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+      float top = st[t][0][0];
+#pragma unroll
+      for (int e = 1; e < 4 * NT; e++) top = fmaxf(top, st[t][e >> 2][e & 3]);
+      top = xlane::bit4(top, xlane::Max{});
+      top = xlane::bit5(top, xlane::Max{});
+      top = fmaxf(top, mx[t]);
+      const float base = top == -INFINITY ? 0.0f : top;
+      if (__any(top != mx[t])) {
+        const float old = mx[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mx[t] - top) * cf[t]);
+        sum[t] *= old;
+#pragma unroll
+        for (int x = 0; x < X; x++) acc[t][x] *= old;
+        mx[t] = top;
+      }
+#pragma unroll
+      for (int e = 0; e < 4 * NT; e++) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(st[t][e >> 2][e & 3] - base, cf[t], 10.0f));
+        sum[t] += p;
+        const _Float16 h = (_Float16)p;
+        ph[t][e >> 3][e & 7] = h;
+        if constexpr (!P16) pl[t][e >> 3][e & 7] = (_Float16)(p - (float)h);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < X; x++)
+#pragma unroll
+      for (int kk = 0; kk < KK; kk++) {
+        const uint32_t *v = buf + KW + (32 * kk + 4 * g + (m >> 2)) * VS + 8 * x + 2 * (m & 3);
+        const u32x2 lo = read_tr(v), hi = read_tr(v + 16 * VS);
+        const half8 vf = __builtin_bit_cast(half8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+          acc[t][x] = mfma(vf, ph[t][kk], acc[t][x]);
+          if constexpr (!P16) acc[t][x] = mfma(vf, pl[t][kk], acc[t][x]);
+        }
+      }
+    if (NODES && odd)  // what the block has zeros for, to the rows that see it
+#pragma unroll 1
+      for (int j = 0; j < min(B, last + 1); j++) {
+        int hd = a.hd;
+        asm volatile("" : "+s"(hd));
+        const T *v = (const T *)a.v + (row0 + j0 + j) * a.stride + (size_t)kh * a.hd;
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+          if (!(node_mask(a, b, min(r0 + 16 * t + m, total - 1) / group, j0 + j) & 1)) continue;
+#pragma unroll
+          for (int x = 0; x < X; x++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) acc[t][x][r] += not_finite(v, 16 * x + 4 * g + r, hd);
+        }
+      }
+  };
+
+  // Blocks begin, begin + 2, .. pass through p0 and the first buffer, the others through p1 and the second.  A buffer is
+  // written again two blocks later, past the barrier that every wavefront reaches after it has read it.
+  uint32_t *const buf0 = words, *const buf1 = words + BUF;
+  int blk = begin;
+  for (; blk + 3 < cached; blk += 2) {
+    store(p0, blk, buf0);
+    load(p0, blk + 2);
+    meet();
+    step(std::false_type{}, blk, buf0);
+    store(p1, blk + 1, buf1);
+    load(p1, blk + 3);
+    meet();
+    step(std::false_type{}, blk + 1, buf1);
+  }
+  for (; blk < cached; blk++) {  // (at most three)
+    const bool even = (blk - begin) % 2 == 0;
+    if (even) store(p0, blk, buf0);
+    else store(p1, blk, buf1);
+    if (even && blk + 2 < cached) load(p0, blk + 2);
+    meet();
+    step(std::false_type{}, blk, even ? buf0 : buf1);
+  }
+  for (; blk < end; blk++) {
+    uint32_t *buf = (blk - begin) % 2 ? buf1 : buf0;
+    const int j0 = (blk - s.cached) * B, last = s.count - 1 - j0;
+    __syncthreads();
+    if (tid == 0) odd = 0;
+    __syncthreads();
+    bool found = false;
+#pragma unroll 1
+    for (int u = tid; u < U; u += threads) {
+      const int row = u % B, d = u / B * 8;
+      const size_t src = (row0 + j0 + min(row, last)) * a.stride + (size_t)kh * a.hd;
+      u32x2 k[2], v[2];
+#pragma unroll
+      for (int y = 0; y < 2; y++) {
+        k[y] = four((const T *)a.k + src + (d < a.hd ? d + 4 * y : 0)), v[y] = four((const T *)a.v + src + (d < a.hd ? d + 4 * y : 0));
+        if (d >= a.hd) k[y] = u32x2{};
+        if (d >= a.hd || row > last) v[y] = u32x2{};
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+          buf[(d / 2 + 2 * y + w) * KS + row] = k[y][w];
+          const uint32_t clean = finite2(v[y][w]);
+          found |= clean != v[y][w];
+          v[y][w] = clean;
+        }
+      }
+      *(u32x4 *)(buf + KW + row * VS + d / 2) = u32x4{v[0][0], v[0][1], v[1][0], v[1][1]};
+    }
+    if (found) odd = 1;
+    __syncthreads();
+    step(std::true_type{}, blk, buf);
+  }
+
+  // Lane 16g + i holds row i's values 16x + 4g + 0 .. 3.
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    sum[t] = xlane::bit4(sum[t], xlane::Add{});
+    sum[t] = xlane::bit5(sum[t], xlane::Add{});
+    const int r = r0 + 16 * t + m;
+    if (r >= total) continue;
+    const int i = r / group, head = kh * group + r % group;
+    const size_t out = ((row0 + i) * a.heads + head) * a.hd;
+    const size_t part = (size_t)split * a.batch * a.rows * a.heads;
+    if (s.used > 1 && g == 0) *(floatx4 *)(a.pml + 4 * (part + (row0 + i) * a.heads + head)) = floatx4{mx[t], sum[t], cf[t], 0.0f};
+    const float inv = s.used > 1 ? 1.0f : sum[t] == 0.0f && !sees_any(a, s, b, i) ? 0.0f : 1.0f / sum[t];
+#pragma unroll
+    for (int x = 0; x < X; x++) {
+      const int d = 16 * x + 4 * g;
+      if (d >= a.hd) continue;
+      const floatx4 f = acc[t][x] * inv;
+      if (s.used > 1) *(floatx4 *)(a.po + part * a.hd + out + d) = f;
+      else if constexpr (P16) *(u32x2_a4 *)((_Float16 *)a.o + out + d) = u32x2{pack2(f[0], f[1]), pack2(f[2], f[3])};
+      else *(floatx4_a4 *)((float *)a.o + out + d) = f;
+    }
   }
 }
 
@@ -564,20 +842,35 @@ int attend_launch(wh_ctx *ctx, const AttendArgs &a) {
     ProfScope prof(ctx, "tree_attend", 4.0 * a.batch * a.rows * a.heads * a.cols * a.hd, 4.0 * a.batch * a.cols * a.kv_heads * a.hd);
     wh_launch(ctx, (attend_kernel<T, HD, QT, P16>), a.batch * a.row_blocks * a.kv_heads * a.splits, 64 * a.qw * a.kw,
               64 * tiles + std::max(queries, merge), a);
-    if (int rc = wh_launched(ctx, "tree attention")) return rc;
+    return wh_launched(ctx, "tree attention");
   }
-  if (a.splits == 1) return WH_OK;
+}
+
+template <bool P16>
+int attend_join(wh_ctx *ctx, const AttendArgs &a) {
   const double heads = (double)a.batch * a.rows * a.heads;
   ProfScope prof(ctx, "tree_attend_join", 0.0, 4.0 * heads * a.splits * (a.hd + 4));
   wh_launch(ctx, attend_join_kernel<P16>, (a.batch * a.rows * a.heads + 3) / 4, 256, 0, a);
   return wh_launched(ctx, "tree attention's join");
 }
 
+template <typename T, int HD, int QT, int W, bool P16>
+int attend_rows_launch(wh_ctx *ctx, const AttendArgs &a) {
+  constexpr int B = rows_block(HD);
+  ProfScope prof(ctx, "tree_attend_rows", 4.0 * a.batch * a.rows * a.heads * a.cols * a.hd, 4.0 * a.batch * a.cols * a.kv_heads * a.hd);
+  wh_launch(ctx, (attend_rows_kernel<T, HD, QT, W, P16>), a.batch * a.row_blocks * a.kv_heads * a.splits, 64 * W,
+            2 * 4 * ((B + 4) * HD / 2 + (HD / 2 + 8) * B), a);
+  return wh_launched(ctx, "tree attention");
+}
+
 template <typename T, bool P16>
-int attend_t(wh_ctx *ctx, const AttendArgs &a, int qt) {
-  if (a.hd <= 64)
-    return qt == 1 ? attend_launch<T, 64, 1, P16>(ctx, a) : qt == 2 ? attend_launch<T, 64, 2, P16>(ctx, a) : attend_launch<T, 64, 4, P16>(ctx, a);
-  return qt == 1 ? attend_launch<T, 128, 1, P16>(ctx, a) : attend_launch<T, 128, 2, P16>(ctx, a);
+int attend_t(wh_ctx *ctx, const AttendArgs &a, int qt, bool rows) {
+  int rc;
+  if (rows && a.hd <= 64) rc = a.qw == 4 ? attend_rows_launch<T, 64, 1, 4, P16>(ctx, a) : attend_rows_launch<T, 64, 1, 8, P16>(ctx, a);
+  else if (rows) rc = a.qw == 4 ? attend_rows_launch<T, 128, 1, 4, P16>(ctx, a) : attend_rows_launch<T, 128, 1, 8, P16>(ctx, a);
+  else if (a.hd <= 64) rc = qt == 1 ? attend_launch<T, 64, 1, P16>(ctx, a) : attend_launch<T, 64, 2, P16>(ctx, a);
+  else rc = qt == 1 ? attend_launch<T, 128, 1, P16>(ctx, a) : attend_launch<T, 128, 2, P16>(ctx, a);
+  return rc || a.splits == 1 ? rc : attend_join<P16>(ctx, a);
 }
 
 }  // namespace
@@ -608,16 +901,20 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
     return wh_fail(ctx, WH_EARG, "tree attention: buffers and rows must be 4-byte aligned");
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "tree attention: %s", hipGetErrorString(e));
   AttendArgs a{q, k, v, stride, kv, kv_stride, o, t->n, t->count, t->mask, t->mask_stride, t->batch, t->rows, (t->rows + 31) / 32,
-               cols, heads, kv_heads, hd, 1.0f / sqrtf((float)hd), 1, 1, 1, 1, nullptr, nullptr};
+               cols, heads, kv_heads, hd, 1.0f / sqrtf((float)hd), 1, 1, 1, 1, KB, nullptr, nullptr};
   const int rows = t->rows * (heads / kv_heads), tiles = (rows + 15) / 16;
-  const int hdp = hd <= 64 ? 64 : 128, qt = tiles == 1 ? 1 : tiles == 2 || hdp == 128 ? 2 : 4, waves = most_waves(hdp, qt);
-  const int qwaves = (tiles + qt - 1) / qt, blocks = (cols + KB - 1) / KB + (t->mask && k ? (t->rows + KB - 1) / KB : 0);
-  a.qw = std::min(qwaves, waves);
+  const int hdp = hd <= 64 ? 64 : 128;
+  const bool many = tiles > 2 && hd % 8 == 0 && cols >= 4;
+  const int qt = many || tiles == 1 ? 1 : 2, waves = many ? 8 : most_waves(hdp, qt), qwaves = (tiles + qt - 1) / qt;
+  if (many) a.block = rows_block(hd);
+  const int blocks = (cols + a.block - 1) / a.block + (t->mask && k ? (t->rows + a.block - 1) / a.block : 0);
+  a.qw = many ? qwaves <= 4 ? 4 : 8 : std::min(qwaves, waves);
   a.row_blocks = (qwaves + a.qw - 1) / a.qw;
-  a.kw = std::max(1, std::min(waves / a.qw, blocks));
+  a.kw = many ? 1 : std::max(1, std::min(waves / a.qw, blocks));
   const size_t units = (size_t)t->batch * kv_heads * a.row_blocks;
   const size_t cus = ctx->cus > 0 ? ctx->cus : 256;
-  a.splits = (int)std::max<size_t>(1, std::min<size_t>((cus + units - 1) / units, (blocks + 2 * a.kw - 1) / (2 * a.kw)));
+  const int least = many ? 8 : 2 * a.kw;  // blocks of a split
+  a.splits = (int)std::max<size_t>(1, std::min<size_t>(((many ? 2 : 1) * cus + units - 1) / units, (blocks + least - 1) / least));
   const size_t nodes = (size_t)t->batch * t->rows;
   if (units * a.splits >= (size_t)1 << 22 || nodes * heads >= (size_t)1 << 25)  // (a launch's threads fit 32 bits)
     return wh_fail(ctx, WH_EARG, "tree attention: %d heads of %zu nodes in one call", heads, nodes);
@@ -626,8 +923,8 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
     if (!(a.po = (float *)wh_scratch(ctx, part * (hd + 4) * sizeof(float)))) return WH_EOOM;
     a.pml = a.po + part * hd;
   }
-  return in16 ? out16 ? attend_t<_Float16, true>(ctx, a, qt) : attend_t<_Float16, false>(ctx, a, qt)
-              : out16 ? attend_t<float, true>(ctx, a, qt) : attend_t<float, false>(ctx, a, qt);
+  return in16 ? out16 ? attend_t<_Float16, true>(ctx, a, qt, many) : attend_t<_Float16, false>(ctx, a, qt, many)
+              : out16 ? attend_t<float, true>(ctx, a, qt, many) : attend_t<float, false>(ctx, a, qt, many);
 }
 
 int launch_tree_accept(wh_ctx *ctx, const wh_tree *t, const uint32_t *picks, const wh_kept *w, int cols, int32_t *path,
