@@ -9,8 +9,6 @@
 
 namespace {
 
-__device__ __forceinline__ float number(const float *p, size_t i) { return p[i]; }
-__device__ __forceinline__ float number(const _Float16 *p, size_t i) { return (float)p[i]; }
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
@@ -33,7 +31,7 @@ struct AttendArgs {
   size_t mask_stride;
   int batch, rows, words, cols, heads, kv_heads, hd;
   float scale;
-  int qw, kw, splits, row_blocks, block;  // (block: keys per block)
+  int kw, splits, row_blocks, block;  // (block: keys per block)
   // splits > 1: unnormalized outputs [split][batch * rows][heads][hd] and (maximum, sum, factor of the maximum's
   // exponent, -) [split][batch * rows][heads] of the splits that are used.
   float *po, *pml;
@@ -41,8 +39,7 @@ struct AttendArgs {
 
 constexpr int KB = 32;  // keys per block of attend_kernel
 
-// Wavefronts of a workgroup, at most: 16 where one needs no more than 128 registers.
-constexpr int most_waves(int hd, int qt) { return hd == 64 && qt == 1 ? 16 : 8; }
+constexpr int WAVES = 8;  // wavefronts of a workgroup, at most
 
 // Positions of a block of attend_rows_kernel.
 constexpr int rows_block(int hd) { return hd <= 64 ? 64 : 32; }
@@ -82,6 +79,14 @@ __device__ __forceinline__ u32x2 four(const float *p) {
   return u32x2{pack2(x[0], x[1]), pack2(x[2], x[3])};
 }
 __device__ __forceinline__ u32x2 four(const _Float16 *p) { return *(const u32x2_a4 *)p; }
+// And in f32.
+__device__ __forceinline__ void values(const float *p, float *f) { *(floatx4 *)f = *(const floatx4_a4 *)p; }
+__device__ __forceinline__ void values(const _Float16 *p, float *f) {
+  typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+  const half4 h = __builtin_bit_cast(half4, four(p));
+#pragma unroll
+  for (int e = 0; e < 4; e++) f[e] = (float)h[e];
+}
 
 // The 8 mask bits of node i from node j on.
 __device__ __forceinline__ uint32_t node_mask(const AttendArgs &a, int b, int i, int j) {
@@ -117,10 +122,54 @@ __device__ __forceinline__ floatx4 mfma(half8 a, half8 b, floatx4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// Attention over a run of key blocks.  A workgroup takes one key head of a sequence, up to 16 * QT * qw of its
-// rows (the heads / kv_heads query heads of a node are rows next to each other) and one split of its key
-// blocks of 32; its wavefronts are qw groups of 16 * QT rows by kw, each of which takes every kw-th block.  A
-// wavefront reads a block's K and V straight into the registers that the matrix cores take:
+// Row (of a key head's: node row / group, query head row % group) and head offset without a division where the heads
+// are not shared.
+__device__ __forceinline__ int node_of(int row, int group) { return group == 1 ? row : row / group; }
+__device__ __forceinline__ int head_of(int row, int group) { return group == 1 ? 0 : row % group; }
+
+// A row's query as the matrix cores take it (lane 16g + i: row i's 8 values from 8g on of every chunk of 32), times a
+// power of two and in two parts for f32: precision is said at attend_kernel.  Gives the factor of its scores' exponents.
+template <typename T, int C>
+__device__ __forceinline__ float query(const T *src, int g, int hd, float scale, half8 (&q)[C][sizeof(T) == 4 ? 2 : 1]) {
+  float f[C][8], top = 0.0f;
+#pragma unroll
+  for (int c = 0; c < C; c++)
+#pragma unroll
+    for (int y = 0; y < 2; y++) {
+      const int d = 32 * c + 8 * g + 4 * y;
+      values(src + (d < hd ? d : 0), &f[c][4 * y]);
+#pragma unroll
+      for (int e = 0; e < 4; e++) f[c][4 * y + e] = d < hd ? f[c][4 * y + e] : 0.0f;
+    }
+  int k = 0;
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int c = 0; c < C; c++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(f[c][e]));
+    top = xlane::bit4(top, xlane::Max{});
+    top = xlane::bit5(top, xlane::Max{});
+    if (top > 0.0f && top < INFINITY) k = min(8 - __builtin_amdgcn_frexp_expf(top), 100);  // its largest value into [2^7, 2^8)
+  }
+#pragma unroll
+  for (int c = 0; c < C; c++)
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      if constexpr (sizeof(T) == 4) {
+        const float y = ldexpf(f[c][e], k);
+        q[c][0][e] = (_Float16)y;
+        q[c][1][e] = (_Float16)(y - (float)q[c][0][e]);
+      } else {
+        q[c][0][e] = (_Float16)f[c][e];
+      }
+    }
+  return ldexpf(scale * 1.44269504088896341f, -k);
+}
+
+// Attention over a run of key blocks, for few rows.  A workgroup takes one key head of a sequence, 16 * QT of its rows
+// (the heads / kv_heads query heads of a node are rows next to each other) and one split of its key blocks of
+// 32, of which each of its kw wavefronts takes every kw-th.  A wavefront reads a block's K and V straight into
+// the registers that the matrix cores take:
 //
 //   Scores transposed, S^T = K Q^T (v_mfma_f32_16x16x32_f16).  The cache holds K as pairs of values, position by
 //   position, so a lane reads two positions of a pair at once: lane 16g + m holds positions 2m and 2m + 1 of the
@@ -131,46 +180,26 @@ __device__ __forceinline__ floatx4 mfma(half8 a, half8 b, floatx4 c) {
 //   A row's softmax state is one lane column's everywhere.
 //
 // The next block's K is loaded as soon as this one's scores are done, and its V after this one's outputs, so that
-// a wavefront always has loads in flight; the first block's before the queries are staged.
+// a wavefront always has loads in flight; the first block's before the queries are looked at.
 //
 // Precision: f32 queries are scaled by a power of two per row and split into two f16 parts, as is every
 // softmax weight for f32 outputs (weights are exp2(s - max + 10), so that the second part is no subnormal):
 // two products each, with an error of 2^-22 against f32's own 2^-24 per sum.  K and V are f16 as stored.
 template <typename T, int HD, int QT, bool P16>
-__global__ __launch_bounds__(64 * most_waves(HD, QT)) void attend_kernel(AttendArgs a) {
+__global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
   constexpr int C = HD / 32, Z = HD / 64, QP = sizeof(T) == 4 ? 2 : 1;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int lane = threadIdx.x & 63, ki = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, m = lane & 15;
-  int at = blockIdx.x;
-  const int split = at % a.splits;
-  at /= a.splits;
-  const int kh = at % a.kv_heads;
-  at /= a.kv_heads;
-  const int rb = at % a.row_blocks, b = at / a.row_blocks;
-  const int group = a.heads / a.kv_heads, tiles = QT * a.qw, r0 = rb * 16 * tiles, all_rows = a.rows * group;
+  const int split = blockIdx.z, kh = blockIdx.y, b = a.row_blocks == 1 ? blockIdx.x : blockIdx.x / a.row_blocks;
+  const int group = a.heads / a.kv_heads, r0 = 16 * QT * (blockIdx.x - b * a.row_blocks);
   const size_t row0 = (size_t)b * a.rows;
-  // Four (or, z = 1 too, eight) values of a row's query: 16 threads per row.
-  auto query = [&](int x, float (&f)[Z][4]) {
-    const int row = min(r0 + (x >> 4), all_rows - 1);
-    const T *q = (const T *)a.q + (row0 + row / group) * a.stride + (size_t)(kh * group + row % group) * a.hd;
-#pragma unroll
-    for (int z = 0; z < Z; z++) {
-      const int d = 64 * z + 4 * (x & 15);
-#pragma unroll
-      for (int e = 0; e < 4; e++) f[z][e] = d < a.hd ? number(q + d, e) : 0.0f;
-    }
-  };
-  float first[Z][4];
-  query(tid, first);
   const Share s = share_of(a, b);
   const int total = s.count * group;
   if (split >= s.used || r0 >= total) return;
-  const int qi = wave % a.qw, ki = wave / a.qw;
   const int half = a.kv_heads * a.hd / 2, pairs = a.hd / 2;
   const uint32_t *kc = a.kv + (size_t)b * a.kv_stride + (size_t)kh * pairs * a.cols;
   const uint32_t *vc = a.kv + (size_t)b * a.kv_stride + (size_t)half * a.cols + kh * pairs;
-  const bool busy = r0 + qi * QT * 16 < total;  // (a wavefront past the last row only meets the others)
 
   u32x2 kw[C][4], vw[8][Z];  // a block's K, pair by pair, and V, position by position
   // The same loads on every way through, so that a wait for one block's does not have to be one for the next block's.
@@ -227,7 +256,7 @@ __global__ __launch_bounds__(64 * most_waves(HD, QT)) void attend_kernel(AttendA
   };
   int blk = split * s.per + ki;
   const int end = min((split + 1) * s.per, s.blocks), cached = min(end, s.cached);
-  if (busy && blk < cached) {
+  if (blk < cached) {
     if (a.cols > 1) {
       load_k(blk);
     } else {  // (a cache of one position: nothing behind it)
@@ -237,60 +266,20 @@ __global__ __launch_bounds__(64 * most_waves(HD, QT)) void attend_kernel(AttendA
         for (int x = 0; x < 4; x++) kw[c][x] = u32x2{16 * c + 4 * g + x < pairs ? kc[16 * c + 4 * g + x] : 0u, 0u};
     }
     load_v(blk);
-  } else if (busy && blk < end) {
+  } else if (blk < end) {
     load_nodes(blk);
   }
 
-  // The queries into LDS, in the operand's order: [tile][chunk of 32 values][part][lane].
-  float *coef = (float *)smem;  // per row: scale * log2(e) / the row's power of two
-  half8 *qs = (half8 *)(smem + 64 * tiles);
-  for (int x = tid; x < 16 * 16 * tiles; x += blockDim.x) {
-    float f[Z][4], top = 0.0f;
-    if (x == tid) {
-#pragma unroll
-      for (int z = 0; z < Z; z++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) f[z][e] = first[z][e];
-    } else {
-      query(x, f);
-    }
-    const int r = x >> 4, l = x & 15;
-    int k = 0;
-    if constexpr (QP == 2) {
-#pragma unroll
-      for (int z = 0; z < Z; z++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) top = fmaxf(top, fabsf(f[z][e]));
-      top = fmaxf(top, xlane::dpp<xlane::XOR1>(top));
-      top = fmaxf(top, xlane::dpp<xlane::XOR2>(top));
-      top = fmaxf(top, xlane::dpp<xlane::HALF_MIRROR>(top));
-      top = fmaxf(top, xlane::dpp<xlane::MIRROR>(top));
-      // The row's largest value into [2^7, 2^8).
-      if (top > 0.0f && top < INFINITY) k = min(7 - ilogbf(top), 100);
-    }
-#pragma unroll
-    for (int z = 0; z < Z; z++) {
-      const int d = 64 * z + 4 * l;
-      uint32_t *w = (uint32_t *)(qs + ((size_t)(r / 16 * C + d / 32) * QP) * 64 + (d % 32) / 8 * 16 + r % 16) + (d % 8) / 2;
-      float y[4];
-#pragma unroll
-      for (int e = 0; e < 4; e++) y[e] = QP == 2 ? ldexpf(f[z][e], k) : f[z][e];
-      w[0] = pack2(y[0], y[1]), w[1] = pack2(y[2], y[3]);
-      if constexpr (QP == 2) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) y[e] -= (float)(_Float16)y[e];
-        w[256] = pack2(y[0], y[1]), w[257] = pack2(y[2], y[3]);
-      }
-    }
-    if (l == 0) coef[r] = ldexpf(a.scale * 1.44269504088896341f, -k);
-  }
-  __syncthreads();
-
+  half8 q[QT][C][QP];
   floatx4 acc[QT][4 * Z];
   float mx[QT], sum[QT], cf[QT];
+  int node[QT];
 #pragma unroll
   for (int t = 0; t < QT; t++) {
-    mx[t] = -INFINITY, sum[t] = 0.0f, cf[t] = coef[(qi * QT + t) * 16 + m];
+    const int row = min(r0 + 16 * t + m, total - 1);
+    node[t] = node_of(row, group);
+    cf[t] = query<T, C>((const T *)a.q + (row0 + node[t]) * a.stride + (size_t)(kh * group + head_of(row, group)) * a.hd, g, a.hd, a.scale, q[t]);
+    mx[t] = -INFINITY, sum[t] = 0.0f;
 #pragma unroll
     for (int x = 0; x < 4 * Z; x++) acc[t][x] = floatx4{};
   }
@@ -300,9 +289,6 @@ __global__ __launch_bounds__(64 * most_waves(HD, QT)) void attend_kernel(AttendA
     constexpr bool all = KIND == 0;
     const int j0 = (KIND == 2 ? blk - s.cached : blk) * KB, last = (KIND == 2 ? s.count : s.n) - 1 - j0;
     const int left = last + 1 - 8 * g;  // of this lane's positions
-    // (read again for every block: with the values in registers all along, a wavefront would spill)
-    uint32_t qat = (qi * QT * C * QP) * 64 + lane;
-    asm volatile("" : "+v"(qat));
     floatx4 st[QT][2];
 #pragma unroll
     for (int t = 0; t < QT; t++) st[t][0] = st[t][1] = floatx4{};
@@ -314,8 +300,7 @@ __global__ __launch_bounds__(64 * most_waves(HD, QT)) void attend_kernel(AttendA
       for (int t = 0; t < QT; t++)
 #pragma unroll
         for (int part = 0; part < QP; part++) {
-          const half8 q = qs[qat + ((t * C + c) * QP + part) * 64];
-          st[t][0] = mfma(k0, q, st[t][0]), st[t][1] = mfma(k1, q, st[t][1]);
+          st[t][0] = mfma(k0, q[t][c][part], st[t][0]), st[t][1] = mfma(k1, q[t][c][part], st[t][1]);
         }
     }
     if constexpr (KIND == 0) load_k(blk + a.kw);
@@ -326,7 +311,7 @@ __global__ __launch_bounds__(64 * most_waves(HD, QT)) void attend_kernel(AttendA
 #pragma unroll
       for (int t = 0; t < QT; t++) {
         uint32_t vis = there;
-        if constexpr (KIND == 2) vis &= node_mask(a, b, min(r0 + (qi * QT + t) * 16 + m, total - 1) / group, j0 + 8 * g);
+        if constexpr (KIND == 2) vis &= node_mask(a, b, node[t], j0 + 8 * g);
 #pragma unroll
         for (int e = 0; e < 8; e++)
           if (!(vis >> e & 1)) st[t][e & 1][e >> 1] = -INFINITY;
@@ -384,8 +369,7 @@ __global__ __launch_bounds__(64 * most_waves(HD, QT)) void attend_kernel(AttendA
           const T *v = (const T *)a.v + (row0 + j0 + j) * a.stride + (size_t)kh * a.hd;
 #pragma unroll
           for (int t = 0; t < QT; t++) {
-            const int i = min(r0 + (qi * QT + t) * 16 + m, total - 1) / group;
-            if (!(node_mask(a, b, i, j0 + j) & 1)) continue;
+            if (!(node_mask(a, b, node[t], j0 + j) & 1)) continue;
 #pragma unroll
             for (int x = 0; x < 4 * Z; x++)
 #pragma unroll
@@ -409,50 +393,55 @@ __global__ __launch_bounds__(64 * most_waves(HD, QT)) void attend_kernel(AttendA
     }
     if constexpr (KIND == 0) load_v(blk + a.kw);
   };
-  if (busy) {
-    bool loaded = true;
-    if (blk < cached) {
-      for (; blk + a.kw < cached; blk += a.kw) step(std::integral_constant<int, 0>{});
-      step(std::integral_constant<int, 1>{});
-      blk += a.kw, loaded = false;
-    }
-    for (; blk < end; blk += a.kw, loaded = false) {
-      if (!loaded) load_nodes(blk);
-      step(std::integral_constant<int, 2>{});
-    }
+  bool loaded = true;
+  if (blk < cached) {
+    for (; blk + a.kw < cached; blk += a.kw) step(std::integral_constant<int, 0>{});
+    step(std::integral_constant<int, 1>{});
+    blk += a.kw, loaded = false;
+  }
+  for (; blk < end; blk += a.kw, loaded = false) {
+    if (!loaded) load_nodes(blk);
+    step(std::integral_constant<int, 2>{});
   }
 
-  // The key groups' results joined through LDS: every wavefront writes its own, then every thread adds up four values
-  // of a row.  Lane 16g + i holds row i's values 16g + 4r + (x % 4) of the chunk of 64 x / 4.
-  floatx4 *merge = (floatx4 *)(smem + 64 * tiles);               // [ki][tile][z][r][lane]
-  float *ml = (float *)(merge + (size_t)a.kw * tiles * Z * 256);  // [ki][tile][maxima, sums][row]
-  __syncthreads();
+  // The wavefronts' results joined through LDS: each writes its own, then every lane adds up four values of a row, all of
+  // its reads at once.  Lane 16g + i holds row i's values 16g + 4r + (x % 4) of the chunk of 64 x / 4.
+  floatx4 *merge = (floatx4 *)smem;                       // [ki][t][z][r][lane]
+  float *ml = (float *)(merge + a.kw * QT * Z * 256);  // [ki][t][maxima, sums][row]
 #pragma unroll
   for (int t = 0; t < QT; t++) {
-    const int tile = ki * tiles + qi * QT + t;
     sum[t] = xlane::bit4(sum[t], xlane::Add{});
     sum[t] = xlane::bit5(sum[t], xlane::Add{});
-    if (g == 0) ml[32 * tile + m] = mx[t], ml[32 * tile + 16 + m] = sum[t];
+    if (g == 0) ml[32 * (ki * QT + t) + m] = mx[t], ml[32 * (ki * QT + t) + 16 + m] = sum[t];
 #pragma unroll
     for (int z = 0; z < Z; z++)
 #pragma unroll
       for (int r = 0; r < 4; r++)
-        merge[((tile * Z + z) * 4 + r) * 64 + lane] = floatx4{acc[t][4 * z][r], acc[t][4 * z + 1][r], acc[t][4 * z + 2][r], acc[t][4 * z + 3][r]};
+        merge[(((ki * QT + t) * Z + z) * 4 + r) * 64 + lane] =
+            floatx4{acc[t][4 * z][r], acc[t][4 * z + 1][r], acc[t][4 * z + 2][r], acc[t][4 * z + 3][r]};
   }
   __syncthreads();
-  for (int x = wave; x < tiles * Z * 4; x += a.qw * a.kw) {
-    const int tile = x / (4 * Z), z = x / 4 % Z, d = 64 * z + 16 * g + 4 * (x % 4), r = r0 + 16 * tile + m;
+  for (int x = ki; x < QT * Z * 4; x += a.kw) {
+    const int t = x / (4 * Z), z = x / 4 % Z, d = 64 * z + 16 * g + 4 * (x % 4), r = r0 + 16 * t + m;
     if (r >= total || d >= a.hd) continue;
-    float top = -INFINITY, l = 0.0f;
-    for (int k = 0; k < a.kw; k++) top = fmaxf(top, ml[32 * (k * tiles + tile) + m]);
-    const float c = coef[16 * tile + m];
-    floatx4 f{};
-    for (int k = 0; k < a.kw; k++) {
-      const float km = ml[32 * (k * tiles + tile) + m], w = km == top ? 1.0f : __builtin_amdgcn_exp2f((km - top) * c);
-      l += w * ml[32 * (k * tiles + tile) + 16 + m];
-      f += w * merge[((k * tiles * Z * 4) + x) * 64 + lane];
+    float km[WAVES], kl[WAVES], top = -INFINITY, l = 0.0f, c = cf[0];
+    if (QT == 2 && t) c = cf[QT - 1];
+    floatx4 kf[WAVES], f{};
+#pragma unroll
+    for (int k = 0; k < WAVES; k++) {
+      const int w = min(k, a.kw - 1) * QT;
+      km[k] = ml[32 * (w + t) + m], kl[k] = ml[32 * (w + t) + 16 + m], kf[k] = merge[(w * Z * 4 + x) * 64 + lane];
+      if (k >= a.kw) km[k] = -INFINITY;
     }
-    const int i = r / group, head = kh * group + r % group;
+#pragma unroll
+    for (int k = 0; k < WAVES; k++) top = fmaxf(top, km[k]);
+#pragma unroll
+    for (int k = 0; k < WAVES; k++) {
+      if (k >= a.kw) break;
+      const float w = km[k] == top ? 1.0f : __builtin_amdgcn_exp2f((km[k] - top) * c);
+      l += w * kl[k], f += w * kf[k];
+    }
+    const int i = node_of(r, group), head = kh * group + head_of(r, group);
     const size_t out = ((row0 + i) * a.heads + head) * a.hd + d;
     if (s.used > 1) {
       const size_t part = (size_t)split * a.batch * a.rows * a.heads;
@@ -482,12 +471,8 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 4 : 3) void attend_rows_kernel(Att
   __shared__ int odd;  // set where a node's value is no finite number
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, m = lane & 15;
   constexpr int threads = 64 * W, MOST = U / threads;  // MOST: pieces per thread
-  int at = blockIdx.x;
-  const int split = at % a.splits;
-  at /= a.splits;
-  const int kh = at % a.kv_heads;
-  at /= a.kv_heads;
-  const int rb = at % a.row_blocks, b = at / a.row_blocks;
+  const int split = blockIdx.z, kh = blockIdx.y, b = a.row_blocks == 1 ? blockIdx.x : blockIdx.x / a.row_blocks;
+  const int rb = blockIdx.x - b * a.row_blocks;
   const int group = a.heads / a.kv_heads, r0 = 16 * QT * (rb * W + wave);
   const size_t row0 = (size_t)b * a.rows;
   const Share s = share_of(a, b);
@@ -508,7 +493,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 4 : 3) void attend_rows_kernel(Att
     for (int i = 0; i < MOST; i++) {
       const int u = tid + threads * i, pair = u / (B / 4), q = u % (B / 4), row = u / (HD / 8), d = u % (HD / 8) * 4;
       p.k[i] = *(const u32x4_a4 *)(kc + (size_t)min(pair, pairs - 1) * a.cols + j0 + min(4 * q, last & ~3));
-      p.v[i] = *(const u32x4_a4 *)(vc + (size_t)j0 * half + (uint32_t)(min(row, last) * half + (d < pairs ? d : 0)));
+      p.v[i] = *(const u32x4_a4 *)(vc + (size_t)j0 * half + (uint32_t)(min(row, last) * half + min(d, pairs - 4)));
     }
   };
   auto store = [&](const Pieces &p, int blk, uint32_t *buf) {
@@ -517,53 +502,29 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 4 : 3) void attend_rows_kernel(Att
     for (int i = 0; i < MOST; i++) {
       const int u = tid + threads * i, pair = u / (B / 4), q = u % (B / 4), row = u / (HD / 8), d = u % (HD / 8) * 4;
       *(u32x4 *)(buf + pair * KS + 4 * q) = pair < pairs ? p.k[i] : u32x4{};
-      *(u32x4 *)(buf + KW + row * VS + d) = row <= last ? p.v[i] : u32x4{};
+      // (a head's last 4 values are the upper half of the piece before its end)
+      const u32x4 v = d == pairs - 2 ? u32x4{p.v[i][2], p.v[i][3], 0, 0} : p.v[i];
+      *(u32x4 *)(buf + KW + row * VS + d) = row <= last ? v : u32x4{};
     }
   };
   Pieces p0, p1;
   if (begin < cached) load(p0, begin);
   if (begin + 1 < cached) load(p1, begin + 1);
 
-  // The queries, scaled as above, in registers.
   half8 q[QT][C][QP];
-  float cf[QT];
+  floatx4 acc[QT][X];
+  float mx[QT], sum[QT], cf[QT];
+  int node[QT];
 #pragma unroll
   for (int t = 0; t < QT; t++) {
     const int row = min(r0 + 16 * t + m, total - 1);
-    const T *src = (const T *)a.q + (row0 + row / group) * a.stride + (size_t)(kh * group + row % group) * a.hd;
-    float f[C][8], top = 0.0f;
-#pragma unroll
-    for (int c = 0; c < C; c++)
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const int d = 32 * c + 8 * g;
-        f[c][e] = d < a.hd ? number(src + d, e) : 0.0f;
-        top = fmaxf(top, fabsf(f[c][e]));
-      }
-    int k = 0;
-    if constexpr (QP == 2) {
-      top = xlane::bit4(top, xlane::Max{});
-      top = xlane::bit5(top, xlane::Max{});
-      if (top > 0.0f && top < INFINITY) k = min(7 - ilogbf(top), 100);
-    }
-    cf[t] = ldexpf(a.scale * 1.44269504088896341f, -k);
-#pragma unroll
-    for (int c = 0; c < C; c++)
-#pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float y = QP == 2 ? ldexpf(f[c][e], k) : f[c][e];
-        q[t][c][0][e] = (_Float16)y;
-        if constexpr (QP == 2) q[t][c][1][e] = (_Float16)(y - (float)q[t][c][0][e]);
-      }
-  }
-  floatx4 acc[QT][X];
-  float mx[QT], sum[QT];
-#pragma unroll
-  for (int t = 0; t < QT; t++) {
+    node[t] = node_of(row, group);
+    cf[t] = query<T, C>((const T *)a.q + (row0 + node[t]) * a.stride + (size_t)(kh * group + head_of(row, group)) * a.hd, g, a.hd, a.scale, q[t]);
     mx[t] = -INFINITY, sum[t] = 0.0f;
 #pragma unroll
     for (int x = 0; x < X; x++) acc[t][x] = floatx4{};
   }
+  const bool busy = r0 < total;  // (a wavefront past the last row only loads)
 
   // One block from LDS; nodes: a block of nodes, otherwise the cache's.
   auto step = [&](auto nodes, int blk, const uint32_t *buf) {
@@ -592,7 +553,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 4 : 3) void attend_rows_kernel(Att
         for (int kk = 0; kk < KK; kk++) {
           const int left = last + 1 - 32 * kk;
           uint32_t vis = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u;
-          if constexpr (NODES) vis &= node_mask(a, b, min(r0 + 16 * t + m, total - 1) / group, j0 + 32 * kk);
+          if constexpr (NODES) vis &= node_mask(a, b, node[t], j0 + 32 * kk);
 #pragma unroll
           for (int e = 0; e < 8; e++)
             if (!(vis >> (16 * (e >> 2) + 4 * g + (e & 3)) & 1)) st[t][2 * kk + (e >> 2)][e & 3] = -INFINITY;
@@ -645,7 +606,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 4 : 3) void attend_rows_kernel(Att
         const T *v = (const T *)a.v + (row0 + j0 + j) * a.stride + (size_t)kh * a.hd;
 #pragma unroll
         for (int t = 0; t < QT; t++) {
-          if (!(node_mask(a, b, min(r0 + 16 * t + m, total - 1) / group, j0 + j) & 1)) continue;
+          if (!(node_mask(a, b, node[t], j0 + j) & 1)) continue;
 #pragma unroll
           for (int x = 0; x < X; x++)
 #pragma unroll
@@ -662,11 +623,11 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 4 : 3) void attend_rows_kernel(Att
     store(p0, blk, buf0);
     load(p0, blk + 2);
     meet();
-    step(std::false_type{}, blk, buf0);
+    if (busy) step(std::false_type{}, blk, buf0);
     store(p1, blk + 1, buf1);
     load(p1, blk + 3);
     meet();
-    step(std::false_type{}, blk + 1, buf1);
+    if (busy) step(std::false_type{}, blk + 1, buf1);
   }
   for (; blk < cached; blk++) {  // (at most three)
     const bool even = (blk - begin) % 2 == 0;
@@ -674,7 +635,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 4 : 3) void attend_rows_kernel(Att
     else store(p1, blk, buf1);
     if (even && blk + 2 < cached) load(p0, blk + 2);
     meet();
-    step(std::false_type{}, blk, even ? buf0 : buf1);
+    if (busy) step(std::false_type{}, blk, even ? buf0 : buf1);
   }
   for (; blk < end; blk++) {
     uint32_t *buf = (blk - begin) % 2 ? buf1 : buf0;
@@ -690,9 +651,10 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 4 : 3) void attend_rows_kernel(Att
       u32x2 k[2], v[2];
 #pragma unroll
       for (int y = 0; y < 2; y++) {
-        k[y] = four((const T *)a.k + src + (d < a.hd ? d + 4 * y : 0)), v[y] = four((const T *)a.v + src + (d < a.hd ? d + 4 * y : 0));
-        if (d >= a.hd) k[y] = u32x2{};
-        if (d >= a.hd || row > last) v[y] = u32x2{};
+        const bool in = d + 4 * y < a.hd;
+        k[y] = four((const T *)a.k + src + (in ? d + 4 * y : 0)), v[y] = four((const T *)a.v + src + (in ? d + 4 * y : 0));
+        if (!in) k[y] = u32x2{};
+        if (!in || row > last) v[y] = u32x2{};
 #pragma unroll
         for (int w = 0; w < 2; w++) {
           buf[(d / 2 + 2 * y + w) * KS + row] = k[y][w];
@@ -705,7 +667,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 4 : 3) void attend_rows_kernel(Att
     }
     if (found) odd = 1;
     __syncthreads();
-    step(std::true_type{}, blk, buf);
+    if (busy) step(std::true_type{}, blk, buf);
   }
 
   // Lane 16g + i holds row i's values 16x + 4g + 0 .. 3.
@@ -715,7 +677,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 4 : 3) void attend_rows_kernel(Att
     sum[t] = xlane::bit5(sum[t], xlane::Add{});
     const int r = r0 + 16 * t + m;
     if (r >= total) continue;
-    const int i = r / group, head = kh * group + r % group;
+    const int i = node[t], head = kh * group + head_of(r, group);
     const size_t out = ((row0 + i) * a.heads + head) * a.hd;
     const size_t part = (size_t)split * a.batch * a.rows * a.heads;
     if (s.used > 1 && g == 0) *(floatx4 *)(a.pml + 4 * (part + (row0 + i) * a.heads + head)) = floatx4{mx[t], sum[t], cf[t], 0.0f};
@@ -836,14 +798,10 @@ __global__ __launch_bounds__(256) void keep_kernel(KeepArgs a) {
 
 template <typename T, int HD, int QT, bool P16>
 int attend_launch(wh_ctx *ctx, const AttendArgs &a) {
-  const size_t tiles = QT * a.qw, queries = tiles * HD / 32 * (sizeof(T) == 4 ? 2 : 1) * 1024;
-  const size_t merge = a.kw * tiles * (HD / 64 * 4096 + 128);
-  {
-    ProfScope prof(ctx, "tree_attend", 4.0 * a.batch * a.rows * a.heads * a.cols * a.hd, 4.0 * a.batch * a.cols * a.kv_heads * a.hd);
-    wh_launch(ctx, (attend_kernel<T, HD, QT, P16>), a.batch * a.row_blocks * a.kv_heads * a.splits, 64 * a.qw * a.kw,
-              64 * tiles + std::max(queries, merge), a);
-    return wh_launched(ctx, "tree attention");
-  }
+  ProfScope prof(ctx, "tree_attend", 4.0 * a.batch * a.rows * a.heads * a.cols * a.hd, 4.0 * a.batch * a.cols * a.kv_heads * a.hd);
+  wh_launch(ctx, (attend_kernel<T, HD, QT, P16>), dim3(a.batch * a.row_blocks, a.kv_heads, a.splits), 64 * a.kw,
+            (size_t)a.kw * QT * (HD / 64 * 4096 + 128), a);
+  return wh_launched(ctx, "tree attention");
 }
 
 template <bool P16>
@@ -854,22 +812,23 @@ int attend_join(wh_ctx *ctx, const AttendArgs &a) {
   return wh_launched(ctx, "tree attention's join");
 }
 
-template <typename T, int HD, int QT, int W, bool P16>
+template <typename T, int HD, int W, bool P16>
 int attend_rows_launch(wh_ctx *ctx, const AttendArgs &a) {
   constexpr int B = rows_block(HD);
   ProfScope prof(ctx, "tree_attend_rows", 4.0 * a.batch * a.rows * a.heads * a.cols * a.hd, 4.0 * a.batch * a.cols * a.kv_heads * a.hd);
-  wh_launch(ctx, (attend_rows_kernel<T, HD, QT, W, P16>), a.batch * a.row_blocks * a.kv_heads * a.splits, 64 * W,
+  wh_launch(ctx, (attend_rows_kernel<T, HD, 1, W, P16>), dim3(a.batch * a.row_blocks, a.kv_heads, a.splits), 64 * W,
             2 * 4 * ((B + 4) * HD / 2 + (HD / 2 + 8) * B), a);
   return wh_launched(ctx, "tree attention");
 }
 
+// waves: of attend_rows_kernel's workgroups, or 0: attend_kernel with qt tiles of rows.
 template <typename T, bool P16>
-int attend_t(wh_ctx *ctx, const AttendArgs &a, int qt, bool rows) {
+int attend_t(wh_ctx *ctx, const AttendArgs &a, int qt, int waves) {
   int rc;
-  if (rows && a.hd <= 64) rc = a.qw == 4 ? attend_rows_launch<T, 64, 1, 4, P16>(ctx, a) : attend_rows_launch<T, 64, 1, 8, P16>(ctx, a);
-  else if (rows) rc = a.qw == 4 ? attend_rows_launch<T, 128, 1, 4, P16>(ctx, a) : attend_rows_launch<T, 128, 1, 8, P16>(ctx, a);
+  if (waves && a.hd <= 64) rc = waves == 4 ? attend_rows_launch<T, 64, 4, P16>(ctx, a) : attend_rows_launch<T, 64, 8, P16>(ctx, a);
+  else if (waves) rc = waves == 4 ? attend_rows_launch<T, 128, 4, P16>(ctx, a) : attend_rows_launch<T, 128, 8, P16>(ctx, a);
   else if (a.hd <= 64) rc = qt == 1 ? attend_launch<T, 64, 1, P16>(ctx, a) : attend_launch<T, 64, 2, P16>(ctx, a);
-  else rc = qt == 1 ? attend_launch<T, 128, 1, P16>(ctx, a) : attend_launch<T, 128, 2, P16>(ctx, a);
+  else rc = attend_launch<T, 128, 1, P16>(ctx, a);
   return rc || a.splits == 1 ? rc : attend_join<P16>(ctx, a);
 }
 
@@ -901,20 +860,18 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
     return wh_fail(ctx, WH_EARG, "tree attention: buffers and rows must be 4-byte aligned");
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "tree attention: %s", hipGetErrorString(e));
   AttendArgs a{q, k, v, stride, kv, kv_stride, o, t->n, t->count, t->mask, t->mask_stride, t->batch, t->rows, (t->rows + 31) / 32,
-               cols, heads, kv_heads, hd, 1.0f / sqrtf((float)hd), 1, 1, 1, 1, KB, nullptr, nullptr};
+               cols, heads, kv_heads, hd, 1.0f / sqrtf((float)hd), 1, 1, 1, KB, nullptr, nullptr};
   const int rows = t->rows * (heads / kv_heads), tiles = (rows + 15) / 16;
-  const int hdp = hd <= 64 ? 64 : 128;
-  const bool many = tiles > 2 && hd % 8 == 0 && cols >= 4;
-  const int qt = many || tiles == 1 ? 1 : 2, waves = many ? 8 : most_waves(hdp, qt), qwaves = (tiles + qt - 1) / qt;
-  if (many) a.block = rows_block(hd);
+  const int most = hd <= 64 ? 2 : 1;  // tiles of attend_kernel
+  const int waves = tiles > most && hd >= 8 && cols >= 4 ? tiles <= 4 ? 4 : 8 : 0, qt = std::min(tiles, most);
+  if (waves) a.block = rows_block(hd);
   const int blocks = (cols + a.block - 1) / a.block + (t->mask && k ? (t->rows + a.block - 1) / a.block : 0);
-  a.qw = many ? qwaves <= 4 ? 4 : 8 : std::min(qwaves, waves);
-  a.row_blocks = (qwaves + a.qw - 1) / a.qw;
-  a.kw = many ? 1 : std::max(1, std::min(waves / a.qw, blocks));
+  a.row_blocks = (tiles + (waves ? waves : qt) - 1) / (waves ? waves : qt);
+  a.kw = waves ? 1 : std::min(WAVES, blocks);
   const size_t units = (size_t)t->batch * kv_heads * a.row_blocks;
   const size_t cus = ctx->cus > 0 ? ctx->cus : 256;
-  const int least = many ? 8 : 2 * a.kw;  // blocks of a split
-  a.splits = (int)std::max<size_t>(1, std::min<size_t>(((many ? 2 : 1) * cus + units - 1) / units, (blocks + least - 1) / least));
+  const int least = waves ? 8 : 2 * a.kw;  // blocks of a split
+  a.splits = (int)std::max<size_t>(1, std::min<size_t>(((waves ? 2 : 1) * cus + units - 1) / units, (blocks + least - 1) / least));
   const size_t nodes = (size_t)t->batch * t->rows;
   if (units * a.splits >= (size_t)1 << 22 || nodes * heads >= (size_t)1 << 25)  // (a launch's threads fit 32 bits)
     return wh_fail(ctx, WH_EARG, "tree attention: %d heads of %zu nodes in one call", heads, nodes);
@@ -923,8 +880,8 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
     if (!(a.po = (float *)wh_scratch(ctx, part * (hd + 4) * sizeof(float)))) return WH_EOOM;
     a.pml = a.po + part * hd;
   }
-  return in16 ? out16 ? attend_t<_Float16, true>(ctx, a, qt, many) : attend_t<_Float16, false>(ctx, a, qt, many)
-              : out16 ? attend_t<float, true>(ctx, a, qt, many) : attend_t<float, false>(ctx, a, qt, many);
+  return in16 ? out16 ? attend_t<_Float16, true>(ctx, a, qt, waves) : attend_t<_Float16, false>(ctx, a, qt, waves)
+              : out16 ? attend_t<float, true>(ctx, a, qt, waves) : attend_t<float, false>(ctx, a, qt, waves);
 }
 
 int launch_tree_accept(wh_ctx *ctx, const wh_tree *t, const uint32_t *picks, const wh_kept *w, int cols, int32_t *path,
