@@ -37,12 +37,11 @@ struct AttendArgs {
   float *po, *pml;
 };
 
-constexpr int KB = 32;  // keys per block of attend_kernel
 
 constexpr int WAVES = 8;  // wavefronts of a workgroup, at most
 
-// Positions of a block of attend_rows_kernel.
-constexpr int rows_block(int hd) { return hd <= 64 ? 64 : 32; }
+constexpr int few_block(int hd) { return hd <= 64 ? 64 : 32; }   // positions of a block of attend_kernel
+constexpr int rows_block(int hd) { return hd <= 64 ? 64 : 32; }  // and of attend_rows_kernel
 
 // The blocks of keys of a sequence (the cache's, then the nodes'), and how its `splits` workgroups share them:
 // runs of `per` blocks, at least one for each wavefront, so that a short sequence uses fewer of them.
@@ -55,8 +54,11 @@ __device__ __forceinline__ Share share_of(const AttendArgs &a, int b) {
   s.count = a.count ? min(max(a.count[b], 0), a.rows) : a.rows;
   s.cached = (s.n + a.block - 1) / a.block;
   s.blocks = s.cached + (a.mask && a.k ? (s.count + a.block - 1) / a.block : 0);
-  s.per = max((s.blocks + a.splits - 1) / a.splits, a.kw);
-  s.used = max((s.blocks + s.per - 1) / s.per, 1);
+  s.per = s.blocks, s.used = 1;
+  if (a.splits > 1) {
+    s.per = max((s.blocks + a.splits - 1) / a.splits, a.kw);
+    s.used = max((s.blocks + s.per - 1) / s.per, 1);
+  }
   return s;
 }
 
@@ -127,11 +129,11 @@ __device__ __forceinline__ floatx4 mfma(half8 a, half8 b, floatx4 c) {
 __device__ __forceinline__ int node_of(int row, int group) { return group == 1 ? row : row / group; }
 __device__ __forceinline__ int head_of(int row, int group) { return group == 1 ? 0 : row % group; }
 
-// A row's query as the matrix cores take it (lane 16g + i: row i's 8 values from 8g on of every chunk of 32), times a
-// power of two and in two parts for f32: precision is said at attend_kernel.  Gives the factor of its scores' exponents.
+// A row's query as the matrix cores take it (lane 16g + i: row i's 8 values from 8g on of every chunk of 32): its values,
+// and those times a power of two and in two parts for f32 (precision is said at attend_kernel), with the factor of its
+// scores' exponents.
 template <typename T, int C>
-__device__ __forceinline__ float query(const T *src, int g, int hd, float scale, half8 (&q)[C][sizeof(T) == 4 ? 2 : 1]) {
-  float f[C][8], top = 0.0f;
+__device__ __forceinline__ void load_query(const T *src, int g, int hd, float (&f)[C][8]) {
 #pragma unroll
   for (int c = 0; c < C; c++)
 #pragma unroll
@@ -141,8 +143,12 @@ __device__ __forceinline__ float query(const T *src, int g, int hd, float scale,
 #pragma unroll
       for (int e = 0; e < 4; e++) f[c][4 * y + e] = d < hd ? f[c][4 * y + e] : 0.0f;
     }
+}
+template <int C, int QP>
+__device__ __forceinline__ float split_query(const float (&f)[C][8], float scale, half8 (&q)[C][QP]) {
   int k = 0;
-  if constexpr (sizeof(T) == 4) {
+  if constexpr (QP == 2) {
+    float top = 0.0f;
 #pragma unroll
     for (int c = 0; c < C; c++)
 #pragma unroll
@@ -155,29 +161,25 @@ __device__ __forceinline__ float query(const T *src, int g, int hd, float scale,
   for (int c = 0; c < C; c++)
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-      if constexpr (sizeof(T) == 4) {
-        const float y = ldexpf(f[c][e], k);
-        q[c][0][e] = (_Float16)y;
-        q[c][1][e] = (_Float16)(y - (float)q[c][0][e]);
-      } else {
-        q[c][0][e] = (_Float16)f[c][e];
-      }
+      const float y = QP == 2 ? ldexpf(f[c][e], k) : f[c][e];
+      q[c][0][e] = (_Float16)y;
+      if constexpr (QP == 2) q[c][1][e] = (_Float16)(y - (float)q[c][0][e]);
     }
   return ldexpf(scale * 1.44269504088896341f, -k);
 }
 
 // Attention over a run of key blocks, for few rows.  A workgroup takes one key head of a sequence, 16 * QT of its rows
-// (the heads / kv_heads query heads of a node are rows next to each other) and one split of its key blocks of
-// 32, of which each of its kw wavefronts takes every kw-th.  A wavefront reads a block's K and V straight into
-// the registers that the matrix cores take:
+// (the heads / kv_heads query heads of a node are rows next to each other) and one split of its key blocks
+// (64 positions for heads of up to 64 values, 32 for larger ones), of which each of its kw wavefronts takes every
+// kw-th.  A wavefront reads a block's K and V straight into the registers that the matrix cores take:
 //
 //   Scores transposed, S^T = K Q^T (v_mfma_f32_16x16x32_f16).  The cache holds K as pairs of values, position by
-//   position, so a lane reads two positions of a pair at once: lane 16g + m holds positions 2m and 2m + 1 of the
-//   pairs of 8 values from 8g on, which are the operand rows of two tiles, tile u with position 2m + u in row m.
-//   In the products, lane 16g + i then holds row i's scores of the 8 positions from 8g on.
-//   Outputs transposed, O^T = V^T P^T: those scores are the operand of P as they stand, k = 8g + e meaning position
-//   8g + e.  A lane reads 4 values (from 4m on) of its 8 positions of V, and v_perm pairs those of two positions.
-//   A row's softmax state is one lane column's everywhere.
+//   position, so a lane reads KP = 4 or 2 positions of a pair at once: lane 16g + m holds the positions from KP m on
+//   of the pairs of 8 values from 8g on, which are the operand rows of KP tiles, tile u with position KP m + u in
+//   row m.  In the products, lane 16g + i then holds row i's scores of the NP = 4 KP positions from NP g on.
+//   Outputs transposed, O^T = V^T P^T: those scores are the operand of P as they stand, k = 8g + e of instruction kk
+//   meaning position NP g + 8kk + e.  A lane reads 4 values (from 4m on) of its NP positions of V, and v_perm
+//   pairs those of two positions.  A row's softmax state is one lane column's everywhere.
 //
 // The next block's K is loaded as soon as this one's scores are done, and its V after this one's outputs, so that
 // a wavefront always has loads in flight; the first block's before the queries are looked at.
@@ -188,12 +190,23 @@ __device__ __forceinline__ float query(const T *src, int g, int hd, float scale,
 template <typename T, int HD, int QT, bool P16>
 __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
   constexpr int C = HD / 32, Z = HD / 64, QP = sizeof(T) == 4 ? 2 : 1;
+  constexpr int KP = few_block(HD) / 16, NP = 4 * KP, KB = 16 * KP, KK = KP / 2;
+  typedef uint32_t Words __attribute__((ext_vector_type(KP)));
+  typedef Words Words_a4 __attribute__((aligned(4)));
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int lane = threadIdx.x & 63, ki = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, m = lane & 15;
   const int split = blockIdx.z, kh = blockIdx.y, b = a.row_blocks == 1 ? blockIdx.x : blockIdx.x / a.row_blocks;
   const int group = a.heads / a.kv_heads, r0 = 16 * QT * (blockIdx.x - b * a.row_blocks);
   const size_t row0 = (size_t)b * a.rows;
+  float f[QT][C][8];
+  int node[QT];
+#pragma unroll
+  for (int t = 0; t < QT; t++) {  // (of rows that are not there, too: nothing is known of the lengths yet)
+    const int row = min(r0 + 16 * t + m, a.rows * group - 1);
+    node[t] = node_of(row, group);
+    load_query<T, C>((const T *)a.q + (row0 + node[t]) * a.stride + (size_t)(kh * group + head_of(row, group)) * a.hd, g, a.hd, f[t]);
+  }
   const Share s = share_of(a, b);
   const int total = s.count * group;
   if (split >= s.used || r0 >= total) return;
@@ -201,25 +214,26 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
   const uint32_t *kc = a.kv + (size_t)b * a.kv_stride + (size_t)kh * pairs * a.cols;
   const uint32_t *vc = a.kv + (size_t)b * a.kv_stride + (size_t)half * a.cols + kh * pairs;
 
-  u32x2 kw[C][4], vw[8][Z];  // a block's K, pair by pair, and V, position by position
+  Words kw[C][4];
+  u32x2 vw[NP][Z];  // a block's K, pair by pair, and V, position by position
   // The same loads on every way through, so that a wait for one block's does not have to be one for the next block's.
   auto load_k = [&](int blk) {
     // (made anew for every block: what follows from them would otherwise be kept in more registers than there are)
     int hd = a.hd, cols = a.cols;
     asm volatile("" : "+s"(hd), "+s"(cols));
-    const int j0 = blk * KB, last = s.n - 1 - j0, jk = min(2 * m, last & ~1);  // (a position past the row's end: the next row, or V)
+    const int j0 = blk * KB, last = s.n - 1 - j0, jk = min(KP * m, last & ~(KP - 1));  // (a position past the row's end: the next row, or V)
 #pragma unroll
     for (int c = 0; c < C; c++) {
       const uint32_t *base = kc + (size_t)(16 * c) * cols + j0;
       const int top = hd / 2 - 1 - 16 * c;  // the last pair of this chunk, where it has not 16
       if (top >= 15) {
 #pragma unroll
-        for (int x = 0; x < 4; x++) kw[c][x] = *(const u32x2_a4 *)(base + (size_t)x * cols + (uint32_t)(4 * g * cols + jk));
+        for (int x = 0; x < 4; x++) kw[c][x] = *(const Words_a4 *)(base + (size_t)x * cols + (uint32_t)(4 * g * cols + jk));
       } else {
 #pragma unroll
         for (int x = 0; x < 4; x++) {
-          kw[c][x] = *(const u32x2_a4 *)(base + (int64_t)max(min(4 * g + x, top), -16 * c) * cols + jk);
-          if (top < 4 * g + x) kw[c][x] = u32x2{};
+          kw[c][x] = *(const Words_a4 *)(base + (int64_t)max(min(4 * g + x, top), -16 * c) * cols + jk);
+          if (top < 4 * g + x) kw[c][x] = Words{};
         }
       }
     }
@@ -228,10 +242,10 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
     const int j0 = blk * KB, last = s.n - 1 - j0;
     const uint32_t *base = vc + (size_t)j0 * half;
 #pragma unroll
-    for (int e = 0; e < 8; e++)
+    for (int e = 0; e < NP; e++)
 #pragma unroll
       for (int z = 0; z < Z; z++)
-        vw[e][z] = *(const u32x2_a4 *)(base + (uint32_t)(min(8 * g + e, last) * half + (64 * z + 4 * m < a.hd ? 32 * z + 2 * m : 0)));
+        vw[e][z] = *(const u32x2_a4 *)(base + (uint32_t)(min(NP * g + e, last) * half + (64 * z + 4 * m < a.hd ? 32 * z + 2 * m : 0)));
   };
   auto load_nodes = [&](int blk) {
     const int j0 = (blk - s.cached) * KB, last = s.count - 1 - j0;
@@ -240,8 +254,8 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
 #pragma unroll
     for (int c = 0; c < C; c++)
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
-        const T *src = k + (uint32_t)min(2 * m + u, last) * (uint32_t)a.stride;
+      for (int u = 0; u < KP; u++) {
+        const T *src = k + (uint32_t)min(KP * m + u, last) * (uint32_t)a.stride;
         const int d = 32 * c + 8 * g;
         u32x2 lo = four(src + (d < a.hd ? d : 0)), hi = four(src + (d + 4 < a.hd ? d + 4 : 0));
         if (d >= a.hd) lo = u32x2{};
@@ -249,21 +263,26 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
         kw[c][0][u] = lo[0], kw[c][1][u] = lo[1], kw[c][2][u] = hi[0], kw[c][3][u] = hi[1];
       }
 #pragma unroll
-    for (int e = 0; e < 8; e++)
+    for (int e = 0; e < NP; e++)
 #pragma unroll
       for (int z = 0; z < Z; z++)
-        vw[e][z] = four(v + (uint32_t)min(8 * g + e, last) * (uint32_t)a.stride + (64 * z + 4 * m < a.hd ? 64 * z + 4 * m : 0));
+        vw[e][z] = four(v + (uint32_t)min(NP * g + e, last) * (uint32_t)a.stride + (64 * z + 4 * m < a.hd ? 64 * z + 4 * m : 0));
   };
   int blk = split * s.per + ki;
   const int end = min((split + 1) * s.per, s.blocks), cached = min(end, s.cached);
   if (blk < cached) {
-    if (a.cols > 1) {
+    if (a.cols >= KP) {
       load_k(blk);
-    } else {  // (a cache of one position: nothing behind it)
+    } else {  // (a cache of so few positions: nothing behind them)
 #pragma unroll
       for (int c = 0; c < C; c++)
 #pragma unroll
-        for (int x = 0; x < 4; x++) kw[c][x] = u32x2{16 * c + 4 * g + x < pairs ? kc[16 * c + 4 * g + x] : 0u, 0u};
+        for (int x = 0; x < 4; x++)
+#pragma unroll
+          for (int u = 0; u < KP; u++) {
+            const int p = 16 * c + 4 * g + x;
+            kw[c][x][u] = p < pairs ? kc[p * a.cols + min(u, a.cols - 1)] : 0u;
+          }
     }
     load_v(blk);
   } else if (blk < end) {
@@ -273,12 +292,9 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
   half8 q[QT][C][QP];
   floatx4 acc[QT][4 * Z];
   float mx[QT], sum[QT], cf[QT];
-  int node[QT];
 #pragma unroll
   for (int t = 0; t < QT; t++) {
-    const int row = min(r0 + 16 * t + m, total - 1);
-    node[t] = node_of(row, group);
-    cf[t] = query<T, C>((const T *)a.q + (row0 + node[t]) * a.stride + (size_t)(kh * group + head_of(row, group)) * a.hd, g, a.hd, a.scale, q[t]);
+    cf[t] = split_query(f[t], a.scale, q[t]);
     mx[t] = -INFINITY, sum[t] = 0.0f;
 #pragma unroll
     for (int x = 0; x < 4 * Z; x++) acc[t][x] = floatx4{};
@@ -288,41 +304,42 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
     constexpr int KIND = which;
     constexpr bool all = KIND == 0;
     const int j0 = (KIND == 2 ? blk - s.cached : blk) * KB, last = (KIND == 2 ? s.count : s.n) - 1 - j0;
-    const int left = last + 1 - 8 * g;  // of this lane's positions
-    floatx4 st[QT][2];
+    const int left = last + 1 - NP * g;  // of this lane's positions
+    floatx4 st[QT][KP];
 #pragma unroll
-    for (int t = 0; t < QT; t++) st[t][0] = st[t][1] = floatx4{};
+    for (int t = 0; t < QT; t++)
 #pragma unroll
-    for (int c = 0; c < C; c++) {
-      const half8 k0 = __builtin_bit_cast(half8, u32x4{kw[c][0][0], kw[c][1][0], kw[c][2][0], kw[c][3][0]});
-      const half8 k1 = __builtin_bit_cast(half8, u32x4{kw[c][0][1], kw[c][1][1], kw[c][2][1], kw[c][3][1]});
+      for (int u = 0; u < KP; u++) st[t][u] = floatx4{};
 #pragma unroll
-      for (int t = 0; t < QT; t++)
+    for (int c = 0; c < C; c++)
 #pragma unroll
-        for (int part = 0; part < QP; part++) {
-          st[t][0] = mfma(k0, q[t][c][part], st[t][0]), st[t][1] = mfma(k1, q[t][c][part], st[t][1]);
-        }
-    }
+      for (int u = 0; u < KP; u++) {
+        const half8 k = __builtin_bit_cast(half8, u32x4{kw[c][0][u], kw[c][1][u], kw[c][2][u], kw[c][3][u]});
+#pragma unroll
+        for (int t = 0; t < QT; t++)
+#pragma unroll
+          for (int part = 0; part < QP; part++) st[t][u] = mfma(k, q[t][c][part], st[t][u]);
+      }
     if constexpr (KIND == 0) load_k(blk + a.kw);
 
-    // The softmax: element 2r + u of the lane's 8 positions is st[u][r].
+    // The softmax: element KP r + u of the lane's NP positions is st[u][r].
     if constexpr (!all) {
-      const uint32_t there = left >= 8 ? 0xffu : left > 0 ? (1u << left) - 1u : 0u;
+      const uint32_t there = left >= NP ? (1u << NP) - 1u : left > 0 ? (1u << left) - 1u : 0u;
 #pragma unroll
       for (int t = 0; t < QT; t++) {
         uint32_t vis = there;
-        if constexpr (KIND == 2) vis &= node_mask(a, b, node[t], j0 + 8 * g);
+        if constexpr (KIND == 2) vis &= node_mask(a, b, node[t], j0 + NP * g);
 #pragma unroll
-        for (int e = 0; e < 8; e++)
-          if (!(vis >> e & 1)) st[t][e & 1][e >> 1] = -INFINITY;
+        for (int e = 0; e < NP; e++)
+          if (!(vis >> e & 1)) st[t][e % KP][e / KP] = -INFINITY;
       }
     }
-    half8 ph[QT], pl[QT];
+    half8 ph[QT][KK], pl[QT][KK];
 #pragma unroll
     for (int t = 0; t < QT; t++) {
       float top = st[t][0][0];
 #pragma unroll
-      for (int e = 1; e < 8; e++) top = fmaxf(top, st[t][e & 1][e >> 1]);
+      for (int e = 1; e < NP; e++) top = fmaxf(top, st[t][e % KP][e / KP]);
       top = xlane::bit4(top, xlane::Max{});
       top = xlane::bit5(top, xlane::Max{});
       top = fmaxf(top, mx[t]);
@@ -335,12 +352,12 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
         mx[t] = top;
       }
 #pragma unroll
-      for (int e = 0; e < 8; e++) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(st[t][e & 1][e >> 1] - base, cf[t], 10.0f));
+      for (int e = 0; e < NP; e++) {
+        const float p = __builtin_amdgcn_exp2f(fmaf(st[t][e % KP][e / KP] - base, cf[t], 10.0f));
         sum[t] += p;
         const _Float16 h = (_Float16)p;
-        ph[t][e] = h;
-        if constexpr (!P16) pl[t][e] = (_Float16)(p - (float)h);
+        ph[t][e >> 3][e & 7] = h;
+        if constexpr (!P16) pl[t][e >> 3][e & 7] = (_Float16)(p - (float)h);
       }
     }
 
@@ -349,7 +366,7 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
       // meet the zero weights of the rows that do not see them, and are added to the others' outputs one by one.
       u16x2 big{};
 #pragma unroll
-      for (int e = 0; e < 8; e++)
+      for (int e = 0; e < NP; e++)
 #pragma unroll
         for (int z = 0; z < Z; z++) {
           if (e >= left) vw[e][z] = u32x2{};
@@ -359,7 +376,7 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
         }
       if (KIND == 2 && __any(big[0] >= 0x7c00 || big[1] >= 0x7c00)) {
 #pragma unroll
-        for (int e = 0; e < 8; e++)
+        for (int e = 0; e < NP; e++)
 #pragma unroll
           for (int z = 0; z < Z; z++) vw[e][z] = u32x2{finite2(vw[e][z][0]), finite2(vw[e][z][1])};
 #pragma unroll 1
@@ -379,18 +396,21 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
       }
     }
 #pragma unroll
-    for (int x = 0; x < 4 * Z; x++) {
-      u32x4 w;
+    for (int x = 0; x < 4 * Z; x++)
 #pragma unroll
-      for (int y = 0; y < 4; y++)
-        w[y] = __builtin_amdgcn_perm(vw[2 * y + 1][x / 4][x % 4 / 2], vw[2 * y][x / 4][x % 4 / 2], x & 1 ? 0x07060302u : 0x05040100u);
-      const half8 vf = __builtin_bit_cast(half8, w);
+      for (int kk = 0; kk < KK; kk++) {
+        u32x4 w;
 #pragma unroll
-      for (int t = 0; t < QT; t++) {
-        acc[t][x] = mfma(vf, ph[t], acc[t][x]);
-        if constexpr (!P16) acc[t][x] = mfma(vf, pl[t], acc[t][x]);
+        for (int y = 0; y < 4; y++)
+          w[y] = __builtin_amdgcn_perm(vw[8 * kk + 2 * y + 1][x / 4][x % 4 / 2], vw[8 * kk + 2 * y][x / 4][x % 4 / 2],
+                                       x & 1 ? 0x07060302u : 0x05040100u);
+        const half8 vf = __builtin_bit_cast(half8, w);
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+          acc[t][x] = mfma(vf, ph[t][kk], acc[t][x]);
+          if constexpr (!P16) acc[t][x] = mfma(vf, pl[t][kk], acc[t][x]);
+        }
       }
-    }
     if constexpr (KIND == 0) load_v(blk + a.kw);
   };
   bool loaded = true;
@@ -519,7 +539,9 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 4 : 3) void attend_rows_kernel(Att
   for (int t = 0; t < QT; t++) {
     const int row = min(r0 + 16 * t + m, total - 1);
     node[t] = node_of(row, group);
-    cf[t] = query<T, C>((const T *)a.q + (row0 + node[t]) * a.stride + (size_t)(kh * group + head_of(row, group)) * a.hd, g, a.hd, a.scale, q[t]);
+    float f[C][8];
+    load_query<T, C>((const T *)a.q + (row0 + node[t]) * a.stride + (size_t)(kh * group + head_of(row, group)) * a.hd, g, a.hd, f);
+    cf[t] = split_query(f, a.scale, q[t]);
     mx[t] = -INFINITY, sum[t] = 0.0f;
 #pragma unroll
     for (int x = 0; x < X; x++) acc[t][x] = floatx4{};
@@ -860,7 +882,7 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
     return wh_fail(ctx, WH_EARG, "tree attention: buffers and rows must be 4-byte aligned");
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "tree attention: %s", hipGetErrorString(e));
   AttendArgs a{q, k, v, stride, kv, kv_stride, o, t->n, t->count, t->mask, t->mask_stride, t->batch, t->rows, (t->rows + 31) / 32,
-               cols, heads, kv_heads, hd, 1.0f / sqrtf((float)hd), 1, 1, 1, KB, nullptr, nullptr};
+               cols, heads, kv_heads, hd, 1.0f / sqrtf((float)hd), 1, 1, 1, few_block(hd), nullptr, nullptr};
   const int rows = t->rows * (heads / kv_heads), tiles = (rows + 15) / 16;
   const int most = hd <= 64 ? 2 : 1;  // tiles of attend_kernel
   const int waves = tiles > most && hd >= 8 && cols >= 4 ? tiles <= 4 ? 4 : 8 : 0, qt = std::min(tiles, most);
