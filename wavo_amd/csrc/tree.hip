@@ -31,7 +31,7 @@ struct AttendArgs {
   size_t mask_stride;
   int batch, rows, words, cols, heads, kv_heads, hd;
   float scale;
-  int kw, splits, row_blocks, block;  // (block: keys per block)
+  int kw, splits, row_blocks, block, node_block;  // (positions per block of the cache and of the nodes)
   // splits > 1: unnormalized outputs [split][batch * rows][heads][hd] and (maximum, sum, factor of the maximum's
   // exponent, -) [split][batch * rows][heads] of the splits that are used.
   float *po, *pml;
@@ -40,7 +40,8 @@ struct AttendArgs {
 
 constexpr int WAVES = 8;  // wavefronts of a workgroup, at most
 
-constexpr int few_block(int hd) { return hd <= 64 ? 64 : 32; }   // positions of a block of attend_kernel
+constexpr int few_block(int hd) { return hd <= 64 ? 64 : 32; }   // positions of a block of attend_kernel's
+constexpr int NODES = 32;                                         // (of its nodes: this many)
 constexpr int rows_block(int hd) { return hd <= 64 ? 64 : 32; }  // and of attend_rows_kernel
 
 // The blocks of keys of a sequence (the cache's, then the nodes'), and how its `splits` workgroups share them:
@@ -53,7 +54,7 @@ __device__ __forceinline__ Share share_of(const AttendArgs &a, int b) {
   s.n = min(max(a.n[b], 0), a.cols);
   s.count = a.count ? min(max(a.count[b], 0), a.rows) : a.rows;
   s.cached = (s.n + a.block - 1) / a.block;
-  s.blocks = s.cached + (a.mask && a.k ? (s.count + a.block - 1) / a.block : 0);
+  s.blocks = s.cached + (a.mask && a.k ? (s.count + a.node_block - 1) / a.node_block : 0);
   s.per = s.blocks, s.used = 1;
   if (a.splits > 1) {
     s.per = max((s.blocks + a.splits - 1) / a.splits, a.kw);
@@ -75,17 +76,26 @@ __device__ bool sees_any(const AttendArgs &a, const Share &s, int b, int i) {
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)lo) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)hi) << 16;
 }
-// Four values of a row as f16 pairs.
-__device__ __forceinline__ u32x2 four(const float *p) {
-  const floatx4 x = *(const floatx4_a4 *)p;
-  return u32x2{pack2(x[0], x[1]), pack2(x[2], x[3])};
-}
-__device__ __forceinline__ u32x2 four(const _Float16 *p) { return *(const u32x2_a4 *)p; }
+// Four values of a row as they stand, and as f16 pairs.
+template <typename T>
+struct Four {
+  typedef floatx4 type;
+};
+template <>
+struct Four<_Float16> {
+  typedef u32x2 type;
+};
+__device__ __forceinline__ floatx4 raw4(const float *p) { return *(const floatx4_a4 *)p; }
+__device__ __forceinline__ u32x2 raw4(const _Float16 *p) { return *(const u32x2_a4 *)p; }
+__device__ __forceinline__ u32x2 pairs4(floatx4 x) { return u32x2{pack2(x[0], x[1]), pack2(x[2], x[3])}; }
+__device__ __forceinline__ u32x2 pairs4(u32x2 x) { return x; }
+template <typename T>
+__device__ __forceinline__ u32x2 four(const T *p) { return pairs4(raw4(p)); }
 // And in f32.
-__device__ __forceinline__ void values(const float *p, float *f) { *(floatx4 *)f = *(const floatx4_a4 *)p; }
+__device__ __forceinline__ void values(const float *p, float *f) { *(floatx4 *)f = raw4(p); }
 __device__ __forceinline__ void values(const _Float16 *p, float *f) {
   typedef _Float16 half4 __attribute__((ext_vector_type(4)));
-  const half4 h = __builtin_bit_cast(half4, four(p));
+  const half4 h = __builtin_bit_cast(half4, raw4(p));
 #pragma unroll
   for (int e = 0; e < 4; e++) f[e] = (float)h[e];
 }
@@ -170,7 +180,7 @@ __device__ __forceinline__ float split_query(const float (&f)[C][8], float scale
 
 // Attention over a run of key blocks, for few rows.  A workgroup takes one key head of a sequence, 16 * QT of its rows
 // (the heads / kv_heads query heads of a node are rows next to each other) and one split of its key blocks
-// (64 positions for heads of up to 64 values, 32 for larger ones), of which each of its kw wavefronts takes every
+// (64 positions for heads of up to 64 values, 32 for larger ones and of nodes), of which each of its kw wavefronts takes every
 // kw-th.  A wavefront reads a block's K and V straight into the registers that the matrix cores take:
 //
 //   Scores transposed, S^T = K Q^T (v_mfma_f32_16x16x32_f16).  The cache holds K as pairs of values, position by
@@ -190,8 +200,8 @@ __device__ __forceinline__ float split_query(const float (&f)[C][8], float scale
 template <typename T, int HD, int QT, bool P16>
 __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
   constexpr int C = HD / 32, Z = HD / 64, QP = sizeof(T) == 4 ? 2 : 1;
-  constexpr int KP = few_block(HD) / 16, NP = 4 * KP, KB = 16 * KP, KK = KP / 2;
-  typedef uint32_t Words __attribute__((ext_vector_type(KP)));
+  constexpr int KPC = few_block(HD) / 16, KB = 16 * KPC;
+  typedef uint32_t Words __attribute__((ext_vector_type(KPC)));
   typedef Words Words_a4 __attribute__((aligned(4)));
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int lane = threadIdx.x & 63, ki = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -215,13 +225,13 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
   const uint32_t *vc = a.kv + (size_t)b * a.kv_stride + (size_t)half * a.cols + kh * pairs;
 
   Words kw[C][4];
-  u32x2 vw[NP][Z];  // a block's K, pair by pair, and V, position by position
+  u32x2 vw[4 * KPC][Z];  // a block's K, pair by pair, and V, position by position
   // The same loads on every way through, so that a wait for one block's does not have to be one for the next block's.
   auto load_k = [&](int blk) {
     // (made anew for every block: what follows from them would otherwise be kept in more registers than there are)
     int hd = a.hd, cols = a.cols;
     asm volatile("" : "+s"(hd), "+s"(cols));
-    const int j0 = blk * KB, last = s.n - 1 - j0, jk = min(KP * m, last & ~(KP - 1));  // (a position past the row's end: the next row, or V)
+    const int j0 = blk * KB, last = s.n - 1 - j0, jk = min(KPC * m, last & ~(KPC - 1));  // (a position past the row's end: the next row, or V)
 #pragma unroll
     for (int c = 0; c < C; c++) {
       const uint32_t *base = kc + (size_t)(16 * c) * cols + j0;
@@ -242,36 +252,55 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
     const int j0 = blk * KB, last = s.n - 1 - j0;
     const uint32_t *base = vc + (size_t)j0 * half;
 #pragma unroll
-    for (int e = 0; e < NP; e++)
+    for (int e = 0; e < 4 * KPC; e++)
 #pragma unroll
       for (int z = 0; z < Z; z++)
-        vw[e][z] = *(const u32x2_a4 *)(base + (uint32_t)(min(NP * g + e, last) * half + (64 * z + 4 * m < a.hd ? 32 * z + 2 * m : 0)));
+        vw[e][z] = *(const u32x2_a4 *)(base + (uint32_t)(min(4 * KPC * g + e, last) * half + (64 * z + 4 * m < a.hd ? 32 * z + 2 * m : 0)));
   };
   auto load_nodes = [&](int blk) {
-    const int j0 = (blk - s.cached) * KB, last = s.count - 1 - j0;
+    const int j0 = (blk - s.cached) * NODES, last = s.count - 1 - j0;
     const T *k = (const T *)a.k + (row0 + j0) * a.stride + (size_t)kh * a.hd;
     const T *v = (const T *)a.v + (row0 + j0) * a.stride + (size_t)kh * a.hd;
+    // (every row's loads before the first one is rounded; larger heads' K first and then V, for want of registers)
+    typename Four<T>::type rk[C][2][2], rv[8][Z];
+    auto round_k = [&] {
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int c = 0; c < C; c++)
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int y = 0; y < 2; y++) {
+            const u32x2 w = 32 * c + 8 * g + 4 * y < a.hd ? pairs4(rk[c][u][y]) : u32x2{};
+            kw[c][2 * y][u] = w[0], kw[c][2 * y + 1][u] = w[1];
+          }
+    };
 #pragma unroll
     for (int c = 0; c < C; c++)
 #pragma unroll
-      for (int u = 0; u < KP; u++) {
-        const T *src = k + (uint32_t)min(KP * m + u, last) * (uint32_t)a.stride;
-        const int d = 32 * c + 8 * g;
-        u32x2 lo = four(src + (d < a.hd ? d : 0)), hi = four(src + (d + 4 < a.hd ? d + 4 : 0));
-        if (d >= a.hd) lo = u32x2{};
-        if (d + 4 >= a.hd) hi = u32x2{};
-        kw[c][0][u] = lo[0], kw[c][1][u] = lo[1], kw[c][2][u] = hi[0], kw[c][3][u] = hi[1];
-      }
+      for (int u = 0; u < 2; u++)
 #pragma unroll
-    for (int e = 0; e < NP; e++)
+        for (int y = 0; y < 2; y++) {
+          const int d = 32 * c + 8 * g + 4 * y;
+          rk[c][u][y] = raw4(k + (uint32_t)min(2 * m + u, last) * (uint32_t)a.stride + (d < a.hd ? d : 0));
+        }
+    if constexpr (Z == 2) round_k();
+#pragma unroll
+    for (int e = 0; e < 8; e++)
 #pragma unroll
       for (int z = 0; z < Z; z++)
-        vw[e][z] = four(v + (uint32_t)min(NP * g + e, last) * (uint32_t)a.stride + (64 * z + 4 * m < a.hd ? 64 * z + 4 * m : 0));
+        rv[e][z] = raw4(v + (uint32_t)min(8 * g + e, last) * (uint32_t)a.stride + (64 * z + 4 * m < a.hd ? 64 * z + 4 * m : 0));
+    if constexpr (Z == 1) round_k();
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+#pragma unroll
+      for (int z = 0; z < Z; z++) vw[e][z] = pairs4(rv[e][z]);
   };
   int blk = split * s.per + ki;
   const int end = min((split + 1) * s.per, s.blocks), cached = min(end, s.cached);
   if (blk < cached) {
-    if (a.cols >= KP) {
+    if (a.cols >= KPC) {
       load_k(blk);
     } else {  // (a cache of so few positions: nothing behind them)
 #pragma unroll
@@ -279,7 +308,7 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
 #pragma unroll
         for (int x = 0; x < 4; x++)
 #pragma unroll
-          for (int u = 0; u < KP; u++) {
+          for (int u = 0; u < KPC; u++) {
             const int p = 16 * c + 4 * g + x;
             kw[c][x][u] = p < pairs ? kc[p * a.cols + min(u, a.cols - 1)] : 0u;
           }
@@ -303,7 +332,8 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
   auto step = [&](auto which) {
     constexpr int KIND = which;
     constexpr bool all = KIND == 0;
-    const int j0 = (KIND == 2 ? blk - s.cached : blk) * KB, last = (KIND == 2 ? s.count : s.n) - 1 - j0;
+    constexpr int KP = KIND == 2 ? 2 : KPC, NP = 4 * KP, KK = KP / 2;
+    const int j0 = KIND == 2 ? (blk - s.cached) * NODES : blk * KB, last = (KIND == 2 ? s.count : s.n) - 1 - j0;
     const int left = last + 1 - NP * g;  // of this lane's positions
     floatx4 st[QT][KP];
 #pragma unroll
@@ -380,7 +410,7 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
 #pragma unroll
           for (int z = 0; z < Z; z++) vw[e][z] = u32x2{finite2(vw[e][z][0]), finite2(vw[e][z][1])};
 #pragma unroll 1
-        for (int j = 0; j < min(KB, last + 1); j++) {
+        for (int j = 0; j < min(NODES, last + 1); j++) {
           int hd = a.hd;
           asm volatile("" : "+s"(hd));  // (nothing of this loop is worth a register outside)
           const T *v = (const T *)a.v + (row0 + j0 + j) * a.stride + (size_t)kh * a.hd;
@@ -882,17 +912,17 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
     return wh_fail(ctx, WH_EARG, "tree attention: buffers and rows must be 4-byte aligned");
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "tree attention: %s", hipGetErrorString(e));
   AttendArgs a{q, k, v, stride, kv, kv_stride, o, t->n, t->count, t->mask, t->mask_stride, t->batch, t->rows, (t->rows + 31) / 32,
-               cols, heads, kv_heads, hd, 1.0f / sqrtf((float)hd), 1, 1, 1, few_block(hd), nullptr, nullptr};
+               cols, heads, kv_heads, hd, 1.0f / sqrtf((float)hd), 1, 1, 1, few_block(hd), NODES, nullptr, nullptr};
   const int rows = t->rows * (heads / kv_heads), tiles = (rows + 15) / 16;
   const int most = hd <= 64 ? 2 : 1;  // tiles of attend_kernel
   const int waves = tiles > most && hd >= 8 && cols >= 4 ? tiles <= 4 ? 4 : 8 : 0, qt = std::min(tiles, most);
-  if (waves) a.block = rows_block(hd);
-  const int blocks = (cols + a.block - 1) / a.block + (t->mask && k ? (t->rows + a.block - 1) / a.block : 0);
+  if (waves) a.block = a.node_block = rows_block(hd);
+  const int blocks = (cols + a.block - 1) / a.block + (t->mask && k ? (t->rows + a.node_block - 1) / a.node_block : 0);
   a.row_blocks = (tiles + (waves ? waves : qt) - 1) / (waves ? waves : qt);
   a.kw = waves ? 1 : std::min(WAVES, blocks);
   const size_t units = (size_t)t->batch * kv_heads * a.row_blocks;
   const size_t cus = ctx->cus > 0 ? ctx->cus : 256;
-  const int least = waves ? 8 : 2 * a.kw;  // blocks of a split
+  const int least = waves ? 8 : 4 * a.kw;  // blocks of a split
   a.splits = (int)std::max<size_t>(1, std::min<size_t>(((waves ? 2 : 1) * cus + units - 1) / units, (blocks + least - 1) / least));
   const size_t nodes = (size_t)t->batch * t->rows;
   if (units * a.splits >= (size_t)1 << 22 || nodes * heads >= (size_t)1 << 25)  // (a launch's threads fit 32 bits)
