@@ -505,29 +505,32 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
   }
 }
 
-// The same for more rows than two tiles of one key head: every wavefront takes 16 * QT rows, and all of them go
-// through the same key blocks (64 positions for heads of up to 64 values, 32 for larger ones: 16 KiB) one after
-// the other.  The workgroup's threads load a block two blocks ahead, each its share of 16-byte pieces, and write
-// it to one of two LDS buffers, from which the wavefronts read operands as they stand: a pair's position from
-// each of 4 rows of K (rows 4 words longer than a block, so that the 4 lane groups hit distinct banks), and V
-// transposed by ds_read_b64_tr_b16 (rows 32 bytes longer, for the same reason).  Tile u's row r is position
-// 16u + r, so lane 16g + i's scores are those of positions 16u + 4g + 0 .. 3 of every u.
-template <typename T, int HD, int QT, int W, bool P16>
-__global__ __launch_bounds__(64 * W, W == 8 ? 4 : 3) void attend_rows_kernel(AttendArgs a) {
+// The same for more rows of a key head: a workgroup's 8 wavefronts are KG groups of RT with 16 rows each, and a group
+// goes through every KG-th key block (64 positions for heads of up to 64 values, 32 for larger ones: 16 KiB), one
+// after the other.  Its threads load a block two blocks ahead, each its share of 16-byte pieces, and write it to
+// one of two LDS buffers, from which its wavefronts read operands as they stand: a pair's position from each of 4
+// rows of K (rows 4 words longer than a block, so that the 4 lane groups hit distinct banks), and V transposed by
+// ds_read_b64_tr_b16 (rows 32 bytes longer, for the same reason).  Tile u's row r is position 16u + r, so lane
+// 16g + i's scores are those of positions 16u + 4g + 0 .. 3 of every u.  128 registers, so that two workgroups
+// share a CU.
+template <typename T, int HD, int RT, bool P16>
+__global__ __launch_bounds__(64 * WAVES, 4) void attend_rows_kernel(AttendArgs a) {
+  constexpr int KG = WAVES / RT, QT = 1;
   constexpr int C = HD / 32, X = HD / 16, QP = sizeof(T) == 4 ? 2 : 1, B = rows_block(HD), NT = B / 16, KK = B / 32;
   constexpr int KS = B + 4, VS = HD / 2 + 8;  // words per row of K and of V in LDS
   constexpr int KW = KS * HD / 2, BUF = KW + VS * B, U = 512;  // words of K and of a buffer; 16-byte pieces of K or V
   extern __shared__ __attribute__((aligned(16))) uint32_t words[];
-  __shared__ int odd;  // set where a node's value is no finite number
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, m = lane & 15;
-  constexpr int threads = 64 * W, MOST = U / threads;  // MOST: pieces per thread
+  __shared__ int odd[KG];  // set where a node's value is no finite number
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, m = lane & 15;
+  const int kg = wave / RT, tid = threadIdx.x - 64 * RT * kg;
+  constexpr int threads = 64 * RT, MOST = U / threads;  // MOST: pieces per thread
   const int split = blockIdx.z, kh = blockIdx.y, b = a.row_blocks == 1 ? blockIdx.x : blockIdx.x / a.row_blocks;
   const int rb = blockIdx.x - b * a.row_blocks;
-  const int group = a.heads / a.kv_heads, r0 = 16 * QT * (rb * W + wave);
+  const int group = a.heads / a.kv_heads, r0 = 16 * (rb * RT + wave % RT);
   const size_t row0 = (size_t)b * a.rows;
   const Share s = share_of(a, b);
   const int total = s.count * group;
-  if (split >= s.used || 16 * QT * W * rb >= total) return;
+  if (split >= s.used || 16 * RT * rb >= total) return;
   const int half = a.kv_heads * a.hd / 2, pairs = a.hd / 2;
   const uint32_t *kc = a.kv + (size_t)b * a.kv_stride + (size_t)kh * pairs * a.cols;
   const uint32_t *vc = a.kv + (size_t)b * a.kv_stride + (size_t)half * a.cols + kh * pairs;
@@ -558,8 +561,9 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 4 : 3) void attend_rows_kernel(Att
     }
   };
   Pieces p0, p1;
-  if (begin < cached) load(p0, begin);
-  if (begin + 1 < cached) load(p1, begin + 1);
+  int blk = begin + kg;
+  if (blk < cached) load(p0, blk);
+  if (blk + KG < cached) load(p1, blk + KG);
 
   half8 q[QT][C][QP];
   floatx4 acc[QT][X];
@@ -650,7 +654,7 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 4 : 3) void attend_rows_kernel(Att
           if constexpr (!P16) acc[t][x] = mfma(vf, pl[t][kk], acc[t][x]);
         }
       }
-    if (NODES && odd)  // what the block has zeros for, to the rows that see it
+    if (NODES && odd[kg])  // what the block has zeros for, to the rows that see it
 #pragma unroll 1
       for (int j = 0; j < min(B, last + 1); j++) {
         int hd = a.hd;
@@ -667,66 +671,90 @@ __global__ __launch_bounds__(64 * W, W == 8 ? 4 : 3) void attend_rows_kernel(Att
       }
   };
 
-  // Blocks begin, begin + 2, .. pass through p0 and the first buffer, the others through p1 and the second.  A buffer is
-  // written again two blocks later, past the barrier that every wavefront reaches after it has read it.
-  uint32_t *const buf0 = words, *const buf1 = words + BUF;
-  int blk = begin;
-  for (; blk + 3 < cached; blk += 2) {
+  // A group's blocks pass in turn through p0 and its first buffer and through p1 and the second.  A buffer is written
+  // again two blocks later, past the barrier that every wavefront reaches after it has read it.  The groups have
+  // as many barriers each: as long as all of them have four more blocks, and then as many as the first one.
+  uint32_t *const buf0 = words + 2 * BUF * kg, *const buf1 = buf0 + BUF;
+  for (; blk - kg + 4 * KG <= cached; blk += 2 * KG) {
     store(p0, blk, buf0);
-    load(p0, blk + 2);
+    load(p0, blk + 2 * KG);
     meet();
     if (busy) step(std::false_type{}, blk, buf0);
-    store(p1, blk + 1, buf1);
-    load(p1, blk + 3);
+    store(p1, blk + KG, buf1);
+    load(p1, blk + 3 * KG);
     meet();
-    if (busy) step(std::false_type{}, blk + 1, buf1);
+    if (busy) step(std::false_type{}, blk + KG, buf1);
   }
-  for (; blk < cached; blk++) {  // (at most three)
-    const bool even = (blk - begin) % 2 == 0;
-    if (even) store(p0, blk, buf0);
-    else store(p1, blk, buf1);
-    if (even && blk + 2 < cached) load(p0, blk + 2);
+  for (bool even = true; blk - kg < cached; blk += KG, even = !even) {
+    const bool mine = blk < cached, next = blk + 2 * KG < cached;
+    if (even) {
+      if (mine) store(p0, blk, buf0);
+      if (next) load(p0, blk + 2 * KG);
+    } else {
+      if (mine) store(p1, blk, buf1);
+      if (next) load(p1, blk + 2 * KG);
+    }
     meet();
-    if (busy) step(std::false_type{}, blk, even ? buf0 : buf1);
+    if (busy && mine) step(std::false_type{}, blk, even ? buf0 : buf1);
   }
-  for (; blk < end; blk++) {
-    uint32_t *buf = (blk - begin) % 2 ? buf1 : buf0;
+  for (blk = max(begin, s.cached) + kg; blk - kg < end; blk += KG) {
     const int j0 = (blk - s.cached) * B, last = s.count - 1 - j0;
     __syncthreads();
-    if (tid == 0) odd = 0;
+    if (tid == 0) odd[kg] = 0;
     __syncthreads();
     bool found = false;
+    if (blk < end)
 #pragma unroll 1
-    for (int u = tid; u < U; u += threads) {
-      const int row = u % B, d = u / B * 8;
-      const size_t src = (row0 + j0 + min(row, last)) * a.stride + (size_t)kh * a.hd;
-      u32x2 k[2], v[2];
+      for (int u = tid; u < U; u += threads) {
+        const int row = u % B, d = u / B * 8;
+        const size_t src = (row0 + j0 + min(row, last)) * a.stride + (size_t)kh * a.hd;
+        u32x2 k[2], v[2];
 #pragma unroll
-      for (int y = 0; y < 2; y++) {
-        const bool in = d + 4 * y < a.hd;
-        k[y] = four((const T *)a.k + src + (in ? d + 4 * y : 0)), v[y] = four((const T *)a.v + src + (in ? d + 4 * y : 0));
-        if (!in) k[y] = u32x2{};
-        if (!in || row > last) v[y] = u32x2{};
+        for (int y = 0; y < 2; y++) {
+          const bool in = d + 4 * y < a.hd;
+          k[y] = four((const T *)a.k + src + (in ? d + 4 * y : 0)), v[y] = four((const T *)a.v + src + (in ? d + 4 * y : 0));
+          if (!in) k[y] = u32x2{};
+          if (!in || row > last) v[y] = u32x2{};
 #pragma unroll
-        for (int w = 0; w < 2; w++) {
-          buf[(d / 2 + 2 * y + w) * KS + row] = k[y][w];
-          const uint32_t clean = finite2(v[y][w]);
-          found |= clean != v[y][w];
-          v[y][w] = clean;
+          for (int w = 0; w < 2; w++) {
+            buf0[(d / 2 + 2 * y + w) * KS + row] = k[y][w];
+            const uint32_t clean = finite2(v[y][w]);
+            found |= clean != v[y][w];
+            v[y][w] = clean;
+          }
         }
+        *(u32x4 *)(buf0 + KW + row * VS + d / 2) = u32x4{v[0][0], v[0][1], v[1][0], v[1][1]};
       }
-      *(u32x4 *)(buf + KW + row * VS + d / 2) = u32x4{v[0][0], v[0][1], v[1][0], v[1][1]};
-    }
-    if (found) odd = 1;
+    if (found) odd[kg] = 1;
     __syncthreads();
-    if (busy) step(std::true_type{}, blk, buf);
+    if (busy && blk < end) step(std::true_type{}, blk, buf0);
   }
 
+  // The groups' results joined by the first one, through LDS.
+  sum[0] = xlane::bit4(sum[0], xlane::Add{});
+  sum[0] = xlane::bit5(sum[0], xlane::Add{});
+  if constexpr (KG > 1) {
+    static_assert(KG == 2);
+    floatx4 *slot = (floatx4 *)words + (wave % RT) * (X * 64 + 32);
+    float *ml = (float *)(slot + X * 64);
+    __syncthreads();
+    if (kg) {
+#pragma unroll
+      for (int x = 0; x < X; x++) slot[64 * x + lane] = acc[0][x];
+      ml[lane] = mx[0], ml[64 + lane] = sum[0];
+    }
+    __syncthreads();
+    if (kg) return;
+    const float om = ml[lane], os = ml[64 + lane], top = fmaxf(mx[0], om);
+    const float f = mx[0] == top ? 1.0f : __builtin_amdgcn_exp2f((mx[0] - top) * cf[0]);
+    const float of = om == top ? 1.0f : __builtin_amdgcn_exp2f((om - top) * cf[0]);
+    sum[0] = sum[0] * f + os * of, mx[0] = top;
+#pragma unroll
+    for (int x = 0; x < X; x++) acc[0][x] = acc[0][x] * f + slot[64 * x + lane] * of;
+  }
   // Lane 16g + i holds row i's values 16x + 4g + 0 .. 3.
 #pragma unroll
   for (int t = 0; t < QT; t++) {
-    sum[t] = xlane::bit4(sum[t], xlane::Add{});
-    sum[t] = xlane::bit5(sum[t], xlane::Add{});
     const int r = r0 + 16 * t + m;
     if (r >= total) continue;
     const int i = node[t], head = kh * group + head_of(r, group);
@@ -864,21 +892,21 @@ int attend_join(wh_ctx *ctx, const AttendArgs &a) {
   return wh_launched(ctx, "tree attention's join");
 }
 
-template <typename T, int HD, int W, bool P16>
+template <typename T, int HD, int RT, bool P16>
 int attend_rows_launch(wh_ctx *ctx, const AttendArgs &a) {
   constexpr int B = rows_block(HD);
   ProfScope prof(ctx, "tree_attend_rows", 4.0 * a.batch * a.rows * a.heads * a.cols * a.hd, 4.0 * a.batch * a.cols * a.kv_heads * a.hd);
-  wh_launch(ctx, (attend_rows_kernel<T, HD, 1, W, P16>), dim3(a.batch * a.row_blocks, a.kv_heads, a.splits), 64 * W,
-            2 * 4 * ((B + 4) * HD / 2 + (HD / 2 + 8) * B), a);
+  wh_launch(ctx, (attend_rows_kernel<T, HD, RT, P16>), dim3(a.batch * a.row_blocks, a.kv_heads, a.splits), 64 * WAVES,
+            WAVES / RT * 2 * 4 * ((B + 4) * HD / 2 + (HD / 2 + 8) * B), a);
   return wh_launched(ctx, "tree attention");
 }
 
-// waves: of attend_rows_kernel's workgroups, or 0: attend_kernel with qt tiles of rows.
+// rt: row tiles of attend_rows_kernel's workgroups, or 0: attend_kernel with qt tiles of rows.
 template <typename T, bool P16>
-int attend_t(wh_ctx *ctx, const AttendArgs &a, int qt, int waves) {
+int attend_t(wh_ctx *ctx, const AttendArgs &a, int qt, int rt) {
   int rc;
-  if (waves && a.hd <= 64) rc = waves == 4 ? attend_rows_launch<T, 64, 4, P16>(ctx, a) : attend_rows_launch<T, 64, 8, P16>(ctx, a);
-  else if (waves) rc = waves == 4 ? attend_rows_launch<T, 128, 4, P16>(ctx, a) : attend_rows_launch<T, 128, 8, P16>(ctx, a);
+  if (rt && a.hd <= 64) rc = rt == 4 ? attend_rows_launch<T, 64, 4, P16>(ctx, a) : attend_rows_launch<T, 64, 8, P16>(ctx, a);
+  else if (rt) rc = rt == 4 ? attend_rows_launch<T, 128, 4, P16>(ctx, a) : attend_rows_launch<T, 128, 8, P16>(ctx, a);
   else if (a.hd <= 64) rc = qt == 1 ? attend_launch<T, 64, 1, P16>(ctx, a) : attend_launch<T, 64, 2, P16>(ctx, a);
   else rc = attend_launch<T, 128, 1, P16>(ctx, a);
   return rc || a.splits == 1 ? rc : attend_join<P16>(ctx, a);
@@ -915,15 +943,15 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
                cols, heads, kv_heads, hd, 1.0f / sqrtf((float)hd), 1, 1, 1, few_block(hd), NODES, nullptr, nullptr};
   const int rows = t->rows * (heads / kv_heads), tiles = (rows + 15) / 16;
   const int most = hd <= 64 ? 2 : 1;  // tiles of attend_kernel
-  const int waves = tiles > most && hd >= 8 && cols >= 4 ? tiles <= 4 ? 4 : 8 : 0, qt = std::min(tiles, most);
-  if (waves) a.block = a.node_block = rows_block(hd);
+  const int rt = tiles > most && hd >= 8 && cols >= 4 ? tiles <= 4 ? 4 : 8 : 0, qt = std::min(tiles, most);
+  if (rt) a.block = a.node_block = rows_block(hd);
   const int blocks = (cols + a.block - 1) / a.block + (t->mask && k ? (t->rows + a.node_block - 1) / a.node_block : 0);
-  a.row_blocks = (tiles + (waves ? waves : qt) - 1) / (waves ? waves : qt);
-  a.kw = waves ? 1 : std::min(WAVES, blocks);
+  a.row_blocks = (tiles + (rt ? rt : qt) - 1) / (rt ? rt : qt);
+  a.kw = rt ? WAVES / rt : std::min(WAVES, blocks);
   const size_t units = (size_t)t->batch * kv_heads * a.row_blocks;
   const size_t cus = ctx->cus > 0 ? ctx->cus : 256;
-  const int least = waves ? 8 : 4 * a.kw;  // blocks of a split
-  a.splits = (int)std::max<size_t>(1, std::min<size_t>(((waves ? 2 : 1) * cus + units - 1) / units, (blocks + least - 1) / least));
+  const int least = (rt ? 8 : 4) * a.kw;  // blocks of a split
+  a.splits = (int)std::max<size_t>(1, std::min<size_t>(((rt ? 2 : 1) * cus + units - 1) / units, (blocks + least - 1) / least));
   const size_t nodes = (size_t)t->batch * t->rows;
   if (units * a.splits >= (size_t)1 << 22 || nodes * heads >= (size_t)1 << 25)  // (a launch's threads fit 32 bits)
     return wh_fail(ctx, WH_EARG, "tree attention: %d heads of %zu nodes in one call", heads, nodes);
@@ -932,8 +960,8 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
     if (!(a.po = (float *)wh_scratch(ctx, part * (hd + 4) * sizeof(float)))) return WH_EOOM;
     a.pml = a.po + part * hd;
   }
-  return in16 ? out16 ? attend_t<_Float16, true>(ctx, a, qt, waves) : attend_t<_Float16, false>(ctx, a, qt, waves)
-              : out16 ? attend_t<float, true>(ctx, a, qt, waves) : attend_t<float, false>(ctx, a, qt, waves);
+  return in16 ? out16 ? attend_t<_Float16, true>(ctx, a, qt, rt) : attend_t<_Float16, false>(ctx, a, qt, rt)
+              : out16 ? attend_t<float, true>(ctx, a, qt, rt) : attend_t<float, false>(ctx, a, qt, rt);
 }
 
 int launch_tree_accept(wh_ctx *ctx, const wh_tree *t, const uint32_t *picks, const wh_kept *w, int cols, int32_t *path,
