@@ -385,7 +385,7 @@ typedef struct wh_tree {
  * positions of kv_heads * hd values each, kv_stride words apart (0: one cache for all).  o:
  * [batch * rows][heads * hd], f32 or (out16) f16.  Products of f32 queries and of the f32 softmax keep
  * their precision (each is split into two f16 parts); f16 queries are exact, and with out16 the softmax
- * weights are rounded to f16.  Masked keys and values may hold anything.  hd % 4 == 0, hd <= 128,
+ * weights are rounded to f16.  Masked keys and values may hold anything.  hd % 4 == 0, hd <= 128, cols <= 2^24,
  * heads % kv_heads == 0; f32 pointers and f16 rows 4-byte aligned (stride even for f16). */
 int wh_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void *k, const void *v, size_t stride,
                    int in16, const uint32_t *kv, size_t kv_stride, int cols, void *o, int out16, int heads,

@@ -38,6 +38,7 @@ struct AttendArgs {
 };
 
 
+constexpr float SLACK = 4.0f;
 constexpr int WAVES = 8;  // wavefronts of a workgroup, at most
 
 constexpr int few_block(int hd) { return hd <= 64 ? 64 : 32; }   // positions of a block of attend_kernel's
@@ -195,8 +196,9 @@ __device__ __forceinline__ float split_query(const float (&f)[C][8], float scale
 // a wavefront always has loads in flight; the first block's before the queries are looked at.
 //
 // Precision: f32 queries are scaled by a power of two per row and split into two f16 parts, as is every
-// softmax weight for f32 outputs (weights are exp2(s - max + 10), so that the second part is no subnormal):
-// two products each, with an error of 2^-22 against f32's own 2^-24 per sum.  K and V are f16 as stored.
+// softmax weight for f32 outputs: two products each, with an error of 2^-22 against f32's own 2^-24 per sum.  Weights
+// are exp2(s - max + 10), so that the second part is no subnormal; a maximum that grows by less than SLACK binary
+// digits is left as it is, since they still fit f16 then.  K and V are f16 as stored.
 template <typename T, int HD, int QT, bool P16>
 __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
   constexpr int C = HD / 32, Z = HD / 64, QP = sizeof(T) == 4 ? 2 : 1;
@@ -206,8 +208,8 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int lane = threadIdx.x & 63, ki = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, m = lane & 15;
-  const int split = blockIdx.z, kh = blockIdx.y, b = a.row_blocks == 1 ? blockIdx.x : blockIdx.x / a.row_blocks;
-  const int group = a.heads / a.kv_heads, r0 = 16 * QT * (blockIdx.x - b * a.row_blocks);
+  const int split = blockIdx.z, kh = blockIdx.x, b = a.row_blocks == 1 ? blockIdx.y : blockIdx.y / a.row_blocks;
+  const int group = a.heads / a.kv_heads, r0 = 16 * QT * (blockIdx.y - b * a.row_blocks);
   const size_t row0 = (size_t)b * a.rows;
   float f[QT][C][8];
   int node[QT];
@@ -320,10 +322,10 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
 
   half8 q[QT][C][QP];
   floatx4 acc[QT][4 * Z];
-  float mx[QT], sum[QT], cf[QT];
+  float mx[QT], sum[QT], cf[QT], slack[QT];
 #pragma unroll
   for (int t = 0; t < QT; t++) {
-    cf[t] = split_query(f[t], a.scale, q[t]);
+    cf[t] = split_query(f[t], a.scale, q[t]), slack[t] = SLACK / cf[t];
     mx[t] = -INFINITY, sum[t] = 0.0f;
 #pragma unroll
     for (int x = 0; x < 4 * Z; x++) acc[t][x] = floatx4{};
@@ -372,15 +374,15 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
       for (int e = 1; e < NP; e++) top = fmaxf(top, st[t][e % KP][e / KP]);
       top = xlane::bit4(top, xlane::Max{});
       top = xlane::bit5(top, xlane::Max{});
-      top = fmaxf(top, mx[t]);
-      const float base = top == -INFINITY ? 0.0f : top;
-      if (__any(top != mx[t])) {
+      if (__any(top > mx[t] + slack[t])) {
+        top = fmaxf(top, mx[t]);
         const float old = mx[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mx[t] - top) * cf[t]);
         sum[t] *= old;
 #pragma unroll
         for (int x = 0; x < 4 * Z; x++) acc[t][x] *= old;
         mx[t] = top;
       }
+      const float base = mx[t] == -INFINITY ? 0.0f : mx[t];
 #pragma unroll
       for (int e = 0; e < NP; e++) {
         const float p = __builtin_amdgcn_exp2f(fmaf(st[t][e % KP][e / KP] - base, cf[t], 10.0f));
@@ -508,24 +510,23 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
 // The same for more rows of a key head: a workgroup's 8 wavefronts are KG groups of RT with 16 rows each, and a group
 // goes through every KG-th key block (64 positions for heads of up to 64 values, 32 for larger ones: 16 KiB), one
 // after the other.  Its threads load a block two blocks ahead, each its share of 16-byte pieces, and write it to
-// one of two LDS buffers, from which its wavefronts read operands as they stand: a pair's position from each of 4
-// rows of K (rows 4 words longer than a block, so that the 4 lane groups hit distinct banks), and V transposed by
-// ds_read_b64_tr_b16 (rows 32 bytes longer, for the same reason).  Tile u's row r is position 16u + r, so lane
+// one of two LDS buffers, K position by position too, from which its wavefronts read operands as they stand: 8 values
+// of a position of K, and V transposed by ds_read_b64_tr_b16 (rows 16 and 32 bytes longer, for the banks' sake).  Tile u's row r is position 16u + r, so lane
 // 16g + i's scores are those of positions 16u + 4g + 0 .. 3 of every u.  128 registers, so that two workgroups
 // share a CU.
 template <typename T, int HD, int RT, bool P16>
 __global__ __launch_bounds__(64 * WAVES, 4) void attend_rows_kernel(AttendArgs a) {
   constexpr int KG = WAVES / RT, QT = 1;
   constexpr int C = HD / 32, X = HD / 16, QP = sizeof(T) == 4 ? 2 : 1, B = rows_block(HD), NT = B / 16, KK = B / 32;
-  constexpr int KS = B + 4, VS = HD / 2 + 8;  // words per row of K and of V in LDS
-  constexpr int KW = KS * HD / 2, BUF = KW + VS * B, U = 512;  // words of K and of a buffer; 16-byte pieces of K or V
+  constexpr int KS = HD / 2 + 4, VS = HD / 2 + 8;  // words per position of K and of V in LDS
+  constexpr int KW = KS * B, BUF = KW + VS * B, U = 512;  // words of K and of a buffer; 16-byte pieces of K or V
   extern __shared__ __attribute__((aligned(16))) uint32_t words[];
   __shared__ int odd[KG];  // set where a node's value is no finite number
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, m = lane & 15;
   const int kg = wave / RT, tid = threadIdx.x - 64 * RT * kg;
   constexpr int threads = 64 * RT, MOST = U / threads;  // MOST: pieces per thread
-  const int split = blockIdx.z, kh = blockIdx.y, b = a.row_blocks == 1 ? blockIdx.x : blockIdx.x / a.row_blocks;
-  const int rb = blockIdx.x - b * a.row_blocks;
+  const int split = blockIdx.z, kh = blockIdx.x, b = a.row_blocks == 1 ? blockIdx.y : blockIdx.y / a.row_blocks;
+  const int rb = blockIdx.y - b * a.row_blocks;
   const int group = a.heads / a.kv_heads, r0 = 16 * (rb * RT + wave % RT);
   const size_t row0 = (size_t)b * a.rows;
   const Share s = share_of(a, b);
@@ -540,24 +541,40 @@ __global__ __launch_bounds__(64 * WAVES, 4) void attend_rows_kernel(AttendArgs a
   struct Pieces {
     u32x4 k[MOST], v[MOST];
   };
+  // Piece u of K: 4 positions from 4q on of a pair, 4 such next to each other in memory and 16 pairs per wavefront, so that
+  // a position's words go to different banks; of V: 8 values of a position.
+  uint32_t kat[MOST], vat[MOST];  // words from the block's first ones
+  int kq[MOST], kpair[MOST], vrow[MOST], vd[MOST];
+#pragma unroll
+  for (int i = 0; i < MOST; i++) {
+    const int u = tid + threads * i;
+    kq[i] = 4 * (u % 4 + 4 * (u / 64 % (B / 16))), kpair[i] = u % 64 / 4 + 16 * (u / 64 / (B / 16));
+    vrow[i] = u / (HD / 8), vd[i] = u % (HD / 8) * 4;
+    kat[i] = (uint32_t)min(kpair[i], pairs - 1) * (uint32_t)a.cols, vat[i] = (uint32_t)min(vd[i], pairs - 4);
+  }
   auto load = [&](Pieces &p, int blk) {
     const int j0 = blk * B, last = s.n - 1 - j0;
+    const bool inside = j0 + B <= a.cols;  // (positions past n are there to be read, at least)
+    const uint32_t *kb = kc + j0, *vb = vc + (size_t)j0 * half;
 #pragma unroll
     for (int i = 0; i < MOST; i++) {
-      const int u = tid + threads * i, pair = u / (B / 4), q = u % (B / 4), row = u / (HD / 8), d = u % (HD / 8) * 4;
-      p.k[i] = *(const u32x4_a4 *)(kc + (size_t)min(pair, pairs - 1) * a.cols + j0 + min(4 * q, last & ~3));
-      p.v[i] = *(const u32x4_a4 *)(vc + (size_t)j0 * half + (uint32_t)(min(row, last) * half + min(d, pairs - 4)));
+      p.k[i] = *(const u32x4_a4 *)(kb + (kat[i] + (inside ? kq[i] : min(kq[i], last & ~3))));
+      p.v[i] = *(const u32x4_a4 *)(vb + (vat[i] + (inside ? vrow[i] : min(vrow[i], last)) * half));
     }
   };
   auto store = [&](const Pieces &p, int blk, uint32_t *buf) {
     const int last = s.n - 1 - blk * B;
 #pragma unroll
     for (int i = 0; i < MOST; i++) {
-      const int u = tid + threads * i, pair = u / (B / 4), q = u % (B / 4), row = u / (HD / 8), d = u % (HD / 8) * 4;
-      *(u32x4 *)(buf + pair * KS + 4 * q) = pair < pairs ? p.k[i] : u32x4{};
-      // (a head's last 4 values are the upper half of the piece before its end)
-      const u32x4 v = d == pairs - 2 ? u32x4{p.v[i][2], p.v[i][3], 0, 0} : p.v[i];
-      *(u32x4 *)(buf + KW + row * VS + d) = row <= last ? v : u32x4{};
+      u32x4 k = p.k[i], v = p.v[i];
+      if (a.hd < HD) {  // (a head's last 4 values can be the upper half of the piece before its end)
+        if (kpair[i] >= pairs) k = u32x4{};
+        if (vd[i] == pairs - 2) v = u32x4{v[2], v[3], 0, 0};
+      }
+      if (last < B - 1 && vrow[i] > last) v = u32x4{};
+#pragma unroll
+      for (int e = 0; e < 4; e++) buf[(kq[i] + e) * KS + kpair[i]] = k[e];
+      *(u32x4 *)(buf + KW + vrow[i] * VS + vd[i]) = v;
     }
   };
   Pieces p0, p1;
@@ -567,7 +584,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void attend_rows_kernel(AttendArgs a
 
   half8 q[QT][C][QP];
   floatx4 acc[QT][X];
-  float mx[QT], sum[QT], cf[QT];
+  float mx[QT], sum[QT], cf[QT], slack[QT];
   int node[QT];
 #pragma unroll
   for (int t = 0; t < QT; t++) {
@@ -575,7 +592,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void attend_rows_kernel(AttendArgs a
     node[t] = node_of(row, group);
     float f[C][8];
     load_query<T, C>((const T *)a.q + (row0 + node[t]) * a.stride + (size_t)(kh * group + head_of(row, group)) * a.hd, g, a.hd, f);
-    cf[t] = split_query(f, a.scale, q[t]);
+    cf[t] = split_query(f, a.scale, q[t]), slack[t] = SLACK / cf[t];
     mx[t] = -INFINITY, sum[t] = 0.0f;
 #pragma unroll
     for (int x = 0; x < X; x++) acc[t][x] = floatx4{};
@@ -595,8 +612,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void attend_rows_kernel(AttendArgs a
     for (int c = 0; c < C; c++)
 #pragma unroll
       for (int u = 0; u < NT; u++) {
-        const uint32_t *k = buf + (16 * c + 4 * g) * KS + 16 * u + m;
-        const half8 kf = __builtin_bit_cast(half8, u32x4{k[0], k[KS], k[2 * KS], k[3 * KS]});
+        const half8 kf = *(const half8 *)(buf + (16 * u + m) * KS + 16 * c + 4 * g);
 #pragma unroll
         for (int t = 0; t < QT; t++)
 #pragma unroll
@@ -623,15 +639,15 @@ __global__ __launch_bounds__(64 * WAVES, 4) void attend_rows_kernel(AttendArgs a
       for (int e = 1; e < 4 * NT; e++) top = fmaxf(top, st[t][e >> 2][e & 3]);
       top = xlane::bit4(top, xlane::Max{});
       top = xlane::bit5(top, xlane::Max{});
-      top = fmaxf(top, mx[t]);
-      const float base = top == -INFINITY ? 0.0f : top;
-      if (__any(top != mx[t])) {
+      if (__any(top > mx[t] + slack[t])) {
+        top = fmaxf(top, mx[t]);
         const float old = mx[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mx[t] - top) * cf[t]);
         sum[t] *= old;
 #pragma unroll
         for (int x = 0; x < X; x++) acc[t][x] *= old;
         mx[t] = top;
       }
+      const float base = mx[t] == -INFINITY ? 0.0f : mx[t];
 #pragma unroll
       for (int e = 0; e < 4 * NT; e++) {
         const float p = __builtin_amdgcn_exp2f(fmaf(st[t][e >> 2][e & 3] - base, cf[t], 10.0f));
@@ -706,7 +722,7 @@ __global__ __launch_bounds__(64 * WAVES, 4) void attend_rows_kernel(AttendArgs a
     if (blk < end)
 #pragma unroll 1
       for (int u = tid; u < U; u += threads) {
-        const int row = u % B, d = u / B * 8;
+        const int row = u / (HD / 8), d = u % (HD / 8) * 8;
         const size_t src = (row0 + j0 + min(row, last)) * a.stride + (size_t)kh * a.hd;
         u32x2 k[2], v[2];
 #pragma unroll
@@ -717,12 +733,12 @@ __global__ __launch_bounds__(64 * WAVES, 4) void attend_rows_kernel(AttendArgs a
           if (!in || row > last) v[y] = u32x2{};
 #pragma unroll
           for (int w = 0; w < 2; w++) {
-            buf0[(d / 2 + 2 * y + w) * KS + row] = k[y][w];
             const uint32_t clean = finite2(v[y][w]);
             found |= clean != v[y][w];
             v[y][w] = clean;
           }
         }
+        *(u32x4 *)(buf0 + row * KS + d / 2) = u32x4{k[0][0], k[0][1], k[1][0], k[1][1]};
         *(u32x4 *)(buf0 + KW + row * VS + d / 2) = u32x4{v[0][0], v[0][1], v[1][0], v[1][1]};
       }
     if (found) odd[kg] = 1;
@@ -879,7 +895,7 @@ __global__ __launch_bounds__(256) void keep_kernel(KeepArgs a) {
 template <typename T, int HD, int QT, bool P16>
 int attend_launch(wh_ctx *ctx, const AttendArgs &a) {
   ProfScope prof(ctx, "tree_attend", 4.0 * a.batch * a.rows * a.heads * a.cols * a.hd, 4.0 * a.batch * a.cols * a.kv_heads * a.hd);
-  wh_launch(ctx, (attend_kernel<T, HD, QT, P16>), dim3(a.batch * a.row_blocks, a.kv_heads, a.splits), 64 * a.kw,
+  wh_launch(ctx, (attend_kernel<T, HD, QT, P16>), dim3(a.kv_heads, a.batch * a.row_blocks, a.splits), 64 * a.kw,
             (size_t)a.kw * QT * (HD / 64 * 4096 + 128), a);
   return wh_launched(ctx, "tree attention");
 }
@@ -896,8 +912,8 @@ template <typename T, int HD, int RT, bool P16>
 int attend_rows_launch(wh_ctx *ctx, const AttendArgs &a) {
   constexpr int B = rows_block(HD);
   ProfScope prof(ctx, "tree_attend_rows", 4.0 * a.batch * a.rows * a.heads * a.cols * a.hd, 4.0 * a.batch * a.cols * a.kv_heads * a.hd);
-  wh_launch(ctx, (attend_rows_kernel<T, HD, RT, P16>), dim3(a.batch * a.row_blocks, a.kv_heads, a.splits), 64 * WAVES,
-            WAVES / RT * 2 * 4 * ((B + 4) * HD / 2 + (HD / 2 + 8) * B), a);
+  wh_launch(ctx, (attend_rows_kernel<T, HD, RT, P16>), dim3(a.kv_heads, a.batch * a.row_blocks, a.splits), 64 * WAVES,
+            WAVES / RT * 2 * 4 * (HD + 12) * B, a);
   return wh_launched(ctx, "tree attention");
 }
 
@@ -929,7 +945,7 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
                        const uint32_t *kv, size_t kv_stride, int cols, void *o, int out16, int heads, int kv_heads, int hd) {
   if (int rc = tree_check(ctx, "tree attention", t)) return rc;
   if (!q || !kv || !o || !k != !v) return wh_fail(ctx, WH_EARG, "tree attention: q, the cache, o, and k with v are needed");
-  if (heads <= 0 || heads > ATTEND_HEADS || kv_heads <= 0 || heads % kv_heads || hd <= 0 || hd > 128 || hd % 4 || cols <= 0 || cols > 1 << 26)
+  if (heads <= 0 || heads > ATTEND_HEADS || kv_heads <= 0 || heads % kv_heads || hd <= 0 || hd > 128 || hd % 4 || cols <= 0 || cols > 1 << 24)
     return wh_fail(ctx, WH_EARG, "tree attention: bad shape (heads %d, key heads %d, head_dim %d, cols %d)", heads, kv_heads, hd,
                    cols);
   if (stride < (size_t)heads * hd || stride > (size_t)1 << 23)
@@ -953,7 +969,7 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
   const int least = (rt ? 8 : 4) * a.kw;  // blocks of a split
   a.splits = (int)std::max<size_t>(1, std::min<size_t>(((rt ? 2 : 1) * cus + units - 1) / units, (blocks + least - 1) / least));
   const size_t nodes = (size_t)t->batch * t->rows;
-  if (units * a.splits >= (size_t)1 << 22 || nodes * heads >= (size_t)1 << 25)  // (a launch's threads fit 32 bits)
+  if ((size_t)t->batch * a.row_blocks > 65535 || units * a.splits >= (size_t)1 << 22 || nodes * heads >= (size_t)1 << 25)  // (a launch's limits)
     return wh_fail(ctx, WH_EARG, "tree attention: %d heads of %zu nodes in one call", heads, nodes);
   if (a.splits > 1) {
     const size_t part = (size_t)a.splits * nodes * heads;
