@@ -507,27 +507,26 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
   }
 }
 
-// The same for more rows of a key head: a workgroup's 8 wavefronts are KG groups of RT with 16 rows each, and a group
-// goes through every KG-th key block (64 positions for heads of up to 64 values, 32 for larger ones: 16 KiB), one
-// after the other.  Its threads load a block two blocks ahead, each its share of 16-byte pieces, and write it to
-// one of two LDS buffers, K position by position too, from which its wavefronts read operands as they stand: 8 values
-// of a position of K, and V transposed by ds_read_b64_tr_b16 (rows 16 and 32 bytes longer, for the banks' sake).  Tile u's row r is position 16u + r, so lane
-// 16g + i's scores are those of positions 16u + 4g + 0 .. 3 of every u.  128 registers, so that two workgroups
-// share a CU.
+// The same for more rows of a key head: a workgroup's RT wavefronts have 16 rows each and go through the key blocks
+// (64 positions for heads of up to 64 values, 32 for larger ones: 16 KiB) one after the other.  Its threads load a
+// block two blocks ahead, each its share of 16-byte pieces, and write it to one of two LDS buffers, K position by
+// position too, from which the wavefronts read operands as they stand: 8 values of a position of K, and V
+// transposed by ds_read_b64_tr_b16 (rows 16 and 32 bytes longer, for the banks' sake).  Tile u's row r is position
+// 16u + r, so lane 16g + i's scores are those of positions 16u + 4g + 0 .. 3 of every u.  Workgroups of 8 wavefronts
+// get by with 128 registers, so that two share a CU, those of 4 with 168 for three.
 template <typename T, int HD, int RT, bool P16>
-__global__ __launch_bounds__(64 * WAVES, 4) void attend_rows_kernel(AttendArgs a) {
-  constexpr int KG = WAVES / RT, QT = 1;
+__global__ __launch_bounds__(64 * RT, RT == 8 ? 4 : 3) void attend_rows_kernel(AttendArgs a) {
   constexpr int C = HD / 32, X = HD / 16, QP = sizeof(T) == 4 ? 2 : 1, B = rows_block(HD), NT = B / 16, KK = B / 32;
   constexpr int KS = HD / 2 + 4, VS = HD / 2 + 8;  // words per position of K and of V in LDS
   constexpr int KW = KS * B, BUF = KW + VS * B, U = 512;  // words of K and of a buffer; 16-byte pieces of K or V
   extern __shared__ __attribute__((aligned(16))) uint32_t words[];
-  __shared__ int odd[KG];  // set where a node's value is no finite number
+  __shared__ int odd;  // set where a node's value is no finite number
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 4, m = lane & 15;
-  const int kg = wave / RT, tid = threadIdx.x - 64 * RT * kg;
+  const int tid = threadIdx.x;
   constexpr int threads = 64 * RT, MOST = U / threads;  // MOST: pieces per thread
   const int split = blockIdx.z, kh = blockIdx.x, b = a.row_blocks == 1 ? blockIdx.y : blockIdx.y / a.row_blocks;
   const int rb = blockIdx.y - b * a.row_blocks;
-  const int group = a.heads / a.kv_heads, r0 = 16 * (rb * RT + wave % RT);
+  const int group = a.heads / a.kv_heads, r0 = 16 * (rb * RT + wave);
   const size_t row0 = (size_t)b * a.rows;
   const Share s = share_of(a, b);
   const int total = s.count * group;
@@ -578,84 +577,69 @@ __global__ __launch_bounds__(64 * WAVES, 4) void attend_rows_kernel(AttendArgs a
     }
   };
   Pieces p0, p1;
-  int blk = begin + kg;
+  int blk = begin;
   if (blk < cached) load(p0, blk);
-  if (blk + KG < cached) load(p1, blk + KG);
+  if (blk + 1 < cached) load(p1, blk + 1);
 
-  half8 q[QT][C][QP];
-  floatx4 acc[QT][X];
-  float mx[QT], sum[QT], cf[QT], slack[QT];
-  int node[QT];
+  half8 q[C][QP];
+  floatx4 acc[X];
+  float mx = -INFINITY, sum = 0.0f;
+  const int row = min(r0 + m, total - 1), node = node_of(row, group), head = kh * group + head_of(row, group);
+  float f[C][8];
+  load_query<T, C>((const T *)a.q + (row0 + node) * a.stride + (size_t)head * a.hd, g, a.hd, f);
+  const float cf = split_query(f, a.scale, q), slack = SLACK / cf;
 #pragma unroll
-  for (int t = 0; t < QT; t++) {
-    const int row = min(r0 + 16 * t + m, total - 1);
-    node[t] = node_of(row, group);
-    float f[C][8];
-    load_query<T, C>((const T *)a.q + (row0 + node[t]) * a.stride + (size_t)(kh * group + head_of(row, group)) * a.hd, g, a.hd, f);
-    cf[t] = split_query(f, a.scale, q[t]), slack[t] = SLACK / cf[t];
-    mx[t] = -INFINITY, sum[t] = 0.0f;
-#pragma unroll
-    for (int x = 0; x < X; x++) acc[t][x] = floatx4{};
-  }
+  for (int x = 0; x < X; x++) acc[x] = floatx4{};
   const bool busy = r0 < total;  // (a wavefront past the last row only loads)
 
   // One block from LDS; nodes: a block of nodes, otherwise the cache's.
   auto step = [&](auto nodes, int blk, const uint32_t *buf) {
     constexpr bool NODES = nodes;
     const int j0 = (NODES ? blk - s.cached : blk) * B, last = (NODES ? s.count : s.n) - 1 - j0;
-    floatx4 st[QT][NT];
+    floatx4 st[NT];
 #pragma unroll
-    for (int t = 0; t < QT; t++)
-#pragma unroll
-      for (int u = 0; u < NT; u++) st[t][u] = floatx4{};
+    for (int u = 0; u < NT; u++) st[u] = floatx4{};
 #pragma unroll
     for (int c = 0; c < C; c++)
 #pragma unroll
       for (int u = 0; u < NT; u++) {
         const half8 kf = *(const half8 *)(buf + (16 * u + m) * KS + 16 * c + 4 * g);
 #pragma unroll
-        for (int t = 0; t < QT; t++)
-#pragma unroll
-          for (int part = 0; part < QP; part++) st[t][u] = mfma(kf, q[t][c][part], st[t][u]);
+        for (int part = 0; part < QP; part++) st[u] = mfma(kf, q[c][part], st[u]);
       }
     if (NODES || last < B - 1) {
 #pragma unroll
-      for (int t = 0; t < QT; t++)
+      for (int kk = 0; kk < KK; kk++) {
+        const int left = last + 1 - 32 * kk;
+        uint32_t vis = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u;
+        if constexpr (NODES) vis &= node_mask(a, b, node, j0 + 32 * kk);
 #pragma unroll
-        for (int kk = 0; kk < KK; kk++) {
-          const int left = last + 1 - 32 * kk;
-          uint32_t vis = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1u : 0u;
-          if constexpr (NODES) vis &= node_mask(a, b, node[t], j0 + 32 * kk);
-#pragma unroll
-          for (int e = 0; e < 8; e++)
-            if (!(vis >> (16 * (e >> 2) + 4 * g + (e & 3)) & 1)) st[t][2 * kk + (e >> 2)][e & 3] = -INFINITY;
-        }
+        for (int e = 0; e < 8; e++)
+          if (!(vis >> (16 * (e >> 2) + 4 * g + (e & 3)) & 1)) st[2 * kk + (e >> 2)][e & 3] = -INFINITY;
+      }
     }
-    half8 ph[QT][KK], pl[QT][KK];
+    half8 ph[KK], pl[KK];
+    float top = st[0][0];
 #pragma unroll
-    for (int t = 0; t < QT; t++) {
-      float top = st[t][0][0];
+    for (int e = 1; e < 4 * NT; e++) top = fmaxf(top, st[e >> 2][e & 3]);
+    top = xlane::bit4(top, xlane::Max{});
+    top = xlane::bit5(top, xlane::Max{});
+    if (__any(top > mx + slack)) {
+      top = fmaxf(top, mx);
+      const float old = mx == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mx - top) * cf);
+      sum *= old;
 #pragma unroll
-      for (int e = 1; e < 4 * NT; e++) top = fmaxf(top, st[t][e >> 2][e & 3]);
-      top = xlane::bit4(top, xlane::Max{});
-      top = xlane::bit5(top, xlane::Max{});
-      if (__any(top > mx[t] + slack[t])) {
-        top = fmaxf(top, mx[t]);
-        const float old = mx[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mx[t] - top) * cf[t]);
-        sum[t] *= old;
+      for (int x = 0; x < X; x++) acc[x] *= old;
+      mx = top;
+    }
+    const float base = mx == -INFINITY ? 0.0f : mx;
 #pragma unroll
-        for (int x = 0; x < X; x++) acc[t][x] *= old;
-        mx[t] = top;
-      }
-      const float base = mx[t] == -INFINITY ? 0.0f : mx[t];
-#pragma unroll
-      for (int e = 0; e < 4 * NT; e++) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(st[t][e >> 2][e & 3] - base, cf[t], 10.0f));
-        sum[t] += p;
-        const _Float16 h = (_Float16)p;
-        ph[t][e >> 3][e & 7] = h;
-        if constexpr (!P16) pl[t][e >> 3][e & 7] = (_Float16)(p - (float)h);
-      }
+    for (int e = 0; e < 4 * NT; e++) {
+      const float p = __builtin_amdgcn_exp2f(fmaf(st[e >> 2][e & 3] - base, cf, 10.0f));
+      sum += p;
+      const _Float16 h = (_Float16)p;
+      ph[e >> 3][e & 7] = h;
+      if constexpr (!P16) pl[e >> 3][e & 7] = (_Float16)(p - (float)h);
     }
 #pragma unroll
     for (int x = 0; x < X; x++)
@@ -664,134 +648,106 @@ __global__ __launch_bounds__(64 * WAVES, 4) void attend_rows_kernel(AttendArgs a
         const uint32_t *v = buf + KW + (32 * kk + 4 * g + (m >> 2)) * VS + 8 * x + 2 * (m & 3);
         const u32x2 lo = read_tr(v), hi = read_tr(v + 16 * VS);
         const half8 vf = __builtin_bit_cast(half8, u32x4{lo[0], lo[1], hi[0], hi[1]});
-#pragma unroll
-        for (int t = 0; t < QT; t++) {
-          acc[t][x] = mfma(vf, ph[t][kk], acc[t][x]);
-          if constexpr (!P16) acc[t][x] = mfma(vf, pl[t][kk], acc[t][x]);
-        }
+        acc[x] = mfma(vf, ph[kk], acc[x]);
+        if constexpr (!P16) acc[x] = mfma(vf, pl[kk], acc[x]);
       }
-    if (NODES && odd[kg])  // what the block has zeros for, to the rows that see it
+    if (NODES && odd)  // what the block has zeros for, to the rows that see it
 #pragma unroll 1
       for (int j = 0; j < min(B, last + 1); j++) {
         int hd = a.hd;
         asm volatile("" : "+s"(hd));
+        if (!(node_mask(a, b, node, j0 + j) & 1)) continue;
         const T *v = (const T *)a.v + (row0 + j0 + j) * a.stride + (size_t)kh * a.hd;
 #pragma unroll
-        for (int t = 0; t < QT; t++) {
-          if (!(node_mask(a, b, node[t], j0 + j) & 1)) continue;
+        for (int x = 0; x < X; x++)
 #pragma unroll
-          for (int x = 0; x < X; x++)
-#pragma unroll
-            for (int r = 0; r < 4; r++) acc[t][x][r] += not_finite(v, 16 * x + 4 * g + r, hd);
-        }
+          for (int r = 0; r < 4; r++) acc[x][r] += not_finite(v, 16 * x + 4 * g + r, hd);
       }
   };
 
-  // A group's blocks pass in turn through p0 and its first buffer and through p1 and the second.  A buffer is written
-  // again two blocks later, past the barrier that every wavefront reaches after it has read it.  The groups have
-  // as many barriers each: as long as all of them have four more blocks, and then as many as the first one.
-  uint32_t *const buf0 = words + 2 * BUF * kg, *const buf1 = buf0 + BUF;
-  for (; blk - kg + 4 * KG <= cached; blk += 2 * KG) {
+  // The blocks pass in turn through p0 and the first buffer and through p1 and the second.  A buffer is written again
+  // two blocks later, past the barrier that every wavefront reaches after it has read it.
+  uint32_t *const buf0 = words, *const buf1 = buf0 + BUF;
+  for (; blk + 4 <= cached; blk += 2) {
     store(p0, blk, buf0);
-    load(p0, blk + 2 * KG);
+    load(p0, blk + 2);
     meet();
     if (busy) step(std::false_type{}, blk, buf0);
-    store(p1, blk + KG, buf1);
-    load(p1, blk + 3 * KG);
+    store(p1, blk + 1, buf1);
+    load(p1, blk + 3);
     meet();
-    if (busy) step(std::false_type{}, blk + KG, buf1);
+    if (busy) step(std::false_type{}, blk + 1, buf1);
   }
-  for (bool even = true; blk - kg < cached; blk += KG, even = !even) {
-    const bool mine = blk < cached, next = blk + 2 * KG < cached;
+  for (bool even = true; blk < cached; blk++, even = !even) {  // (three at most)
     if (even) {
-      if (mine) store(p0, blk, buf0);
-      if (next) load(p0, blk + 2 * KG);
+      store(p0, blk, buf0);
+      if (blk + 2 < cached) load(p0, blk + 2);
     } else {
-      if (mine) store(p1, blk, buf1);
-      if (next) load(p1, blk + 2 * KG);
+      store(p1, blk, buf1);
     }
     meet();
-    if (busy && mine) step(std::false_type{}, blk, even ? buf0 : buf1);
+    if (busy) step(std::false_type{}, blk, even ? buf0 : buf1);
   }
-  for (blk = max(begin, s.cached) + kg; blk - kg < end; blk += KG) {
+  for (; blk < end; blk++) {
     const int j0 = (blk - s.cached) * B, last = s.count - 1 - j0;
     __syncthreads();
-    if (tid == 0) odd[kg] = 0;
+    if (tid == 0) odd = 0;
     __syncthreads();
     bool found = false;
-    if (blk < end)
-#pragma unroll 1
-      for (int u = tid; u < U; u += threads) {
-        const int row = u / (HD / 8), d = u % (HD / 8) * 8;
-        const size_t src = (row0 + j0 + min(row, last)) * a.stride + (size_t)kh * a.hd;
-        u32x2 k[2], v[2];
+    typename Four<T>::type rk[MOST][2], rv[MOST][2];  // (every row's loads before the first one is rounded)
 #pragma unroll
-        for (int y = 0; y < 2; y++) {
-          const bool in = d + 4 * y < a.hd;
-          k[y] = four((const T *)a.k + src + (in ? d + 4 * y : 0)), v[y] = four((const T *)a.v + src + (in ? d + 4 * y : 0));
-          if (!in) k[y] = u32x2{};
-          if (!in || row > last) v[y] = u32x2{};
+    for (int i = 0; i < MOST; i++) {
+      const int u = tid + threads * i, row = u / (HD / 8), d = u % (HD / 8) * 8;
+      const size_t src = (row0 + j0 + min(row, last)) * a.stride + (size_t)kh * a.hd;
 #pragma unroll
-          for (int w = 0; w < 2; w++) {
-            const uint32_t clean = finite2(v[y][w]);
-            found |= clean != v[y][w];
-            v[y][w] = clean;
-          }
-        }
-        *(u32x4 *)(buf0 + row * KS + d / 2) = u32x4{k[0][0], k[0][1], k[1][0], k[1][1]};
-        *(u32x4 *)(buf0 + KW + row * VS + d / 2) = u32x4{v[0][0], v[0][1], v[1][0], v[1][1]};
+      for (int y = 0; y < 2; y++) {
+        const int at = d + 4 * y < a.hd ? d + 4 * y : 0;
+        rk[i][y] = raw4((const T *)a.k + src + at), rv[i][y] = raw4((const T *)a.v + src + at);
       }
-    if (found) odd[kg] = 1;
+    }
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < MOST; i++) {
+      const int u = tid + threads * i, row = u / (HD / 8), d = u % (HD / 8) * 8;
+      u32x2 k[2], v[2];
+#pragma unroll
+      for (int y = 0; y < 2; y++) {
+        const bool in = d + 4 * y < a.hd;
+        k[y] = in ? pairs4(rk[i][y]) : u32x2{}, v[y] = in && row <= last ? pairs4(rv[i][y]) : u32x2{};
+        const u32x2 clean{finite2(v[y][0]), finite2(v[y][1])};
+        found |= clean[0] != v[y][0] || clean[1] != v[y][1];
+        v[y] = clean;
+      }
+      *(u32x4 *)(buf0 + row * KS + d / 2) = u32x4{k[0][0], k[0][1], k[1][0], k[1][1]};
+      *(u32x4 *)(buf0 + KW + row * VS + d / 2) = u32x4{v[0][0], v[0][1], v[1][0], v[1][1]};
+    }
+    if (found) odd = 1;
     __syncthreads();
-    if (busy && blk < end) step(std::true_type{}, blk, buf0);
+    if (busy) step(std::true_type{}, blk, buf0);
   }
 
-  // The groups' results joined by the first one, through LDS.
-  sum[0] = xlane::bit4(sum[0], xlane::Add{});
-  sum[0] = xlane::bit5(sum[0], xlane::Add{});
-  if constexpr (KG > 1) {
-    static_assert(KG == 2);
-    floatx4 *slot = (floatx4 *)words + (wave % RT) * (X * 64 + 32);
-    float *ml = (float *)(slot + X * 64);
-    __syncthreads();
-    if (kg) {
-#pragma unroll
-      for (int x = 0; x < X; x++) slot[64 * x + lane] = acc[0][x];
-      ml[lane] = mx[0], ml[64 + lane] = sum[0];
-    }
-    __syncthreads();
-    if (kg) return;
-    const float om = ml[lane], os = ml[64 + lane], top = fmaxf(mx[0], om);
-    const float f = mx[0] == top ? 1.0f : __builtin_amdgcn_exp2f((mx[0] - top) * cf[0]);
-    const float of = om == top ? 1.0f : __builtin_amdgcn_exp2f((om - top) * cf[0]);
-    sum[0] = sum[0] * f + os * of, mx[0] = top;
-#pragma unroll
-    for (int x = 0; x < X; x++) acc[0][x] = acc[0][x] * f + slot[64 * x + lane] * of;
-  }
+  sum = xlane::bit4(sum, xlane::Add{});
+  sum = xlane::bit5(sum, xlane::Add{});
+  if (r0 + m >= total) return;
   // Lane 16g + i holds row i's values 16x + 4g + 0 .. 3.
+  const size_t out = ((row0 + node) * a.heads + head) * a.hd, part = (size_t)split * a.batch * a.rows * a.heads;
+  if (s.used > 1 && g == 0) *(floatx4 *)(a.pml + 4 * (part + (row0 + node) * a.heads + head)) = floatx4{mx, sum, cf, 0.0f};
+  const float inv = s.used > 1 ? 1.0f : sum == 0.0f && !sees_any(a, s, b, node) ? 0.0f : 1.0f / sum;
 #pragma unroll
-  for (int t = 0; t < QT; t++) {
-    const int r = r0 + 16 * t + m;
-    if (r >= total) continue;
-    const int i = node[t], head = kh * group + head_of(r, group);
-    const size_t out = ((row0 + i) * a.heads + head) * a.hd;
-    const size_t part = (size_t)split * a.batch * a.rows * a.heads;
-    if (s.used > 1 && g == 0) *(floatx4 *)(a.pml + 4 * (part + (row0 + i) * a.heads + head)) = floatx4{mx[t], sum[t], cf[t], 0.0f};
-    const float inv = s.used > 1 ? 1.0f : sum[t] == 0.0f && !sees_any(a, s, b, i) ? 0.0f : 1.0f / sum[t];
-#pragma unroll
-    for (int x = 0; x < X; x++) {
-      const int d = 16 * x + 4 * g;
-      if (d >= a.hd) continue;
-      const floatx4 f = acc[t][x] * inv;
-      if (s.used > 1) *(floatx4 *)(a.po + part * a.hd + out + d) = f;
-      else if constexpr (P16) *(u32x2_a4 *)((_Float16 *)a.o + out + d) = u32x2{pack2(f[0], f[1]), pack2(f[2], f[3])};
-      else *(floatx4_a4 *)((float *)a.o + out + d) = f;
-    }
+  for (int x = 0; x < X; x++) {
+    const int d = 16 * x + 4 * g;
+    if (d >= a.hd) continue;
+    const floatx4 o = acc[x] * inv;
+    if (s.used > 1) *(floatx4 *)(a.po + part * a.hd + out + d) = o;
+    else if constexpr (P16) *(u32x2_a4 *)((_Float16 *)a.o + out + d) = u32x2{pack2(o[0], o[1]), pack2(o[2], o[3])};
+    else *(floatx4_a4 *)((float *)a.o + out + d) = o;
   }
 }
 
 // The splits' outputs of one head of a node rescaled to their common maximum, summed and divided; one wavefront
-// each, two values a lane.
+// each: split x's maximum and sum in lane x, then two values a lane, 8 splits' at a time.
+constexpr int SPLITS = 64;
+
 template <bool P16>
 __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
   const int lane = threadIdx.x & 63, at = blockIdx.x * 4 + (threadIdx.x >> 6), heads = a.batch * a.rows * a.heads;
@@ -799,23 +755,31 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a) {
   const int row = at / a.heads, b = row / a.rows, i = row % a.rows;
   const Share s = share_of(a, b);
   if (s.used == 1 || i >= s.count) return;
-  float top = -INFINITY;
-  for (int x = 0; x < s.used; x++) top = fmaxf(top, a.pml[4 * ((size_t)x * heads + at)]);
-  const int d = 2 * lane;
-  const float c = a.pml[4 * (size_t)at + 2];
-  float sum = 0.0f, o0 = 0.0f, o1 = 0.0f;
-  for (int x = 0; x < s.used; x++) {
-    const float mx = a.pml[4 * ((size_t)x * heads + at)], f = mx == top ? 1.0f : __builtin_amdgcn_exp2f((mx - top) * c);
-    sum += f * a.pml[4 * ((size_t)x * heads + at) + 1];
-    if (d < a.hd) {
-      const float2 p = *(const float2 *)(a.po + ((size_t)x * heads + at) * a.hd + d);
-      o0 += f * p.x, o1 += f * p.y;
+  const floatx4 ml = *(const floatx4 *)(a.pml + 4 * ((size_t)min(lane, s.used - 1) * heads + at));
+  const bool mine = lane < s.used;
+  const float top = xlane::wave_max(mine ? ml[0] : -INFINITY);
+  const float w = !mine ? 0.0f : ml[0] == top ? 1.0f : __builtin_amdgcn_exp2f((ml[0] - top) * ml[2]);
+  const float sum = xlane::wave_sum(mine ? w * ml[1] : 0.0f);
+  const int d = min(2 * lane, a.hd - 2);
+  float o0 = 0.0f, o1 = 0.0f;
+  for (int x = 0; x < s.used; x += 8) {
+    float2 p[8];
+#pragma unroll
+    for (int y = 0; y < 8; y++) p[y] = *(const float2 *)(a.po + ((size_t)min(x + y, s.used - 1) * heads + at) * a.hd + d);
+#pragma unroll
+    for (int y = 0; y < 8; y++) {
+      const float f = __shfl(w, x + y);
+      if (x + y < s.used) o0 += f * p[y].x, o1 += f * p[y].y;
     }
   }
-  if (d >= a.hd) return;
+  if (2 * lane >= a.hd) return;
   const float inv = sum == 0.0f && !sees_any(a, s, b, i) ? 0.0f : 1.0f / sum;
-  if constexpr (P16) *(uint32_t *)((_Float16 *)a.o + (size_t)at * a.hd + d) = pack2(o0 * inv, o1 * inv);
-  else *(float *)((float *)a.o + (size_t)at * a.hd + d) = o0 * inv, *(float *)((float *)a.o + (size_t)at * a.hd + d + 1) = o1 * inv;
+  if constexpr (P16) {
+    *(uint32_t *)((_Float16 *)a.o + (size_t)at * a.hd + d) = pack2(o0 * inv, o1 * inv);
+  } else {
+    float *o = (float *)a.o + (size_t)at * a.hd + d;
+    o[0] = o0 * inv, o[1] = o1 * inv;
+  }
 }
 
 // ------------------------------------------------------------------------------------- the kept path
@@ -912,8 +876,7 @@ template <typename T, int HD, int RT, bool P16>
 int attend_rows_launch(wh_ctx *ctx, const AttendArgs &a) {
   constexpr int B = rows_block(HD);
   ProfScope prof(ctx, "tree_attend_rows", 4.0 * a.batch * a.rows * a.heads * a.cols * a.hd, 4.0 * a.batch * a.cols * a.kv_heads * a.hd);
-  wh_launch(ctx, (attend_rows_kernel<T, HD, RT, P16>), dim3(a.kv_heads, a.batch * a.row_blocks, a.splits), 64 * WAVES,
-            WAVES / RT * 2 * 4 * (HD + 12) * B, a);
+  wh_launch(ctx, (attend_rows_kernel<T, HD, RT, P16>), dim3(a.kv_heads, a.batch * a.row_blocks, a.splits), 64 * RT, 2 * 4 * (HD + 12) * B, a);
   return wh_launched(ctx, "tree attention");
 }
 
@@ -963,11 +926,11 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
   if (rt) a.block = a.node_block = rows_block(hd);
   const int blocks = (cols + a.block - 1) / a.block + (t->mask && k ? (t->rows + a.node_block - 1) / a.node_block : 0);
   a.row_blocks = (tiles + (rt ? rt : qt) - 1) / (rt ? rt : qt);
-  a.kw = rt ? WAVES / rt : std::min(WAVES, blocks);
   const size_t units = (size_t)t->batch * kv_heads * a.row_blocks;
   const size_t cus = ctx->cus > 0 ? ctx->cus : 256;
+  a.kw = rt ? 1 : std::min(WAVES, blocks);
   const int least = (rt ? 8 : 4) * a.kw;  // blocks of a split
-  a.splits = (int)std::max<size_t>(1, std::min<size_t>(((rt ? 2 : 1) * cus + units - 1) / units, (blocks + least - 1) / least));
+  a.splits = (int)std::max<size_t>(1, std::min<size_t>({((rt ? 2 : 1) * cus + units - 1) / units, ((size_t)blocks + least - 1) / least, SPLITS}));
   const size_t nodes = (size_t)t->batch * t->rows;
   if ((size_t)t->batch * a.row_blocks > 65535 || units * a.splits >= (size_t)1 << 22 || nodes * heads >= (size_t)1 << 25)  // (a launch's limits)
     return wh_fail(ctx, WH_EARG, "tree attention: %d heads of %zu nodes in one call", heads, nodes);
