@@ -1,12 +1,13 @@
 // The requests' rules on rows of logits (include/wavo_hip.h, wh_logit_rules): penalties for ids that the
 // text holds, biases, masks, the first maximum and its log-softmax.
 //
-// Bound by reading and writing the rows.  A workgroup takes 4096 ids of a sequence and several of its rows (nodes):
-// what the sequence's text and biases say of an id is the same for all of them, so it is counted once, in LDS, and
-// then kept in the registers of the thread that has the id (16 ids a thread).  Only ids among the tokens of the
-// tree differ from node to node; a workgroup that has any counts them for every node again.  Otherwise its
-// wavefronts go through the rows without meeting, each with the next row's loads under way, and leave a maximum and a
-// sum of their own, which a second launch joins (one wavefront a row).
+// A workgroup takes 2048 ids of a sequence and several of its rows (nodes).  What the sequence's text and biases say of
+// an id is the same for all of them: it is counted once, in LDS, and each wavefront lists those of its 512 ids that a
+// rule can change (few, but for the most frequent ids).  Then the wavefronts go through the rows without meeting, two
+// rows' loads ahead: a row's values go to LDS, the listed ones are changed there, a lane for each, and come back.  The
+// tree's tokens differ from node to node: those on a node's path are added to the counts before its row and taken
+// back after it.  Each wavefront leaves a maximum and a sum of its own, which a second launch joins (one wavefront a
+// row).
 //
 // The log-softmax is kept as the sum of exp(x − max) over every id but the maximum itself, so that a row
 // with one likely id keeps its precision: logprob = −log1p(sum).
@@ -18,8 +19,7 @@
 
 namespace {
 
-constexpr int RT = 256, PER = 16, IDS = PER * RT;  // threads, ids per thread and per workgroup
-constexpr int NODES = TREE_ROWS;
+constexpr int RT = 256, PER = 8, IDS = PER * RT, WIDS = 64 * PER;  // threads; ids per thread, workgroup and wavefront
 
 struct RulePart {
   float best, rest;
@@ -48,16 +48,6 @@ struct RuleArgs {
 
 __device__ __forceinline__ bool better(float ov, int oi, float v, int i) { return ov > v || (ov == v && oi < i); }
 
-// x / r rounded once, for many x: from the reciprocal ri = 1 / r (rounded once), twice corrected by the remainder
-// (P. Markstein, "Computation of elementary functions on the IBM RISC System/6000 processor", 1990).  exact: r is
-// where the remainders are numbers; quotients that are not are divided as they stand.
-__device__ __forceinline__ float divide(float x, float r, float ri, bool exact) {
-  float q = x * ri;
-  if (!(exact && q > 0x1p-60f && q < 0x1p60f)) return x / r;
-  q = __builtin_fmaf(__builtin_fmaf(-q, r, x), ri, q);
-  return __builtin_fmaf(__builtin_fmaf(-q, r, x), ri, q);
-}
-
 // 16 bytes of a row of any alignment: 4 or 8 values.
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
@@ -75,77 +65,81 @@ struct Piece<_Float16> {
   static constexpr int N = 8;
 };
 
+// Keeps what a wavefront does in LDS in the order it is written in (its accesses are served in order).
+__device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
+
 template <typename T>
-__global__ __launch_bounds__(RT) void rules_kernel(RuleArgs a) {
+__global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
 #pragma clang fp contract(off)  // the rules' sums and products are rounded one by one
   constexpr int V = Piece<T>::N, G = PER / V;  // ids per load, loads
+  typedef typename Piece<T>::type P;
+  // times: twice an id's count, and 1 where a node has it as its token.  bias: the entry, then its value.  list: the ids of
+  // each wavefront that a rule can change.  who, what: the nodes whose tokens are among these ids, and those.
   __shared__ uint32_t times[IDS];
-  __shared__ int entry[IDS];
-  __shared__ uint16_t who[NODES], what[NODES];  // the nodes whose tokens are among these ids
+  __shared__ float bias[IDS];
+  __shared__ __attribute__((aligned(16))) float values[IDS];
+  __shared__ uint16_t list[IDS], who[TREE_ROWS], what[TREE_ROWS];
   __shared__ int whos;
-  const int tid = threadIdx.x;
-  const int chunk = blockIdx.x % a.chunks, rest_ = blockIdx.x / a.chunks, part_of = rest_ % a.groups, b = rest_ / a.groups;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int chunk = blockIdx.x % a.chunks, of = blockIdx.x / a.chunks, b = of / a.groups;
   const int count = a.count ? min(max(a.count[b], 0), a.rows) : a.rows;
-  const int i0 = part_of * a.group, i1 = min(i0 + a.group, count);
+  const int i0 = (of - b * a.groups) * a.group, i1 = min(i0 + a.group, count);
   if (i0 >= i1) return;
   const int id0 = chunk * IDS;
-  // This thread's ids: V from id0 + V * (tid + RT * t) on, t < G.
-  const bool whole = id0 + IDS <= a.vocab;
-  typedef typename Piece<T>::type P;
-  P now[G];
-  uint32_t ok[G];
-  auto load = [&](int i) {
-    const size_t row = (size_t)b * a.rows + i;
-    const T *in = (const T *)a.logits + row * a.ld + id0;
-    const uint32_t *allow = a.allow ? a.allow + row * ((a.vocab + 31) / 32) + id0 / 32 : nullptr;
+  // This thread's ids: V from id0 + first + V * RT * t on, t < G.
+  const int first = V * tid;
+  auto mine = [&](int e) { return first + V * RT * (e / V) + e % V; };
+  struct Row {
+    P x[G];
+    uint32_t ok;    // a bit per id of this thread
+    uint32_t path;  // the mask's word with the lane's listed node
+  };
+  int listed = 0, node = 0, token = 0;
+  const size_t row0 = (size_t)b * a.rows;
+  auto load = [&](Row &w, int i) {
+    const T *in = (const T *)a.logits + (row0 + i) * a.ld + id0;
+    const uint32_t *allow = a.allow ? a.allow + (row0 + i) * ((a.vocab + 31) / 32) + id0 / 32 : nullptr;
+    w.ok = 0xffu;
 #pragma unroll
     for (int t = 0; t < G; t++) {
-      const int l = V * (tid + RT * t);
-      if (whole) {
-        now[t] = *(const typename Piece<T>::any *)(in + l);
+      const int l = first + V * RT * t, left = a.vocab - id0 - l;
+      if (left >= V) {
+        w.x[t] = *(const typename Piece<T>::any *)(in + l);
       } else {
 #pragma unroll
-        for (int e = 0; e < V; e++) now[t][e] = id0 + l + e < a.vocab ? in[l + e] : (T)-INFINITY;
+        for (int e = 0; e < V; e++) w.x[t][e] = e < left ? in[l + e] : (T)-INFINITY;
       }
-      ok[t] = allow && (whole || id0 + l < a.vocab) ? allow[l / 32] >> (l % 32) : 0xffffffffu;
+      if (allow) {
+        const uint32_t bits = left > 0 ? allow[l / 32] >> (l % 32) : 0u;
+        w.ok = t ? (w.ok & ((1u << V) - 1u)) | bits << V : bits;
+      }
     }
+    if (listed) w.path = a.mask[(size_t)b * a.mask_stride + (size_t)i * a.words + node / 32];
   };
-  load(i0);
+  Row now{}, next{};
+  load(now, i0);
+  if (i0 + 1 < i1) load(next, i0 + 1);
 
-  // How often each id stands in the sequence's text, and its bias entry.
   const bool counted = a.penalty != nullptr, biased = a.bias_start != nullptr;
-  float fc[PER], bias[PER], r = 1.0f, ri = 1.0f, f = 0.0f, p = 0.0f;
-  uint32_t hit = 0;
-#pragma unroll
-  for (int e = 0; e < PER; e++) fc[e] = 0.0f, bias[e] = 0.0f;
-  auto look = [&] {  // the counts of this thread's ids
-    hit = 0;
-#pragma unroll
-    for (int t = 0; t < G; t++)
-#pragma unroll
-      for (int e = 0; e < V; e++) {
-        const uint32_t c = times[V * (tid + RT * t) + e];
-        fc[V * t + e] = f * (float)c;
-        hit |= (c ? 1u : 0u) << (V * t + e);
-      }
-  };
-  int listed = 0;
+  float r = 1.0f, f = 0.0f, p = 0.0f;
+  int changes = 0;  // of this wavefront's list
   if (counted || biased) {
-    for (int x = tid; x < IDS; x += RT) times[x] = 0, entry[x] = -1;
+    int *entry = (int *)bias;
+#pragma unroll
+    for (int e = 0; e < PER; e++) times[tid + RT * e] = 0, entry[tid + RT * e] = -1;
     if (tid == 0) whos = 0;
     __syncthreads();
     if (counted) {
       r = a.penalty[3 * b], f = a.penalty[3 * b + 1], p = a.penalty[3 * b + 2];
-      ri = 1.0f / r;
       const int n = a.history ? min(max(a.n[b], 0), a.history_cols) : 0;
       const uint32_t *text = a.history + (size_t)b * a.history_cols;
-      for (int x = a.from + tid; x < n; x += 8 * RT) {  // (8 ids' loads at a time)
-        uint32_t id[8];
+      for (int x = a.from + tid; x < n; x += 16 * RT) {  // (16 ids' loads at a time)
+        uint32_t id[16];
 #pragma unroll
-        for (int y = 0; y < 8; y++) id[y] = text[min(x + RT * y, n - 1)] - (uint32_t)id0;
+        for (int y = 0; y < 16; y++) id[y] = text[min(x + RT * y, n - 1)] - (uint32_t)id0;
 #pragma unroll
-        for (int y = 0; y < 8; y++)
-          if (x + RT * y < n && id[y] < (uint32_t)IDS) atomicAdd(&times[id[y]], 1u);
+        for (int y = 0; y < 16; y++)
+          if (x + RT * y < n && id[y] < (uint32_t)IDS) atomicAdd(&times[id[y]], 2u);
       }
       if (a.mask)
         for (int j = tid; j < count; j += RT) {
@@ -153,6 +147,7 @@ __global__ __launch_bounds__(RT) void rules_kernel(RuleArgs a) {
           if (id < (uint32_t)IDS) {
             const int at = atomicAdd(&whos, 1);
             who[at] = (uint16_t)j, what[at] = (uint16_t)id;
+            atomicOr(&times[id], 1u);
           }
         }
     }
@@ -165,89 +160,114 @@ __global__ __launch_bounds__(RT) void rules_kernel(RuleArgs a) {
     }
     __syncthreads();
     listed = whos;
-    if (biased)
+    if (listed) {
+      node = who[min(lane, listed - 1)], token = what[min(lane, listed - 1)];
+      const uint32_t *mask = a.mask + (size_t)b * a.mask_stride + node / 32;
+      now.path = mask[(size_t)i0 * a.words];
+      if (i0 + 1 < i1) next.path = mask[(size_t)(i0 + 1) * a.words];
+    }
 #pragma unroll
-      for (int t = 0; t < G; t++)
-#pragma unroll
-        for (int e = 0; e < V; e++) {
-          const int at = entry[V * (tid + RT * t) + e];
-          if (at >= 0) bias[V * t + e] = a.bias[at];
-        }
-    if (counted && !listed) look();
+    for (int e = 0; e < PER; e++) {
+      const int l = mine(e), at = entry[l];
+      const uint64_t all = __ballot(times[l] || at >= 0);
+      if (all >> lane & 1) list[WIDS * wave + changes + __popcll(all & ((1ull << lane) - 1ull))] = (uint16_t)l;
+      changes += __popcll(all);
+      bias[l] = at >= 0 ? a.bias[at] : 0.0f;
+    }
+    in_order();
   }
-  const bool exact = r > 0x1p-30f && r < 0x1p30f;
 
   for (int i = i0; i < i1; i++) {
-    if (listed) {  // (every wavefront's: the tokens of the nodes that node i sees)
-      const uint32_t *mask = a.mask + (size_t)b * a.mask_stride + (size_t)i * a.words;
-      __syncthreads();
-      for (int x = tid; x < listed; x += RT)
-        if (mask[who[x] / 32] >> (who[x] % 32) & 1) atomicAdd(&times[what[x]], 1u);
-      __syncthreads();
-      look();
-      __syncthreads();
-      for (int x = tid; x < listed; x += RT)
-        if (mask[who[x] / 32] >> (who[x] % 32) & 1) atomicAdd(&times[what[x]], 0xffffffffu);
-    }
     float v[PER];
 #pragma unroll
-    for (int t = 0; t < G; t++)
-#pragma unroll
-      for (int e = 0; e < V; e++) v[V * t + e] = (float)now[t][e];
-    uint32_t allowed[G];
-#pragma unroll
-    for (int t = 0; t < G; t++) allowed[t] = ok[t];
-    if (i + 1 < i1) load(i + 1);
-    const size_t row = (size_t)b * a.rows + i;
-    T *out = a.out ? (T *)a.out + row * a.ld + id0 : nullptr;
-#pragma unroll
-    for (int t = 0; t < G; t++) {
-      if (counted && __any((hit >> (V * t) & ((1u << V) - 1u)) != 0))
-#pragma unroll
-        for (int e = 0; e < V; e++) {
-          const float x = v[V * t + e], y = x > 0.0f ? divide(x, r, ri, exact) : x * r;
-          if (hit >> (V * t + e) & 1) v[V * t + e] = (y - fc[V * t + e]) - p;
+    for (int e = 0; e < PER; e++) v[e] = (float)now.x[e / V][e % V];
+    const uint32_t ok = now.ok, path = now.path;
+    now = next;
+    if (i + 2 < i1) load(next, i + 2);
+    if (changes) {
+      // The tokens on node i's path among this wavefront's ids: one more of each (or, from < 0, one less).
+      auto add = [&](uint32_t more) {
+        for (int x = lane; x < listed; x += 64) {
+          const int j = x < 64 ? node : who[x], id = x < 64 ? token : what[x];
+          const uint32_t word = x < 64 ? path : a.mask[(size_t)b * a.mask_stride + (size_t)i * a.words + j / 32];
+          if (id / V % RT / 64 == wave && (word >> (j % 32) & 1)) atomicAdd(&times[id], more);
         }
+      };
+      add(2u);
 #pragma unroll
-      for (int e = 0; e < V; e++) {
-        const float x = v[V * t + e] + bias[V * t + e];
-        v[V * t + e] = allowed[t] >> e & 1 ? x : -INFINITY;
+      for (int t = 0; t < PER / 4; t++)
+        *(floatx4 *)(values + mine(4 * t)) = floatx4{v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]};
+      in_order();
+      for (int x = lane; x < changes; x += 64) {
+        const int l = list[WIDS * wave + x];
+        const uint32_t c = times[l] >> 1;
+        float y = values[l];
+        if (c) y = ((y > 0.0f ? y / r : y * r) - f * (float)c) - p;
+        values[l] = y + bias[l];
       }
+      in_order();
+#pragma unroll
+      for (int t = 0; t < PER / 4; t++) {
+        const floatx4 y = *(const floatx4 *)(values + mine(4 * t));
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[4 * t + e] = y[e];
+      }
+      add(0u - 2u);
+      in_order();
     }
-    if (out)
+    if (a.allow)
+#pragma unroll
+      for (int e = 0; e < PER; e++) v[e] = ok >> e & 1 ? v[e] : -INFINITY;
+    if (a.out) {
+      T *out = (T *)a.out + (row0 + i) * a.ld + id0;
 #pragma unroll
       for (int t = 0; t < G; t++) {
-        const int l = V * (tid + RT * t);
+        const int l = first + V * RT * t, left = a.vocab - id0 - l;
         P w;
 #pragma unroll
         for (int e = 0; e < V; e++) w[e] = (T)v[V * t + e];
-        if (whole) {
+        if (left >= V) {
           *(typename Piece<T>::any *)(out + l) = w;
         } else {
 #pragma unroll
           for (int e = 0; e < V; e++)
-            if (id0 + l + e < a.vocab) out[l + e] = w[e];
+            if (e < left) out[l + e] = w[e];
         }
       }
+    }
     if (!a.part) continue;
-    float best = -INFINITY;
+    float best = v[0];  // (ids that are not there hold −∞, as masked ones do)
 #pragma unroll
-    for (int e = 0; e < PER; e++) best = fmaxf(best, v[e]);
+    for (int e = 1; e < PER; e++) best = fmaxf(best, v[e]);
     best = xlane::wave_max(best);
-    // Its first place (ids that are not there hold −∞, as masked ones do), and the others' mass against it.
+    // Its first place, and the others' mass against it.
     int at = INT_MAX;
-    if (best > -INFINITY)
+    if (best > -INFINITY) {
 #pragma unroll
-      for (int e = PER - 1; e >= 0; e--)
-        if (v[e] == best) at = V * (tid + RT * (e / V)) + e % V;
-    for (int d = 32; d; d >>= 1) at = min(at, __shfl_xor(at, d));
+      for (int t = G - 1; t >= 0; t--) {
+        uint64_t any = 0;
+#pragma unroll
+        for (int e = 0; e < V; e++) any |= __ballot(v[V * t + e] == best);
+        if (any) at = V * (64 * wave + (int)__builtin_ctzll(any) + RT * t);
+      }
+      int e0 = PER;
+      if (at / V % 64 == lane)
+#pragma unroll
+        for (int e = V - 1; e >= 0; e--)
+#pragma unroll
+          for (int t = 0; t < G; t++)
+            if (t == at / V / RT && v[V * t + e] == best) e0 = V * t + e;
+      if (e0 < PER)
+#pragma unroll
+        for (int e = 0; e < PER; e++) v[e] = e == e0 ? -INFINITY : v[e];
+      at += __builtin_amdgcn_readlane(e0, at / V % 64) % V;
+    }
     float rest = 0.0f;
     const float m = best == -INFINITY ? 0.0f : best;
 #pragma unroll
-    for (int e = 0; e < PER; e++)
-      if (V * (tid + RT * (e / V)) + e % V != at) rest += __expf(v[e] - m);
+    for (int e = 0; e < PER; e++) rest += __expf(v[e] - m);
     rest = xlane::wave_sum(rest);
-    if ((tid & 63) == 0) a.part[(row * a.chunks + chunk) * (RT / 64) + tid / 64] = {best, rest, at == INT_MAX ? at : id0 + at, 0};
+    if (lane == 0) a.part[((row0 + i) * a.chunks + chunk) * (RT / 64) + wave] = {best, rest, at == INT_MAX ? at : id0 + at, 0};
   }
 }
 
@@ -308,8 +328,8 @@ int launch_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *r, const v
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "logit rules: %s", hipGetErrorString(e));
   const size_t nodes = (size_t)t->batch * t->rows;
   const int chunks = (vocab + IDS - 1) / IDS, parts = chunks * (RT / 64);
-  // Rows per workgroup: all of a sequence's, or as many as leave 4 workgroups a CU.
-  const size_t want = 4 * (size_t)(ctx->cus > 0 ? ctx->cus : 256), each = (size_t)chunks * t->batch;
+  // Rows per workgroup: all of a sequence's, or as many as leave 5 workgroups a CU.
+  const size_t want = 5 * (size_t)(ctx->cus > 0 ? ctx->cus : 256), each = (size_t)chunks * t->batch;
   int groups = (int)std::min<size_t>(t->rows, (want + each - 1) / each);
   const int group = (t->rows + groups - 1) / groups;
   groups = (t->rows + group - 1) / group;
