@@ -74,11 +74,11 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
   constexpr int V = Piece<T>::N, G = PER / V;  // ids per load, loads
   typedef typename Piece<T>::type P;
   // times: twice an id's count, and 1 where a node has it as its token.  bias: the entry, then its value.  list: the ids of
-  // each wavefront that a rule can change.  who, what: the nodes whose tokens are among these ids, and those.
+  // each wavefront that a rule can change.  who: the nodes whose tokens are among these ids.
   __shared__ uint32_t times[IDS];
   __shared__ float bias[IDS];
   __shared__ __attribute__((aligned(16))) float values[IDS];
-  __shared__ uint16_t list[IDS], who[TREE_ROWS], what[TREE_ROWS];
+  __shared__ uint16_t list[IDS], who[TREE_ROWS];
   __shared__ int whos;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int chunk = blockIdx.x % a.chunks, of = blockIdx.x / a.chunks, b = of / a.groups;
@@ -146,7 +146,7 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
           const uint32_t id = a.tokens[(size_t)b * a.rows + j] - (uint32_t)id0;
           if (id < (uint32_t)IDS) {
             const int at = atomicAdd(&whos, 1);
-            who[at] = (uint16_t)j, what[at] = (uint16_t)id;
+            who[at] = (uint16_t)j;
             atomicOr(&times[id], 1u);
           }
         }
@@ -161,7 +161,7 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
     __syncthreads();
     listed = whos;
     if (listed) {
-      node = who[min(lane, listed - 1)], token = what[min(lane, listed - 1)];
+      node = who[min(lane, listed - 1)], token = (int)a.tokens[(size_t)b * a.rows + node] - id0;
       const uint32_t *mask = a.mask + (size_t)b * a.mask_stride + node / 32;
       now.path = mask[(size_t)i0 * a.words];
       if (i0 + 1 < i1) next.path = mask[(size_t)(i0 + 1) * a.words];
@@ -188,7 +188,7 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
       // The tokens on node i's path among this wavefront's ids: one more of each (or, from < 0, one less).
       auto add = [&](uint32_t more) {
         for (int x = lane; x < listed; x += 64) {
-          const int j = x < 64 ? node : who[x], id = x < 64 ? token : what[x];
+          const int j = x < 64 ? node : who[x], id = x < 64 ? token : (int)a.tokens[(size_t)b * a.rows + j] - id0;
           const uint32_t word = x < 64 ? path : a.mask[(size_t)b * a.mask_stride + (size_t)i * a.words + j / 32];
           if (id / V % RT / 64 == wave && (word >> (j % 32) & 1)) atomicAdd(&times[id], more);
         }
