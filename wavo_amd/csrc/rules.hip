@@ -50,6 +50,7 @@ __device__ __forceinline__ bool better(float ov, int oi, float v, int i) { retur
 
 // 16 bytes of a row of any alignment: 4 or 8 values.
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_a4 __attribute__((aligned(4)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 template <typename T>
@@ -96,21 +97,22 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
   };
   int listed = 0, node = 0, token = 0;
   const size_t row0 = (size_t)b * a.rows;
+  const bool whole = id0 + IDS <= a.vocab;
   auto load = [&](Row &w, int i) {
     const T *in = (const T *)a.logits + (row0 + i) * a.ld + id0;
     const uint32_t *allow = a.allow ? a.allow + (row0 + i) * ((a.vocab + 31) / 32) + id0 / 32 : nullptr;
     w.ok = 0xffu;
 #pragma unroll
     for (int t = 0; t < G; t++) {
-      const int l = first + V * RT * t, left = a.vocab - id0 - l;
-      if (left >= V) {
+      const int l = first + V * RT * t, left = whole ? V : a.vocab - id0 - l;
+      if (whole || left >= V) {
         w.x[t] = *(const typename Piece<T>::any *)(in + l);
       } else {
 #pragma unroll
         for (int e = 0; e < V; e++) w.x[t][e] = e < left ? in[l + e] : (T)-INFINITY;
       }
       if (allow) {
-        const uint32_t bits = left > 0 ? allow[l / 32] >> (l % 32) : 0u;
+        const uint32_t bits = whole || left > 0 ? allow[l / 32] >> (l % 32) : 0u;
         w.ok = t ? (w.ok & ((1u << V) - 1u)) | bits << V : bits;
       }
     }
@@ -133,13 +135,25 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
       r = a.penalty[3 * b], f = a.penalty[3 * b + 1], p = a.penalty[3 * b + 2];
       const int n = a.history ? min(max(a.n[b], 0), a.history_cols) : 0;
       const uint32_t *text = a.history + (size_t)b * a.history_cols;
-      for (int x = a.from + tid; x < n; x += 16 * RT) {  // (16 ids' loads at a time)
+      auto add = [&](uint32_t id) {
+        id -= (uint32_t)id0;
+        if (id < (uint32_t)IDS) atomicAdd(&times[id], 2u);
+      };
+      int x = a.from;
+      for (; x + 16 * RT <= n; x += 16 * RT) {  // (16 ids a thread at a time)
+        u32x4 id[4];
+#pragma unroll
+        for (int y = 0; y < 4; y++) id[y] = *(const u32x4_a4 *)(text + x + 4 * (tid + RT * y));
+#pragma unroll
+        for (int y = 0; y < 16; y++) add(id[y / 4][y % 4]);
+      }
+      if (x < n) {
         uint32_t id[16];
 #pragma unroll
-        for (int y = 0; y < 16; y++) id[y] = text[min(x + RT * y, n - 1)] - (uint32_t)id0;
+        for (int y = 0; y < 16; y++) id[y] = text[min(x + RT * y + tid, n - 1)];
 #pragma unroll
         for (int y = 0; y < 16; y++)
-          if (x + RT * y < n && id[y] < (uint32_t)IDS) atomicAdd(&times[id[y]], 2u);
+          if (x + RT * y + tid < n) add(id[y]);
       }
       if (a.mask)
         for (int j = tid; j < count; j += RT) {
@@ -217,16 +231,19 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
     }
     if (a.allow)
 #pragma unroll
-      for (int e = 0; e < PER; e++) v[e] = ok >> e & 1 ? v[e] : -INFINITY;
+      for (int e = 0; e < PER; e++) {
+        const uint32_t keep = (uint32_t)((int32_t)(ok << (31 - e)) >> 31);
+        v[e] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, v[e]) & keep) | (0xff800000u & ~keep));
+      }
     if (a.out) {
       T *out = (T *)a.out + (row0 + i) * a.ld + id0;
 #pragma unroll
       for (int t = 0; t < G; t++) {
-        const int l = first + V * RT * t, left = a.vocab - id0 - l;
+        const int l = first + V * RT * t, left = whole ? V : a.vocab - id0 - l;
         P w;
 #pragma unroll
         for (int e = 0; e < V; e++) w[e] = (T)v[V * t + e];
-        if (left >= V) {
+        if (whole || left >= V) {
           *(typename Piece<T>::any *)(out + l) = w;
         } else {
 #pragma unroll
@@ -236,32 +253,31 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
       }
     }
     if (!a.part) continue;
-    float best = v[0];  // (ids that are not there hold −∞, as masked ones do)
+    float tops[G], best = -INFINITY;  // (ids that are not there hold −∞, as masked ones do)
 #pragma unroll
-    for (int e = 1; e < PER; e++) best = fmaxf(best, v[e]);
-    best = xlane::wave_max(best);
-    // Its first place, and the others' mass against it.
-    int at = INT_MAX;
-    if (best > -INFINITY) {
+    for (int t = 0; t < G; t++) {
+      tops[t] = v[V * t];
 #pragma unroll
-      for (int t = G - 1; t >= 0; t--) {
-        uint64_t any = 0;
-#pragma unroll
-        for (int e = 0; e < V; e++) any |= __ballot(v[V * t + e] == best);
-        if (any) at = V * (64 * wave + (int)__builtin_ctzll(any) + RT * t);
-      }
-      int e0 = PER;
-      if (at / V % 64 == lane)
-#pragma unroll
-        for (int e = V - 1; e >= 0; e--)
-#pragma unroll
-          for (int t = 0; t < G; t++)
-            if (t == at / V / RT && v[V * t + e] == best) e0 = V * t + e;
-      if (e0 < PER)
-#pragma unroll
-        for (int e = 0; e < PER; e++) v[e] = e == e0 ? -INFINITY : v[e];
-      at += __builtin_amdgcn_readlane(e0, at / V % 64) % V;
+      for (int e = 1; e < V; e++) tops[t] = fmaxf(tops[t], v[V * t + e]);
+      best = fmaxf(best, tops[t]);
     }
+    best = xlane::wave_max(best);
+    // Its first place, which the others' mass against it leaves out.
+    int at = INT_MAX;
+    if (best > -INFINITY)
+#pragma unroll
+      for (int t = 0; t < G; t++) {
+        const uint64_t any = __ballot(tops[t] == best);
+        if (!any || at != INT_MAX) continue;
+        const int l = (int)__builtin_ctzll(any);
+#pragma unroll
+        for (int e = 0; e < V; e++) {
+          const int x = __builtin_bit_cast(int, v[V * t + e]);
+          if (at != INT_MAX || __builtin_bit_cast(float, __builtin_amdgcn_readlane(x, l)) != best) continue;
+          at = V * (64 * wave + l + RT * t) + e;
+          if (lane == l) v[V * t + e] = -INFINITY;
+        }
+      }
     float rest = 0.0f;
     const float m = best == -INFINITY ? 0.0f : best;
 #pragma unroll
@@ -328,9 +344,11 @@ int launch_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *r, const v
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "logit rules: %s", hipGetErrorString(e));
   const size_t nodes = (size_t)t->batch * t->rows;
   const int chunks = (vocab + IDS - 1) / IDS, parts = chunks * (RT / 64);
-  // Rows per workgroup: all of a sequence's, or as many as leave 5 workgroups a CU.
+  // Rows per workgroup: about ten (fewer count the text too often, more leave the last workgroups alone: 61 rows of
+  // 131071 f16 ids for 8 requests took 115, 107, 107, 113 and 142 us with 4, 8, 12, 16 and 32 of them), or so few that
+  // there are 5 workgroups a CU.
   const size_t want = 5 * (size_t)(ctx->cus > 0 ? ctx->cus : 256), each = (size_t)chunks * t->batch;
-  int groups = (int)std::min<size_t>(t->rows, (want + each - 1) / each);
+  int groups = (int)std::min<size_t>(t->rows, std::max<size_t>((want + each - 1) / each, (t->rows + 9) / 10));
   const int group = (t->rows + groups - 1) / groups;
   groups = (t->rows + group - 1) / group;
   if (each * groups >= (size_t)1 << 24) return wh_fail(ctx, WH_EARG, "logit rules: %zu rows of %d ids", nodes, vocab);
