@@ -13,6 +13,7 @@
 // with one likely id keeps its precision: logprob = −log1p(sum).
 #include <algorithm>
 #include <climits>
+#include <type_traits>
 
 #include "internal.h"
 #include "xlane.h"
@@ -69,7 +70,9 @@ struct Piece<_Float16> {
 // Keeps what a wavefront does in LDS in the order it is written in (its accesses are served in order).
 __device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
 
-template <typename T>
+// ALLOW, OUT, whole: what a row's pass loads and stores has to be the same for every row, so that a wait for one row's
+// loads is not one for the next rows' (61 rows of 131071 f16 ids for 8 requests: @@ us).
+template <typename T, bool ALLOW, bool OUT>
 __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
 #pragma clang fp contract(off)  // the rules' sums and products are rounded one by one
   constexpr int V = Piece<T>::N, G = PER / V;  // ids per load, loads
@@ -80,6 +83,7 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
   __shared__ float bias[IDS];
   __shared__ __attribute__((aligned(16))) float values[IDS];
   __shared__ uint16_t list[IDS], who[TREE_ROWS];
+  __shared__ uint64_t paths[64];  // per row of this workgroup: which nodes in `who` it sees, where both are so few
   __shared__ int whos;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int chunk = blockIdx.x % a.chunks, of = blockIdx.x / a.chunks, b = of / a.groups;
@@ -92,39 +96,33 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
   auto mine = [&](int e) { return first + V * RT * (e / V) + e % V; };
   struct Row {
     P x[G];
-    uint32_t ok;    // a bit per id of this thread
-    uint32_t path;  // the mask's word with the lane's listed node
+    uint32_t ok[G];  // from bit 0 on, a bit per id
   };
-  int listed = 0, node = 0, token = 0;
   const size_t row0 = (size_t)b * a.rows;
   const bool whole = id0 + IDS <= a.vocab;
-  auto load = [&](Row &w, int i) {
+  auto load = [&](auto all, Row &w, int i) {
     const T *in = (const T *)a.logits + (row0 + i) * a.ld + id0;
-    const uint32_t *allow = a.allow ? a.allow + (row0 + i) * ((a.vocab + 31) / 32) + id0 / 32 : nullptr;
-    w.ok = 0xffu;
+    const uint32_t *allow = ALLOW ? a.allow + (row0 + i) * ((a.vocab + 31) / 32) + id0 / 32 : nullptr;
 #pragma unroll
     for (int t = 0; t < G; t++) {
-      const int l = first + V * RT * t, left = whole ? V : a.vocab - id0 - l;
-      if (whole || left >= V) {
+      const int l = first + V * RT * t, left = a.vocab - id0 - l;
+      if constexpr (all) {
         w.x[t] = *(const typename Piece<T>::any *)(in + l);
       } else {
 #pragma unroll
         for (int e = 0; e < V; e++) w.x[t][e] = e < left ? in[l + e] : (T)-INFINITY;
       }
-      if (allow) {
-        const uint32_t bits = whole || left > 0 ? allow[l / 32] >> (l % 32) : 0u;
-        w.ok = t ? (w.ok & ((1u << V) - 1u)) | bits << V : bits;
-      }
+      if constexpr (ALLOW) w.ok[t] = all || left > 0 ? allow[l / 32] >> (l % 32) : 0u;
     }
-    if (listed) w.path = a.mask[(size_t)b * a.mask_stride + (size_t)i * a.words + node / 32];
   };
-  Row now{}, next{};
-  load(now, i0);
-  if (i0 + 1 < i1) load(next, i0 + 1);
+  Row even, odd;  // rows i0, i0 + 2, .. and the others: each loaded again as soon as its values are in use
+  if (whole) load(std::true_type{}, even, i0), load(std::true_type{}, odd, min(i0 + 1, i1 - 1));
+  else load(std::false_type{}, even, i0), load(std::false_type{}, odd, min(i0 + 1, i1 - 1));
 
   const bool counted = a.penalty != nullptr, biased = a.bias_start != nullptr;
   float r = 1.0f, f = 0.0f, p = 0.0f;
-  int changes = 0;  // of this wavefront's list
+  int changes = 0, listed = 0, token = -1;  // of this wavefront's list; nodes in `who`; the lane's, if it is this wavefront's
+  bool few = false;
   if (counted || biased) {
     int *entry = (int *)bias;
 #pragma unroll
@@ -174,11 +172,17 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
     }
     __syncthreads();
     listed = whos;
-    if (listed) {
-      node = who[min(lane, listed - 1)], token = (int)a.tokens[(size_t)b * a.rows + node] - id0;
-      const uint32_t *mask = a.mask + (size_t)b * a.mask_stride + node / 32;
-      now.path = mask[(size_t)i0 * a.words];
-      if (i0 + 1 < i1) next.path = mask[(size_t)(i0 + 1) * a.words];
+    few = listed <= 64 && i1 - i0 <= 64;
+    if (listed && few) {
+      const int j = who[min(lane, listed - 1)];
+      token = (int)a.tokens[(size_t)b * a.rows + j] - id0;
+      for (int i = i0 + wave; i < i1; i += RT / 64) {
+        const uint32_t word = a.mask[(size_t)b * a.mask_stride + (size_t)i * a.words + j / 32];
+        const uint64_t seen = __ballot(lane < listed && (word >> (j % 32) & 1));
+        if (lane == 0) paths[i - i0] = seen;
+      }
+      __syncthreads();
+      if (token / V % RT / 64 != wave) token = -1;
     }
 #pragma unroll
     for (int e = 0; e < PER; e++) {
@@ -191,20 +195,25 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
     in_order();
   }
 
-  for (int i = i0; i < i1; i++) {
+  auto row = [&](auto all, Row &now, int i) {
     float v[PER];
 #pragma unroll
     for (int e = 0; e < PER; e++) v[e] = (float)now.x[e / V][e % V];
-    const uint32_t ok = now.ok, path = now.path;
-    now = next;
-    if (i + 2 < i1) load(next, i + 2);
+    uint32_t ok[G];
+#pragma unroll
+    for (int t = 0; t < G; t++) ok[t] = now.ok[t];
+    load(all, now, min(i + 2, i1 - 1));
     if (changes) {
-      // The tokens on node i's path among this wavefront's ids: one more of each (or, from < 0, one less).
+      // The tokens on node i's path among this wavefront's ids: one more of each (or one less).
       auto add = [&](uint32_t more) {
+        if (few) {
+          if (token >= 0 && (paths[i - i0] >> lane & 1)) atomicAdd(&times[token], more);
+          return;
+        }
         for (int x = lane; x < listed; x += 64) {
-          const int j = x < 64 ? node : who[x], id = x < 64 ? token : (int)a.tokens[(size_t)b * a.rows + j] - id0;
-          const uint32_t word = x < 64 ? path : a.mask[(size_t)b * a.mask_stride + (size_t)i * a.words + j / 32];
-          if (id / V % RT / 64 == wave && (word >> (j % 32) & 1)) atomicAdd(&times[id], more);
+          const int j = who[x], id = (int)a.tokens[(size_t)b * a.rows + j] - id0;
+          if (id / V % RT / 64 == wave && (a.mask[(size_t)b * a.mask_stride + (size_t)i * a.words + j / 32] >> (j % 32) & 1))
+            atomicAdd(&times[id], more);
         }
       };
       add(2u);
@@ -229,21 +238,21 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
       add(0u - 2u);
       in_order();
     }
-    if (a.allow)
+    if constexpr (ALLOW)
 #pragma unroll
       for (int e = 0; e < PER; e++) {
-        const uint32_t keep = (uint32_t)((int32_t)(ok << (31 - e)) >> 31);
+        const uint32_t keep = (uint32_t)((int32_t)(ok[e / V] << (31 - e % V)) >> 31);
         v[e] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, v[e]) & keep) | (0xff800000u & ~keep));
       }
-    if (a.out) {
+    if constexpr (OUT) {
       T *out = (T *)a.out + (row0 + i) * a.ld + id0;
 #pragma unroll
       for (int t = 0; t < G; t++) {
-        const int l = first + V * RT * t, left = whole ? V : a.vocab - id0 - l;
+        const int l = first + V * RT * t, left = a.vocab - id0 - l;
         P w;
 #pragma unroll
         for (int e = 0; e < V; e++) w[e] = (T)v[V * t + e];
-        if (whole || left >= V) {
+        if constexpr (all) {
           *(typename Piece<T>::any *)(out + l) = w;
         } else {
 #pragma unroll
@@ -252,7 +261,7 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
         }
       }
     }
-    if (!a.part) continue;
+    if (!a.part) return;
     float tops[G], best = -INFINITY;  // (ids that are not there hold −∞, as masked ones do)
 #pragma unroll
     for (int t = 0; t < G; t++) {
@@ -284,7 +293,17 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
     for (int e = 0; e < PER; e++) rest += __expf(v[e] - m);
     rest = xlane::wave_sum(rest);
     if (lane == 0) a.part[((row0 + i) * a.chunks + chunk) * (RT / 64) + wave] = {best, rest, at == INT_MAX ? at : id0 + at, 0};
-  }
+  };
+  auto rows = [&](auto all) {
+    for (int i = i0;;) {
+      row(all, even, i);
+      if (++i == i1) return;
+      row(all, odd, i);
+      if (++i == i1) return;
+    }
+  };
+  if (whole) rows(std::true_type{});
+  else rows(std::false_type{});
 }
 
 // (best, rest, at) of two runs of ids: the greater maximum, and the other one's mass against it.
@@ -326,6 +345,15 @@ __global__ __launch_bounds__(64) void rules_pick_kernel(const RulePart *part, co
   if (logprob) logprob[row] = rest != rest ? rest : best == -INFINITY ? best : (best - best) - log1pf(rest);
 }
 
+template <typename T>
+int rules_launch(wh_ctx *ctx, const RuleArgs &a, int grid) {
+  if (a.allow && a.out) wh_launch(ctx, (rules_kernel<T, true, true>), grid, RT, 0, a);
+  else if (a.allow) wh_launch(ctx, (rules_kernel<T, true, false>), grid, RT, 0, a);
+  else if (a.out) wh_launch(ctx, (rules_kernel<T, false, true>), grid, RT, 0, a);
+  else wh_launch(ctx, (rules_kernel<T, false, false>), grid, RT, 0, a);
+  return wh_launched(ctx, "logit rules");
+}
+
 }  // namespace
 
 int launch_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *r, const void *logits, void *out, int vocab, size_t ld,
@@ -359,9 +387,7 @@ int launch_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *r, const v
                    chunks, group, groups, ld, part};
   {
     ProfScope prof(ctx, "logit_rules", 0.0, (double)nodes * vocab * (f16 ? 2 : 4) * (out ? 2 : 1));
-    if (f16) wh_launch(ctx, rules_kernel<_Float16>, (int)each * groups, RT, 0, a);
-    else wh_launch(ctx, rules_kernel<float>, (int)each * groups, RT, 0, a);
-    if (int rc = wh_launched(ctx, "logit rules")) return rc;
+    if (int rc = f16 ? rules_launch<_Float16>(ctx, a, (int)each * groups) : rules_launch<float>(ctx, a, (int)each * groups)) return rc;
   }
   if (!part) return WH_OK;
   ProfScope prof(ctx, "logit_pick", 0.0, (double)sizeof(RulePart) * parts * nodes);
