@@ -21,6 +21,7 @@
 namespace {
 
 constexpr int RT = 256, PER = 8, IDS = PER * RT, WIDS = 64 * PER;  // threads; ids per thread, workgroup and wavefront
+constexpr int GROUP = 10, WORDS = TREE_ROWS / 64;  // rows of a workgroup, at most; 64-bit words of a node's path
 
 struct RulePart {
   float best, rest;
@@ -71,20 +72,21 @@ struct Piece<_Float16> {
 __device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
 
 // ALLOW, OUT, whole: what a row's pass loads and stores has to be the same for every row, so that a wait for one row's
-// loads is not one for the next rows' (61 rows of 131071 f16 ids for 8 requests: @@ us).
+// loads is not one for the next rows'.  61 rows of 131071 f16 ids for 8 requests, 16000 ids of text and 1000 biases
+// each: 94 us (2.1 TB/s; 104 with one row's registers only).  A copy
+// of these rows alone in the same form takes 42 us: the rest is issue, 236 vector instructions a wavefront and row.
 template <typename T, bool ALLOW, bool OUT>
 __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
 #pragma clang fp contract(off)  // the rules' sums and products are rounded one by one
   constexpr int V = Piece<T>::N, G = PER / V;  // ids per load, loads
   typedef typename Piece<T>::type P;
   // times: twice an id's count, and 1 where a node has it as its token.  bias: the entry, then its value.  list: the ids of
-  // each wavefront that a rule can change.  who: the nodes whose tokens are among these ids.
+  // each wavefront that a rule can change.  who: the nodes whose tokens are among these ids, then those tokens.
   __shared__ uint32_t times[IDS];
   __shared__ float bias[IDS];
   __shared__ __attribute__((aligned(16))) float values[IDS];
   __shared__ uint16_t list[IDS], who[TREE_ROWS];
-  __shared__ uint64_t paths[64];  // per row of this workgroup: which nodes in `who` it sees, where both are so few
-  __shared__ int whos;
+  __shared__ uint64_t paths[GROUP][WORDS];  // per row of this workgroup: which nodes of `who` it sees
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int chunk = blockIdx.x % a.chunks, of = blockIdx.x / a.chunks, b = of / a.groups;
   const int count = a.count ? min(max(a.count[b], 0), a.rows) : a.rows;
@@ -121,10 +123,12 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
 
   const bool counted = a.penalty != nullptr, biased = a.bias_start != nullptr;
   float r = 1.0f, f = 0.0f, p = 0.0f;
-  int changes = 0, listed = 0, token = -1;  // of this wavefront's list; nodes in `who`; the lane's, if it is this wavefront's
-  bool few = false;
+  int changes = 0, listed = 0;  // of this wavefront's list; of `who`
+  int one = 0, token = -1;      // the lane's id on the list; its token of `who`, if it is this wavefront's
+  float onebias = 0.0f;
+  const int span = min(IDS, a.vocab - id0);
   if (counted || biased) {
-    int *entry = (int *)bias;
+    int *entry = (int *)bias, &whos = *(int *)values;
 #pragma unroll
     for (int e = 0; e < PER; e++) times[tid + RT * e] = 0, entry[tid + RT * e] = -1;
     if (tid == 0) whos = 0;
@@ -135,7 +139,7 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
       const uint32_t *text = a.history + (size_t)b * a.history_cols;
       auto add = [&](uint32_t id) {
         id -= (uint32_t)id0;
-        if (id < (uint32_t)IDS) atomicAdd(&times[id], 2u);
+        if (id < (uint32_t)span) atomicAdd(&times[id], 2u);
       };
       int x = a.from;
       for (; x + 16 * RT <= n; x += 16 * RT) {  // (16 ids a thread at a time)
@@ -156,7 +160,7 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
       if (a.mask)
         for (int j = tid; j < count; j += RT) {
           const uint32_t id = a.tokens[(size_t)b * a.rows + j] - (uint32_t)id0;
-          if (id < (uint32_t)IDS) {
+          if (id < (uint32_t)span) {
             const int at = atomicAdd(&whos, 1);
             who[at] = (uint16_t)j;
             atomicOr(&times[id], 1u);
@@ -167,22 +171,25 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
       const int e0 = max(a.bias_start[b], 0), e1 = min(a.bias_start[b + 1], a.bias_len);
       for (int x = e0 + tid; x < e1; x += RT) {
         const uint32_t id = a.bias_id[x] - (uint32_t)id0;
-        if (id < (uint32_t)IDS) atomicMax(&entry[id], x);
+        if (id < (uint32_t)span) atomicMax(&entry[id], x);
       }
     }
     __syncthreads();
     listed = whos;
-    few = listed <= 64 && i1 - i0 <= 64;
-    if (listed && few) {
-      const int j = who[min(lane, listed - 1)];
-      token = (int)a.tokens[(size_t)b * a.rows + j] - id0;
-      for (int i = i0 + wave; i < i1; i += RT / 64) {
-        const uint32_t word = a.mask[(size_t)b * a.mask_stride + (size_t)i * a.words + j / 32];
-        const uint64_t seen = __ballot(lane < listed && (word >> (j % 32) & 1));
-        if (lane == 0) paths[i - i0] = seen;
-      }
+    __syncthreads();  // (the rows' values take its place)
+    if (listed) {
+      for (int i = i0 + wave; i < i1; i += RT / 64)
+        for (int x = 0; x < listed; x += 64) {
+          const int j = who[min(x + lane, listed - 1)];
+          const uint32_t word = a.mask[(size_t)b * a.mask_stride + (size_t)i * a.words + j / 32];
+          const uint64_t seen = __ballot(x + lane < listed && (word >> (j % 32) & 1));
+          if (lane == 0) paths[i - i0][x / 64] = seen;
+        }
       __syncthreads();
-      if (token / V % RT / 64 != wave) token = -1;
+      for (int x = tid; x < listed; x += RT) who[x] = (uint16_t)(a.tokens[(size_t)b * a.rows + who[x]] - (uint32_t)id0);
+      __syncthreads();
+      token = who[min(lane, listed - 1)];
+      if (lane >= listed || token / V % RT / 64 != wave) token = -1;
     }
 #pragma unroll
     for (int e = 0; e < PER; e++) {
@@ -193,6 +200,8 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
       bias[l] = at >= 0 ? a.bias[at] : 0.0f;
     }
     in_order();
+    one = lane < changes ? list[WIDS * wave + lane] : first;
+    onebias = bias[one];
   }
 
   auto row = [&](auto all, Row &now, int i) {
@@ -206,14 +215,10 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
     if (changes) {
       // The tokens on node i's path among this wavefront's ids: one more of each (or one less).
       auto add = [&](uint32_t more) {
-        if (few) {
-          if (token >= 0 && (paths[i - i0] >> lane & 1)) atomicAdd(&times[token], more);
-          return;
-        }
-        for (int x = lane; x < listed; x += 64) {
-          const int j = who[x], id = (int)a.tokens[(size_t)b * a.rows + j] - id0;
-          if (id / V % RT / 64 == wave && (a.mask[(size_t)b * a.mask_stride + (size_t)i * a.words + j / 32] >> (j % 32) & 1))
-            atomicAdd(&times[id], more);
+        if (token >= 0 && (paths[i - i0][0] >> lane & 1)) atomicAdd(&times[token], more);
+        for (int x = 64 + lane; x < listed; x += 64) {
+          const int id = who[x];
+          if (id / V % RT / 64 == wave && (paths[i - i0][x / 64] >> lane & 1)) atomicAdd(&times[id], more);
         }
       };
       add(2u);
@@ -221,12 +226,16 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
       for (int t = 0; t < PER / 4; t++)
         *(floatx4 *)(values + mine(4 * t)) = floatx4{v[4 * t], v[4 * t + 1], v[4 * t + 2], v[4 * t + 3]};
       in_order();
-      for (int x = lane; x < changes; x += 64) {
-        const int l = list[WIDS * wave + x];
+      auto change = [&](int l, float add) {
         const uint32_t c = times[l] >> 1;
         float y = values[l];
         if (c) y = ((y > 0.0f ? y / r : y * r) - f * (float)c) - p;
-        values[l] = y + bias[l];
+        values[l] = y + add;
+      };
+      if (lane < changes) change(one, onebias);
+      for (int x = 64 + lane; x < changes; x += 64) {
+        const int l = list[WIDS * wave + x];
+        change(l, bias[l]);
       }
       in_order();
 #pragma unroll
@@ -273,20 +282,19 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
     best = xlane::wave_max(best);
     // Its first place, which the others' mass against it leaves out.
     int at = INT_MAX;
-    if (best > -INFINITY)
+    if (best > -INFINITY) {
 #pragma unroll
-      for (int t = 0; t < G; t++) {
+      for (int t = G - 1; t >= 0; t--) {
+        int e0 = V - 1;
+#pragma unroll
+        for (int e = V - 2; e >= 0; e--) e0 = v[V * t + e] == best ? e : e0;
         const uint64_t any = __ballot(tops[t] == best);
-        if (!any || at != INT_MAX) continue;
-        const int l = (int)__builtin_ctzll(any);
-#pragma unroll
-        for (int e = 0; e < V; e++) {
-          const int x = __builtin_bit_cast(int, v[V * t + e]);
-          if (at != INT_MAX || __builtin_bit_cast(float, __builtin_amdgcn_readlane(x, l)) != best) continue;
-          at = V * (64 * wave + l + RT * t) + e;
-          if (lane == l) v[V * t + e] = -INFINITY;
-        }
+        const int l = any ? (int)__builtin_ctzll(any) : 0, place = V * (64 * wave + l + RT * t) + __builtin_amdgcn_readlane(e0, l);
+        at = any ? place : at;
       }
+#pragma unroll
+      for (int e = 0; e < PER; e++) v[e] = at - first == V * RT * (e / V) + e % V ? -INFINITY : v[e];
+    }
     float rest = 0.0f;
     const float m = best == -INFINITY ? 0.0f : best;
 #pragma unroll
@@ -376,7 +384,7 @@ int launch_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *r, const v
   // 131071 f16 ids for 8 requests took 115, 107, 107, 113 and 142 us with 4, 8, 12, 16 and 32 of them), or so few that
   // there are 5 workgroups a CU.
   const size_t want = 5 * (size_t)(ctx->cus > 0 ? ctx->cus : 256), each = (size_t)chunks * t->batch;
-  int groups = (int)std::min<size_t>(t->rows, std::max<size_t>((want + each - 1) / each, (t->rows + 9) / 10));
+  int groups = (int)std::min<size_t>(t->rows, std::max<size_t>((want + each - 1) / each, (t->rows + GROUP - 1) / GROUP));
   const int group = (t->rows + groups - 1) / groups;
   groups = (t->rows + group - 1) / group;
   if (each * groups >= (size_t)1 << 24) return wh_fail(ctx, WH_EARG, "logit rules: %zu rows of %d ids", nodes, vocab);

@@ -840,19 +840,45 @@ struct KeepArgs {
   int rows, cols, d, parts;
 };
 
-// The kept nodes' K and V into the caches: a thread per pair of values, K's pairs and then V's.
+// The kept nodes' K and V into the caches: a thread per pair of values, K's pairs and then V's.  Bound by its chain of
+// loads and by K's layout, whose words of a position lie `cols` apart: AT positions' rows are loaded side by side, and
+// four neighbouring positions' words of a pair of K go in one store (9 nodes of 1280 values for 32 sequences and 4
+// layers: 9.7 us, 1.9 TB/s; word by word 11.4).
 template <typename T>
 __global__ __launch_bounds__(256) void keep_kernel(KeepArgs a) {
+  typedef T Pair __attribute__((ext_vector_type(2)));
+  typedef Pair any __attribute__((aligned(4)));
+  typedef uint32_t Words __attribute__((ext_vector_type(4)));
+  typedef Words words_at __attribute__((aligned(4)));
+  constexpr int AT = 8;
   const int part = blockIdx.x % a.parts, b = blockIdx.x / a.parts, layer = blockIdx.y;
   const int i = part * 256 + threadIdx.x, half = a.d / 2;
   if (i >= a.d) return;
-  const int kept = a.kept[b], n = a.n_out[b] - kept, c = i < half ? i : i - half;
+  const int c = i < half ? i : i - half;
   const T *x = (const T *)(i < half ? a.k : a.v) + layer * a.layer_stride + (size_t)b * a.rows * a.stride + 2 * c;
-  uint32_t *y = a.kv + layer * a.kv_layer_stride + b * a.kv_stride;
-  for (int s = 0; s < kept; s++) {
-    const T *p = x + (size_t)a.path[(size_t)b * a.rows + s] * a.stride;
-    const uint32_t lo = __builtin_bit_cast(uint16_t, (_Float16)p[0]), hi = __builtin_bit_cast(uint16_t, (_Float16)p[1]);
-    y[i < half ? (size_t)c * a.cols + n + s : (size_t)half * a.cols + (size_t)(n + s) * half + c] = lo | hi << 16;
+  const int32_t *path = a.path + (size_t)b * a.rows;
+  const int kept = a.kept[b], n = a.n_out[b] - kept;
+  uint32_t *y = a.kv + layer * a.kv_layer_stride + b * a.kv_stride +
+                (i < half ? (size_t)c * a.cols + n : (size_t)half * a.cols + (size_t)n * half + c);
+  const size_t step = i < half ? 1 : half;
+  for (int s = 0; s < kept; s += AT) {
+    Pair p[AT];
+#pragma unroll
+    for (int e = 0; e < AT; e++) p[e] = *(const any *)(x + (size_t)max(path[min(s + e, a.rows - 1)], 0) * a.stride);
+#pragma unroll
+    for (int e = 0; e < AT; e += 4) {
+      Words w;
+#pragma unroll
+      for (int f = 0; f < 4; f++)
+        w[f] = __builtin_bit_cast(uint16_t, (_Float16)p[e + f][0]) | (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)p[e + f][1]) << 16;
+      if (i < half && s + e + 4 <= kept) {
+        *(words_at *)(y + s + e) = w;
+      } else {
+#pragma unroll
+        for (int f = 0; f < 4; f++)
+          if (s + e + f < kept) y[(s + e + f) * step] = w[f];
+      }
+    }
   }
 }
 
