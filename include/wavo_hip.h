@@ -385,8 +385,10 @@ typedef struct wh_tree {
  * positions of kv_heads * hd values each, kv_stride words apart (0: one cache for all).  o:
  * [batch * rows][heads * hd], f32 or (out16) f16.  Products of f32 queries and of the f32 softmax keep
  * their precision (each is split into two f16 parts); f16 queries are exact, and with out16 the softmax
- * weights are rounded to f16.  Masked keys and values may hold anything.  hd % 4 == 0, hd <= 128, cols <= 2^24,
- * heads % kv_heads == 0; f32 pointers and f16 rows 4-byte aligned (stride even for f16). */
+ * weights are rounded to f16.  Masked keys and values may hold anything.  o overlaps none of the inputs.
+ * hd % 4 == 0, hd <= 128, cols <= 2^24, heads % kv_heads == 0, heads <= 1024, stride <= 2^23; pointers
+ * 4-byte aligned (stride even for f16).  batch <= 65535 for up to 16 rows of a key head (rows * heads /
+ * kv_heads), fewer for more (one for every 64 or 128 of them), and batch * rows * heads < 2^25. */
 int wh_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void *k, const void *v, size_t stride,
                    int in16, const uint32_t *kv, size_t kv_stride, int cols, void *o, int out16, int heads,
                    int kv_heads, int hd);
@@ -415,9 +417,10 @@ typedef struct wh_rules {
  * f16; vocab values each), in the order penalties, bias, mask, in f32: into out (the same layout;
  * may be logits itself, or NULL: not written), with pick[r] the first maximum (0xffffffff where
  * nothing is left; NaN is never picked) and logprob[r] its log-softmax over the row (minus infinity
- * where nothing is left, NaN where the row holds one), either of which may be NULL.  Pick and log-probability are those of the f32
- * values, before an f16 output is rounded.  Ids past vocab in history, tokens and bias_id are passed
- * over.  search::decode's `pick` for rows of many requests (src/whisper/search.rs:46-59). */
+ * where nothing is left, NaN where the row holds one), either of which may be NULL.  Pick and
+ * log-probability are those of the f32 values, before an f16 output is rounded.  Ids past vocab in
+ * history, tokens and bias_id are passed over.  vocab <= 2^28; batch * vocab / 2048 workgroups of ten
+ * rows have to be fewer than 2^24.  search::decode's `pick` for rows of many requests (src/whisper/search.rs:46-59). */
 int wh_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *rules, const void *logits, void *out, int vocab,
                    size_t ld, int f16, uint32_t *pick, float *logprob);
 
@@ -437,7 +440,7 @@ typedef struct wh_kept {
  * token is the pick of its parent (picks[b][i], wh_logit_rules' pick of node i), as long as there is one
  * and the sequence has room in its `cols` positions.  path[b]: the kept nodes, then -1; kept[b]: their
  * number; next[b]: the token after them (the last kept node's pick; the root's token where there was no
- * room for it; as it was where the sequence has no nodes); n_out[b] = n[b] + kept[b] (may be n itself).
+ * room for it; as it was where the sequence has no nodes; may be tokens itself where rows is 1); n_out[b] = n[b] + kept[b] (may be n itself).
  * history [batch][history_cols] (or NULL) gets the kept tokens at n[b] .. (and then has to have room,
  * too), and, with where != NULL, the caches get the kept nodes' keys and values there.  The masks are
  * those of trees: bit j of i for j = i and all ancestors, so that i's parent is the highest one below i. */

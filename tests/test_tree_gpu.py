@@ -171,6 +171,36 @@ def test_attend(gpu, shape, in16, out16):
     check_attend(got, q, k, v, seen, n, None, kc, vc, heads, kv_heads, hd, in16, out16)
 
 
+# Many rows of the smallest heads, and of caches shorter than a load: several row blocks of the kernel for few rows.
+NARROW = [(3, 70, 2, 2, 4, 333, [333, 0, 200]), (2, 70, 3, 1, 64, 3, [3, 2]), (2, 41, 2, 2, 128, 2, [1, 2]), (1, 90, 1, 1, 4, 1, [1]),
+          (1, 75, 2, 1, 8, 5, [5]), (2, 70, 1, 1, 12, 4, [4, 3])]
+
+
+@pytest.mark.parametrize("in16,out16", [(False, False), (True, True)])
+@pytest.mark.parametrize("shape", NARROW, ids=lambda s: "x".join(str(x) for x in s[:6]))
+def test_attend_narrow(gpu, shape, in16, out16):
+    test_attend(gpu, shape, in16, out16)
+
+
+@pytest.mark.parametrize("rows", [2, 70])
+def test_attend_splits_of_very_different_scores(gpu, rows):
+    """A long cache whose thirds have scores near -1e34, 0 and 1e34, with the large ones first, last and in the middle:
+    shares of a row that are joined across wavefronts and workgroups, one of which carries all of it."""
+    batch, heads, hd, cols = 3, 1, 64, 6000
+    rng, q, _, _, _, kc, vc = case(9, batch, rows, heads, heads, hd, cols)
+    q[:] = 0
+    q[:, :, 0] = 1e33
+    kc[:, :, 0] = 0
+    n = [6000, 5999, 5000]
+    for b, top in enumerate((0, 2000, 4000)):
+        kc[b, (np.arange(2000) + top + 2000) % 6000, 0] = -8
+        kc[b, top:top + 2000:7, 0] = 8
+    got = attend(gpu, q, None, None, None, n, None, kc, vc, heads, heads, hd)
+    for b, top in enumerate((0, 2000, 4000)):  # equal scores there, and weights of zero everywhere else
+        vals = vc[b, top:min(top + 2000, n[b]):7].astype(np.float64)
+        assert np.all(np.abs(got[b] - vals.mean(0)) <= (2 * len(vals) * EPS + 2.0**-20) * np.abs(vals).max())
+
+
 @pytest.mark.parametrize("in16", [False, True])
 @pytest.mark.parametrize("heads,kv_heads,hd", [(4, 4, 64), (6, 2, 128), (2, 1, 40)])
 def test_attend_ragged_any_mask_and_masked_garbage(gpu, heads, kv_heads, hd, in16):
@@ -406,6 +436,7 @@ def check_rules(c, f16, o, pick, logprob, ld_more=0, penalty=True, bias=True, al
 
 RULES = [(1, 1, 1, 1, 0), (1, 1, 33, 3, 5), (2, 5, 1000, 20, 30), (1, 3, 4096, 10, 4), (3, 1, 4097, 300, 100), (2, 33, 5000, 64, 10),
          (1, 70, 12289, 700, 400), (1, 2, 51866, 448, 100), (5, 9, 8191, 5, 1)]
+CROWDED = [(2, 300, 2500, 100, 1900), (1, 1024, 700, 30, 5), (1, 130, 2049, 9000, 3000)]  # nodes and listed ids past 64 in a run of ids
 
 
 @pytest.mark.parametrize("f16", [False, True])
@@ -414,6 +445,29 @@ def test_rules(gpu, shape, f16):
     for seed, ld_more, out in ((1, 0, "new"), (2, 1, "same"), (3, 38, "none")):
         c = rules_case(seed, *shape, f16)
         check_rules(c, f16, *run_rules(gpu, c, f16, ld_more, out=out), ld_more, out=out)
+
+
+@pytest.mark.parametrize("f16", [False, True])
+@pytest.mark.parametrize("shape", CROWDED, ids=lambda s: "x".join(str(x) for x in s))
+def test_rules_crowded(gpu, shape, f16):
+    c = rules_case(11, *shape, f16)
+    check_rules(c, f16, *run_rules(gpu, c, f16), out="new")
+
+
+def test_rules_infinite_biases_past_the_vocabulary(gpu):
+    """Ids from vocab on, inside the last run of ids: infinite biases and penalties there must not reach the sums."""
+    batch, rows, vocab = 2, 3, 2050
+    c = rules_case(12, batch, rows, vocab, 20, 0, False)
+    c["start"] = np.array([0, 2, 4])
+    c["bias_id"], c["bias"] = np.array([2050, 4095, 2051, 3000]), np.array([np.inf, np.nan, np.inf, np.inf], np.float32)
+    c["history"][:, :3] = [2050, 4095, 2060]
+    c["n"][:] = 20
+    c["tokens"][:] = 2055
+    c["penalty"][:] = [0.0, -np.inf, np.nan]
+    c["history"][:, 3:] = 2070
+    got = run_rules(gpu, c, False, penalty=True)
+    check_rules(c, False, *got)
+    assert np.isfinite(got[2][got[2] != 77]).all()
 
 
 @pytest.mark.parametrize("f16", [False, True])
@@ -557,6 +611,26 @@ def test_accept_forms(gpu, in_place):
     run_accept(gpu, 4, *shape, False, in_place=in_place, history_more=-9, vocab=1)
     run_accept(gpu, 5, *shape, True, in_place=in_place, history_more=9, vocab=1)
     run_accept(gpu, 6, *shape, False, in_place=in_place, move=False, history=False)
+
+
+def test_accept_root_alone_in_place(gpu):
+    """Steps without drafts: the next tokens take the roots' place, their lengths grow, the texts get what they were."""
+    batch, steps = 5, 3
+    picks = np.arange(100, 100 + batch * steps, dtype=np.uint32).reshape(steps, batch)
+    tokens, n = gpu.upload(np.arange(batch, dtype=np.uint32)), gpu.upload(np.array([0, 1, 2, 8, 9], np.int32))
+    mask, text = gpu.upload(np.ones((batch, 1), np.uint32)), gpu.upload(np.full((batch, 10), 7, np.uint32))
+    path, kept = gpu.buffer(batch), gpu.buffer(batch)
+    for p in picks:
+        pb = gpu.upload(p)
+        gpu.tree_accept(wa.Tree(batch, 1, n, None, tokens, mask, 1), pb, None, None, 0, 0, None, 0, 0, 0, 10, 0, path, kept, tokens, n,
+                        text, 10)
+    got = gpu.read(text, (batch, 10), np.uint32)
+    for b, first in enumerate((0, 1, 2, 8, 9)):
+        made = [b, *picks[:, b].tolist()]
+        room = min(steps, 10 - first)
+        assert got[b].tolist() == [7] * first + made[:room] + [7] * (10 - first - room)
+        assert gpu.read(n, (batch,), np.int32)[b] == first + room
+        assert gpu.read(tokens, (batch,), np.uint32)[b] == made[room]
 
 
 def test_accept_one_tree_for_all(gpu):

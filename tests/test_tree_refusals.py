@@ -101,6 +101,12 @@ int main() {
   attend("misaligned q", "aligned", [](Attend &a) { a.q = at<void>(4098); });
   attend("misaligned cache", "aligned", [](Attend &a) { a.kv = at<uint32_t>(4097); });
   attend("odd f16 rows", "aligned", [](Attend &a) { a.in16 = 1, a.stride = 961; });
+  attend("sequences past a launch", "in one call", [](Attend &a) { a.t.batch = 65536, a.t.rows = 1; });
+  attend("heads past a launch", "in one call", [](Attend &a) {
+    a.t.batch = 4096, a.t.rows = 64, a.t.mask_stride = 0, a.heads = a.kv_heads = 128, a.hd = 4, a.kv_stride = 0;
+  });
+  attend("positions past the most", "shape", [](Attend &a) { a.cols = (1 << 24) + 1, a.kv_stride = 0; });
+  attend("rows just too far", "apart", [](Attend &a) { a.stride = ((size_t)1 << 23) + 1; });
   rules("no rules", "needed", [](RulesCall &) {}, false);
   rules("no logits", "needed", [](RulesCall &a) { a.logits = nullptr; });
   rules("no output", "needed", [](RulesCall &a) { a.out = nullptr, a.pick = nullptr, a.logprob = nullptr; });
@@ -116,6 +122,7 @@ int main() {
   rules("misaligned logits", "misaligned", [](RulesCall &a) { a.logits = at<void>(4098); });
   rules("misaligned f16 logits", "misaligned", [](RulesCall &a) { a.f16 = 1, a.logits = at<void>(4097); });
   rules("misaligned picks", "misaligned", [](RulesCall &a) { a.pick = at<uint32_t>(4098); });
+  rules("rows past a launch", "rows of", [](RulesCall &a) { a.t.batch = 1 << 18, a.t.rows = 1, a.vocab = 1 << 20, a.ld = 1 << 20; });
   rules("no lengths", "tree", [](RulesCall &a) { a.t.n = nullptr; });
   accept("no tokens", "needed", [](Accept &a) { a.t.tokens = nullptr; });
   accept("no masks", "needed", [](Accept &a) { a.t.mask = nullptr; });
@@ -137,6 +144,9 @@ int main() {
   accept("caches too close", "apart", [](Accept &a) { a.w.kv_stride = 159; });
   accept("layers' caches too close", "apart", [](Accept &a) { a.w.kv_layer_stride = 159; });
   accept("misaligned keys", "aligned", [](Accept &a) { a.w.k = at<void>(4098); });
+  accept("rows past a launch", "in one call", [](Accept &a) {
+    a.t.batch = 1 << 20, a.t.rows = 1, a.t.mask_stride = 0, a.w.d = 1 << 16, a.w.stride = 1 << 16, a.w.layers = 1, a.w.kv_stride = 5 << 16;
+  });
   accept("odd f16 rows", "aligned", [](Accept &a) { a.w.in16 = 1, a.w.stride = 97; });
   printf("%d calls, %d not refused\n", calls, bad);
   return bad != 0;

@@ -377,7 +377,6 @@ int launch_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *r, const v
   if (((uintptr_t)r->penalty | (uintptr_t)r->history | (uintptr_t)r->bias_start | (uintptr_t)r->bias_id | (uintptr_t)r->bias |
        (uintptr_t)r->allow | (uintptr_t)pick | (uintptr_t)logprob) % 4 || ((uintptr_t)logits | (uintptr_t)out) % (f16 ? 2 : 4))
     return wh_fail(ctx, WH_EARG, "logit rules: misaligned arrays");
-  if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "logit rules: %s", hipGetErrorString(e));
   const size_t nodes = (size_t)t->batch * t->rows;
   const int chunks = (vocab + IDS - 1) / IDS, parts = chunks * (RT / 64);
   // Rows per workgroup: about ten (fewer count the text too often, more leave the last workgroups alone: 61 rows of
@@ -388,6 +387,7 @@ int launch_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *r, const v
   const int group = (t->rows + groups - 1) / groups;
   groups = (t->rows + group - 1) / group;
   if (each * groups >= (size_t)1 << 24) return wh_fail(ctx, WH_EARG, "logit rules: %zu rows of %d ids", nodes, vocab);
+  if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "logit rules: %s", hipGetErrorString(e));
   RulePart *part = nullptr;
   if ((pick || logprob) && !(part = (RulePart *)wh_scratch(ctx, sizeof(RulePart) * parts * nodes))) return WH_EOOM;
   const RuleArgs a{t->n, t->count, t->tokens, t->mask, t->mask_stride, t->rows, (t->rows + 31) / 32, r->penalty, r->history,

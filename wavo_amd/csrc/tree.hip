@@ -822,13 +822,14 @@ __global__ __launch_bounds__(256) void accept_kernel(AcceptArgs a) {
     for (int i = 0; i < count && k < room; i = child[i]) path[k++] = i;
     kept = k;
     a.kept[b] = k;
-    if (count) a.next[b] = k ? picks[path[k - 1]] : tokens[0];
     a.n_out[b] = n + k;
   }
   __syncthreads();
   for (int i = tid; i < a.rows; i += 256) a.path[(size_t)b * a.rows + i] = i < kept ? path[i] : -1;
   if (a.history)
     for (int i = tid; i < kept; i += 256) a.history[(size_t)b * a.history_cols + n + i] = tokens[path[i]];
+  __syncthreads();  // (next may be the tokens themselves, where a root is all there is)
+  if (tid == 0 && count) a.next[b] = kept ? picks[path[kept - 1]] : tokens[0];
 }
 
 struct KeepArgs {
@@ -943,7 +944,6 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
     return wh_fail(ctx, WH_EARG, "tree attention: caches of %zu words %zu apart", (size_t)cols * kv_heads * hd, kv_stride);
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)kv | (uintptr_t)o) % 4 || (in16 && stride % 2))
     return wh_fail(ctx, WH_EARG, "tree attention: buffers and rows must be 4-byte aligned");
-  if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "tree attention: %s", hipGetErrorString(e));
   AttendArgs a{q, k, v, stride, kv, kv_stride, o, t->n, t->count, t->mask, t->mask_stride, t->batch, t->rows, (t->rows + 31) / 32,
                cols, heads, kv_heads, hd, 1.0f / sqrtf((float)hd), 1, 1, 1, few_block(hd), NODES, nullptr, nullptr};
   const int rows = t->rows * (heads / kv_heads), tiles = (rows + 15) / 16;
@@ -960,6 +960,7 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
   const size_t nodes = (size_t)t->batch * t->rows;
   if ((size_t)t->batch * a.row_blocks > 65535 || units * a.splits >= (size_t)1 << 22 || nodes * heads >= (size_t)1 << 25)  // (a launch's limits)
     return wh_fail(ctx, WH_EARG, "tree attention: %d heads of %zu nodes in one call", heads, nodes);
+  if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "tree attention: %s", hipGetErrorString(e));
   if (a.splits > 1) {
     const size_t part = (size_t)a.splits * nodes * heads;
     if (!(a.po = (float *)wh_scratch(ctx, part * (hd + 4) * sizeof(float)))) return WH_EOOM;
@@ -984,6 +985,8 @@ int launch_tree_accept(wh_ctx *ctx, const wh_tree *t, const uint32_t *picks, con
     const size_t cache = (size_t)cols * w->d;
     if ((t->batch > 1 && w->kv_stride < cache) || (w->layers > 1 && w->kv_layer_stride < cache))
       return wh_fail(ctx, WH_EARG, "tree accept: caches of %zu words %zu and %zu apart", cache, w->kv_stride, w->kv_layer_stride);
+    if ((size_t)t->batch * ((w->d + 255) / 256) >= (size_t)1 << 24)  // (a launch's limit)
+      return wh_fail(ctx, WH_EARG, "tree accept: %d sequences' rows of %d values in one call", t->batch, w->d);
     if (((uintptr_t)w->k | (uintptr_t)w->v | (uintptr_t)w->kv) % 4 || (w->in16 && (w->stride % 2 || w->layer_stride % 2)))
       return wh_fail(ctx, WH_EARG, "tree accept: buffers and rows must be 4-byte aligned");
   }
