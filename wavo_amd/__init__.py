@@ -249,8 +249,8 @@ class _Tensor(ctypes.Structure):
 
 def _p(x):
     """A device pointer argument: Buffer, int or None."""
-    if x is None:
-        return None
+    if x is None or type(x) is int:
+        return x
     if isinstance(x, Buffer):
         return x.ptr
     return int(x)

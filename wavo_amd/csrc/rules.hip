@@ -6,8 +6,8 @@
 // rule can change (few, but for the most frequent ids).  Then the wavefronts go through the rows without meeting, two
 // rows' loads ahead: a row's values go to LDS, the listed ones are changed there, a lane for each, and come back.  The
 // tree's tokens differ from node to node: those on a node's path are added to the counts before its row and taken
-// back after it.  Each wavefront leaves a maximum and a sum of its own, which a second launch joins (one wavefront a
-// row).
+// back after it.  Each wavefront leaves a maximum and a sum of its own, which the last workgroup of a run of rows to
+// be through joins, or a second launch (one wavefront a row).
 //
 // The log-softmax is kept as the sum of exp(x − max) over every id but the maximum itself, so that a row
 // with one likely id keeps its precision: logprob = −log1p(sum).
@@ -27,6 +27,17 @@ struct RulePart {
   float best, rest;
   int at, pad;
 };
+// For parts that pass between workgroups of one launch: each half is stored to and loaded from where all XCDs see it.
+__device__ __forceinline__ void store_part(RulePart *p, RulePart x) {
+  const uint64_t *w = (const uint64_t *)&x;
+  for (int e = 0; e < 2; e++) __hip_atomic_store((uint64_t *)p + e, w[e], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ RulePart load_part(const RulePart *p) {
+  RulePart x;
+  for (int e = 0; e < 2; e++)
+    ((uint64_t *)&x)[e] = __hip_atomic_load((const uint64_t *)p + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return x;
+}
 
 struct RuleArgs {
   const int32_t *n, *count;
@@ -46,6 +57,9 @@ struct RuleArgs {
   int vocab, chunks, group, groups;  // rows per workgroup; workgroups per sequence and chunk
   size_t ld;
   RulePart *part;  // [batch * rows][chunks][wavefront], or NULL: neither picks nor log-probabilities are asked for
+  uint32_t *pick;
+  float *logprob;
+  int *done;  // [batch * groups] workgroups that are through (0 between launches), or NULL: another launch joins the parts
 };
 
 __device__ __forceinline__ bool better(float ov, int oi, float v, int i) { return ov > v || (ov == v && oi < i); }
@@ -67,6 +81,42 @@ struct Piece<_Float16> {
   typedef half8 any __attribute__((aligned(2)));
   static constexpr int N = 8;
 };
+
+// (best, rest, at) of two runs of ids: the greater maximum, and the other one's mass against it.
+__device__ __forceinline__ void join(float &best, float &rest, int &at, float ob, float orest, int oat) {
+  if (better(ob, oat, best, at)) {
+    float x = best;
+    best = ob, ob = x;
+    x = rest, rest = orest, orest = x;
+    const int y = at;
+    at = oat, oat = y;
+  }
+  if (ob == -INFINITY) rest += orest;  // (nothing there, or NaN)
+  else rest += (1.0f + orest) * __expf(ob - best);
+}
+
+// One wavefront joins a row's parts.
+__device__ __forceinline__ void join_row(const RulePart *part, int parts, int lane, uint32_t *pick, float *logprob) {
+  float best = -INFINITY, rest = 0.0f;
+  int at = INT_MAX;
+  for (int c = lane; c < parts; c += 256) {  // (4 loads at a time)
+    RulePart p[4];
+#pragma unroll
+    for (int y = 0; y < 4; y++) p[y] = load_part(part + min(c + 64 * y, parts - 1));
+#pragma unroll
+    for (int y = 0; y < 4; y++)
+      if (c + 64 * y < parts) join(best, rest, at, p[y].best, p[y].rest, p[y].at);
+  }
+  for (int d = 32; d; d >>= 1) {
+    const float ob = __shfl_xor(best, d), orest = __shfl_xor(rest, d);
+    const int oat = __shfl_xor(at, d);
+    join(best, rest, at, ob, orest, oat);
+  }
+  if (lane) return;
+  if (pick) *pick = best == -INFINITY ? 0xffffffffu : (uint32_t)at;
+  // (best − best: NaN beside an infinity, as in the quotient it stands for)
+  if (logprob) *logprob = rest != rest ? rest : best == -INFINITY ? best : (best - best) - log1pf(rest);
+}
 
 // Keeps what a wavefront does in LDS in the order it is written in (its accesses are served in order).
 __device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
@@ -300,7 +350,12 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
 #pragma unroll
     for (int e = 0; e < PER; e++) rest += __expf(v[e] - m);
     rest = xlane::wave_sum(rest);
-    if (lane == 0) a.part[((row0 + i) * a.chunks + chunk) * (RT / 64) + wave] = {best, rest, at == INT_MAX ? at : id0 + at, 0};
+    if (lane == 0) {
+      RulePart *p = a.part + ((row0 + i) * a.chunks + chunk) * (RT / 64) + wave;
+      const RulePart x{best, rest, at == INT_MAX ? at : id0 + at, 0};
+      if (a.done) store_part(p, x);
+      else *p = x;
+    }
   };
   auto rows = [&](auto all) {
     for (int i = i0;;) {
@@ -312,45 +367,25 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
   };
   if (whole) rows(std::true_type{});
   else rows(std::false_type{});
+
+  if (!a.done) return;
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // (this wavefront's parts are out)
+  __syncthreads();
+  int &last = *(int *)times, at = b * a.groups + i0 / a.group;
+  if (tid == 0) last = atomicAdd(&a.done[at], 1) == a.chunks - 1;
+  __syncthreads();
+  if (!last) return;
+  const int parts = a.chunks * (RT / 64);
+  for (int i = i0 + wave; i < i1; i += RT / 64)
+    join_row(a.part + (row0 + i) * parts, parts, lane, a.pick ? a.pick + row0 + i : nullptr, a.logprob ? a.logprob + row0 + i : nullptr);
+  if (tid == 0) a.done[at] = 0;
 }
 
-// (best, rest, at) of two runs of ids: the greater maximum, and the other one's mass against it.
-__device__ __forceinline__ void join(float &best, float &rest, int &at, float ob, float orest, int oat) {
-  if (better(ob, oat, best, at)) {
-    float x = best;
-    best = ob, ob = x;
-    x = rest, rest = orest, orest = x;
-    const int y = at;
-    at = oat, oat = y;
-  }
-  if (ob == -INFINITY) rest += orest;  // (nothing there, or NaN)
-  else rest += (1.0f + orest) * __expf(ob - best);
-}
-
-// One wave per row joins its parts.
 __global__ __launch_bounds__(64) void rules_pick_kernel(const RulePart *part, const int32_t *counts, int rows, int parts,
                                                         uint32_t *pick, float *logprob) {
-  const int row = blockIdx.x, lane = threadIdx.x;
+  const int row = blockIdx.x;
   if (counts && row % rows >= counts[row / rows]) return;
-  float best = -INFINITY, rest = 0.0f;
-  int at = INT_MAX;
-  for (int c = lane; c < parts; c += 256) {  // (4 loads at a time)
-    RulePart p[4];
-#pragma unroll
-    for (int y = 0; y < 4; y++) p[y] = part[(size_t)row * parts + min(c + 64 * y, parts - 1)];
-#pragma unroll
-    for (int y = 0; y < 4; y++)
-      if (c + 64 * y < parts) join(best, rest, at, p[y].best, p[y].rest, p[y].at);
-  }
-  for (int d = 32; d; d >>= 1) {
-    const float ob = __shfl_xor(best, d), orest = __shfl_xor(rest, d);
-    const int oat = __shfl_xor(at, d);
-    join(best, rest, at, ob, orest, oat);
-  }
-  if (lane) return;
-  if (pick) pick[row] = best == -INFINITY ? 0xffffffffu : (uint32_t)at;
-  // (best − best: NaN beside an infinity, as in the quotient it stands for)
-  if (logprob) logprob[row] = rest != rest ? rest : best == -INFINITY ? best : (best - best) - log1pf(rest);
+  join_row(part + (size_t)row * parts, parts, threadIdx.x, pick ? pick + row : nullptr, logprob ? logprob + row : nullptr);
 }
 
 template <typename T>
@@ -382,7 +417,8 @@ int launch_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *r, const v
   // Rows per workgroup: about ten (fewer count the text too often, more leave the last workgroups alone: 61 rows of
   // 131071 f16 ids for 8 requests took 115, 107, 107, 113 and 142 us with 4, 8, 12, 16 and 32 of them), or so few that
   // there are 5 workgroups a CU.
-  const size_t want = 5 * (size_t)(ctx->cus > 0 ? ctx->cus : 256), each = (size_t)chunks * t->batch;
+  const int cus = ctx->cus > 0 ? ctx->cus : 256;
+  const size_t want = 5 * (size_t)cus, each = (size_t)chunks * t->batch;
   int groups = (int)std::min<size_t>(t->rows, std::max<size_t>((want + each - 1) / each, (t->rows + GROUP - 1) / GROUP));
   const int group = (t->rows + groups - 1) / groups;
   groups = (t->rows + group - 1) / group;
@@ -390,14 +426,17 @@ int launch_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *r, const v
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "logit rules: %s", hipGetErrorString(e));
   RulePart *part = nullptr;
   if ((pick || logprob) && !(part = (RulePart *)wh_scratch(ctx, sizeof(RulePart) * parts * nodes))) return WH_EOOM;
+  // Who joins the parts: up to a workgroup a CU their last one (a row of 51866 f32 ids 9.7 us, 11.2 with a second launch,
+  // whose start costs more than the counting); more of them wait for each other's counts (18 such rows 13.5 us counted,
+  // 12.7 in two launches, 48 of them 18.7 and 14.7).
   const RuleArgs a{t->n, t->count, t->tokens, t->mask, t->mask_stride, t->rows, (t->rows + 31) / 32, r->penalty, r->history,
                    r->history_cols, r->from, r->bias_start, r->bias_id, r->bias, r->bias_len, r->allow, logits, out, vocab,
-                   chunks, group, groups, ld, part};
+                   chunks, group, groups, ld, part, pick, logprob, part && each * groups <= (size_t)cus && t->batch * groups <= ATTEND_HEADS ? ctx->attend_count : nullptr};
   {
     ProfScope prof(ctx, "logit_rules", 0.0, (double)nodes * vocab * (f16 ? 2 : 4) * (out ? 2 : 1));
     if (int rc = f16 ? rules_launch<_Float16>(ctx, a, (int)each * groups) : rules_launch<float>(ctx, a, (int)each * groups)) return rc;
   }
-  if (!part) return WH_OK;
+  if (!part || a.done) return WH_OK;
   ProfScope prof(ctx, "logit_pick", 0.0, (double)sizeof(RulePart) * parts * nodes);
   wh_launch(ctx, rules_pick_kernel, (int)nodes, 64, 0, (const RulePart *)part, t->count, t->rows, parts, pick, logprob);
   return wh_launched(ctx, "logit pick");

@@ -796,12 +796,10 @@ struct AcceptArgs {
   int history_cols;
 };
 
-// One workgroup per sequence: every node's parent (the highest bit below its own) and whether its token is
-// the parent's pick; of a parent's agreeing children the first; then the walk from the root.
-__global__ __launch_bounds__(256) void accept_kernel(AcceptArgs a) {
-  __shared__ int child[TREE_ROWS], path[TREE_ROWS], kept;
-  const int tid = threadIdx.x, b = blockIdx.x;
-  const int n = min(max(a.n[b], 0), a.cols), count = a.count ? min(max(a.count[b], 0), a.rows) : a.rows;
+// The walk of sequence b, by a whole workgroup: every node's parent (the highest bit below its own) and whether its
+// token is the parent's pick; of a parent's agreeing children the first; then from the root on.  path: LDS.
+__device__ __forceinline__ int walk(const AcceptArgs &a, int b, int n, int count, int *child, int *path, int *kept) {
+  const int tid = threadIdx.x;
   const uint32_t *tokens = a.tokens + (size_t)b * a.rows, *picks = a.picks + (size_t)b * a.rows;
   for (int i = tid; i < count; i += 256) child[i] = INT_MAX;
   __syncthreads();
@@ -820,25 +818,41 @@ __global__ __launch_bounds__(256) void accept_kernel(AcceptArgs a) {
     if (a.history) room = min(room, a.history_cols - n);
     int k = 0;
     for (int i = 0; i < count && k < room; i = child[i]) path[k++] = i;
-    kept = k;
-    a.kept[b] = k;
-    a.n_out[b] = n + k;
+    *kept = k;
   }
   __syncthreads();
+  return *kept;
+}
+
+// What the walk says of sequence b.
+__device__ __forceinline__ void tell(const AcceptArgs &a, int b, int n, int count, const int *path, int kept) {
+  const int tid = threadIdx.x;
+  const uint32_t *tokens = a.tokens + (size_t)b * a.rows, *picks = a.picks + (size_t)b * a.rows;
   for (int i = tid; i < a.rows; i += 256) a.path[(size_t)b * a.rows + i] = i < kept ? path[i] : -1;
   if (a.history)
     for (int i = tid; i < kept; i += 256) a.history[(size_t)b * a.history_cols + n + i] = tokens[path[i]];
   __syncthreads();  // (next may be the tokens themselves, where a root is all there is)
-  if (tid == 0 && count) a.next[b] = kept ? picks[path[kept - 1]] : tokens[0];
+  if (tid == 0) {
+    a.kept[b] = kept;
+    a.n_out[b] = n + kept;
+    if (count) a.next[b] = kept ? picks[path[kept - 1]] : tokens[0];
+  }
+}
+
+__global__ __launch_bounds__(256) void accept_kernel(AcceptArgs a) {
+  __shared__ int child[TREE_ROWS], path[TREE_ROWS], kept;
+  const int b = blockIdx.x, n = min(max(a.n[b], 0), a.cols), count = a.count ? min(max(a.count[b], 0), a.rows) : a.rows;
+  const int k = walk(a, b, n, count, child, path, &kept);
+  tell(a, b, n, count, path, k);
 }
 
 struct KeepArgs {
-  const int32_t *path, *kept, *n_out;
   const void *k, *v;
   size_t stride, layer_stride;
   uint32_t *kv;
   size_t kv_stride, kv_layer_stride;
-  int rows, cols, d, parts;
+  int d, parts;
+  bool walks;  // the workgroups walk the trees themselves; otherwise the outputs are there
 };
 
 // The kept nodes' K and V into the caches: a thread per pair of values, K's pairs and then V's.  Bound by its chain of
@@ -846,26 +860,36 @@ struct KeepArgs {
 // four neighbouring positions' words of a pair of K go in one store (9 nodes of 1280 values for 32 sequences and 4
 // layers: 9.7 us, 1.9 TB/s; word by word 11.4).
 template <typename T>
-__global__ __launch_bounds__(256) void keep_kernel(KeepArgs a) {
+__global__ __launch_bounds__(256) void keep_kernel(AcceptArgs t, KeepArgs a) {
   typedef T Pair __attribute__((ext_vector_type(2)));
   typedef Pair any __attribute__((aligned(4)));
   typedef uint32_t Words __attribute__((ext_vector_type(4)));
   typedef Words words_at __attribute__((aligned(4)));
   constexpr int AT = 8;
+  __shared__ int child[TREE_ROWS], path[TREE_ROWS], found;
   const int part = blockIdx.x % a.parts, b = blockIdx.x / a.parts, layer = blockIdx.y;
+  int kept, n;
+  if (a.walks) {
+    n = min(max(t.n[b], 0), t.cols);
+    const int count = t.count ? min(max(t.count[b], 0), t.rows) : t.rows;
+    kept = walk(t, b, n, count, child, path, &found);
+    if (part == 0 && layer == 0) tell(t, b, n, count, path, kept);
+  } else {
+    kept = t.kept[b], n = t.n_out[b] - kept;
+    for (int i = threadIdx.x; i < kept; i += 256) path[i] = t.path[(size_t)b * t.rows + i];
+    __syncthreads();
+  }
   const int i = part * 256 + threadIdx.x, half = a.d / 2;
   if (i >= a.d) return;
   const int c = i < half ? i : i - half;
-  const T *x = (const T *)(i < half ? a.k : a.v) + layer * a.layer_stride + (size_t)b * a.rows * a.stride + 2 * c;
-  const int32_t *path = a.path + (size_t)b * a.rows;
-  const int kept = a.kept[b], n = a.n_out[b] - kept;
+  const T *x = (const T *)(i < half ? a.k : a.v) + layer * a.layer_stride + (size_t)b * t.rows * a.stride + 2 * c;
   uint32_t *y = a.kv + layer * a.kv_layer_stride + b * a.kv_stride +
-                (i < half ? (size_t)c * a.cols + n : (size_t)half * a.cols + (size_t)n * half + c);
+                (i < half ? (size_t)c * t.cols + n : (size_t)half * t.cols + (size_t)n * half + c);
   const size_t step = i < half ? 1 : half;
   for (int s = 0; s < kept; s += AT) {
     Pair p[AT];
 #pragma unroll
-    for (int e = 0; e < AT; e++) p[e] = *(const any *)(x + (size_t)max(path[min(s + e, a.rows - 1)], 0) * a.stride);
+    for (int e = 0; e < AT; e++) p[e] = *(const any *)(x + (size_t)path[min(s + e, kept - 1)] * a.stride);
 #pragma unroll
     for (int e = 0; e < AT; e += 4) {
       Words w;
@@ -993,18 +1017,31 @@ int launch_tree_accept(wh_ctx *ctx, const wh_tree *t, const uint32_t *picks, con
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "tree accept: %s", hipGetErrorString(e));
   const AcceptArgs a{t->n, t->count, t->tokens, t->mask, picks, t->mask_stride, t->rows, (t->rows + 31) / 32, cols,
                      path, kept, next, n_out, history, history_cols};
-  {
-    ProfScope prof(ctx, "tree_accept", 0.0, 16.0 * t->batch * t->rows);
+  const size_t nodes = (size_t)t->batch * t->rows, masks = t->mask_stride ? t->mask_stride * t->batch : (size_t)t->rows * a.words;
+  // One launch, each of whose workgroups walks its sequence's tree for itself, unless an output lies in what they read (32
+  // sequences' 9 of 61 nodes in 4 layers of 1280 values 10.2 us, 12.5 in two launches; trees of 1000 nodes 15.5 and 18.8).
+  auto apart = [&](const void *y, size_t words) {
+    const struct {
+      const void *p;
+      size_t words;
+    } in[] = {{t->n, (size_t)t->batch}, {t->count, (size_t)t->batch}, {t->tokens, nodes}, {t->mask, masks}, {picks, nodes}};
+    for (const auto &x : in)
+      if (x.p && y && (uintptr_t)y < (uintptr_t)x.p + 4 * x.words && (uintptr_t)x.p < (uintptr_t)y + 4 * words) return false;
+    return true;
+  };
+  const bool one = w && apart(path, nodes) && apart(kept, t->batch) && apart(next, t->batch) && apart(n_out, t->batch) &&
+                   apart(history, (size_t)t->batch * history_cols);
+  if (!one) {
+    ProfScope prof(ctx, "tree_accept", 0.0, 16.0 * nodes);
     wh_launch(ctx, accept_kernel, t->batch, 256, 0, a);
     if (int rc = wh_launched(ctx, "tree accept")) return rc;
   }
   if (!w) return WH_OK;
   const int parts = (w->d + 255) / 256;
-  const KeepArgs ka{path, kept, n_out, w->k, w->v, w->stride, w->layer_stride, w->kv, w->kv_stride, w->kv_layer_stride,
-                    t->rows, cols, w->d, parts};
+  const KeepArgs ka{w->k, w->v, w->stride, w->layer_stride, w->kv, w->kv_stride, w->kv_layer_stride, w->d, parts, one};
   const dim3 grid(t->batch * parts, w->layers);
   ProfScope prof(ctx, "tree_keep", 0.0, 0.0);
-  if (w->in16) wh_launch(ctx, keep_kernel<_Float16>, grid, 256, 0, ka);
-  else wh_launch(ctx, keep_kernel<float>, grid, 256, 0, ka);
+  if (w->in16) wh_launch(ctx, keep_kernel<_Float16>, grid, 256, 0, a, ka);
+  else wh_launch(ctx, keep_kernel<float>, grid, 256, 0, a, ka);
   return wh_launched(ctx, "tree keep");
 }
