@@ -114,6 +114,8 @@ int main() {
   rules("ids past the most", "needed", [](RulesCall &a) { a.vocab = (1 << 28) + 1, a.ld = 1 << 29; });
   rules("rows too close", "needed", [](RulesCall &a) { a.ld = 999; });
   rules("no texts' size", "texts", [](RulesCall &a) { a.r.history_cols = 0; });
+  rules("texts past the most", "texts", [](RulesCall &a) { a.r.history_cols = (1 << 30) + 1; });
+  rules("biases past the most", "biases", [](RulesCall &a) { a.r.bias_len = (1 << 30) + 1; });
   rules("texts from -1", "texts", [](RulesCall &a) { a.r.from = -1; });
   rules("biases without ids", "biases", [](RulesCall &a) { a.r.bias_id = nullptr; });
   rules("biases without values", "biases", [](RulesCall &a) { a.r.bias = nullptr; });

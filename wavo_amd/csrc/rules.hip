@@ -139,10 +139,7 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
   __shared__ uint64_t paths[GROUP][WORDS];  // per row of this workgroup: which nodes of `who` it sees
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int chunk = blockIdx.x % a.chunks, of = blockIdx.x / a.chunks, b = of / a.groups;
-  const int count = a.count ? min(max(a.count[b], 0), a.rows) : a.rows;
-  const int i0 = (of - b * a.groups) * a.group, i1 = min(i0 + a.group, count);
-  if (i0 >= i1) return;
-  const int id0 = chunk * IDS;
+  const int i0 = (of - b * a.groups) * a.group, id0 = chunk * IDS;
   // This thread's ids: V from id0 + first + V * RT * t on, t < G.
   const int first = V * tid;
   auto mine = [&](int e) { return first + V * RT * (e / V) + e % V; };
@@ -168,11 +165,27 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
     }
   };
   Row even, odd;  // rows i0, i0 + 2, .. and the others: each loaded again as soon as its values are in use
-  if (whole) load(std::true_type{}, even, i0), load(std::true_type{}, odd, min(i0 + 1, i1 - 1));
-  else load(std::false_type{}, even, i0), load(std::false_type{}, odd, min(i0 + 1, i1 - 1));
+  auto load_first = [&](int last) {
+    if (whole) load(std::true_type{}, even, i0), load(std::true_type{}, odd, min(i0 + 1, last));
+    else load(std::false_type{}, even, i0), load(std::false_type{}, odd, min(i0 + 1, last));
+  };
+  // What is asked for before the sequence's numbers are known: its first rows and the text's first EARLY ids a thread (a
+  // row of 51866 ids 9.1 us, 9.7 asked for afterwards).
+  constexpr int EARLY = 2;
+  const bool counted = a.penalty != nullptr, biased = a.bias_start != nullptr, has_text = counted && a.history;
+  const uint32_t *text = has_text ? a.history + (size_t)b * a.history_cols : nullptr;
+  uint32_t early[EARLY];
+  if (has_text)
+#pragma unroll
+    for (int y = 0; y < EARLY; y++) early[y] = text[min(min(a.from, a.history_cols - 1) + RT * y + tid, a.history_cols - 1)];
+  if (i0 == 0) load_first(a.rows - 1);
+  const int count = a.count ? min(max(a.count[b], 0), a.rows) : a.rows, i1 = min(i0 + a.group, count);
+  const int n = has_text ? min(max(a.n[b], 0), a.history_cols) : 0;
+  const float r = counted ? a.penalty[3 * b] : 1.0f, f = counted ? a.penalty[3 * b + 1] : 0.0f, p = counted ? a.penalty[3 * b + 2] : 0.0f;
+  const int e0 = biased ? max(a.bias_start[b], 0) : 0, e1 = biased ? min(a.bias_start[b + 1], a.bias_len) : 0;
+  if (i0 >= i1) return;
+  if (i0) load_first(i1 - 1);
 
-  const bool counted = a.penalty != nullptr, biased = a.bias_start != nullptr;
-  float r = 1.0f, f = 0.0f, p = 0.0f;
   int changes = 0, listed = 0;  // of this wavefront's list; of `who`
   int one = 0, token = -1;      // the lane's id on the list; its token of `who`, if it is this wavefront's
   float onebias = 0.0f;
@@ -184,14 +197,14 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
     if (tid == 0) whos = 0;
     __syncthreads();
     if (counted) {
-      r = a.penalty[3 * b], f = a.penalty[3 * b + 1], p = a.penalty[3 * b + 2];
-      const int n = a.history ? min(max(a.n[b], 0), a.history_cols) : 0;
-      const uint32_t *text = a.history + (size_t)b * a.history_cols;
       auto add = [&](uint32_t id) {
         id -= (uint32_t)id0;
         if (id < (uint32_t)span) atomicAdd(&times[id], 2u);
       };
-      int x = a.from;
+#pragma unroll
+      for (int y = 0; y < EARLY; y++)
+        if (a.from < n && a.from + RT * y + tid < n) add(early[y]);
+      int x = a.from < n ? a.from + EARLY * RT : n;
       for (; x + 16 * RT <= n; x += 16 * RT) {  // (16 ids a thread at a time)
         u32x4 id[4];
 #pragma unroll
@@ -217,12 +230,9 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
           }
         }
     }
-    if (biased) {
-      const int e0 = max(a.bias_start[b], 0), e1 = min(a.bias_start[b + 1], a.bias_len);
-      for (int x = e0 + tid; x < e1; x += RT) {
-        const uint32_t id = a.bias_id[x] - (uint32_t)id0;
-        if (id < (uint32_t)span) atomicMax(&entry[id], x);
-      }
+    for (int x = e0 + tid; x < e1; x += RT) {
+      const uint32_t id = a.bias_id[x] - (uint32_t)id0;
+      if (id < (uint32_t)span) atomicMax(&entry[id], x);
     }
     __syncthreads();
     listed = whos;
@@ -404,9 +414,9 @@ int launch_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *r, const v
   if (int rc = tree_check(ctx, "logit rules", t)) return rc;
   if (!r || !logits || (!out && !pick && !logprob) || vocab <= 0 || vocab > 1 << 28 || ld < (size_t)vocab)
     return wh_fail(ctx, WH_EARG, "logit rules: rules, logits, an output and rows of %d ids (%zu apart) are needed", vocab, ld);
-  if (r->history && (r->history_cols <= 0 || r->from < 0))
+  if (r->history && (r->history_cols <= 0 || r->history_cols > 1 << 30 || r->from < 0))
     return wh_fail(ctx, WH_EARG, "logit rules: texts of %d ids from %d on", r->history_cols, r->from);
-  if (r->bias_start && (!r->bias_id || !r->bias || r->bias_len < 0))
+  if (r->bias_start && (!r->bias_id || !r->bias || r->bias_len < 0 || r->bias_len > 1 << 30))
     return wh_fail(ctx, WH_EARG, "logit rules: biases need their ids, values and number");
   if (r->penalty && t->mask && !t->tokens) return wh_fail(ctx, WH_EARG, "logit rules: the nodes' tokens are needed");
   if (((uintptr_t)r->penalty | (uintptr_t)r->history | (uintptr_t)r->bias_start | (uintptr_t)r->bias_id | (uintptr_t)r->bias |
@@ -426,7 +436,7 @@ int launch_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *r, const v
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "logit rules: %s", hipGetErrorString(e));
   RulePart *part = nullptr;
   if ((pick || logprob) && !(part = (RulePart *)wh_scratch(ctx, sizeof(RulePart) * parts * nodes))) return WH_EOOM;
-  // Who joins the parts: up to a workgroup a CU their last one (a row of 51866 f32 ids 9.7 us, 11.2 with a second launch,
+  // Who joins the parts: up to a workgroup a CU their last one (a row of 51866 f32 ids 9.1 us, 10.7 with a second launch,
   // whose start costs more than the counting); more of them wait for each other's counts (18 such rows 13.5 us counted,
   // 12.7 in two launches, 48 of them 18.7 and 14.7).
   const RuleArgs a{t->n, t->count, t->tokens, t->mask, t->mask_stride, t->rows, (t->rows + 31) / 32, r->penalty, r->history,
