@@ -11,6 +11,8 @@ namespace {
 
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+typedef float floatx2 __attribute__((ext_vector_type(2)));
 typedef float floatx4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -39,6 +41,9 @@ struct AttendArgs {
 
 
 constexpr float SLACK = 4.0f;
+// Exponents are taken as score * factor + (10 − maximum * factor), whose sum in brackets is rounded like a score; past
+// this it would be off by whole digits, and the maximum is subtracted first.
+constexpr float FAR = 65536.0f;
 constexpr int WAVES = 8;  // wavefronts of a workgroup, at most
 
 constexpr int few_block(int hd) { return hd <= 64 ? 64 : 32; }   // positions of a block of attend_kernel's
@@ -133,6 +138,21 @@ __device__ __forceinline__ void meet() {
 
 __device__ __forceinline__ floatx4 mfma(half8 a, half8 b, floatx4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// Softmax weights p0 and p1 as f16, and (unless P16) what that leaves of them.
+template <bool P16>
+__device__ __forceinline__ void weights2(float p0, float p1, half8 &h, half8 &l, int e) {
+  const half2 w = __builtin_convertvector((floatx2{p0, p1}), half2);
+  h[e] = w[0], h[e + 1] = w[1];
+  if constexpr (!P16) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, w);
+    floatx2 r;  // p − w, a product and a sum with a half as it stands
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[0,0,0] op_sel_hi:[1,0,0]" : "=v"(r[0]) : "v"(u), "v"(p0));
+    asm("v_fma_mix_f32 %0, -%1, 1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r[1]) : "v"(u), "v"(p1));
+    const half2 x = __builtin_convertvector(r, half2);
+    l[e] = x[0], l[e + 1] = x[1];
+  }
 }
 
 // Row (of a key head's: node row / group, query head row % group) and head offset without a division where the heads
@@ -383,13 +403,18 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
         mx[t] = top;
       }
       const float base = mx[t] == -INFINITY ? 0.0f : mx[t];
+      float shift = fmaf(-base, cf[t], 10.0f);
+      if (__any(fabsf(shift) > FAR)) {
+        shift = 10.0f;
 #pragma unroll
-      for (int e = 0; e < NP; e++) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(st[t][e % KP][e / KP] - base, cf[t], 10.0f));
-        sum[t] += p;
-        const _Float16 h = (_Float16)p;
-        ph[t][e >> 3][e & 7] = h;
-        if constexpr (!P16) pl[t][e >> 3][e & 7] = (_Float16)(p - (float)h);
+        for (int u = 0; u < KP; u++) st[t][u] -= base;
+      }
+#pragma unroll
+      for (int e = 0; e < NP; e += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(st[t][e % KP][e / KP], cf[t], shift));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(st[t][(e + 1) % KP][(e + 1) / KP], cf[t], shift));
+        sum[t] += p0, sum[t] += p1;
+        weights2<P16>(p0, p1, ph[t][e >> 3], pl[t][e >> 3], e & 7);
       }
     }
 
@@ -633,13 +658,18 @@ __global__ __launch_bounds__(64 * RT, RT == 8 ? 4 : 3) void attend_rows_kernel(A
       mx = top;
     }
     const float base = mx == -INFINITY ? 0.0f : mx;
+    float shift = fmaf(-base, cf, 10.0f);
+    if (__any(fabsf(shift) > FAR)) {
+      shift = 10.0f;
 #pragma unroll
-    for (int e = 0; e < 4 * NT; e++) {
-      const float p = __builtin_amdgcn_exp2f(fmaf(st[e >> 2][e & 3] - base, cf, 10.0f));
-      sum += p;
-      const _Float16 h = (_Float16)p;
-      ph[e >> 3][e & 7] = h;
-      if constexpr (!P16) pl[e >> 3][e & 7] = (_Float16)(p - (float)h);
+      for (int u = 0; u < NT; u++) st[u] -= base;
+    }
+#pragma unroll
+    for (int e = 0; e < 4 * NT; e += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(st[e >> 2][e & 3], cf, shift));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(st[e >> 2][(e + 1) & 3], cf, shift));
+      sum += p0, sum += p1;
+      weights2<P16>(p0, p1, ph[e >> 3], pl[e >> 3], e & 7);
     }
 #pragma unroll
     for (int x = 0; x < X; x++)
