@@ -9,7 +9,6 @@
 
 namespace {
 
-
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef float floatx2 __attribute__((ext_vector_type(2)));
@@ -39,15 +38,15 @@ struct AttendArgs {
   float *po, *pml;
 };
 
-
+// How far scores may pass a row's maximum, in binary digits, before it is moved.
 constexpr float SLACK = 4.0f;
 // Exponents are taken as score * factor + (10 − maximum * factor), whose sum in brackets is rounded like a score; past
 // this it would be off by whole digits, and the maximum is subtracted first.
 constexpr float FAR = 65536.0f;
 constexpr int WAVES = 8;  // wavefronts of a workgroup, at most
 
-constexpr int few_block(int hd) { return hd <= 64 ? 64 : 32; }   // positions of a block of attend_kernel's
-constexpr int NODES = 32;                                         // (of its nodes: this many)
+constexpr int few_block(int hd) { return hd <= 64 ? 64 : 32; }   // positions of a block of attend_kernel
+constexpr int NODES = 32;                                        // (of its nodes: this many)
 constexpr int rows_block(int hd) { return hd <= 64 ? 64 : 32; }  // and of attend_rows_kernel
 
 // The blocks of keys of a sequence (the cache's, then the nodes'), and how its `splits` workgroups share them:
@@ -213,7 +212,9 @@ __device__ __forceinline__ float split_query(const float (&f)[C][8], float scale
 //   pairs those of two positions.  A row's softmax state is one lane column's everywhere.
 //
 // The next block's K is loaded as soon as this one's scores are done, and its V after this one's outputs, so that
-// a wavefront always has loads in flight; the first block's before the queries are looked at.
+// a wavefront always has loads in flight; the first block's before the queries are looked at.  Bound by the cache's bytes
+// where it is long (4 requests' 16 rows over 32 k keys of 8 heads of 128 values 98 us, 4.7 TB/s) and by its chain of
+// loads where it is short (16 rows of 20 heads of 64 values over 391 keys 8.5 us a call, of which 7 are the host's).
 //
 // Precision: f32 queries are scaled by a power of two per row and split into two f16 parts, as is every
 // softmax weight for f32 outputs: two products each, with an error of 2^-22 against f32's own 2^-24 per sum.  Weights
@@ -538,7 +539,10 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
 // position too, from which the wavefronts read operands as they stand: 8 values of a position of K, and V
 // transposed by ds_read_b64_tr_b16 (rows 16 and 32 bytes longer, for the banks' sake).  Tile u's row r is position
 // 16u + r, so lane 16g + i's scores are those of positions 16u + 4g + 0 .. 3 of every u.  Workgroups of 8 wavefronts
-// get by with 128 registers, so that two share a CU, those of 4 with 168 for three.
+// get by with 128 registers, so that two share a CU, those of 4 with 168 for three.  Its wavefronts wait for each other
+// block by block, so the matrix cores, LDS and the softmax's instructions share the time rather than overlap (200 rows of
+// f32 queries on 64 values: vector instructions 54 % of it, matrix cores 26 %): 4 requests' 100 f16 rows over 28 k keys of
+// 8 heads of 128 values 115 us (4.0 TB/s, 305 TFLOP/s), 16 requests' 61 rows over up to 448 keys of 20 heads 15.7 us.
 template <typename T, int HD, int RT, bool P16>
 __global__ __launch_bounds__(64 * RT, RT == 8 ? 4 : 3) void attend_rows_kernel(AttendArgs a) {
   constexpr int C = HD / 32, X = HD / 16, QP = sizeof(T) == 4 ? 2 : 1, B = rows_block(HD), NT = B / 16, KK = B / 32;
@@ -1001,6 +1005,11 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
   AttendArgs a{q, k, v, stride, kv, kv_stride, o, t->n, t->count, t->mask, t->mask_stride, t->batch, t->rows, (t->rows + 31) / 32,
                cols, heads, kv_heads, hd, 1.0f / sqrtf((float)hd), 1, 1, 1, few_block(hd), NODES, nullptr, nullptr};
   const int rows = t->rows * (heads / kv_heads), tiles = (rows + 15) / 16;
+  // Which kernel: up to 32 rows (16 of larger heads, for want of registers) attend_kernel, as it shares nothing (4
+  // requests' 16 rows of 20 heads of 64 values over 448 keys 8.5 us, 12.3 by attend_rows_kernel; 32 rows 10.6 and 12.9).
+  // More rows need the blocks shared.  attend_rows_kernel's workgroups have 4 wavefronts where that is all the rows there
+  // are (64 rows over 4000 keys 29.2 us, 32.3 with 8) and 8 otherwise (100 rows of 128 values over 28 k keys 119 us, 141
+  // with 4).
   const int most = hd <= 64 ? 2 : 1;  // tiles of attend_kernel
   const int rt = tiles > most && hd >= 8 && cols >= 4 ? tiles <= 4 ? 4 : 8 : 0, qt = std::min(tiles, most);
   if (rt) a.block = a.node_block = rows_block(hd);
@@ -1009,8 +1018,21 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
   const size_t units = (size_t)t->batch * kv_heads * a.row_blocks;
   const size_t cus = ctx->cus > 0 ? ctx->cus : 256;
   a.kw = rt ? 1 : std::min(WAVES, blocks);
-  const int least = (rt ? 8 : 4) * a.kw;  // blocks of a split
-  a.splits = (int)std::max<size_t>(1, std::min<size_t>({((rt ? 2 : 1) * cus + units - 1) / units, ((size_t)blocks + least - 1) / least, SPLITS}));
+  // A second launch joins the splits, so a cache that one workgroup gets through in 4 blocks a wavefront (8 of
+  // attend_rows_kernel's) stays whole (1500 keys of 8 heads of 64 values for 4 requests 11.9 us, 13.5 in parts).  Of a
+  // longer one each has at least half as many (4000 keys 14.9 us, 17.8 with as many), and there are as many as keep the
+  // rounds of workgroups that the CUs hold at once short and full (1500 keys of 20 heads of 100 values for 5 requests
+  // 21.8 us with 2 splits, 28.5 with 3, whose last round has 44 workgroups for 256 CUs; 300 nodes of 32 heads over 28 k
+  // keys 253 us, 299 with one round's number rounded up).
+  const int least = (rt ? 4 : 2) * a.kw;
+  if (blocks > 2 * least) {
+    const size_t slots = cus * (rt ? 2 : 1);
+    size_t best = SIZE_MAX;
+    for (int x = 1; x <= std::min(SPLITS, (blocks + least - 1) / least); x++) {
+      const size_t cost = (units * x + slots - 1) / slots * ((blocks + x - 1) / x + least);
+      if (cost < best) best = cost, a.splits = x;
+    }
+  }
   const size_t nodes = (size_t)t->batch * t->rows;
   if ((size_t)t->batch * a.row_blocks > 65535 || units * a.splits >= (size_t)1 << 22 || nodes * heads >= (size_t)1 << 25)  // (a launch's limits)
     return wh_fail(ctx, WH_EARG, "tree attention: %d heads of %zu nodes in one call", heads, nodes);
