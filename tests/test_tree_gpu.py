@@ -812,6 +812,29 @@ def test_recorded_passes_share_the_scratch(gpu):
         p.free()
 
 
+def test_rules_calls_in_a_row(gpu):
+    """Small calls whose last workgroup joins the parts, many behind each other over the same scratch, with other rows and
+    row counts each: a part read before it is there, or one of an earlier call, gives another pick."""
+    batch, rows, vocab, sets, calls = 3, 4, 30011, 5, 60
+    rng = np.random.default_rng(13)
+    x = (3 * rng.standard_normal((sets, batch * rows, vocab))).astype(np.float32)
+    count = rng.integers(1, rows + 1, (sets, batch)).astype(np.int32)
+    xb, cb, nb = [gpu.upload(a) for a in x], [gpu.upload(a) for a in count], gpu.upload(np.zeros(batch, np.int32))
+    pick, logprob = gpu.upload(np.full((calls, batch * rows), 77, np.uint32)), gpu.upload(np.full((calls, batch * rows), 77, np.float32))
+    for i in range(calls):
+        gpu.logit_rules(wa.Tree(batch, rows, nb, cb[i % sets]), wa.Rules(), xb[i % sets], None, vocab, vocab,
+                        pick=pick.ptr + 4 * i * batch * rows, logprob=logprob.ptr + 4 * i * batch * rows)
+    p, l = gpu.read(pick, (calls, batch, rows), np.uint32), gpu.read(logprob, (calls, batch, rows))
+    y = x.astype(np.float64)
+    there = np.arange(rows) < count[:, :, None]
+    best = np.where(there, x.argmax(2).reshape(sets, batch, rows), 77)
+    total = -np.log(np.exp(y - y.max(2, keepdims=True)).sum(2)).reshape(sets, batch, rows)
+    for i in range(calls):
+        assert np.array_equal(p[i], best[i % sets])
+        # (as in check_rules, with rest / (1 + rest) < 1 and a log1p below 16)
+        assert np.all(np.abs(l[i] - np.where(there[i % sets], total[i % sets], 77)) <= 104 * 2.0**-23 + 2.0**-21 + 64 * EPS + 2.0**-18)
+
+
 def test_two_contexts(gpu):
     """The same calls queued on two contexts (streams) at once, without waits between."""
     other = wa.Gpu(0)
