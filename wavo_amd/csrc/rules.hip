@@ -124,7 +124,8 @@ __device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
 // ALLOW, OUT, whole: what a row's pass loads and stores has to be the same for every row, so that a wait for one row's
 // loads is not one for the next rows'.  61 rows of 131071 f16 ids for 8 requests, 16000 ids of text and 1000 biases
 // each: 94 us (2.1 TB/s; 104 with one row's registers only).  A copy
-// of these rows alone in the same form takes 42 us: the rest is issue, 236 vector instructions a wavefront and row.
+// of these rows alone in the same form takes 42 us; the rest is each row's chain of LDS trips, cross-lane sums and 232
+// vector instructions, in as many wavefronts as LDS has room for (five workgroups a CU; 126 us with four).
 template <typename T, bool ALLOW, bool OUT>
 __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
 #pragma clang fp contract(off)  // the rules' sums and products are rounded one by one
