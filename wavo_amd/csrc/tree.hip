@@ -647,6 +647,17 @@ __global__ __launch_bounds__(64 * RT, RT == 8 ? 4 : 3) void attend_rows_kernel(A
           if (!(vis >> (16 * (e >> 2) + 4 * g + (e & 3)) & 1)) st[2 * kk + (e >> 2)][e & 3] = -INFINITY;
       }
     }
+    // V's operands are read a step ahead of their products.
+    half8 vf[2][KK];
+    auto read_v = [&](int x) {
+#pragma unroll
+      for (int kk = 0; kk < KK; kk++) {
+        const uint32_t *v = buf + KW + (32 * kk + 4 * g + (m >> 2)) * VS + 8 * x + 2 * (m & 3);
+        const u32x2 lo = read_tr(v), hi = read_tr(v + 16 * VS);
+        vf[x & 1][kk] = __builtin_bit_cast(half8, u32x4{lo[0], lo[1], hi[0], hi[1]});
+      }
+    };
+    read_v(0);
     half8 ph[KK], pl[KK];
     float top = st[0][0];
 #pragma unroll
@@ -676,15 +687,15 @@ __global__ __launch_bounds__(64 * RT, RT == 8 ? 4 : 3) void attend_rows_kernel(A
       weights2<P16>(p0, p1, ph[e >> 3], pl[e >> 3], e & 7);
     }
 #pragma unroll
-    for (int x = 0; x < X; x++)
+    for (int x = 0; x < X; x++) {
+      if (x + 1 < X) read_v(x + 1);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int kk = 0; kk < KK; kk++) {
-        const uint32_t *v = buf + KW + (32 * kk + 4 * g + (m >> 2)) * VS + 8 * x + 2 * (m & 3);
-        const u32x2 lo = read_tr(v), hi = read_tr(v + 16 * VS);
-        const half8 vf = __builtin_bit_cast(half8, u32x4{lo[0], lo[1], hi[0], hi[1]});
-        acc[x] = mfma(vf, ph[kk], acc[x]);
-        if constexpr (!P16) acc[x] = mfma(vf, pl[kk], acc[x]);
+        acc[x] = mfma(vf[x & 1][kk], ph[kk], acc[x]);
+        if constexpr (!P16) acc[x] = mfma(vf[x & 1][kk], pl[kk], acc[x]);
       }
+    }
     if (NODES && odd)  // what the block has zeros for, to the rows that see it
 #pragma unroll 1
       for (int j = 0; j < min(B, last + 1); j++) {
