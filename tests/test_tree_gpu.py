@@ -246,6 +246,20 @@ def test_attend_bad_node_stays_on_its_path(gpu, bad, in16):
             assert not np.isfinite(got[b, i, spoiled]).any()
 
 
+@pytest.mark.parametrize("rows,hd", [(13, 64), (20, 64), (9, 128), (40, 64), (40, 128)])
+@pytest.mark.parametrize("what", [np.nan, np.inf, 1e30, -3.0])
+def test_attend_rows_past_the_count_change_nothing(gpu, rows, hd, what):
+    """Whatever stands in the queries, keys and values of nodes past the count: the same bits."""
+    batch, heads, cols = 2, 3, 300
+    _, q, k, v, seen, kc, vc = case(14, batch, rows, heads, heads, hd, cols)
+    n, count = [290, 0], [rows // 2, rows - 1]
+    want = attend(gpu, q, k, v, seen, n, count, kc, vc, heads, heads, hd)
+    for b in range(batch):
+        for x in (q, k, v):
+            x[b, count[b]:] = what
+    assert np.array_equal(attend(gpu, q, k, v, seen, n, count, kc, vc, heads, heads, hd), want)
+
+
 @pytest.mark.parametrize("rows", [1, 13, 70])
 def test_attend_cache_alone(gpu, rows):
     """No mask, or no nodes' keys: cross attention, one cache for all sequences or one each."""

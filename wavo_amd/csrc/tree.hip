@@ -346,7 +346,9 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
   float mx[QT], sum[QT], cf[QT], slack[QT];
 #pragma unroll
   for (int t = 0; t < QT; t++) {
-    cf[t] = split_query(f[t], a.scale, q[t]), slack[t] = SLACK / cf[t];
+    cf[t] = split_query(f[t], a.scale, q[t]);
+    if (r0 + 16 * t + m >= total) cf[t] = 0.0f;  // (whatever stands in a row past the last: no maximum, no far score)
+    slack[t] = SLACK / cf[t];
     mx[t] = -INFINITY, sum[t] = 0.0f;
 #pragma unroll
     for (int x = 0; x < 4 * Z; x++) acc[t][x] = floatx4{};
@@ -542,7 +544,7 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
 // get by with 128 registers, so that two share a CU, those of 4 with 168 for three.  Its wavefronts wait for each other
 // block by block, so the matrix cores, LDS and the softmax's instructions share the time rather than overlap (200 rows of
 // f32 queries on 64 values: vector instructions 54 % of it, matrix cores 26 %): 4 requests' 100 f16 rows over 28 k keys of
-// 8 heads of 128 values 115 us (4.0 TB/s, 305 TFLOP/s), 16 requests' 61 rows over up to 448 keys of 20 heads 15.7 us.
+// 8 heads of 128 values 115 us (4.0 TB/s, 305 TFLOP/s), 16 requests' 61 rows over up to 448 keys of 20 heads 15.2 us.
 template <typename T, int HD, int RT, bool P16>
 __global__ __launch_bounds__(64 * RT, RT == 8 ? 4 : 3) void attend_rows_kernel(AttendArgs a) {
   constexpr int C = HD / 32, X = HD / 16, QP = sizeof(T) == 4 ? 2 : 1, B = rows_block(HD), NT = B / 16, KK = B / 32;
