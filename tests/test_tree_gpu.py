@@ -312,6 +312,27 @@ def test_attend_equal_keys_give_the_mean(gpu):
     assert np.all(np.abs(got[0] - want) <= 2 * 1000 * EPS * np.abs(vc[0]).max())
 
 
+@pytest.mark.parametrize("in16", [False, True])
+@pytest.mark.parametrize("rows,heads,hd", [(1, 8, 64), (20, 8, 64), (7, 4, 128), (5, 4, 100), (40, 4, 128)])
+def test_attend_caches_of_many_positions(gpu, rows, heads, hd, in16):
+    """Caches past what the chip keeps (300 MB), of which a few positions are there: the split of a long one, the loads past
+    the chip's caches."""
+    n, d = 700, heads * hd
+    cols = 75_000_003 // d
+    _, q, k, v, seen, kc, vc = case(15, 1, rows, heads, heads, hd, n, in16)
+    kv = gpu.buffer(cols * d)
+    gpu.zero(kv)
+    gpu.pack(gpu.upload(np.concatenate([kc[0], vc[0]], 1).astype(np.float32)), 0, 2 * d, kv, n, d, cols, 0)
+    x = gpu.upload(np.concatenate([q, k, v], 2))
+    size = 2 if in16 else 4
+    o = gpu.buffer(rows * d)
+    t = wa.Tree(1, rows, gpu.upload(np.array([n], np.int32)), None, None, gpu.upload(bits(seen)), 0)
+    gpu.tree_attend(t, x, x.ptr + size * d, x.ptr + 2 * size * d, 3 * d, kv, cols * d, cols, o, heads, heads, hd, in16, in16)
+    got = gpu.read(o, (1, rows, d), np.float16 if in16 else np.float32)
+    kv.free()
+    check_attend(got, q, k, v, seen, [n], None, kc, vc, heads, heads, hd, in16, in16)
+
+
 def test_attend_offsets_past_32_bits(gpu):
     """A cache of 2^31 words and more to its values (17 GB): keys of zeros but for the last ones, which are large."""
     heads, hd, cols, rows, last = 8, 128, (1 << 22) + 3, 2, 50

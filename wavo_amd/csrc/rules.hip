@@ -123,9 +123,10 @@ __device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
 
 // ALLOW, OUT, whole: what a row's pass loads and stores has to be the same for every row, so that a wait for one row's
 // loads is not one for the next rows'.  61 rows of 131071 f16 ids for 8 requests, 16000 ids of text and 1000 biases
-// each: 94 us (2.1 TB/s; 104 with one row's registers only).  A copy
-// of these rows alone in the same form takes 42 us; the rest is each row's chain of LDS trips, cross-lane sums and 232
-// vector instructions, in as many wavefronts as LDS has room for (five workgroups a CU; 126 us with four).
+// each: 91 us (2.2 TB/s; 96 where the stores stay in L2, 104 with one row's registers only); 24 rows of 51866 f32 ids for
+// 16 requests: 33 us (3.7 TB/s; 40).  A copy of the former rows in the same form takes 42 us; the rest is each row's chain
+// of LDS trips, cross-lane sums and 232 vector instructions, in as many wavefronts as LDS has room for (five workgroups a
+// CU; 126 us with four).
 template <typename T, bool ALLOW, bool OUT>
 __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
 #pragma clang fp contract(off)  // the rules' sums and products are rounded one by one
@@ -323,7 +324,7 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
 #pragma unroll
         for (int e = 0; e < V; e++) w[e] = (T)v[V * t + e];
         if constexpr (all) {
-          *(typename Piece<T>::any *)(out + l) = w;
+          __builtin_nontemporal_store(w, (typename Piece<T>::any *)(out + l));  // (not read again here)
         } else {
 #pragma unroll
           for (int e = 0; e < V; e++)

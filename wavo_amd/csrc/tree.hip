@@ -213,14 +213,16 @@ __device__ __forceinline__ float split_query(const float (&f)[C][8], float scale
 //
 // The next block's K is loaded as soon as this one's scores are done, and its V after this one's outputs, so that
 // a wavefront always has loads in flight; the first block's before the queries are looked at.  Bound by the cache's bytes
-// where it is long (4 requests' 16 rows over 32 k keys of 8 heads of 128 values 98 us, 4.7 TB/s) and by its chain of
+// where it is long (4 requests' 4 rows over 28 k keys of 8 heads of 128 values 88 us, 5.3 TB/s) and by its chain of
 // loads where it is short (16 rows of 20 heads of 64 values over 391 keys 8.5 us a call, of which 7 are the host's).
 //
 // Precision: f32 queries are scaled by a power of two per row and split into two f16 parts, as is every
 // softmax weight for f32 outputs: two products each, with an error of 2^-22 against f32's own 2^-24 per sum.  Weights
 // are exp2(s - max + 10), so that the second part is no subnormal; a maximum that grows by less than SLACK binary
 // digits is left as it is, since they still fit f16 then.  K and V are f16 as stored.
-template <typename T, int HD, int QT, bool P16>
+//
+// ONCE: the cache is read past the chip's own caches.
+template <typename T, int HD, int QT, bool P16, bool ONCE>
 __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
   constexpr int C = HD / 32, Z = HD / 64, QP = sizeof(T) == 4 ? 2 : 1;
   constexpr int KPC = few_block(HD) / 16, KB = 16 * KPC;
@@ -261,7 +263,11 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
       const int top = hd / 2 - 1 - 16 * c;  // the last pair of this chunk, where it has not 16
       if (top >= 15) {
 #pragma unroll
-        for (int x = 0; x < 4; x++) kw[c][x] = *(const Words_a4 *)(base + (size_t)x * cols + (uint32_t)(4 * g * cols + jk));
+        for (int x = 0; x < 4; x++) {
+          const Words_a4 *p = (const Words_a4 *)(base + (size_t)x * cols + (uint32_t)(4 * g * cols + jk));
+          if constexpr (ONCE) kw[c][x] = __builtin_nontemporal_load(p);
+          else kw[c][x] = *p;
+        }
       } else {
 #pragma unroll
         for (int x = 0; x < 4; x++) {
@@ -277,8 +283,11 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
 #pragma unroll
     for (int e = 0; e < 4 * KPC; e++)
 #pragma unroll
-      for (int z = 0; z < Z; z++)
-        vw[e][z] = *(const u32x2_a4 *)(base + (uint32_t)(min(4 * KPC * g + e, last) * half + (64 * z + 4 * m < a.hd ? 32 * z + 2 * m : 0)));
+      for (int z = 0; z < Z; z++) {
+        const u32x2_a4 *p = (const u32x2_a4 *)(base + (uint32_t)(min(4 * KPC * g + e, last) * half + (64 * z + 4 * m < a.hd ? 32 * z + 2 * m : 0)));
+        if constexpr (ONCE) vw[e][z] = __builtin_nontemporal_load(p);
+        else vw[e][z] = *p;
+      }
   };
   auto load_nodes = [&](int blk) {
     const int j0 = (blk - s.cached) * NODES, last = s.count - 1 - j0;
@@ -955,10 +964,12 @@ __global__ __launch_bounds__(256) void keep_kernel(AcceptArgs t, KeepArgs a) {
 }
 
 template <typename T, int HD, int QT, bool P16>
-int attend_launch(wh_ctx *ctx, const AttendArgs &a) {
+int attend_launch(wh_ctx *ctx, const AttendArgs &a, bool once) {
   ProfScope prof(ctx, "tree_attend", 4.0 * a.batch * a.rows * a.heads * a.cols * a.hd, 4.0 * a.batch * a.cols * a.kv_heads * a.hd);
-  wh_launch(ctx, (attend_kernel<T, HD, QT, P16>), dim3(a.kv_heads, a.batch * a.row_blocks, a.splits), 64 * a.kw,
-            (size_t)a.kw * QT * (HD / 64 * 4096 + 128), a);
+  const dim3 grid(a.kv_heads, a.batch * a.row_blocks, a.splits);
+  const size_t shm = (size_t)a.kw * QT * (HD / 64 * 4096 + 128);
+  if (once) wh_launch(ctx, (attend_kernel<T, HD, QT, P16, true>), grid, 64 * a.kw, shm, a);
+  else wh_launch(ctx, (attend_kernel<T, HD, QT, P16, false>), grid, 64 * a.kw, shm, a);
   return wh_launched(ctx, "tree attention");
 }
 
@@ -978,14 +989,14 @@ int attend_rows_launch(wh_ctx *ctx, const AttendArgs &a) {
   return wh_launched(ctx, "tree attention");
 }
 
-// rt: row tiles of attend_rows_kernel's workgroups, or 0: attend_kernel with qt tiles of rows.
+// rt: row tiles of attend_rows_kernel's workgroups, or 0: attend_kernel with qt tiles of rows; once: see there.
 template <typename T, bool P16>
-int attend_t(wh_ctx *ctx, const AttendArgs &a, int qt, int rt) {
+int attend_t(wh_ctx *ctx, const AttendArgs &a, int qt, int rt, bool once) {
   int rc;
   if (rt && a.hd <= 64) rc = rt == 4 ? attend_rows_launch<T, 64, 4, P16>(ctx, a) : attend_rows_launch<T, 64, 8, P16>(ctx, a);
   else if (rt) rc = rt == 4 ? attend_rows_launch<T, 128, 4, P16>(ctx, a) : attend_rows_launch<T, 128, 8, P16>(ctx, a);
-  else if (a.hd <= 64) rc = qt == 1 ? attend_launch<T, 64, 1, P16>(ctx, a) : attend_launch<T, 64, 2, P16>(ctx, a);
-  else rc = attend_launch<T, 128, 1, P16>(ctx, a);
+  else if (a.hd <= 64) rc = qt == 1 ? attend_launch<T, 64, 1, P16>(ctx, a, once) : attend_launch<T, 64, 2, P16>(ctx, a, once);
+  else rc = attend_launch<T, 128, 1, P16>(ctx, a, once);
   return rc || a.splits == 1 ? rc : attend_join<P16>(ctx, a);
 }
 
@@ -1055,8 +1066,12 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
     if (!(a.po = (float *)wh_scratch(ctx, part * (hd + 4) * sizeof(float)))) return WH_EOOM;
     a.pml = a.po + part * hd;
   }
-  return in16 ? out16 ? attend_t<_Float16, true>(ctx, a, qt, rt) : attend_t<_Float16, false>(ctx, a, qt, rt)
-              : out16 ? attend_t<float, true>(ctx, a, qt, rt) : attend_t<float, false>(ctx, a, qt, rt);
+  // Caches of more than the 256 MB that the chip keeps are read past it (4 requests' 4 rows over 28 k keys of 8 heads of 128
+  // values: 88 us, 98 through it); smaller ones may be found there by the next step (4 requests' 13 rows over 1300 keys:
+  // 11.5 us, 15.0 past it).  attend_rows_kernel gains nothing by it.
+  const bool once = kv_stride && a.row_blocks == 1 && 4 * (size_t)t->batch * kv_heads * hd * cols > (size_t)256 << 20;
+  return in16 ? out16 ? attend_t<_Float16, true>(ctx, a, qt, rt, once) : attend_t<_Float16, false>(ctx, a, qt, rt, once)
+              : out16 ? attend_t<float, true>(ctx, a, qt, rt, once) : attend_t<float, false>(ctx, a, qt, rt, once);
 }
 
 int launch_tree_accept(wh_ctx *ctx, const wh_tree *t, const uint32_t *picks, const wh_kept *w, int cols, int32_t *path,
