@@ -35,7 +35,8 @@ struct wh_ctx {
   int device = 0;
   hipStream_t stream = nullptr;
   int cus = 0;
-  // Per head, the parts of an attend launch done so far (0 between launches: the last part resets it).
+  // Per head, the parts of an attend launch done so far, or per run of rows the workgroups of a logit rules launch (0
+  // between launches: the last one resets it).
   int *attend_count = nullptr;
   // GEMM launch-plan override set by wh_tune("gemm_plan", "bm,bn,wm,wn,slots,split[,pipeline[,kgroups]]") (tuning
   // sweeps only): all zero = chosen per shape.
