@@ -399,7 +399,7 @@ typedef struct wh_rules {
    * the sequence's text gets x = ((x > 0 ? x / r : x * r) - f * c) - p. */
   const float *penalty;
   /* [batch][history_cols]: the sequences' ids; the text of a node is ids from .. n[b] - 1 and the
-   * tokens of the nodes that it sees.  NULL: those tokens alone. */
+   * tokens of the nodes that it sees.  NULL: those tokens alone.  from >= 0. */
   const uint32_t *history;
   int history_cols, from;
   /* Biases added to single ids: entries bias_start[b] .. bias_start[b + 1] - 1 of bias_id and bias (of

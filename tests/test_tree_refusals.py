@@ -177,3 +177,29 @@ def test_no_context(name):
 
     args = [0 if t in (wa._i, wa._sz) else None for t in wa.SIGNATURES[name][1]]
     assert getattr(wa.lib(), name)(*args) == wa.EARG
+
+
+def run_calls(tmp_path, calls):
+    """The same program with other calls: its output, an error if one of them is not refused."""
+    head = SOURCE[:SOURCE.index("int main() {")]
+    tail = '  printf("%d calls, %d not refused\\n", calls, bad);\n  return bad != 0;\n}\n'
+    src, obj, exe = tmp_path / "main.cpp", tmp_path / "main.o", tmp_path / "main"
+    src.write_text(head + "int main() {\n" + calls + tail)
+    hipcc = ["/opt/rocm/bin/hipcc", "--offload-arch=gfx950"]
+    for args in (["-std=c++17", "-x", "hip", "--cuda-host-only", str(src), "-I", os.path.join(ROOT, "wavo_amd", "csrc"), "-c", "-o", str(obj)],
+                 [str(obj), os.path.join(ROOT, "wavo_amd", "libwavo_hip.a"), "-o", str(exe)]):
+        subprocess.run(hipcc + args, check=True, capture_output=True, timeout=300)
+    out = subprocess.run([str(exe)], capture_output=True, text=True, timeout=120)
+    assert out.returncode == 0, out.stdout + out.stderr
+    return out.stdout
+
+
+def test_texts_from_below_zero_are_refused_without_texts_too(tmp_path):
+    """Penalties alone count the tree's tokens; a start below zero would have had the kernel count a text that is not there."""
+    out = run_calls(tmp_path, r'''
+  for (int from : {-1, -1000, INT32_MIN})
+    for (int cols : {0, 100})
+      rules("no texts, from below zero", "texts", [&](RulesCall &a) { a.r.history = nullptr, a.r.history_cols = cols, a.r.from = from; });
+  rules("texts from the lowest", "texts", [](RulesCall &a) { a.r.from = INT32_MIN; });
+''')
+    assert "7 calls, 0 not refused" in out

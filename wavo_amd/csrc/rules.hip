@@ -416,7 +416,8 @@ int launch_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *r, const v
   if (int rc = tree_check(ctx, "logit rules", t)) return rc;
   if (!r || !logits || (!out && !pick && !logprob) || vocab <= 0 || vocab > 1 << 28 || ld < (size_t)vocab)
     return wh_fail(ctx, WH_EARG, "logit rules: rules, logits, an output and rows of %d ids (%zu apart) are needed", vocab, ld);
-  if (r->history && (r->history_cols <= 0 || r->history_cols > 1 << 30 || r->from < 0))
+  // (from without a history, too: penalties compare it with a text's length of zero)
+  if ((r->history && (r->history_cols <= 0 || r->history_cols > 1 << 30)) || ((r->history || r->penalty) && r->from < 0))
     return wh_fail(ctx, WH_EARG, "logit rules: texts of %d ids from %d on", r->history_cols, r->from);
   if (r->bias_start && (!r->bias_id || !r->bias || r->bias_len < 0 || r->bias_len > 1 << 30))
     return wh_fail(ctx, WH_EARG, "logit rules: biases need their ids, values and number");
