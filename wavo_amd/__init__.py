@@ -257,17 +257,18 @@ def _p(x):
 
 
 class Tree(ctypes.Structure):
-    """wh_tree: a decoder step over drafted tokens (device pointers: Buffer, int or None)."""
+    """wh_tree: a decoder step over drafted tokens (device pointers: Buffer, int or None; buffers are kept)."""
 
     _fields_ = [("batch", _i), ("rows", _i), ("n", _vp), ("count", _vp), ("tokens", _vp), ("mask", _vp),
                 ("mask_stride", _sz)]
 
     def __init__(self, batch, rows, n, count=None, tokens=None, mask=None, mask_stride=0):
         super().__init__(batch, rows, _p(n), _p(count), _p(tokens), _p(mask), mask_stride)
+        self._keep = n, count, tokens, mask
 
 
 class Rules(ctypes.Structure):
-    """wh_rules: the requests' penalties, biases and masks on their logits (device pointers)."""
+    """wh_rules: the requests' penalties, biases and masks on their logits (device pointers, as Tree's)."""
 
     _fields_ = [("penalty", _vp), ("history", _vp), ("history_cols", _i), ("from_", _i), ("bias_start", _vp),
                 ("bias_id", _vp), ("bias", _vp), ("bias_len", _i), ("allow", _vp)]
@@ -276,6 +277,7 @@ class Rules(ctypes.Structure):
                  bias_len=0, allow=None):
         super().__init__(_p(penalty), _p(history), history_cols, from_, _p(bias_start), _p(bias_id), _p(bias), bias_len,
                          _p(allow))
+        self._keep = penalty, history, bias_start, bias_id, bias, allow
 
 
 class _Kept(ctypes.Structure):
