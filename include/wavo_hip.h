@@ -419,7 +419,8 @@ typedef struct wh_rules {
  * nothing is left; NaN is never picked) and logprob[r] its log-softmax over the row (minus infinity
  * where nothing is left, NaN where the row holds one), either of which may be NULL.  Pick and
  * log-probability are those of the f32 values, before an f16 output is rounded.  Ids past vocab in
- * history, tokens and bias_id are passed over.  vocab <= 2^28, history_cols and bias_len <= 2^30; batch * vocab / 2048 workgroups of ten
+ * history, tokens and bias_id are passed over.  pick may lie in the tree's tokens (which are then gone); apart
+ * from that, and out from logits, outputs overlap no input.  vocab <= 2^28, history_cols and bias_len <= 2^30; batch * vocab / 2048 workgroups of ten
  * rows have to be fewer than 2^24.  search::decode's `pick` for rows of many requests (src/whisper/search.rs:46-59). */
 int wh_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *rules, const void *logits, void *out, int vocab,
                    size_t ld, int f16, uint32_t *pick, float *logprob);

@@ -870,6 +870,33 @@ def test_rules_calls_in_a_row(gpu):
         assert np.all(np.abs(l[i] - np.where(there[i % sets], total[i % sets], 77)) <= 104 * 2.0**-23 + 2.0**-21 + 64 * EPS + 2.0**-18)
 
 
+@pytest.mark.parametrize("batch,rows,vocab", [(3, 4, 30011), (1, 20, 9000), (5, 1, 51866), (2, 64, 4097), (60, 3, 20000)])
+@pytest.mark.parametrize("shift", [0, 1, -1])
+def test_rules_picks_in_the_tokens_place(gpu, batch, rows, vocab, shift):
+    """Picks written over the tokens that the penalties count (or a place off them): those of picks of their own.  Rows of
+    one sequence in several workgroups must have read their tokens before the first of them is through."""
+    c = rules_case(15, batch, rows, vocab, 40, 10, False)
+    c["count"][:] = rows
+    total = batch * rows
+    x, n, mask = gpu.upload(c["logits"]), gpu.upload(c["n"].astype(np.int32)), gpu.upload(bits(c["seen"]))
+    penalty, text = gpu.upload(c["penalty"]), gpu.upload(c["history"].astype(np.uint32))
+    rules = wa.Rules(penalty, text, c["history"].shape[1])
+    tokens = np.full(total + 2, 5, np.uint32)
+    tokens[1:total + 1] = c["tokens"].reshape(-1)
+    tb, own, logprob = gpu.upload(tokens), gpu.buffer(total), gpu.buffer(total)
+    tree = wa.Tree(batch, rows, n, None, tb.ptr + 4, mask, rows * ((rows + 31) // 32))
+    gpu.logit_rules(tree, rules, x, None, vocab, vocab, pick=own, logprob=logprob)
+    want, prob = gpu.read(own, (total,), np.uint32), gpu.read(logprob, (total,))
+    for _ in range(5):
+        gpu.write(tb, tokens)
+        gpu.logit_rules(tree, rules, x, None, vocab, vocab, pick=tb.ptr + 4 + 4 * shift, logprob=logprob)
+        got = gpu.read(tb, (total + 2,), np.uint32)
+        assert np.array_equal(got[1 + shift:1 + shift + total], want)
+        assert got[:1 + shift].tolist() == tokens[:1 + shift].tolist()
+        assert got[1 + shift + total:].tolist() == tokens[1 + shift + total:].tolist()
+        assert np.array_equal(gpu.read(logprob, (total,)), prob)
+
+
 def test_two_contexts(gpu):
     """The same calls queued on two contexts (streams) at once, without waits between."""
     other = wa.Gpu(0)

@@ -442,9 +442,14 @@ int launch_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *r, const v
   // Who joins the parts: up to a workgroup a CU their last one (a row of 51866 f32 ids 9.1 us, 10.7 with a second launch,
   // whose start costs more than the counting); more of them wait for each other's counts (18 such rows 13.5 us counted,
   // 12.7 in two launches, 48 of them 18.7 and 14.7).
+  // Picks that lie in the tokens are written when all that read those are through: by a second launch, unless they take
+  // the very places of tokens that one run of rows alone reads.
+  const uintptr_t p0 = (uintptr_t)pick, t0 = (uintptr_t)t->tokens;
+  const bool over = pick && t->tokens && p0 < t0 + 4 * nodes && t0 < p0 + 4 * nodes && (p0 != t0 || groups > 1);
   const RuleArgs a{t->n, t->count, t->tokens, t->mask, t->mask_stride, t->rows, (t->rows + 31) / 32, r->penalty, r->history,
                    r->history_cols, r->from, r->bias_start, r->bias_id, r->bias, r->bias_len, r->allow, logits, out, vocab,
-                   chunks, group, groups, ld, part, pick, logprob, part && each * groups <= (size_t)cus && t->batch * groups <= ATTEND_HEADS ? ctx->attend_count : nullptr};
+                   chunks, group, groups, ld, part, pick, logprob,
+                   part && !over && each * groups <= (size_t)cus && t->batch * groups <= ATTEND_HEADS ? ctx->attend_count : nullptr};
   {
     ProfScope prof(ctx, "logit_rules", 0.0, (double)nodes * vocab * (f16 ? 2 : 4) * (out ? 2 : 1));
     if (int rc = f16 ? rules_launch<_Float16>(ctx, a, (int)each * groups) : rules_launch<float>(ctx, a, (int)each * groups)) return rc;
