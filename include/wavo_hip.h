@@ -383,12 +383,17 @@ typedef struct wh_tree {
  * x / (heads / kv_heads).  k and v are taken as the cache will hold them (rounded to f16); with k and v
  * NULL, or without a mask, the cache is all that is seen (cross attention).  kv: the caches, cols
  * positions of kv_heads * hd values each, kv_stride words apart (0: one cache for all).  o:
- * [batch * rows][heads * hd], f32 or (out16) f16.  Products of f32 queries and of the f32 softmax keep
- * their precision (each is split into two f16 parts); f16 queries are exact, and with out16 the softmax
- * weights are rounded to f16.  Masked keys and values may hold anything.  o overlaps none of the inputs.
+ * [batch * rows][heads * hd], f32 or (out16) f16.  f32 queries and, for f32 outputs, the softmax weights are
+ * taken in two f16 parts, which leaves 2^-22 of them; f16 queries are exact, and with out16 the weights
+ * are rounded to f16 once (half a step, 2^-11; their sum stays f32).  Masked keys and values may hold
+ * anything, and so may the rows past count[b], which are read; a row that sees a key or value that is no
+ * finite number in f16 may get NaN where the formula has an infinity or a zero weight.  o overlaps none
+ * of the inputs.
  * hd % 4 == 0, hd <= 128, cols <= 2^24, heads % kv_heads == 0, heads <= 1024, stride <= 2^23; pointers
- * 4-byte aligned (stride even for f16).  batch <= 65535 for up to 16 rows of a key head (rows * heads /
- * kv_heads), fewer for more (one for every 64 or 128 of them), and batch * rows * heads < 2^25. */
+ * 4-byte aligned (stride even for f16).  A workgroup takes 16, 32, 64 or 128 rows of a key head (of its
+ * rows * heads / kv_heads): batch times such blocks <= 65535, that times kv_heads and the splits of a long
+ * cache < 2^22 (splits are made where there are few workgroups), and batch * rows * heads < 2^25.
+ * Splits and loads are planned from cols, whatever part of the cache is in use. */
 int wh_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void *k, const void *v, size_t stride,
                    int in16, const uint32_t *kv, size_t kv_stride, int cols, void *o, int out16, int heads,
                    int kv_heads, int hd);
@@ -420,8 +425,9 @@ typedef struct wh_rules {
  * where nothing is left, NaN where the row holds one), either of which may be NULL.  Pick and
  * log-probability are those of the f32 values, before an f16 output is rounded.  Ids past vocab in
  * history, tokens and bias_id are passed over.  pick may lie in the tree's tokens (which are then gone); apart
- * from that, and out from logits, outputs overlap no input.  vocab <= 2^28, history_cols and bias_len <= 2^30; batch * vocab / 2048 workgroups of ten
- * rows have to be fewer than 2^24.  search::decode's `pick` for rows of many requests (src/whisper/search.rs:46-59). */
+ * from that, and out from logits, outputs overlap no input.  vocab <= 2^28, history_cols and
+ * bias_len <= 2^30; batch * vocab / 2048 workgroups of ten rows have to be fewer than 2^24.
+ * search::decode's `pick` for rows of many requests (src/whisper/search.rs:46-59). */
 int wh_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *rules, const void *logits, void *out, int vocab,
                    size_t ld, int f16, uint32_t *pick, float *logprob);
 

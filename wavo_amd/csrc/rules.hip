@@ -123,10 +123,9 @@ __device__ __forceinline__ void in_order() { asm volatile("" ::: "memory"); }
 
 // ALLOW, OUT, whole: what a row's pass loads and stores has to be the same for every row, so that a wait for one row's
 // loads is not one for the next rows'.  61 rows of 131071 f16 ids for 8 requests, 16000 ids of text and 1000 biases
-// each: 91 us (2.2 TB/s; 96 where the stores stay in L2, 104 with one row's registers only); 24 rows of 51866 f32 ids for
-// 16 requests: 33 us (3.7 TB/s; 40).  A copy of the former rows in the same form takes 42 us; the rest is each row's chain
-// of LDS trips, cross-lane sums and 232 vector instructions, in as many wavefronts as LDS has room for (five workgroups a
-// CU; 126 us with four).
+// each: 91 us (2.2 TB/s; 97 where the stores stay in L2); 24 rows of 51866 f32 ids for 16 requests: 33 us (3.7 TB/s; 40).
+// A copy of the former rows in the same form takes 42 us; the rest is each row's chain of LDS trips, cross-lane sums and 232
+// vector instructions, in as many wavefronts as LDS has room for (five workgroups a CU; 95 us with four).
 template <typename T, bool ALLOW, bool OUT>
 __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
 #pragma clang fp contract(off)  // the rules' sums and products are rounded one by one
@@ -171,8 +170,9 @@ __global__ __launch_bounds__(RT, 5) void rules_kernel(RuleArgs a) {
     if (whole) load(std::true_type{}, even, i0), load(std::true_type{}, odd, min(i0 + 1, last));
     else load(std::false_type{}, even, i0), load(std::false_type{}, odd, min(i0 + 1, last));
   };
-  // What is asked for before the sequence's numbers are known: its first rows and the text's first EARLY ids a thread (a
-  // row of 51866 ids 9.1 us, 9.7 asked for afterwards).
+  // What is asked for before the sequence's numbers are known: its first rows and the text's first EARLY ids a thread (61
+  // rows of 131071 ids for 8 requests 91.5 us, 93 asked for afterwards, 48 requests' one row of 51866 13.3 and 13.6; one
+  // request's row 8.5 us of kernel either way).
   constexpr int EARLY = 2;
   const bool counted = a.penalty != nullptr, biased = a.bias_start != nullptr, has_text = counted && a.history;
   const uint32_t *text = has_text ? a.history + (size_t)b * a.history_cols : nullptr;
@@ -428,8 +428,8 @@ int launch_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *r, const v
   const size_t nodes = (size_t)t->batch * t->rows;
   const int chunks = (vocab + IDS - 1) / IDS, parts = chunks * (RT / 64);
   // Rows per workgroup: about ten (fewer count the text too often, more leave the last workgroups alone: 61 rows of
-  // 131071 f16 ids for 8 requests took 115, 107, 107, 113 and 142 us with 4, 8, 12, 16 and 32 of them), or so few that
-  // there are 5 workgroups a CU.
+  // 131071 f16 ids for 8 requests take 103, 92, 91, 95, 95 and 100 us with 4, 8, 10, 12, 16 and 32 of them; texts of 448 ids
+  // and 24 rows would rather have 4: 31.2 us against 33.5), or so few that there are 5 workgroups a CU.
   const int cus = ctx->cus > 0 ? ctx->cus : 256;
   const size_t want = 5 * (size_t)cus, each = (size_t)chunks * t->batch;
   int groups = (int)std::min<size_t>(t->rows, std::max<size_t>((want + each - 1) / each, (t->rows + GROUP - 1) / GROUP));
@@ -439,9 +439,10 @@ int launch_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *r, const v
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "logit rules: %s", hipGetErrorString(e));
   RulePart *part = nullptr;
   if ((pick || logprob) && !(part = (RulePart *)wh_scratch(ctx, sizeof(RulePart) * parts * nodes))) return WH_EOOM;
-  // Who joins the parts: up to a workgroup a CU their last one (a row of 51866 f32 ids 9.1 us, 10.7 with a second launch,
-  // whose start costs more than the counting); more of them wait for each other's counts (18 such rows 13.5 us counted,
-  // 12.7 in two launches, 48 of them 18.7 and 14.7).
+  // Who joins the parts: up to a workgroup a CU their last one (a row of 51866 f32 ids 9.5 us, 12.7 with a second launch,
+  // whose start costs more than the counting; 9 such rows 10.8 and 12.5); many more of them wait for each other's counts and
+  // for their rows' stores before those (18 such rows 12.8 us counted, 12.5 in two launches, 48 of them 16.9 and 13.4; 10 to
+  // 14, which two launches take as well, are still 11.1 to 12.3 counted, 12.6 in two).
   // Picks that lie in the tokens are written when all that read those are through: by a second launch, unless they take
   // the very places of tokens that one run of rows alone reads.
   const uintptr_t p0 = (uintptr_t)pick, t0 = (uintptr_t)t->tokens;

@@ -211,15 +211,23 @@ __device__ __forceinline__ float split_query(const float (&f)[C][8], float scale
 //   meaning position NP g + 8kk + e.  A lane reads 4 values (from 4m on) of its NP positions of V, and v_perm
 //   pairs those of two positions.  A row's softmax state is one lane column's everywhere.
 //
-// The next block's K is loaded as soon as this one's scores are done, and its V after this one's outputs, so that
-// a wavefront always has loads in flight; the first block's before the queries are looked at.  Bound by the cache's bytes
-// where it is long (4 requests' 4 rows over 28 k keys of 8 heads of 128 values 88 us, 5.3 TB/s) and by its chain of
-// loads where it is short (16 rows of 20 heads of 64 values over 391 keys 8.5 us a call, of which 7 are the host's).
+// The next block's K is asked for as soon as this one's scores are done, and its V after this one's outputs; the first
+// block's before the queries are looked at.  For heads of 128 values this keeps loads in flight all the time.  In the code
+// made for heads of up to 64, and of any size that is no multiple of 32, it does not: load_k's whole and partial chunks
+// meet in the same registers, and each chunk's loads stand behind a wait for all that are under way, so that a block pays
+// a round trip per chunk of K and one for V.  Both forms' addresses also cost 37 to 126 scalar registers kept in lanes of
+// vector ones.  Bound by the cache's bytes where it is long (4 requests' 4 rows over 28 k keys of 8 heads of 128 values
+// 85 us, 5.4 TB/s) and by that chain of loads where it is short (16 rows of 20 heads of 64 values over 391 keys: 7.6 us of
+// kernel; 4 requests' 13 rows over 1100 to 1500: 11.4 us, twice their bytes' time).
 //
 // Precision: f32 queries are scaled by a power of two per row and split into two f16 parts, as is every
 // softmax weight for f32 outputs: two products each, with an error of 2^-22 against f32's own 2^-24 per sum.  Weights
 // are exp2(s - max + 10), so that the second part is no subnormal; a maximum that grows by less than SLACK binary
 // digits is left as it is, since they still fit f16 then.  K and V are f16 as stored.
+// P16 (f16 outputs): a weight is its first part alone, off by up to 2^-11 of itself, while the weights' sum stays f32.  Of 16
+// requests' 61 f16 rows, values of 0.24, that makes the outputs' error 6.2e-5 (root mean square) where rounding them once
+// leaves 5.0e-5; with both parts it is 5.0e-5 as well, and takes 16.4 us against 15.4 (4 requests' 100 rows over 28 k keys:
+// 1.00e-5, 0.82e-5, and 120 us against 114).
 //
 // ONCE: the cache is read past the chip's own caches.
 template <typename T, int HD, int QT, bool P16, bool ONCE>
@@ -251,7 +259,6 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
 
   Words kw[C][4];
   u32x2 vw[4 * KPC][Z];  // a block's K, pair by pair, and V, position by position
-  // The same loads on every way through, so that a wait for one block's does not have to be one for the next block's.
   auto load_k = [&](int blk) {
     // (made anew for every block: what follows from them would otherwise be kept in more registers than there are)
     int hd = a.hd, cols = a.cols;
@@ -550,10 +557,12 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
 // position too, from which the wavefronts read operands as they stand: 8 values of a position of K, and V
 // transposed by ds_read_b64_tr_b16 (rows 16 and 32 bytes longer, for the banks' sake).  Tile u's row r is position
 // 16u + r, so lane 16g + i's scores are those of positions 16u + 4g + 0 .. 3 of every u.  Workgroups of 8 wavefronts
-// get by with 128 registers, so that two share a CU, those of 4 with 168 for three.  Its wavefronts wait for each other
+// get by with 128 registers, so that two share a CU, those of 4 with 168 for three; f32 queries of heads past 64 values need 8
+// more than the former 128, which are spilled outside the loop over the cache.  Its wavefronts wait for each other
 // block by block, so the matrix cores, LDS and the softmax's instructions share the time rather than overlap (200 rows of
 // f32 queries on 64 values: vector instructions 54 % of it, matrix cores 26 %): 4 requests' 100 f16 rows over 28 k keys of
-// 8 heads of 128 values 115 us (4.0 TB/s, 305 TFLOP/s), 16 requests' 61 rows over up to 448 keys of 20 heads 15.2 us.
+// 8 heads of 128 values 114 us (4.0 TB/s, 305 TFLOP/s), 16 requests' 61 rows over up to 448 keys of 20 heads 15.4 us.
+// The nodes' rows and masks are asked for only when the cache's blocks are done, which such short caches feel.
 template <typename T, int HD, int RT, bool P16>
 __global__ __launch_bounds__(64 * RT, RT == 8 ? 4 : 3) void attend_rows_kernel(AttendArgs a) {
   constexpr int C = HD / 32, X = HD / 16, QP = sizeof(T) == 4 ? 2 : 1, B = rows_block(HD), NT = B / 16, KK = B / 32;
@@ -914,7 +923,7 @@ struct KeepArgs {
 // The kept nodes' K and V into the caches: a thread per pair of values, K's pairs and then V's.  Bound by its chain of
 // loads and by K's layout, whose words of a position lie `cols` apart: AT positions' rows are loaded side by side, and
 // four neighbouring positions' words of a pair of K go in one store (9 nodes of 1280 values for 32 sequences and 4
-// layers: 9.7 us, 1.9 TB/s; word by word 11.4).
+// layers: 10.2 us of kernel, 1.7 TB/s; word by word 12.7).
 template <typename T>
 __global__ __launch_bounds__(256) void keep_kernel(AcceptArgs t, KeepArgs a) {
   typedef T Pair __attribute__((ext_vector_type(2)));
@@ -1030,10 +1039,11 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
                cols, heads, kv_heads, hd, 1.0f / sqrtf((float)hd), 1, 1, 1, few_block(hd), NODES, nullptr, nullptr};
   const int rows = t->rows * (heads / kv_heads), tiles = (rows + 15) / 16;
   // Which kernel: up to 32 rows (16 of larger heads, for want of registers) attend_kernel, as it shares nothing (4
-  // requests' 16 rows of 20 heads of 64 values over 448 keys 8.5 us, 12.3 by attend_rows_kernel; 32 rows 10.6 and 12.9).
+  // requests' 16 rows of 20 heads of 64 values over 448 keys 8.5 us, 12.4 by attend_rows_kernel; 32 rows 10.7 and 12.8).
   // More rows need the blocks shared.  attend_rows_kernel's workgroups have 4 wavefronts where that is all the rows there
-  // are (64 rows over 4000 keys 29.2 us, 32.3 with 8) and 8 otherwise (100 rows of 128 values over 28 k keys 119 us, 141
-  // with 4).
+  // are (4 requests' 60 f32 rows of 8 heads of 128 values over 28 k keys 98 us, 108 with 8; 16 requests' 20 over 448 16.7 and
+  // 18.6; f16 rows and heads of 64 values within 4 % either way) and 8 otherwise (100 f16 rows of 128 values over 28 k keys
+  // 114 us, 135 with 4).
   const int most = hd <= 64 ? 2 : 1;  // tiles of attend_kernel
   const int rt = tiles > most && hd >= 8 && cols >= 4 ? tiles <= 4 ? 4 : 8 : 0, qt = std::min(tiles, most);
   if (rt) a.block = a.node_block = rows_block(hd);
@@ -1043,11 +1053,12 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
   const size_t cus = ctx->cus > 0 ? ctx->cus : 256;
   a.kw = rt ? 1 : std::min(WAVES, blocks);
   // A second launch joins the splits, so a cache that one workgroup gets through in 4 blocks a wavefront (8 of
-  // attend_rows_kernel's) stays whole (1500 keys of 8 heads of 64 values for 4 requests 11.9 us, 13.5 in parts).  Of a
-  // longer one each has at least half as many (4000 keys 14.9 us, 17.8 with as many), and there are as many as keep the
+  // attend_rows_kernel's) stays whole (1500 keys of 8 heads of 64 values for 4 requests 12.2 us, 13.6 in parts).  Of a
+  // longer one each has at least half as many (4000 keys 14.9 us, 17.9 with as many), and there are as many as keep the
   // rounds of workgroups that the CUs hold at once short and full (1500 keys of 20 heads of 100 values for 5 requests
-  // 21.8 us with 2 splits, 28.5 with 3, whose last round has 44 workgroups for 256 CUs; 300 nodes of 32 heads over 28 k
-  // keys 253 us, 299 with one round's number rounded up).
+  // 22.3 us with 2 splits, 28.8 with 3, whose last round has 44 workgroups for 256 CUs; 4 requests' 300 nodes of 8 heads
+  // over 28 k keys 239 us, 276 with one round's number rounded up).  All of this goes by the cache's size, since the lengths
+  // are on the device: a long cache of which little is in use is planned as a full one and pays the second launch.
   const int least = (rt ? 4 : 2) * a.kw;
   if (blocks > 2 * least) {
     const size_t slots = cus * (rt ? 2 : 1);
@@ -1067,8 +1078,8 @@ int launch_tree_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
     a.pml = a.po + part * hd;
   }
   // Caches of more than the 256 MB that the chip keeps are read past it (4 requests' 4 rows over 28 k keys of 8 heads of 128
-  // values: 88 us, 98 through it); smaller ones may be found there by the next step (4 requests' 13 rows over 1300 keys:
-  // 11.5 us, 15.0 past it).  attend_rows_kernel gains nothing by it.
+  // values: 85 us, 95 through it); smaller ones may be found there by the next step (4 requests' 13 rows over 1300 keys:
+  // 11.6 us, 15.1 past it), which a large one of which little is in use goes without.  attend_rows_kernel gains nothing by it.
   const bool once = kv_stride && a.row_blocks == 1 && 4 * (size_t)t->batch * kv_heads * hd * cols > (size_t)256 << 20;
   return in16 ? out16 ? attend_t<_Float16, true>(ctx, a, qt, rt, once) : attend_t<_Float16, false>(ctx, a, qt, rt, once)
               : out16 ? attend_t<float, true>(ctx, a, qt, rt, once) : attend_t<float, false>(ctx, a, qt, rt, once);
@@ -1099,7 +1110,7 @@ int launch_tree_accept(wh_ctx *ctx, const wh_tree *t, const uint32_t *picks, con
                      path, kept, next, n_out, history, history_cols};
   const size_t nodes = (size_t)t->batch * t->rows, masks = t->mask_stride ? t->mask_stride * t->batch : (size_t)t->rows * a.words;
   // One launch, each of whose workgroups walks its sequence's tree for itself, unless an output lies in what they read (32
-  // sequences' 9 of 61 nodes in 4 layers of 1280 values 10.2 us, 12.5 in two launches; trees of 1000 nodes 15.5 and 18.8).
+  // sequences' 9 of 61 nodes in 4 layers of 1280 values 10.4 us, 13.2 in two launches; 4 sequences' 9 of 1000 9.9 and 12.8).
   auto apart = [&](const void *y, size_t words) {
     const struct {
       const void *p;
