@@ -276,6 +276,19 @@ def test_attend_cache_alone(gpu, rows):
     check_attend(one, q, None, None, None, n, count, kc[:1], vc[:1], heads, heads, hd, False, False)
 
 
+@pytest.mark.parametrize("in16", [False, True])
+@pytest.mark.parametrize("batch,rows,heads,kv_heads,hd,cols", [(3, 1, 4, 4, 64, 3000), (2, 25, 8, 2, 128, 5000), (4, 61, 6, 6, 64, 448), (2, 9, 3, 3, 100, 1500)])
+def test_attend_repeats_itself(gpu, batch, rows, heads, kv_heads, hd, cols, in16):
+    """The same call gives the same bits, with splits and without, whatever ran on the device before it."""
+    _, q, k, v, seen, kc, vc = case(16, batch, rows, heads, kv_heads, hd, cols, in16)
+    n = [cols - 3 * b for b in range(batch)]
+    want = attend(gpu, q, k, v, seen, n, None, kc, vc, heads, kv_heads, hd, in16, in16)
+    for turn in range(6):
+        if turn % 2:
+            attend(gpu, -q, v, k, seen, n[::-1], None, vc, kc, heads, kv_heads, hd, in16, in16)
+        assert np.array_equal(attend(gpu, q, k, v, seen, n, None, kc, vc, heads, kv_heads, hd, in16, in16), want)
+
+
 def test_attend_one_tree_for_all(gpu):
     batch, rows, heads, hd, cols = 4, 21, 4, 64, 90
     _, q, k, v, seen, kc, vc = case(5, batch, rows, heads, heads, hd, cols)

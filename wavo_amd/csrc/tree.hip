@@ -560,7 +560,7 @@ __global__ __launch_bounds__(64 * WAVES) void attend_kernel(AttendArgs a) {
 // get by with 128 registers, so that two share a CU, those of 4 with 168 for three; f32 queries of heads past 64 values need 8
 // more than the former 128, which are spilled outside the loop over the cache.  Its wavefronts wait for each other
 // block by block, so the matrix cores, LDS and the softmax's instructions share the time rather than overlap (200 rows of
-// f32 queries on 64 values: vector instructions 54 % of it, matrix cores 26 %): 4 requests' 100 f16 rows over 28 k keys of
+// f32 queries on 64 values over 23 k keys: vector instructions 50 % of it, matrix cores 29 %): 4 requests' 100 f16 rows over 28 k keys of
 // 8 heads of 128 values 114 us (4.0 TB/s, 305 TFLOP/s), 16 requests' 61 rows over up to 448 keys of 20 heads 15.4 us.
 // The nodes' rows and masks are asked for only when the cache's blocks are done, which such short caches feel.
 template <typename T, int HD, int RT, bool P16>
