@@ -73,6 +73,13 @@ SIGNATURES = {
     "wh_tree_attend": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _i, _vp, _sz, _i, _vp, _i, _i, _i, _i]),
     "wh_logit_rules": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _sz, _i, _vp, _vp]),
     "wh_tree_accept": (_i, [_vp, _vp, _vp, _vp, _i, _vp, _vp, _vp, _vp, _vp, _i]),
+    "wh_page_bytes": (_sz, [_i, _i, _i, _i]),
+    "wh_head_norm": (_i, [_vp, _vp, _vp, _vp, _sz, _i, _vp, _sz, _i]),
+    "wh_page_append": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _sz, _i, _vp, _vp, _vp, _vp, _sz, _i, _vp]),
+    "wh_page_read": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _i]),
+    "wh_page_attend": (_i, [_vp, _vp, _vp, _vp, _vp, _sz, _i, _vp, _vp, _i, _i]),
+    "wh_logit_probs": (_i, [_vp, _vp, _vp, _sz, _i, _i, _vp, _vp, _sz]),
+    "wh_tree_sample": (_i, [_vp, _vp, _vp, _vp, _i, _sz, _vp, _vp]),
     "wh_model_load": (_i, [_vp, ctypes.c_char_p, ctypes.POINTER(_vp)]),
     "wh_model_free": (None, [_vp]),
     "wh_model_info": (_i, [_vp] + [ctypes.POINTER(_i)] * 5),
@@ -280,6 +287,33 @@ class Rules(ctypes.Structure):
         self._keep = penalty, history, bias_start, bias_id, bias, allow
 
 
+class Heads(ctypes.Structure):
+    """wh_heads: a projection's heads, and the norms and rotation of queries and keys (device pointers, as Tree's)."""
+
+    _fields_ = [("heads", _i), ("kv_heads", _i), ("hd", _i), ("q_gain", _vp), ("k_gain", _vp), ("eps", _f), ("table", _vp),
+                ("positions", _i), ("rot", _i), ("pairs", _i)]
+
+    def __init__(self, heads, kv_heads, hd, q_gain=None, k_gain=None, eps=1e-6, table=None, positions=0, rot=0, pairs=False):
+        super().__init__(heads, kv_heads, hd, _p(q_gain), _p(k_gain), eps, _p(table), positions, rot, pairs)
+        self._keep = q_gain, k_gain, table
+
+
+def page_bytes(type, page, kv_heads, hd):
+    """Bytes of a page of `page` positions (wh_page_bytes); 0 where its type or sizes are not supported."""
+    return lib().wh_page_bytes(type, page, kv_heads, hd)
+
+
+class Pages(ctypes.Structure):
+    """wh_pages: caches in pages of F16 or Q4_0 keys and values (device pointers, as Tree's)."""
+
+    _fields_ = [("pool", _vp), ("pages", _i), ("table", _vp), ("table_cols", _i), ("table_stride", _sz), ("page", _i), ("type", _i),
+                ("kv_heads", _i), ("hd", _i)]
+
+    def __init__(self, pool, pages, table, table_cols, table_stride, page, type, kv_heads, hd):
+        super().__init__(_p(pool), pages, _p(table), table_cols, table_stride, page, type, kv_heads, hd)
+        self._keep = pool, table
+
+
 class _Kept(ctypes.Structure):
     _fields_ = [("k", _vp), ("v", _vp), ("stride", _sz), ("layer_stride", _sz), ("in16", _i), ("kv", _vp),
                 ("kv_stride", _sz), ("kv_layer_stride", _sz), ("layers", _i), ("d", _i)]
@@ -477,6 +511,34 @@ class Gpu:
             where = ctypes.byref(_Kept(_p(k), _p(v), stride, layer_stride, in16, _p(kv), kv_stride, kv_layer_stride, layers, d))
         self._check(lib().wh_tree_accept(self.h, ctypes.byref(tree), _p(picks), where, cols, _p(path), _p(kept), _p(next),
                                          _p(n_out), _p(history), history_cols))
+
+    # -- sampled decoding over caches in pages
+    def head_norm(self, tree, heads, x, stride, y, y_stride, in16=False, out16=False):
+        """Queries and keys of the rows x normed and rotated (Heads) into y, v copied where y is not x."""
+        self._check(lib().wh_head_norm(self.h, ctypes.byref(tree), ctypes.byref(heads), _p(x), stride, in16, _p(y), y_stride, out16))
+
+    def page_append(self, tree, heads, q, k, v, stride, pages, path=None, kept=None, qo=None, qo_stride=0, n_out=None, in16=False,
+                    out16=False):
+        """Keys and values of the rows (those of `path`) into Pages, keys and queries normed and rotated on the way."""
+        self._check(lib().wh_page_append(self.h, ctypes.byref(tree), ctypes.byref(heads), _p(q), _p(k), _p(v), stride, in16, _p(path),
+                                         _p(kept), ctypes.byref(pages), _p(qo), qo_stride, out16, _p(n_out)))
+
+    def page_read(self, tree, pages, k, v, stride, out16=False):
+        """Keys and values of the sequences' positions from n on out of Pages."""
+        self._check(lib().wh_page_read(self.h, ctypes.byref(tree), ctypes.byref(pages), _p(k), _p(v), stride, out16))
+
+    def page_attend(self, tree, q, k, v, stride, pages, o, heads, in16=False, out16=False):
+        """Attention of every node of `tree` over its sequence's positions in Pages and the nodes that it sees."""
+        self._check(lib().wh_page_attend(self.h, ctypes.byref(tree), _p(q), _p(k), _p(v), stride, in16, ctypes.byref(pages), _p(o), out16,
+                                         heads))
+
+    def logit_probs(self, tree, logits, probs, vocab, ld, probs_ld, temperature=None, half=False):
+        """Softmax of the nodes' logits at their sequence's temperature."""
+        self._check(lib().wh_logit_probs(self.h, ctypes.byref(tree), _p(logits), ld, half, vocab, _p(temperature), _p(probs), probs_ld))
+
+    def tree_sample(self, tree, probs, drafts, vocab, ld, u, picks):
+        """Verifies the drafted tokens against probabilities: the picks that tree_accept follows, and the token after them."""
+        self._check(lib().wh_tree_sample(self.h, ctypes.byref(tree), _p(probs), _p(drafts), vocab, ld, _p(u), _p(picks)))
 
     def im2col(self, x, col, t, ch, kernel, stride, pad):
         self._check(lib().wh_im2col(self.h, _p(x), _p(col), t, ch, kernel, stride, pad))

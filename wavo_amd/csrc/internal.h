@@ -315,6 +315,26 @@ int launch_tree_accept(wh_ctx *ctx, const wh_tree *t, const uint32_t *picks, con
 int launch_logit_rules(wh_ctx *ctx, const wh_tree *t, const wh_rules *r, const void *logits, void *out, int vocab, size_t ld,
                        int f16, uint32_t *pick, float *logprob);
 
+// ---- sampled decoding over caches in pages (pages.hip, page_attend.hip, sample.hip) ----
+namespace pages {
+struct Pages;
+}
+// Bytes of a page, 0 where its type or sizes are not supported; whether a call can run over `p` (its error set if not), and
+// what its kernels take.
+size_t page_bytes(int type, int page, int kv_heads, int hd);
+int pages_check(wh_ctx *ctx, const char *what, const wh_pages *p);
+pages::Pages pages_of(const wh_pages *p);
+int launch_head_norm(wh_ctx *ctx, const wh_tree *t, const wh_heads *h, const void *x, size_t stride, int in16, void *y, size_t y_stride,
+                     int out16);
+int launch_page_append(wh_ctx *ctx, const wh_tree *t, const wh_heads *h, const void *q, const void *k, const void *v, size_t stride, int in16,
+                       const int32_t *path, const int32_t *kept, const wh_pages *p, void *qo, size_t qo_stride, int out16, int32_t *n_out);
+int launch_page_read(wh_ctx *ctx, const wh_tree *t, const wh_pages *p, void *k, void *v, size_t stride, int out16);
+int launch_page_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void *k, const void *v, size_t stride, int in16, const wh_pages *p,
+                       void *o, int out16, int heads);
+int launch_logit_probs(wh_ctx *ctx, const wh_tree *t, const void *logits, size_t ld, int f16, int vocab, const float *temperature, float *probs,
+                       size_t probs_ld);
+int launch_tree_sample(wh_ctx *ctx, const wh_tree *t, const float *probs, const float *drafts, int vocab, size_t ld, const float *u, uint32_t *picks);
+
 // ---- greedy decoding on the device (greedy.hip) ----
 // The TDT loop's state (src/parakeet/decoder.rs:158-191), in device memory: the call's encoder output
 // and (token, frame) list too, so a recorded decision serves every call.

@@ -1,0 +1,557 @@
+// Attention of a step's rows over caches in pages (include/wavo_hip.h, wh_page_attend; pages.h for their layout).
+#include <algorithm>
+#include <type_traits>
+
+#include "internal.h"
+#include "pages.h"
+#include "rows.h"
+#include "xlane.h"
+
+namespace {
+
+using namespace rows;
+using namespace pages;
+
+struct PageAttendArgs {
+  const void *q, *k, *v;
+  size_t stride;
+  Pages pages;
+  void *o;
+  int out16;
+  const int32_t *n, *count;
+  const uint32_t *mask;
+  size_t mask_stride;
+  int batch, rows, words, heads;
+  float scale;
+  int kw, splits, row_blocks;
+  // splits > 1: unnormalized outputs [split][batch * rows][heads][hd] and (maximum, sum, factor of the maximum's exponent,
+  // -) [split][batch * rows][heads] of the splits that are used.
+  float *po, *pml;
+};
+
+constexpr int WAVES = 8;    // wavefronts of a workgroup, at most
+constexpr int SPLITS = 64;  // and splits of a cache
+
+// The tiles of a sequence (the cache's, then the nodes'), and how its `splits` workgroups share them: runs of `per`, at least
+// one tile for each wavefront, so that a short sequence uses fewer of them.
+struct Share {
+  int n, count, cached, tiles, per, used;
+};
+__device__ __forceinline__ Share share_of(const PageAttendArgs &a, int b) {
+  Share s;
+  s.n = min(max(a.n[b], 0), a.pages.room);
+  s.count = a.count ? min(max(a.count[b], 0), a.rows) : a.rows;
+  s.cached = (s.n + TILE - 1) / TILE;
+  s.tiles = s.cached + (a.mask && a.k ? (s.count + TILE - 1) / TILE : 0);
+  s.per = s.tiles, s.used = 1;
+  if (a.splits > 1) {
+    s.per = max((s.tiles + a.splits - 1) / a.splits, a.kw);
+    s.used = max((s.tiles + s.per - 1) / s.per, 1);
+  }
+  return s;
+}
+
+// A tile's share of a lane: words of K and V, and for 4 bits their factors.
+template <int Z, bool Q4>
+struct Tile;
+template <int Z>
+struct Tile<Z, true> {
+  uint32_t k[2 * Z], v[2 * Z];
+  half8 kd[Z], vd[Z];
+  static __device__ __forceinline__ void words(uint32_t (&w)[2 * Z], const uint32_t *p, int lane) {
+    constexpr int T = 2 * Z, whole = T & ~3;
+#pragma unroll
+    for (int t = 0; t < whole; t += 4) {
+      const u32x4 x = *(const u32x4 *)(p + t * 64 + lane * 4);
+      w[t] = x[0], w[t + 1] = x[1], w[t + 2] = x[2], w[t + 3] = x[3];
+    }
+    if constexpr (T > whole) {
+      const u32x2 x = *(const u32x2 *)(p + whole * 64 + lane * 2);
+      w[whole] = x[0], w[whole + 1] = x[1];
+    }
+  }
+  __device__ __forceinline__ void load_k(const uint32_t *p, int lane, int g) {
+    words(k, p, lane);
+#pragma unroll
+    for (int c = 0; c < Z; c++) kd[c] = *(const half8 *)(p + 128 * Z + (g * Z + c) * 4);
+  }
+  __device__ __forceinline__ void load_v(const uint32_t *p, int lane, int g) {
+    words(v, p + 144 * Z, lane);
+#pragma unroll
+    for (int c = 0; c < Z; c++) vd[c] = *(const half8 *)(p + 272 * Z + (g * Z + c) * 4);
+  }
+  // nibble - 8 of the 8 elements, exactly: nibbles are the last bits of 1024 + x and of 64 + x.
+  static __device__ __forceinline__ half8 open(uint32_t w) {
+    u32x4 r;
+#pragma unroll
+    for (int i = 0; i < 2; i++, w >>= 8) {
+      const half2 lo = __builtin_bit_cast(half2, (w & 0x000f000fu) | 0x64006400u) - half2{(_Float16)1032, (_Float16)1032};
+      const half2 hi = __builtin_bit_cast(half2, (w & 0x00f000f0u) | 0x54005400u) - half2{(_Float16)72, (_Float16)72};
+      r[2 * i] = __builtin_bit_cast(uint32_t, lo), r[2 * i + 1] = __builtin_bit_cast(uint32_t, hi);
+    }
+    return __builtin_bit_cast(half8, r);
+  }
+  // What stands in positions that are not there must not meet their zero weights.
+  __device__ __forceinline__ void clear_v(uint32_t there) {
+#pragma unroll
+    for (int c = 0; c < Z; c++)
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (!(there >> e & 1)) vd[c][e] = (_Float16)0;
+  }
+};
+template <int Z>
+struct Tile<Z, false> {
+  u32x4 k[2 * Z], v[2 * Z];
+  __device__ __forceinline__ void load_k(const uint32_t *p, int lane, int) {
+#pragma unroll
+    for (int t = 0; t < 2 * Z; t++) k[t] = *(const u32x4 *)(p + (t * 64 + lane) * 4);
+  }
+  __device__ __forceinline__ void load_v(const uint32_t *p, int lane, int) {
+#pragma unroll
+    for (int t = 0; t < 2 * Z; t++) v[t] = *(const u32x4 *)(p + 512 * Z + (t * 64 + lane) * 4);
+  }
+  static __device__ __forceinline__ half8 open(u32x4 w) { return __builtin_bit_cast(half8, w); }
+  __device__ __forceinline__ void clear_v(uint32_t there) {
+#pragma unroll
+    for (int t = 0; t < 2 * Z; t++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) v[t][e] &= (there >> (2 * e) & 1 ? 0xffffu : 0u) | (there >> (2 * e + 1) & 1 ? 0xffff0000u : 0u);
+  }
+};
+
+// A workgroup takes one key head of a sequence, 16 * QT of its rows (the heads / kv_heads query heads of a node are rows next
+// to each other) and one split of its tiles, of which each of its kw wavefronts takes every kw-th.
+//   Scores transposed, S^T = K Q^T: lane 16g + i holds row i's scores of positions position_of(g, e), e < 8.  For 4 bits the
+//   products are those of nibble - 8, exact in f16, chunk by chunk of 32 values, and every chunk's sum is multiplied by its
+//   position's factor in f32: K is taken as it stands.
+//   Outputs transposed, O^T = V^T P^T, with V's factors in the weights: a chunk's 32 values of V share one factor, so the
+//   operand of P for that chunk is p * d.
+// The next tile's K is asked for as soon as this one's scores are done, and its V after this one's outputs; its page two tiles
+// ahead.
+//
+// Precision: f32 queries are scaled by a power of two per row and split into two f16 parts, as are the weights (p * d) for
+// f32 outputs: two products each, with an error of 2^-22.  Weights are exp2(s - max + 10 - E): the second part is no
+// subnormal, and E, zero until a factor of V reaches 2, keeps p * d within f16.  P16 (f16 outputs): p and p * d are rounded to
+// f16, off by 2^-11 of themselves each, beside the output's own rounding; the weights' sum stays f32.
+template <int Z, int QT, int QP, bool P16, bool Q4>
+__global__ __launch_bounds__(64 * WAVES) void page_attend_kernel(PageAttendArgs a) {
+  typedef typename std::conditional<QP == 2, float, _Float16>::type T;
+  constexpr int hd = 32 * Z;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const int lane = threadIdx.x & 63, ki = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, m = lane & 15;
+  const int split = blockIdx.z, kh = blockIdx.x, b = a.row_blocks == 1 ? blockIdx.y : blockIdx.y / a.row_blocks;
+  const int group = a.heads / a.pages.kv_heads, r0 = 16 * QT * (blockIdx.y - b * a.row_blocks);
+  const size_t row0 = (size_t)b * a.rows;
+  float f[QT][Z][8];
+  int node[QT];
+#pragma unroll
+  for (int t = 0; t < QT; t++) {  // (of rows that are not there, too: nothing is known of the lengths yet)
+    const int row = min(r0 + 16 * t + m, a.rows * group - 1);
+    node[t] = node_of(row, group);
+    load_query<T, Z>((const T *)a.q + (row0 + node[t]) * a.stride + (size_t)(kh * group + head_of(row, group)) * hd, g, hd, f[t]);
+  }
+  const Share s = share_of(a, b);
+  const int total = s.count * group;
+  if (split >= s.used || r0 >= total) return;
+  const int end = min((split + 1) * s.per, s.tiles), cached = min(end, s.cached);
+  const int slot = a.pages.shift - 5;
+  const int32_t *table = a.pages.table + (size_t)b * a.pages.table_stride;
+
+  // The tiles that are there, in turn: `blk` is worked on, `next` is asked for, and the page of `after` is.
+  auto id_of = [&](int tile) { return table[min(tile, cached - 1) >> slot]; };
+  auto skip = [&](int &tile, int &id) {
+    while (tile < cached && (uint32_t)id >= (uint32_t)a.pages.pages) tile += a.kw, id = id_of(tile);
+  };
+  auto at = [&](int tile, int id) {
+    return (const uint32_t *)a.pages.pool + (size_t)id * a.pages.page_words + (size_t)((kh << slot) + (tile & ((1 << slot) - 1))) * tile_words(Q4, hd);
+  };
+  Tile<Z, Q4> w;
+  int blk = split * s.per + ki, next = cached, next_id = -1;
+  if (blk < cached) {
+    int id = id_of(blk);
+    skip(blk, id);
+    if (blk < cached) {
+      const uint32_t *p = at(blk, id);
+      w.load_k(p, lane, g), w.load_v(p, lane, g);
+      next = blk + a.kw, next_id = id_of(next);
+    }
+  }
+
+  half8 q[QT][Z][QP];
+  floatx4 acc[QT][2 * Z];
+  float mx[QT], sum[QT], cf[QT], slack[QT], digits = 10.0f;
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    cf[t] = split_query(f[t], a.scale, q[t]);
+    if (r0 + 16 * t + m >= total) cf[t] = 0.0f;  // (whatever stands in a row past the last: no maximum, no far score)
+    slack[t] = SLACK / cf[t];
+    mx[t] = -INFINITY, sum[t] = 0.0f;
+#pragma unroll
+    for (int x = 0; x < 2 * Z; x++) acc[t][x] = floatx4{};
+  }
+
+  // Scores st of a tile into weights p: exp2 against the running maximum, and their sum.  seen: the lane's positions.
+  auto weights = [&](floatx4 (&st)[2], int t, uint32_t seen, float (&p)[8]) {
+    if (seen != 0xff)
+#pragma unroll
+      for (int e = 0; e < 8; e++)
+        if (!(seen >> e & 1)) st[e >> 2][e & 3] = -INFINITY;
+    float top = st[0][0];
+#pragma unroll
+    for (int e = 1; e < 8; e++) top = fmaxf(top, st[e >> 2][e & 3]);
+    top = xlane::bit4(top, xlane::Max{});
+    top = xlane::bit5(top, xlane::Max{});
+    if (__any(top > mx[t] + slack[t])) {
+      top = fmaxf(top, mx[t]);
+      const float old = mx[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mx[t] - top) * cf[t]);
+      sum[t] *= old;
+#pragma unroll
+      for (int x = 0; x < 2 * Z; x++) acc[t][x] *= old;
+      mx[t] = top;
+    }
+    const float base = mx[t] == -INFINITY ? 0.0f : mx[t];
+    float shift = fmaf(-base, cf[t], digits);
+    if (__any(fabsf(shift) > FAR)) {
+      shift = digits;
+      st[0] -= base, st[1] -= base;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      p[e] = __builtin_amdgcn_exp2f(fmaf(st[e >> 2][e & 3], cf[t], shift));
+      sum[t] += p[e];
+    }
+  };
+  // p times a chunk's factors as an operand, and (unless P16) what that leaves of them.
+  auto operand = [&](const float (&p)[8], const half8 *d, half8 &h, half8 &l) {
+    if constexpr (P16) {
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) weights2<true>(p[e], p[e + 1], h, l, e);
+      if (d) h *= *d;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e += 2)
+        weights2<false>(d ? p[e] * (float)(*d)[e] : p[e], d ? p[e + 1] * (float)(*d)[e + 1] : p[e + 1], h, l, e);
+    }
+  };
+  // Factors of V of 2 and more: the weights that follow are smaller by their largest's power of two.
+  auto room = [&] {
+    if constexpr (Q4) {
+      uint32_t any = 0;
+#pragma unroll
+      for (int c = 0; c < Z; c++) {
+        const u32x4 x = __builtin_bit_cast(u32x4, w.vd[c]);
+        any |= x[0] | x[1] | x[2] | x[3];
+      }
+      if (__any(any & 0x40004000u)) {
+        float most = 0.0f;
+#pragma unroll
+        for (int c = 0; c < Z; c++)
+#pragma unroll
+          for (int e = 0; e < 8; e++) most = fmaxf(most, fabsf((float)w.vd[c][e]));
+        most = xlane::wave_max(most);
+        const float want = 10.0f - fminf((float)(__builtin_amdgcn_frexp_expf(most) - 1), 15.0f);  // (most < 2^(10 - want + 1))
+        if (most >= 2.0f && want < digits) {
+          const float less = __builtin_amdgcn_exp2f(want - digits);
+#pragma unroll
+          for (int t = 0; t < QT; t++) {
+            sum[t] *= less;
+#pragma unroll
+            for (int x = 0; x < 2 * Z; x++) acc[t][x] *= less;
+          }
+          digits = want;
+        }
+      }
+    }
+  };
+
+  auto step = [&](auto more) {
+    int after = next + a.kw, after_id = 0;
+    if constexpr (more) after_id = id_of(after);
+    const uint32_t *np = at(next, next_id);
+    floatx4 st[QT][2];
+#pragma unroll
+    for (int t = 0; t < QT; t++) st[t][0] = st[t][1] = floatx4{};
+#pragma unroll
+    for (int c = 0; c < Z; c++)
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const half8 k = w.open(w.k[2 * c + u]);
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+          if constexpr (Q4) {
+            floatx4 x = mfma(k, q[t][c][0], floatx4{});
+            if constexpr (QP == 2) x = mfma(k, q[t][c][QP - 1], x);
+#pragma unroll
+            for (int r = 0; r < 4; r++) st[t][u][r] = fmaf(x[r], (float)w.kd[c][4 * u + r], st[t][u][r]);
+          } else {
+#pragma unroll
+            for (int part = 0; part < QP; part++) st[t][u] = mfma(k, q[t][c][part], st[t][u]);
+          }
+        }
+      }
+    if constexpr (more) w.load_k(np, lane, g);
+    const int left = s.n - TILE * blk;
+    uint32_t seen = 0xff;
+    if (left < TILE) {
+      const uint32_t there = (1u << left) - 1u;
+      seen = (there >> 4 * g & 15) | (there >> (16 + 4 * g) & 15) << 4;
+      w.clear_v(seen);
+    }
+    room();
+    float p[QT][8];
+#pragma unroll
+    for (int t = 0; t < QT; t++) weights(st[t], t, seen, p[t]);
+#pragma unroll
+    for (int c = 0; c < Z; c++) {
+      const half8 v0 = w.open(w.v[2 * c]), v1 = w.open(w.v[2 * c + 1]);
+#pragma unroll
+      for (int t = 0; t < QT; t++) {
+        half8 h, l;
+        if constexpr (Q4) operand(p[t], &w.vd[c], h, l);
+        else operand(p[t], nullptr, h, l);
+        acc[t][2 * c] = mfma(v0, h, acc[t][2 * c]), acc[t][2 * c + 1] = mfma(v1, h, acc[t][2 * c + 1]);
+        if constexpr (!P16) acc[t][2 * c] = mfma(v0, l, acc[t][2 * c]), acc[t][2 * c + 1] = mfma(v1, l, acc[t][2 * c + 1]);
+      }
+    }
+    if constexpr (more) {
+      w.load_v(np, lane, g);
+      blk = next, next = after, next_id = after_id;
+    }
+  };
+  if (blk < cached) {
+    for (skip(next, next_id); next < cached; skip(next, next_id)) step(std::true_type{});
+    step(std::false_type{});
+  }
+
+  // The nodes, 32 at a time: K and V as f16.
+  const int first = max(split * s.per, s.cached);
+  for (int tile = first + ((ki - (first - split * s.per)) % a.kw + a.kw) % a.kw; tile < end; tile += a.kw) {
+    const int j0 = TILE * (tile - s.cached), last = s.count - 1 - j0;
+    const T *k = (const T *)a.k + (row0 + j0) * a.stride + (size_t)kh * hd, *v = (const T *)a.v + (row0 + j0) * a.stride + (size_t)kh * hd;
+    const uint32_t there = last >= TILE - 1 ? 0xffffffffu : (2u << last) - 1u;
+    floatx4 st[QT][2];
+#pragma unroll
+    for (int t = 0; t < QT; t++) st[t][0] = st[t][1] = floatx4{};
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      const T *row = k + (size_t)min(16 * u + m, last) * a.stride + 8 * g;
+      typename Four<T>::type raw[Z][2];
+#pragma unroll
+      for (int c = 0; c < Z; c++) raw[c][0] = raw4(row + 32 * c), raw[c][1] = raw4(row + 32 * c + 4);
+#pragma unroll
+      for (int c = 0; c < Z; c++) {
+        const u32x2 x = pairs4(raw[c][0]), y = pairs4(raw[c][1]);
+        const half8 kf = __builtin_bit_cast(half8, u32x4{x[0], x[1], y[0], y[1]});
+#pragma unroll
+        for (int t = 0; t < QT; t++)
+#pragma unroll
+          for (int part = 0; part < QP; part++) st[t][u] = mfma(kf, q[t][c][part], st[t][u]);
+      }
+    }
+    float p[QT][8];
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+      const uint32_t sees = there & a.mask[(size_t)b * a.mask_stride + (size_t)node[t] * a.words + j0 / 32];
+      weights(st[t], t, (sees >> 4 * g & 15) | (sees >> (16 + 4 * g) & 15) << 4, p[t]);
+    }
+#pragma unroll
+    for (int c = 0; c < Z; c++) {
+      // Values of nodes that are not there are zeroed, and so are those that are no finite numbers: they must not meet the zero
+      // weights of the rows that do not see them, and are added to the others' outputs one by one.
+      uint32_t x[8];
+      u16x2 big{};
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const T *y = v + (size_t)min(position_of(g, e), last) * a.stride + 32 * c + 2 * m;
+        if constexpr (QP == 2) {
+          typedef floatx2 any __attribute__((aligned(4)));
+          const floatx2 f2 = *(const any *)y;
+          x[e] = pack2(f2[0], f2[1]);
+        } else {
+          x[e] = *(const uint32_t *)y;
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        if (position_of(g, e) > last) x[e] = 0;
+        big = __builtin_elementwise_max(big, __builtin_bit_cast(u16x2, x[e] & 0x7fff7fffu));
+      }
+      if (__any(big[0] >= 0x7c00 || big[1] >= 0x7c00)) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = finite2(x[e]);
+#pragma unroll 1
+        for (int j = 0; j < min(TILE, last + 1); j++) {
+          const T *y = v + (size_t)j * a.stride;
+#pragma unroll
+          for (int t = 0; t < QT; t++) {
+            if (!(a.mask[(size_t)b * a.mask_stride + (size_t)node[t] * a.words + j0 / 32] >> j & 1)) continue;
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+              for (int r = 0; r < 4; r++) acc[t][2 * c + i][r] += not_finite(y, 32 * c + 8 * g + 2 * r + i, hd);
+          }
+        }
+      }
+      u32x4 v0, v1;
+#pragma unroll
+      for (int i = 0; i < 4; i++) {
+        v0[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x05040100u);
+        v1[i] = __builtin_amdgcn_perm(x[2 * i + 1], x[2 * i], 0x07060302u);
+      }
+#pragma unroll
+      for (int t = 0; t < QT; t++) {
+        half8 h, l;
+        operand(p[t], nullptr, h, l);
+        const half8 a0 = __builtin_bit_cast(half8, v0), a1 = __builtin_bit_cast(half8, v1);
+        acc[t][2 * c] = mfma(a0, h, acc[t][2 * c]), acc[t][2 * c + 1] = mfma(a1, h, acc[t][2 * c + 1]);
+        if constexpr (!P16) acc[t][2 * c] = mfma(a0, l, acc[t][2 * c]), acc[t][2 * c + 1] = mfma(a1, l, acc[t][2 * c + 1]);
+      }
+    }
+  }
+
+  // The wavefronts' results joined through LDS: each writes its own, then every lane adds up four values of a row.  Lane
+  // 16g + i holds row i's values 32c + 8g + 2r + x.
+  floatx4 *merge = (floatx4 *)smem;                    // [ki][t][c][half][lane]
+  float *ml = (float *)(merge + a.kw * QT * Z * 128);  // [ki][t][maxima, sums][row]
+  const float more = __builtin_amdgcn_exp2f(10.0f - digits);
+#pragma unroll
+  for (int t = 0; t < QT; t++) {
+    sum[t] = xlane::bit4(sum[t], xlane::Add{});
+    sum[t] = xlane::bit5(sum[t], xlane::Add{});
+    if (g == 0) ml[32 * (ki * QT + t) + m] = mx[t], ml[32 * (ki * QT + t) + 16 + m] = sum[t] * more;
+#pragma unroll
+    for (int c = 0; c < Z; c++)
+#pragma unroll
+      for (int h = 0; h < 2; h++)
+        merge[(((ki * QT + t) * Z + c) * 2 + h) * 64 + lane] =
+            floatx4{acc[t][2 * c][2 * h], acc[t][2 * c + 1][2 * h], acc[t][2 * c][2 * h + 1], acc[t][2 * c + 1][2 * h + 1]} * more;
+  }
+  __syncthreads();
+  for (int x = ki; x < QT * Z * 2; x += a.kw) {
+    const int t = x / (2 * Z), c = x / 2 % Z, d = 32 * c + 8 * g + 4 * (x % 2), r = r0 + 16 * t + m;
+    if (r >= total) continue;
+    float km[WAVES], kl[WAVES], top = -INFINITY, l = 0.0f, scale = cf[0];
+    if (QT == 2 && t) scale = cf[QT - 1];
+    floatx4 kf[WAVES], o{};
+#pragma unroll
+    for (int k = 0; k < WAVES; k++) {
+      const int y = min(k, a.kw - 1) * QT;
+      km[k] = ml[32 * (y + t) + m], kl[k] = ml[32 * (y + t) + 16 + m], kf[k] = merge[(y * Z * 2 + x) * 64 + lane];
+      if (k >= a.kw) km[k] = -INFINITY;
+    }
+#pragma unroll
+    for (int k = 0; k < WAVES; k++) top = fmaxf(top, km[k]);
+#pragma unroll
+    for (int k = 0; k < WAVES; k++) {
+      if (k >= a.kw) break;
+      const float y = km[k] == top ? 1.0f : __builtin_amdgcn_exp2f((km[k] - top) * scale);
+      l += y * kl[k], o += y * kf[k];
+    }
+    const int i = node_of(r, group), head = kh * group + head_of(r, group);
+    const size_t out = ((row0 + i) * a.heads + head) * hd + d;
+    if (s.used > 1) {
+      const size_t part = (size_t)split * a.batch * a.rows * a.heads;
+      if (d == 0) *(floatx4 *)(a.pml + 4 * (part + (row0 + i) * a.heads + head)) = floatx4{top, l, scale, 0.0f};
+      *(floatx4 *)(a.po + part * hd + out) = o;
+      continue;
+    }
+    o *= top == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
+    if (a.out16) *(u32x2_a4 *)((_Float16 *)a.o + out) = u32x2{pack2(o[0], o[1]), pack2(o[2], o[3])};
+    else *(floatx4_a4 *)((float *)a.o + out) = o;
+  }
+}
+
+// The splits of a row's head joined, a lane per four values, 32 lanes a head.
+__global__ __launch_bounds__(256) void page_join_kernel(PageAttendArgs a) {
+  const int hd = a.pages.hd;
+  const size_t unit = (size_t)blockIdx.x * 8 + threadIdx.x / 32, heads = (size_t)a.batch * a.rows * a.heads;
+  const int d = 4 * (threadIdx.x % 32);
+  if (unit >= heads || d >= hd) return;
+  const int row = unit / a.heads, b = row / a.rows, i = row - b * a.rows;
+  const Share s = share_of(a, b);
+  if (i >= s.count || s.used == 1) return;
+  float top = -INFINITY, l = 0.0f;
+  floatx4 o{};
+  for (int k = 0; k < s.used; k++) top = fmaxf(top, a.pml[4 * (k * heads + unit)]);
+  for (int k = 0; k < s.used; k++) {
+    const floatx4 x = *(const floatx4 *)(a.pml + 4 * (k * heads + unit));
+    const float w = x[0] == top ? 1.0f : __builtin_amdgcn_exp2f((x[0] - top) * x[2]);
+    l += w * x[1], o += w * *(const floatx4 *)(a.po + (k * heads + unit) * hd + d);
+  }
+  o *= top == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
+  if (a.out16) *(u32x2_a4 *)((_Float16 *)a.o + unit * hd + d) = u32x2{pack2(o[0], o[1]), pack2(o[2], o[3])};
+  else *(floatx4_a4 *)((float *)a.o + unit * hd + d) = o;
+}
+
+template <int Z, int QT, int QP, bool P16, bool Q4>
+int attend_launch(wh_ctx *ctx, const PageAttendArgs &a) {
+  const double keys = (double)a.batch * a.pages.room;
+  ProfScope prof(ctx, "page_attend", 4.0 * keys * a.rows * a.heads * a.pages.hd, keys * a.pages.kv_heads * a.pages.hd * (Q4 ? 1.125 : 4.0));
+  const size_t shm = (size_t)a.kw * QT * (Z * 2048 + 128);
+  wh_launch(ctx, (page_attend_kernel<Z, QT, QP, P16, Q4>), dim3(a.pages.kv_heads, a.batch * a.row_blocks, a.splits), 64 * a.kw, shm, a);
+  return wh_launched(ctx, "page attention");
+}
+template <int Z, int QP, bool P16, bool Q4>
+int attend_qt(wh_ctx *ctx, const PageAttendArgs &a, int qt) {
+  return qt == 1 ? attend_launch<Z, 1, QP, P16, Q4>(ctx, a) : attend_launch<Z, 2, QP, P16, Q4>(ctx, a);
+}
+template <int QP, bool P16, bool Q4>
+int attend_z(wh_ctx *ctx, const PageAttendArgs &a, int qt) {
+  switch (a.pages.hd / 32) {
+    case 1: return attend_qt<1, QP, P16, Q4>(ctx, a, qt);
+    case 2: return attend_qt<2, QP, P16, Q4>(ctx, a, qt);
+    case 3: return attend_qt<3, QP, P16, Q4>(ctx, a, qt);
+    default: return attend_qt<4, QP, P16, Q4>(ctx, a, qt);
+  }
+}
+template <bool Q4>
+int attend_types(wh_ctx *ctx, const PageAttendArgs &a, int in16, int out16, int qt) {
+  return !in16 ? attend_z<2, false, Q4>(ctx, a, qt) : out16 ? attend_z<1, true, Q4>(ctx, a, qt) : attend_z<1, false, Q4>(ctx, a, qt);
+}
+
+}  // namespace
+
+int launch_page_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void *k, const void *v, size_t stride, int in16, const wh_pages *p,
+                       void *o, int out16, int heads) {
+  if (int rc = tree_check(ctx, "page attention", t)) return rc;
+  if (int rc = pages_check(ctx, "page attention", p)) return rc;
+  if (!q || !o || !k != !v) return wh_fail(ctx, WH_EARG, "page attention: q, o, and k with v are needed");
+  if (heads <= 0 || heads > ATTEND_HEADS || heads % p->kv_heads)
+    return wh_fail(ctx, WH_EARG, "page attention: %d heads over %d of keys", heads, p->kv_heads);
+  if (stride < (size_t)heads * p->hd || stride > (size_t)1 << 23)
+    return wh_fail(ctx, WH_EARG, "page attention: rows of %d queries %zu apart", heads * p->hd, stride);
+  if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o) % 4 || (in16 && stride % 2))
+    return wh_fail(ctx, WH_EARG, "page attention: buffers and rows must be 4-byte aligned");
+  PageAttendArgs a{q, k, v, stride, pages_of(p), o, out16 != 0, t->n, t->count, t->mask, t->mask_stride, t->batch, t->rows, (t->rows + 31) / 32,
+                   heads, 1.0f / sqrtf((float)p->hd), 1, 1, 1, nullptr, nullptr};
+  const int z = p->hd / 32, rows = t->rows * (heads / p->kv_heads), qt = rows > 16 ? 2 : 1;
+  const int tiles = a.pages.room / TILE + (t->mask && k ? (t->rows + TILE - 1) / TILE : 0);
+  a.row_blocks = (rows + 16 * qt - 1) / (16 * qt);
+  a.kw = std::min({WAVES, 32 / (z * qt), tiles});  // (64 KiB of LDS for their join)
+  const size_t units = (size_t)t->batch * p->kv_heads * a.row_blocks;
+  const size_t cus = ctx->cus > 0 ? ctx->cus : 256;
+  const int least = 2 * a.kw;
+  if (tiles > 2 * least) {
+    size_t best = SIZE_MAX;
+    for (int x = 1; x <= std::min(SPLITS, (tiles + least - 1) / least); x++) {
+      const size_t cost = (units * x + cus - 1) / cus * ((tiles + x - 1) / x + least);
+      if (cost < best) best = cost, a.splits = x;
+    }
+  }
+  const size_t nodes = (size_t)t->batch * t->rows;
+  if ((size_t)t->batch * a.row_blocks > 65535 || units * a.splits >= (size_t)1 << 22 || nodes * heads >= (size_t)1 << 25)  // (a launch's limits)
+    return wh_fail(ctx, WH_EARG, "page attention: %d heads of %zu nodes in one call", heads, nodes);
+  if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "page attention: %s", hipGetErrorString(e));
+  if (a.splits > 1) {
+    const size_t part = (size_t)a.splits * nodes * heads;
+    if (!(a.po = (float *)wh_scratch(ctx, part * (p->hd + 4) * sizeof(float)))) return WH_EOOM;
+    a.pml = a.po + part * p->hd;
+  }
+  if (int rc = p->type == WH_Q4_0 ? attend_types<true>(ctx, a, in16, out16, qt) : attend_types<false>(ctx, a, in16, out16, qt)) return rc;
+  if (a.splits == 1) return WH_OK;
+  ProfScope prof(ctx, "page_attend_join", 0.0, 4.0 * nodes * heads * a.splits * (p->hd + 4));
+  wh_launch(ctx, page_join_kernel, (unsigned)((nodes * heads + 7) / 8), 256, 0, a);
+  return wh_launched(ctx, "page attention's join");
+}

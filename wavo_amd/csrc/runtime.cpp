@@ -824,4 +824,41 @@ int wh_tree_accept(wh_ctx *ctx, const wh_tree *t, const uint32_t *picks, const w
   return launch_tree_accept(ctx, t, picks, where, cols, path, kept, next, n_out, history, history_cols);
 }
 
+size_t wh_page_bytes(int type, int page, int kv_heads, int hd) { return page_bytes(type, page, kv_heads, hd); }
+
+int wh_head_norm(wh_ctx *ctx, const wh_tree *t, const wh_heads *heads, const void *x, size_t stride, int in16, void *y, size_t y_stride,
+                 int out16) {
+  if (!ctx) return WH_EARG;
+  return launch_head_norm(ctx, t, heads, x, stride, in16, y, y_stride, out16);
+}
+
+int wh_page_append(wh_ctx *ctx, const wh_tree *t, const wh_heads *heads, const void *q, const void *k, const void *v, size_t stride, int in16,
+                   const int32_t *path, const int32_t *kept, const wh_pages *pages, void *qo, size_t qo_stride, int out16, int32_t *n_out) {
+  if (!ctx) return WH_EARG;
+  return launch_page_append(ctx, t, heads, q, k, v, stride, in16, path, kept, pages, qo, qo_stride, out16, n_out);
+}
+
+int wh_page_read(wh_ctx *ctx, const wh_tree *t, const wh_pages *pages, void *k, void *v, size_t stride, int out16) {
+  if (!ctx) return WH_EARG;
+  return launch_page_read(ctx, t, pages, k, v, stride, out16);
+}
+
+int wh_page_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void *k, const void *v, size_t stride, int in16, const wh_pages *pages,
+                   void *o, int out16, int heads) {
+  if (!ctx) return WH_EARG;
+  return launch_page_attend(ctx, t, q, k, v, stride, in16, pages, o, out16, heads);
+}
+
+int wh_logit_probs(wh_ctx *ctx, const wh_tree *t, const void *logits, size_t ld, int f16, int vocab, const float *temperature, float *probs,
+                   size_t probs_ld) {
+  if (!ctx) return WH_EARG;
+  return launch_logit_probs(ctx, t, logits, ld, f16, vocab, temperature, probs, probs_ld);
+}
+
+int wh_tree_sample(wh_ctx *ctx, const wh_tree *t, const float *probs, const float *drafts, int vocab, size_t ld, const float *u,
+                   uint32_t *picks) {
+  if (!ctx) return WH_EARG;
+  return launch_tree_sample(ctx, t, probs, drafts, vocab, ld, u, picks);
+}
+
 }  // extern "C"
