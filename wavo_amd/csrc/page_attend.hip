@@ -23,7 +23,7 @@ struct PageAttendArgs {
   size_t mask_stride;
   int batch, rows, words, heads;
   float scale;
-  int kw, splits, row_blocks;
+  int kw, splits, per, row_blocks;  // per: tiles of a split
   // splits > 1: unnormalized outputs [split][batch * rows][heads][hd] and (maximum, sum, factor of the maximum's exponent,
   // -) [split][batch * rows][heads] of the splits that are used.
   float *po, *pml;
@@ -31,11 +31,13 @@ struct PageAttendArgs {
 
 constexpr int WAVES = 8;    // wavefronts of a workgroup, at most
 constexpr int SPLITS = 64;  // and splits of a cache
+constexpr float LOWEST = -1e30f;  // the maximum of a row that has seen nothing
+constexpr int JOIN_LDS = 128 << 10;  // bytes in which wavefronts' results are joined
 
-// The tiles of a sequence (the cache's, then the nodes'), and how its `splits` workgroups share them: runs of `per`, at least
-// one tile for each wavefront, so that a short sequence uses fewer of them.
+// The tiles of a sequence (the cache's, then the nodes'): its workgroups take runs of `per`, so that a short sequence uses fewer
+// of them and they all take about as long.
 struct Share {
-  int n, count, cached, tiles, per, used;
+  int n, count, cached, tiles, used;
 };
 __device__ __forceinline__ Share share_of(const PageAttendArgs &a, int b) {
   Share s;
@@ -43,21 +45,19 @@ __device__ __forceinline__ Share share_of(const PageAttendArgs &a, int b) {
   s.count = a.count ? min(max(a.count[b], 0), a.rows) : a.rows;
   s.cached = (s.n + TILE - 1) / TILE;
   s.tiles = s.cached + (a.mask && a.k ? (s.count + TILE - 1) / TILE : 0);
-  s.per = s.tiles, s.used = 1;
-  if (a.splits > 1) {
-    s.per = max((s.tiles + a.splits - 1) / a.splits, a.kw);
-    s.used = max((s.tiles + s.per - 1) / s.per, 1);
-  }
+  s.used = a.splits > 1 ? max((s.tiles + a.per - 1) / a.per, 1) : 1;
   return s;
 }
 
 // A tile's share of a lane: words of K and V, and for 4 bits their factors.
-template <int Z, bool Q4>
+// OWN: of K those of the positions of the lane's own words (halfs for u = 0 and 1), otherwise those of its scores.
+template <int Z, bool Q4, bool OWN>
 struct Tile;
-template <int Z>
-struct Tile<Z, true> {
+template <int Z, bool OWN>
+struct Tile<Z, true, OWN> {
   uint32_t k[2 * Z], v[2 * Z];
-  half8 kd[Z], vd[Z];
+  typename std::conditional<OWN, half2, half8>::type kd[Z];
+  half8 vd[Z];
   static __device__ __forceinline__ void words(uint32_t (&w)[2 * Z], const uint32_t *p, int lane) {
     constexpr int T = 2 * Z, whole = T & ~3;
 #pragma unroll
@@ -72,22 +72,31 @@ struct Tile<Z, true> {
   }
   __device__ __forceinline__ void load_k(const uint32_t *p, int lane, int g) {
     words(k, p, lane);
+    if constexpr (OWN) {
+      const _Float16 *d = (const _Float16 *)(p + 128 * Z) + (lane % 16 / 4) * 8 * Z + lane % 4;
 #pragma unroll
-    for (int c = 0; c < Z; c++) kd[c] = *(const half8 *)(p + 128 * Z + (g * Z + c) * 4);
+      for (int c = 0; c < Z; c++) kd[c] = half2{d[8 * c], d[8 * c + 4]};
+    } else {
+#pragma unroll
+      for (int c = 0; c < Z; c++) kd[c] = *(const half8 *)(p + 128 * Z + (g * Z + c) * 4);
+    }
   }
   __device__ __forceinline__ void load_v(const uint32_t *p, int lane, int g) {
     words(v, p + 144 * Z, lane);
 #pragma unroll
     for (int c = 0; c < Z; c++) vd[c] = *(const half8 *)(p + 272 * Z + (g * Z + c) * 4);
   }
-  // nibble - 8 of the 8 elements, exactly: nibbles are the last bits of 1024 + x and of 64 + x.
-  static __device__ __forceinline__ half8 open(uint32_t w) {
+  // nibble - 8 of the 8 elements, exactly: nibbles are the last bits of 1024 + x and of 64 + x.  (The constants from registers, so
+  // that a mask and its sum are one instruction.)
+  uint32_t low = 0x000f000fu, high = 0x00f000f0u, large = 0x64006400u, small = 0x54005400u;
+  __device__ __forceinline__ Tile() { asm volatile("" : "+s"(low), "+s"(high), "+v"(large), "+v"(small)); }
+  __device__ __forceinline__ half8 open(uint32_t w) const {
     u32x4 r;
 #pragma unroll
     for (int i = 0; i < 2; i++, w >>= 8) {
-      const half2 lo = __builtin_bit_cast(half2, (w & 0x000f000fu) | 0x64006400u) - half2{(_Float16)1032, (_Float16)1032};
-      const half2 hi = __builtin_bit_cast(half2, (w & 0x00f000f0u) | 0x54005400u) - half2{(_Float16)72, (_Float16)72};
-      r[2 * i] = __builtin_bit_cast(uint32_t, lo), r[2 * i + 1] = __builtin_bit_cast(uint32_t, hi);
+      const half2 x = __builtin_bit_cast(half2, (w & low) | large) - half2{(_Float16)1032, (_Float16)1032};
+      const half2 y = __builtin_bit_cast(half2, (w & high) | small) - half2{(_Float16)72, (_Float16)72};
+      r[2 * i] = __builtin_bit_cast(uint32_t, x), r[2 * i + 1] = __builtin_bit_cast(uint32_t, y);
     }
     return __builtin_bit_cast(half8, r);
   }
@@ -100,8 +109,8 @@ struct Tile<Z, true> {
         if (!(there >> e & 1)) vd[c][e] = (_Float16)0;
   }
 };
-template <int Z>
-struct Tile<Z, false> {
+template <int Z, bool OWN>
+struct Tile<Z, false, OWN> {
   u32x4 k[2 * Z], v[2 * Z];
   __device__ __forceinline__ void load_k(const uint32_t *p, int lane, int) {
 #pragma unroll
@@ -111,7 +120,7 @@ struct Tile<Z, false> {
 #pragma unroll
     for (int t = 0; t < 2 * Z; t++) v[t] = *(const u32x4 *)(p + 512 * Z + (t * 64 + lane) * 4);
   }
-  static __device__ __forceinline__ half8 open(u32x4 w) { return __builtin_bit_cast(half8, w); }
+  __device__ __forceinline__ half8 open(u32x4 w) const { return __builtin_bit_cast(half8, w); }
   __device__ __forceinline__ void clear_v(uint32_t there) {
 #pragma unroll
     for (int t = 0; t < 2 * Z; t++)
@@ -134,30 +143,39 @@ struct Tile<Z, false> {
 // f32 outputs: two products each, with an error of 2^-22.  Weights are exp2(s - max + 10 - E): the second part is no
 // subnormal, and E, zero until a factor of V reaches 2, keeps p * d within f16.  P16 (f16 outputs): p and p * d are rounded to
 // f16, off by 2^-11 of themselves each, beside the output's own rounding; the weights' sum stays f32.
+//
+// OPEN (4 bits and P16): K and V are multiplied by their factors as they are opened, once for all rows, and rounded to f16 (2^-11 of
+// themselves, as an f16 cache would hold them), so that weights are operands as they stand.
 template <int Z, int QT, int QP, bool P16, bool Q4>
-__global__ __launch_bounds__(64 * WAVES) void page_attend_kernel(PageAttendArgs a) {
+__global__ __launch_bounds__(64 * WAVES, QT == 1 && (QP == 1 || Z < 4) ? 4 : 2) void page_attend_kernel(PageAttendArgs a) {
   typedef typename std::conditional<QP == 2, float, _Float16>::type T;
   constexpr int hd = 32 * Z;
+  constexpr bool SHARED = QT > 1, OPEN = Q4 && P16;  // SHARED: queries in LDS
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int lane = threadIdx.x & 63, ki = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, m = lane & 15;
   const int split = blockIdx.z, kh = blockIdx.x, b = a.row_blocks == 1 ? blockIdx.y : blockIdx.y / a.row_blocks;
   const int group = a.heads / a.pages.kv_heads, r0 = 16 * QT * (blockIdx.y - b * a.row_blocks);
   const size_t row0 = (size_t)b * a.rows;
-  float f[QT][Z][8];
-  int node[QT];
-#pragma unroll
-  for (int t = 0; t < QT; t++) {  // (of rows that are not there, too: nothing is known of the lengths yet)
-    const int row = min(r0 + 16 * t + m, a.rows * group - 1);
-    node[t] = node_of(row, group);
-    load_query<T, Z>((const T *)a.q + (row0 + node[t]) * a.stride + (size_t)(kh * group + head_of(row, group)) * hd, g, hd, f[t]);
-  }
+  auto query = [&](int row, float (&f)[Z][8]) {  // (of rows that are not there, too: nothing is known of the lengths yet)
+    const int r = min(row, a.rows * group - 1);
+    load_query<T, Z>((const T *)a.q + (row0 + node_of(r, group)) * a.stride + (size_t)(kh * group + head_of(r, group)) * hd, g, hd, f);
+  };
+  float f[Z][8];
+  if constexpr (!SHARED) query(r0 + m, f);
   const Share s = share_of(a, b);
   const int total = s.count * group;
+  if constexpr (!SHARED)  // (asked for above, with the lengths, and not where they are first used)
+#pragma unroll
+    for (int c = 0; c < Z; c++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) asm volatile("" : "+v"(f[c][e]));
   if (split >= s.used || r0 >= total) return;
-  const int end = min((split + 1) * s.per, s.tiles), cached = min(end, s.cached);
+  const int end = a.splits > 1 ? min((split + 1) * a.per, s.tiles) : s.tiles, start = split * a.per, cached = min(end, s.cached);
   const int slot = a.pages.shift - 5;
-  const int32_t *table = a.pages.table + (size_t)b * a.pages.table_stride;
+  // (nothing writes the table meanwhile: its numbers by scalar loads)
+  typedef const __attribute__((address_space(4))) int32_t *Table;
+  const Table table = (Table)(uintptr_t)(a.pages.table + (size_t)b * a.pages.table_stride);
 
   // The tiles that are there, in turn: `blk` is worked on, `next` is asked for, and the page of `after` is.
   auto id_of = [&](int tile) { return table[min(tile, cached - 1) >> slot]; };
@@ -167,68 +185,107 @@ __global__ __launch_bounds__(64 * WAVES) void page_attend_kernel(PageAttendArgs 
   auto at = [&](int tile, int id) {
     return (const uint32_t *)a.pages.pool + (size_t)id * a.pages.page_words + (size_t)((kh << slot) + (tile & ((1 << slot) - 1))) * tile_words(Q4, hd);
   };
-  Tile<Z, Q4> w;
-  int blk = split * s.per + ki, next = cached, next_id = -1;
+  Tile<Z, Q4, OPEN> w;
+  int blk = start + ki, next = cached, next_id = -1;
   if (blk < cached) {
     int id = id_of(blk);
     skip(blk, id);
     if (blk < cached) {
       const uint32_t *p = at(blk, id);
-      w.load_k(p, lane, g), w.load_v(p, lane, g);
+      w.load_k(p, lane, g);
+      __builtin_amdgcn_sched_barrier(0);  // (K first, as in the loop: waits count the loads in between)
+      w.load_v(p, lane, g);
+      __builtin_amdgcn_sched_barrier(0);
       next = blk + a.kw, next_id = id_of(next);
     }
   }
 
-  half8 q[QT][Z][QP];
+  half8 q[SHARED ? 1 : Z][QP];
+  half8 *const qs = (half8 *)smem;                    // [t][c][part][lane]
+  float *const cfs = (float *)(qs + QT * Z * QP * 64);  // [t][row]
   floatx4 acc[QT][2 * Z];
-  float mx[QT], sum[QT], cf[QT], slack[QT], digits = 10.0f;
+  float mx[QT], sum[QT], cf[QP == 2 ? QT : 1], digits = 10.0f;
+  auto factor = [&](int t) { return cf[QP == 2 ? t : 0]; };
+  bool far = false;  // whether a maximum is past FAR
+  // (rows that are not there: zeros, whose scores disturb nobody)
+  auto taken = [&](int row, half8 (&x)[Z][QP]) {
+#pragma unroll
+    for (int c = 0; c < Z; c++)
+#pragma unroll
+      for (int e = 0; e < 8; e++) f[c][e] = row < total ? f[c][e] : 0.0f;
+    return split_query(f, a.scale, x);
+  };
+  if constexpr (SHARED) {
+    for (int t = ki; t < QT; t += a.kw) {
+      half8 x[Z][QP];
+      query(r0 + 16 * t + m, f);
+      const float y = taken(r0 + 16 * t + m, x);
+      if (g == 0) cfs[16 * t + m] = y;
+#pragma unroll
+      for (int c = 0; c < Z; c++)
+#pragma unroll
+        for (int part = 0; part < QP; part++) qs[((t * Z + c) * QP + part) * 64 + lane] = x[c][part];
+    }
+    __syncthreads();
+    if constexpr (QP == 2)
+#pragma unroll
+      for (int t = 0; t < QT; t++) cf[t] = cfs[16 * t + m];
+  } else {
+    cf[0] = taken(r0 + m, q);
+  }
+  if constexpr (QP == 1) cf[0] = a.scale * 1.44269504088896341f;
 #pragma unroll
   for (int t = 0; t < QT; t++) {
-    cf[t] = split_query(f[t], a.scale, q[t]);
-    if (r0 + 16 * t + m >= total) cf[t] = 0.0f;  // (whatever stands in a row past the last: no maximum, no far score)
-    slack[t] = SLACK / cf[t];
-    mx[t] = -INFINITY, sum[t] = 0.0f;
+    mx[t] = LOWEST, sum[t] = 0.0f;
 #pragma unroll
     for (int x = 0; x < 2 * Z; x++) acc[t][x] = floatx4{};
   }
+  int mine = lane;
+  asm volatile("" : "+v"(mine));  // (one address and its offsets: not others made of it that take registers)
+  auto query_of = [&](int t, int c, int part) {
+    if constexpr (SHARED) return qs[mine + ((t * Z + c) * QP + part) * 64];
+    else return q[c][part];
+  };
 
+  typedef float floatx8 __attribute__((ext_vector_type(8)));
+  typedef typename std::conditional<P16, half8, floatx8>::type P;
   // Scores st of a tile into weights p: exp2 against the running maximum, and their sum.  seen: the lane's positions.
-  auto weights = [&](floatx4 (&st)[2], int t, uint32_t seen, float (&p)[8]) {
-    if (seen != 0xff)
+  auto weights = [&](floatx4 (&st)[2], int t, bool masked, uint32_t seen, P &p) {
+    if (masked)
 #pragma unroll
       for (int e = 0; e < 8; e++)
         if (!(seen >> e & 1)) st[e >> 2][e & 3] = -INFINITY;
     float top = st[0][0];
 #pragma unroll
     for (int e = 1; e < 8; e++) top = fmaxf(top, st[e >> 2][e & 3]);
-    top = xlane::bit4(top, xlane::Max{});
-    top = xlane::bit5(top, xlane::Max{});
-    if (__any(top > mx[t] + slack[t])) {
-      top = fmaxf(top, mx[t]);
-      const float old = mx[t] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((mx[t] - top) * cf[t]);
+    // The maximum is moved, for all of a row's lanes, where one of them has a score well past it: otherwise they need not meet.
+    const float c = factor(t);
+    float by = fminf(fmaf(-mx[t], c, digits), -LOWEST);
+    if (__any((far ? fmaf(top - mx[t], c, digits) : fmaf(top, c, by)) > digits + SLACK)) {
+      top = xlane::bit4(top, xlane::Max{});
+      top = fmaxf(xlane::bit5(top, xlane::Max{}), mx[t]);
+      const float old = __builtin_amdgcn_exp2f((mx[t] - top) * c);
       sum[t] *= old;
 #pragma unroll
       for (int x = 0; x < 2 * Z; x++) acc[t][x] *= old;
       mx[t] = top;
+      by = fminf(fmaf(-top, c, digits), -LOWEST);
+      far = far || __any(top != LOWEST && fabsf(by) > FAR);
     }
-    const float base = mx[t] == -INFINITY ? 0.0f : mx[t];
-    float shift = fmaf(-base, cf[t], digits);
-    if (__any(fabsf(shift) > FAR)) {
-      shift = digits;
-      st[0] -= base, st[1] -= base;
-    }
+    if (far) st[0] -= mx[t], st[1] -= mx[t], by = digits;
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      p[e] = __builtin_amdgcn_exp2f(fmaf(st[e >> 2][e & 3], cf[t], shift));
-      sum[t] += p[e];
+    for (int e = 0; e < 8; e += 2) {
+      const float p0 = __builtin_amdgcn_exp2f(fmaf(st[e >> 2][e & 3], c, by));
+      const float p1 = __builtin_amdgcn_exp2f(fmaf(st[e >> 2][e + 1 & 3], c, by));
+      sum[t] += p0, sum[t] += p1;
+      if constexpr (P16) weights2<true>(p0, p1, p, p, e);
+      else p[e] = p0, p[e + 1] = p1;
     }
   };
   // p times a chunk's factors as an operand, and (unless P16) what that leaves of them.
-  auto operand = [&](const float (&p)[8], const half8 *d, half8 &h, half8 &l) {
+  auto operand = [&](const P &p, const half8 *d, half8 &h, half8 &l) {
     if constexpr (P16) {
-#pragma unroll
-      for (int e = 0; e < 8; e += 2) weights2<true>(p[e], p[e + 1], h, l, e);
-      if (d) h *= *d;
+      h = d ? p * *d : p;
     } else {
 #pragma unroll
       for (int e = 0; e < 8; e += 2)
@@ -237,7 +294,7 @@ __global__ __launch_bounds__(64 * WAVES) void page_attend_kernel(PageAttendArgs 
   };
   // Factors of V of 2 and more: the weights that follow are smaller by their largest's power of two.
   auto room = [&] {
-    if constexpr (Q4) {
+    if constexpr (Q4 && !OPEN) {
       uint32_t any = 0;
 #pragma unroll
       for (int c = 0; c < Z; c++) {
@@ -273,24 +330,53 @@ __global__ __launch_bounds__(64 * WAVES) void page_attend_kernel(PageAttendArgs 
     floatx4 st[QT][2];
 #pragma unroll
     for (int t = 0; t < QT; t++) st[t][0] = st[t][1] = floatx4{};
+    // (matrix instructions of a word among the vector ones that open the next)
+    auto open_k = [&](int i) {
+      half8 k = w.open(w.k[i]);
+      if constexpr (OPEN) k *= (half8)w.kd[i / 2][i % 2];
+      return k;
+    };
+    // (and queries asked for when the chunk before them is done)
+    half8 k = open_k(0), x[QT][QP];
 #pragma unroll
-    for (int c = 0; c < Z; c++)
+    for (int t = 0; t < QT; t++)
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
-        const half8 k = w.open(w.k[2 * c + u]);
+      for (int part = 0; part < QP; part++) x[t][part] = query_of(t, 0, part);
+    if constexpr (QT > 1) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int i = 0; i < 2 * Z; i++) {
+      const int c = i / 2, u = i % 2;
+      half8 after = k;
+      if (i + 1 < 2 * Z) after = open_k(i + 1);
+#pragma unroll
+      for (int t = 0; t < QT; t++) {
+        if constexpr (Q4 && !OPEN) {
+          floatx4 y = mfma(k, x[t][0], floatx4{});
+          if constexpr (QP == 2) y = mfma(k, x[t][QP - 1], y);
+#pragma unroll
+          for (int r = 0; r < 4; r++) st[t][u][r] = fmaf(y[r], (float)w.kd[c][4 * u + r], st[t][u][r]);
+        } else {
+#pragma unroll
+          for (int part = 0; part < QP; part++) st[t][u] = mfma(k, x[t][part], st[t][u]);
+        }
+        if (u == 1 && c + 1 < Z)
+#pragma unroll
+          for (int part = 0; part < QP; part++) x[t][part] = query_of(t, c + 1, part);
+      }
+      k = after;
+      if constexpr (QT > 1 && OPEN) {
 #pragma unroll
         for (int t = 0; t < QT; t++) {
-          if constexpr (Q4) {
-            floatx4 x = mfma(k, q[t][c][0], floatx4{});
-            if constexpr (QP == 2) x = mfma(k, q[t][c][QP - 1], x);
-#pragma unroll
-            for (int r = 0; r < 4; r++) st[t][u][r] = fmaf(x[r], (float)w.kd[c][4 * u + r], st[t][u][r]);
-          } else {
-#pragma unroll
-            for (int part = 0; part < QP; part++) st[t][u] = mfma(k, q[t][c][part], st[t][u]);
-          }
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          if (u == 1 && c + 1 < Z) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, (13 + QT - 1) / QT, 0);
         }
+        __builtin_amdgcn_sched_barrier(0);
       }
+    }
+    // (the scores are done before K's registers take the next tile: it would be waited for at the end of this one otherwise)
+#pragma unroll
+    for (int t = 0; t < QT; t++) asm volatile("" : "+v"(st[t][0]), "+v"(st[t][1]));
     if constexpr (more) w.load_k(np, lane, g);
     const int left = s.n - TILE * blk;
     uint32_t seen = 0xff;
@@ -300,19 +386,41 @@ __global__ __launch_bounds__(64 * WAVES) void page_attend_kernel(PageAttendArgs 
       w.clear_v(seen);
     }
     room();
-    float p[QT][8];
+    P p[QT];
 #pragma unroll
-    for (int t = 0; t < QT; t++) weights(st[t], t, seen, p[t]);
+    for (int t = 0; t < QT; t++) {
+      if constexpr (QT > 1) __builtin_amdgcn_sched_barrier(0);
+      weights(st[t], t, left < TILE, seen, p[t]);
+    }
+    auto open_v = [&](int i) {
+      half8 v = w.open(w.v[i]);
+      if constexpr (OPEN) v *= w.vd[i / 2];
+      return v;
+    };
+    half8 v = open_v(0);
+    if constexpr (QT > 1) __builtin_amdgcn_sched_barrier(0);
+    half8 h[QT], l[QT];
 #pragma unroll
-    for (int c = 0; c < Z; c++) {
-      const half8 v0 = w.open(w.v[2 * c]), v1 = w.open(w.v[2 * c + 1]);
+    for (int i = 0; i < 2 * Z; i++) {
+      half8 after = v;
+      if (i + 1 < 2 * Z) after = open_v(i + 1);
 #pragma unroll
       for (int t = 0; t < QT; t++) {
-        half8 h, l;
-        if constexpr (Q4) operand(p[t], &w.vd[c], h, l);
-        else operand(p[t], nullptr, h, l);
-        acc[t][2 * c] = mfma(v0, h, acc[t][2 * c]), acc[t][2 * c + 1] = mfma(v1, h, acc[t][2 * c + 1]);
-        if constexpr (!P16) acc[t][2 * c] = mfma(v0, l, acc[t][2 * c]), acc[t][2 * c + 1] = mfma(v1, l, acc[t][2 * c + 1]);
+        if (i % 2 == 0) {
+          if constexpr (Q4 && !OPEN) operand(p[t], &w.vd[i / 2], h[t], l[t]);
+          else operand(p[t], nullptr, h[t], l[t]);
+        }
+        acc[t][i] = mfma(v, h[t], acc[t][i]);
+        if constexpr (!P16) acc[t][i] = mfma(v, l[t], acc[t][i]);
+      }
+      v = after;
+      if constexpr (QT > 1 && OPEN) {
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+          __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, (13 + QT - 1) / QT, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
     }
     if constexpr (more) {
@@ -326,8 +434,10 @@ __global__ __launch_bounds__(64 * WAVES) void page_attend_kernel(PageAttendArgs 
   }
 
   // The nodes, 32 at a time: K and V as f16.
-  const int first = max(split * s.per, s.cached);
-  for (int tile = first + ((ki - (first - split * s.per)) % a.kw + a.kw) % a.kw; tile < end; tile += a.kw) {
+  const int first = max(start, s.cached);
+  const uint32_t *masks = a.mask ? a.mask + (size_t)b * a.mask_stride : nullptr;
+  auto mask_of = [&](int t, int word) { return masks[(size_t)node_of(min(r0 + 16 * t + m, a.rows * group - 1), group) * a.words + word]; };
+  for (int tile = first + ((ki - (first - start)) % a.kw + a.kw) % a.kw; tile < end; tile += a.kw) {
     const int j0 = TILE * (tile - s.cached), last = s.count - 1 - j0;
     const T *k = (const T *)a.k + (row0 + j0) * a.stride + (size_t)kh * hd, *v = (const T *)a.v + (row0 + j0) * a.stride + (size_t)kh * hd;
     const uint32_t there = last >= TILE - 1 ? 0xffffffffu : (2u << last) - 1u;
@@ -347,14 +457,14 @@ __global__ __launch_bounds__(64 * WAVES) void page_attend_kernel(PageAttendArgs 
 #pragma unroll
         for (int t = 0; t < QT; t++)
 #pragma unroll
-          for (int part = 0; part < QP; part++) st[t][u] = mfma(kf, q[t][c][part], st[t][u]);
+          for (int part = 0; part < QP; part++) st[t][u] = mfma(kf, query_of(t, c, part), st[t][u]);
       }
     }
-    float p[QT][8];
+    P p[QT];
 #pragma unroll
     for (int t = 0; t < QT; t++) {
-      const uint32_t sees = there & a.mask[(size_t)b * a.mask_stride + (size_t)node[t] * a.words + j0 / 32];
-      weights(st[t], t, (sees >> 4 * g & 15) | (sees >> (16 + 4 * g) & 15) << 4, p[t]);
+      const uint32_t sees = there & mask_of(t, j0 / 32);
+      weights(st[t], t, true, (sees >> 4 * g & 15) | (sees >> (16 + 4 * g) & 15) << 4, p[t]);
     }
 #pragma unroll
     for (int c = 0; c < Z; c++) {
@@ -386,7 +496,7 @@ __global__ __launch_bounds__(64 * WAVES) void page_attend_kernel(PageAttendArgs 
           const T *y = v + (size_t)j * a.stride;
 #pragma unroll
           for (int t = 0; t < QT; t++) {
-            if (!(a.mask[(size_t)b * a.mask_stride + (size_t)node[t] * a.words + j0 / 32] >> j & 1)) continue;
+            if (!(mask_of(t, j0 / 32) >> j & 1)) continue;
 #pragma unroll
             for (int i = 0; i < 2; i++)
 #pragma unroll
@@ -411,41 +521,79 @@ __global__ __launch_bounds__(64 * WAVES) void page_attend_kernel(PageAttendArgs 
     }
   }
 
-  // The wavefronts' results joined through LDS: each writes its own, then every lane adds up four values of a row.  Lane
-  // 16g + i holds row i's values 32c + 8g + 2r + x.
-  floatx4 *merge = (floatx4 *)smem;                    // [ki][t][c][half][lane]
-  float *ml = (float *)(merge + a.kw * QT * Z * 128);  // [ki][t][maxima, sums][row]
+  // The wavefronts' results joined through LDS, where the queries were: half of them added to the other half until the rest fit,
+  // which write their own, and every lane adds up four values of a row.  Lane 16g + i holds row i's values 32c + 8g + 2r + x.
+  constexpr int SLOT = QT * Z * 128, FIT = JOIN_LDS / (16 * SLOT);
   const float more = __builtin_amdgcn_exp2f(10.0f - digits);
 #pragma unroll
   for (int t = 0; t < QT; t++) {
     sum[t] = xlane::bit4(sum[t], xlane::Add{});
-    sum[t] = xlane::bit5(sum[t], xlane::Add{});
-    if (g == 0) ml[32 * (ki * QT + t) + m] = mx[t], ml[32 * (ki * QT + t) + 16 + m] = sum[t] * more;
+    sum[t] = xlane::bit5(sum[t], xlane::Add{}) * more;
+    if constexpr (Q4 && !OPEN)
 #pragma unroll
-    for (int c = 0; c < Z; c++)
+      for (int x = 0; x < 2 * Z; x++) acc[t][x] *= more;
+  }
+  int waves = a.kw;
+  floatx4 *merge = (floatx4 *)smem;                             // [wave][...][lane]
+  float *ml = (float *)(merge + min(waves, FIT) * SLOT);  // [wave][t][maxima, sums][row]
+  if constexpr (SHARED) __syncthreads();
+  if constexpr (FIT < WAVES)
+    for (; waves > FIT; waves /= 2) {
+      const int half = waves / 2;
+      if (ki >= half && ki < waves) {
 #pragma unroll
-      for (int h = 0; h < 2; h++)
-        merge[(((ki * QT + t) * Z + c) * 2 + h) * 64 + lane] =
-            floatx4{acc[t][2 * c][2 * h], acc[t][2 * c + 1][2 * h], acc[t][2 * c][2 * h + 1], acc[t][2 * c + 1][2 * h + 1]} * more;
+        for (int t = 0; t < QT; t++) {
+          if (g == 0) ml[32 * ((ki - half) * QT + t) + m] = mx[t], ml[32 * ((ki - half) * QT + t) + 16 + m] = sum[t];
+#pragma unroll
+          for (int x = 0; x < 2 * Z; x++) merge[(ki - half) * SLOT + (t * 2 * Z + x) * 64 + lane] = acc[t][x];
+        }
+      }
+      __syncthreads();
+      if (ki < half) {
+#pragma unroll
+        for (int t = 0; t < QT; t++) {
+          const float om = ml[32 * (ki * QT + t) + m], os = ml[32 * (ki * QT + t) + 16 + m], top = fmaxf(mx[t], om);
+          const float y = mx[t] == top ? 1.0f : __builtin_amdgcn_exp2f((mx[t] - top) * factor(t)), z = om == top ? 1.0f : __builtin_amdgcn_exp2f((om - top) * factor(t));
+          mx[t] = top, sum[t] = sum[t] * y + os * z;
+#pragma unroll
+          for (int x = 0; x < 2 * Z; x++) acc[t][x] = acc[t][x] * y + merge[ki * SLOT + (t * 2 * Z + x) * 64 + lane] * z;
+        }
+      }
+      __syncthreads();
+    }
+  if (ki < waves) {
+#pragma unroll
+    for (int t = 0; t < QT; t++) {
+      if (g == 0) ml[32 * (ki * QT + t) + m] = mx[t], ml[32 * (ki * QT + t) + 16 + m] = sum[t];
+#pragma unroll
+      for (int c = 0; c < Z; c++)
+#pragma unroll
+        for (int h = 0; h < 2; h++)
+          merge[ki * SLOT + ((t * Z + c) * 2 + h) * 64 + lane] =
+              floatx4{acc[t][2 * c][2 * h], acc[t][2 * c + 1][2 * h], acc[t][2 * c][2 * h + 1], acc[t][2 * c + 1][2 * h + 1]};
+    }
   }
   __syncthreads();
   for (int x = ki; x < QT * Z * 2; x += a.kw) {
     const int t = x / (2 * Z), c = x / 2 % Z, d = 32 * c + 8 * g + 4 * (x % 2), r = r0 + 16 * t + m;
     if (r >= total) continue;
-    float km[WAVES], kl[WAVES], top = -INFINITY, l = 0.0f, scale = cf[0];
-    if (QT == 2 && t) scale = cf[QT - 1];
-    floatx4 kf[WAVES], o{};
+    constexpr int MOST = std::min(WAVES, FIT);
+    float km[MOST], kl[MOST], top = -INFINITY, l = 0.0f, scale = cf[0];
+    if constexpr (QP == 2)
 #pragma unroll
-    for (int k = 0; k < WAVES; k++) {
-      const int y = min(k, a.kw - 1) * QT;
-      km[k] = ml[32 * (y + t) + m], kl[k] = ml[32 * (y + t) + 16 + m], kf[k] = merge[(y * Z * 2 + x) * 64 + lane];
-      if (k >= a.kw) km[k] = -INFINITY;
+      for (int y = 1; y < QT; y++) scale = t == y ? cf[y] : scale;
+    floatx4 kf[MOST], o{};
+#pragma unroll
+    for (int k = 0; k < MOST; k++) {
+      const int y = min(k, waves - 1);
+      km[k] = ml[32 * (y * QT + t) + m], kl[k] = ml[32 * (y * QT + t) + 16 + m], kf[k] = merge[y * SLOT + x * 64 + lane];
+      if (k >= waves) km[k] = -INFINITY;
     }
 #pragma unroll
-    for (int k = 0; k < WAVES; k++) top = fmaxf(top, km[k]);
+    for (int k = 0; k < MOST; k++) top = fmaxf(top, km[k]);
 #pragma unroll
-    for (int k = 0; k < WAVES; k++) {
-      if (k >= a.kw) break;
+    for (int k = 0; k < MOST; k++) {
+      if (k >= waves) break;
       const float y = km[k] == top ? 1.0f : __builtin_amdgcn_exp2f((km[k] - top) * scale);
       l += y * kl[k], o += y * kf[k];
     }
@@ -457,7 +605,7 @@ __global__ __launch_bounds__(64 * WAVES) void page_attend_kernel(PageAttendArgs 
       *(floatx4 *)(a.po + part * hd + out) = o;
       continue;
     }
-    o *= top == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
+    o *= l == 0.0f ? 0.0f : 1.0f / l;
     if (a.out16) *(u32x2_a4 *)((_Float16 *)a.o + out) = u32x2{pack2(o[0], o[1]), pack2(o[2], o[3])};
     else *(floatx4_a4 *)((float *)a.o + out) = o;
   }
@@ -480,7 +628,7 @@ __global__ __launch_bounds__(256) void page_join_kernel(PageAttendArgs a) {
     const float w = x[0] == top ? 1.0f : __builtin_amdgcn_exp2f((x[0] - top) * x[2]);
     l += w * x[1], o += w * *(const floatx4 *)(a.po + (k * heads + unit) * hd + d);
   }
-  o *= top == -INFINITY && l == 0.0f ? 0.0f : 1.0f / l;
+  o *= l == 0.0f ? 0.0f : 1.0f / l;
   if (a.out16) *(u32x2_a4 *)((_Float16 *)a.o + unit * hd + d) = u32x2{pack2(o[0], o[1]), pack2(o[2], o[3])};
   else *(floatx4_a4 *)((float *)a.o + unit * hd + d) = o;
 }
@@ -489,12 +637,17 @@ template <int Z, int QT, int QP, bool P16, bool Q4>
 int attend_launch(wh_ctx *ctx, const PageAttendArgs &a) {
   const double keys = (double)a.batch * a.pages.room;
   ProfScope prof(ctx, "page_attend", 4.0 * keys * a.rows * a.heads * a.pages.hd, keys * a.pages.kv_heads * a.pages.hd * (Q4 ? 1.125 : 4.0));
-  const size_t shm = (size_t)a.kw * QT * (Z * 2048 + 128);
+  const size_t join = (size_t)std::min(a.kw, JOIN_LDS / (QT * Z * 2048)) * QT * (Z * 2048 + 128), queries = QT > 1 ? QT * (Z * QP * 1024 + 64) : 0;
+  const size_t shm = std::max(join, queries);
   wh_launch(ctx, (page_attend_kernel<Z, QT, QP, P16, Q4>), dim3(a.pages.kv_heads, a.batch * a.row_blocks, a.splits), 64 * a.kw, shm, a);
   return wh_launched(ctx, "page attention");
 }
 template <int Z, int QP, bool P16, bool Q4>
 int attend_qt(wh_ctx *ctx, const PageAttendArgs &a, int qt) {
+  if constexpr (Q4) {
+    if (qt == 4) return attend_launch<Z, 4, QP, P16, Q4>(ctx, a);
+    if (qt == 3) return attend_launch<Z, 3, QP, P16, Q4>(ctx, a);
+  }
   return qt == 1 ? attend_launch<Z, 1, QP, P16, Q4>(ctx, a) : attend_launch<Z, 2, QP, P16, Q4>(ctx, a);
 }
 template <int QP, bool P16, bool Q4>
@@ -525,21 +678,25 @@ int launch_page_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o) % 4 || (in16 && stride % 2))
     return wh_fail(ctx, WH_EARG, "page attention: buffers and rows must be 4-byte aligned");
   PageAttendArgs a{q, k, v, stride, pages_of(p), o, out16 != 0, t->n, t->count, t->mask, t->mask_stride, t->batch, t->rows, (t->rows + 31) / 32,
-                   heads, 1.0f / sqrtf((float)p->hd), 1, 1, 1, nullptr, nullptr};
-  const int z = p->hd / 32, rows = t->rows * (heads / p->kv_heads), qt = rows > 16 ? 2 : 1;
+                   heads, 1.0f / sqrtf((float)p->hd), 1, 1, 1, 1, nullptr, nullptr};
+  const int rows = (t->rows * (heads / p->kv_heads) + 15) / 16, most = p->type == WH_Q4_0 ? 4 : 2;  // tiles of 16
+  a.row_blocks = (rows + most - 1) / most;
+  const int qt = (rows + a.row_blocks - 1) / a.row_blocks;
+  a.row_blocks = (rows + qt - 1) / qt;
   const int tiles = a.pages.room / TILE + (t->mask && k ? (t->rows + TILE - 1) / TILE : 0);
-  a.row_blocks = (rows + 16 * qt - 1) / (16 * qt);
-  a.kw = std::min({WAVES, 32 / (z * qt), tiles});  // (64 KiB of LDS for their join)
+  while (2 * a.kw <= std::min(WAVES, tiles)) a.kw *= 2;
   const size_t units = (size_t)t->batch * p->kv_heads * a.row_blocks;
   const size_t cus = ctx->cus > 0 ? ctx->cus : 256;
-  const int least = 2 * a.kw;
+  const int least = 4 * a.kw;
   if (tiles > 2 * least) {
+    const size_t slots = cus * (qt == 1 ? 2 : 1);
     size_t best = SIZE_MAX;
     for (int x = 1; x <= std::min(SPLITS, (tiles + least - 1) / least); x++) {
-      const size_t cost = (units * x + cus - 1) / cus * ((tiles + x - 1) / x + least);
+      const size_t cost = (units * x + slots - 1) / slots * ((tiles + x - 1) / x + least);
       if (cost < best) best = cost, a.splits = x;
     }
   }
+  a.per = (tiles + a.splits - 1) / a.splits;
   const size_t nodes = (size_t)t->batch * t->rows;
   if ((size_t)t->batch * a.row_blocks > 65535 || units * a.splits >= (size_t)1 << 22 || nodes * heads >= (size_t)1 << 25)  // (a launch's limits)
     return wh_fail(ctx, WH_EARG, "page attention: %d heads of %zu nodes in one call", heads, nodes);
