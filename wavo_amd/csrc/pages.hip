@@ -189,123 +189,162 @@ __device__ __forceinline__ float single(double x) {
   return f;
 }
 
-// New keys and values of one tile of a key head, by one wavefront, whose lanes hold K and V as the tile's words do
-// (pages.h): a position's K in the four lanes of its row, its V in a group's 16 lanes.  K is normed and rotated in
-// 64 bits: the last bits of f32 would cross a border of f16 for one of 1e3 values and of 4 bits for one of 1e5; as it is, a row
-// leaves the words of its exact values.
-template <typename T, int Z, bool Q4, bool TURN>
-__device__ __forceinline__ void append_tile(const AppendArgs &a, int b, int tile, int kh, int n, int end) {
-  typedef double F;
-  const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15, hd = 32 * Z;
-  uint32_t *out = tile_at(a.pages, Q4, b, tile, kh);
-  if (!out) return;
-  const int j0 = TILE * tile;
-  // The source row of a position, or -1.
-  auto row_of = [&](int j) {
-    const int r = j0 + j - n;
-    if (r < 0 || j0 + j >= end) return -1;
-    if (!a.path) return r;
-    const int p = a.path[(size_t)b * a.rows + r];
-    return (uint32_t)p < (uint32_t)a.rows ? p : -1;
-  };
-  int kr[2], vr[8];
-#pragma unroll
-  for (int u = 0; u < 2; u++) kr[u] = row_of(16 * u + m);
-#pragma unroll
-  for (int e = 0; e < 8; e++) vr[e] = row_of(position_of(g, e));
-  const T *k0 = (const T *)a.k + (size_t)b * a.rows * a.stride + (size_t)kh * hd;
-  const T *v0 = (const T *)a.v + (size_t)b * a.rows * a.stride + (size_t)kh * hd;
+// Where the rows of a tile's new positions are: of position j of the tile, in the sequence's rows, or -1.
+struct Rows {
+  const int32_t *path;
+  int first, end, rows;  // of the tile's first position, in the sequence; one past the last that is stored, from the tile's first
+  __device__ __forceinline__ int operator()(int j) const {
+    const int r = first + j;
+    if (r < 0 || j >= end) return -1;
+    if (!path) return r;
+    const int p = path[r];
+    return (uint32_t)p < (uint32_t)rows ? p : -1;
+  }
+};
 
-  // V: pairs of neighbouring values of a position.
-  uint32_t v[8][Z];
-#pragma unroll
-  for (int e = 0; e < 8; e++)
-#pragma unroll
-    for (int c = 0; c < Z; c++) v[e][c] = pair_at(v0 + (size_t)max(vr[e], 0) * a.stride + 32 * c + 2 * m);
+// How a key is turned: not at all, by values of any lane (read again) or by values of the same one (the head's halves, of 64
+// and 128 values).
+enum { PLAIN, ANY, HALVES };
 
-  // K, row by row.
-  uint32_t kw[2][Z][4];  // pairs of halfs
+// New keys of 16 positions of a tile, by one wavefront, whose lanes hold them as the tile's words do (pages.h): a position's in
+// the four lanes of its row.  They are normed and rotated in 64 bits: the last bits of f32 would cross a border of f16 for
+// one of 1e3 values and of 4 bits for one of 1e5; as it is, a row leaves the words of its exact values.
+template <typename T, int Z, bool Q4, int TURN>
+__device__ __forceinline__ void append_k(const AppendArgs &a, const Rows &rows, const T *k0, uint32_t *out, int j0, int u) {
+  constexpr int hd = 32 * Z;
+  const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15, row = rows(16 * u + m);
+  const T *k = k0 + (size_t)max(row, 0) * a.stride;
+  const float *table = a.turn.table ? a.turn.table + (size_t)min(max(j0 + 16 * u + m, 0), a.turn.positions - 1) * a.turn.rot : nullptr;
+  Eight<T> raw[Z];
 #pragma unroll
-  for (int u = 0; u < 2; u++) {
-    const T *k = k0 + (size_t)max(kr[u], 0) * a.stride;
-    Eight<T> raw[Z];
+  for (int c = 0; c < Z; c++) raw[c] = raw8(k + 32 * c + 8 * g);
+  uint32_t w[Z][4];  // pairs of halfs
+  if constexpr (TURN == PLAIN) {
 #pragma unroll
-    for (int c = 0; c < Z; c++) raw[c] = raw8(k + 32 * c + 8 * g);
-    if constexpr (TURN) {
-      F r = 1, x[Z][8];
-      if (a.turn.k_gain) {
-        F sum = 0;
-#pragma unroll
-        for (int c = 0; c < Z; c++)
-#pragma unroll
-          for (int e = 0; e < 8; e++) sum += (F)at8(raw[c], e) * (F)at8(raw[c], e);
-        sum = xlane::bit4(sum, xlane::Add{});
-        sum = xlane::bit5(sum, xlane::Add{});
-        r = (F)1 / sqrt(sum / (F)hd + (F)a.turn.eps);
-      }
-      auto normed = [&](float y, int d) { return a.turn.k_gain ? (F)y * r * (F)a.turn.k_gain[d] : (F)y; };
+    for (int c = 0; c < Z; c++) {
+      const u32x2 p = pairs4(raw[c].a), q = pairs4(raw[c].b);
+      w[c][0] = p[0], w[c][1] = p[1], w[c][2] = q[0], w[c][3] = q[1];
+    }
+  } else {
+    double r = 1.0;
+    if (a.turn.k_gain) {
+      double sum = 0.0, more = 0.0;
 #pragma unroll
       for (int c = 0; c < Z; c++)
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[c][e] = normed(at8(raw[c], e), 32 * c + 8 * g + e);
-      if (a.turn.table) {
-        const int half = a.turn.rot / 2, position = min(max(j0 + 16 * u + m, 0), a.turn.positions - 1);
-        const float *t = a.turn.table + (size_t)position * a.turn.rot;
+        for (int e = 0; e < 8; e += 2) {
+          const double x = at8(raw[c], e), y = at8(raw[c], e + 1);
+          sum = fma(x, x, sum), more = fma(y, y, more);
+        }
+      sum = xlane::bit4(sum + more, xlane::Add{});
+      sum = xlane::bit5(sum, xlane::Add{});
+      r = 1.0 / sqrt(sum / hd + (double)a.turn.eps);
+    }
+    auto normed = [&](float y, float gain) { return a.turn.k_gain ? (double)y * r * (double)gain : (double)y; };
+    auto gain4 = [&](int d) { return a.turn.k_gain ? raw4(a.turn.k_gain + d) : floatx4{}; };
+    if constexpr (TURN == HALVES) {
 #pragma unroll
-        for (int c = 0; c < Z; c++)
+      for (int c = 0; c < Z / 2; c++)
 #pragma unroll
-          for (int y = 0; y < 2; y++) {
-            const int d = 32 * c + 8 * g + 4 * y;
-            if (d >= a.turn.rot) continue;
+        for (int y = 0; y < 2; y++) {
+          const int d = 32 * c + 8 * g + 4 * y;
+          const floatx4 cs = raw4(table + d), sn = raw4(table + hd / 2 + d), ga = gain4(d), gb = gain4(hd / 2 + d);
+          float p[4], q[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const double x = normed(at8(raw[c], 4 * y + e), ga[e]), z = normed(at8(raw[c + Z / 2], 4 * y + e), gb[e]);
+            p[e] = single(x * cs[e] - z * sn[e]), q[e] = single(z * cs[e] + x * sn[e]);
+          }
+          w[c][2 * y] = pack2(p[0], p[1]), w[c][2 * y + 1] = pack2(p[2], p[3]);
+          w[c + Z / 2][2 * y] = pack2(q[0], q[1]), w[c + Z / 2][2 * y + 1] = pack2(q[2], q[3]);
+        }
+    } else {
+      const int half = a.turn.rot / 2;
+#pragma unroll
+      for (int c = 0; c < Z; c++)
+#pragma unroll
+        for (int y = 0; y < 2; y++) {
+          const int d = 32 * c + 8 * g + 4 * y;
+          const floatx4 gain = gain4(d);
+          double x[4];
+#pragma unroll
+          for (int e = 0; e < 4; e++) x[e] = normed(at8(raw[c], 4 * y + e), gain[e]);
+          if (d < a.turn.rot) {
             if (a.turn.pairs) {
 #pragma unroll
-              for (int e = 4 * y; e < 4 * y + 4; e += 2) {
-                const F cs = t[(32 * c + 8 * g + e) / 2], sn = t[half + (32 * c + 8 * g + e) / 2], p = x[c][e], q = x[c][e + 1];
-                x[c][e] = p * cs - q * sn, x[c][e + 1] = q * cs + p * sn;
+              for (int e = 0; e < 4; e += 2) {
+                const double cs = table[(d + e) / 2], sn = table[half + (d + e) / 2], p = x[e], q = x[e + 1];
+                x[e] = p * cs - q * sn, x[e + 1] = q * cs + p * sn;
               }
             } else {
-              // (the other half's values are another lane's, for most sizes: read again)
               const bool low = d < half;
               const int other = low ? d + half : d - half, i = low ? d : d - half;
-              const floatx4 f = load4(k, other, sizeof(T) == 2);
+              const floatx4 f = load4(k, other, sizeof(T) == 2), cs = raw4(table + i), sn = raw4(table + half + i), go = gain4(other);
 #pragma unroll
               for (int e = 0; e < 4; e++) {
-                const F cs = t[i + e], sn = t[half + i + e], p = x[c][4 * y + e], q = normed(f[e], other + e);
-                x[c][4 * y + e] = low ? p * cs - q * sn : p * cs + q * sn;
+                const double q = normed(f[e], go[e]);
+                x[e] = low ? x[e] * cs[e] - q * sn[e] : x[e] * cs[e] + q * sn[e];
               }
             }
           }
-      }
-#pragma unroll
-      for (int c = 0; c < Z; c++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) kw[u][c][e] = pack2(single(x[c][2 * e]), single(x[c][2 * e + 1]));
-    } else {
-#pragma unroll
-      for (int c = 0; c < Z; c++) {
-        const u32x2 p = pairs4(raw[c].a), q = pairs4(raw[c].b);
-        kw[u][c][0] = p[0], kw[u][c][1] = p[1], kw[u][c][2] = q[0], kw[u][c][3] = q[1];
-      }
+          w[c][2 * y] = pack2(single(x[0]), single(x[1])), w[c][2 * y + 1] = pack2(single(x[2]), single(x[3]));
+        }
     }
   }
 
-  uint32_t vnew = 0;  // of this lane's positions, those that are stored
-#pragma unroll
-  for (int e = 0; e < 8; e++) vnew |= vr[e] >= 0 ? 1u << e : 0u;
   if constexpr (!Q4) {
-    // (e's two values of V to the two words that they belong to)
-    _Float16 *const kh16 = (_Float16 *)out, *const vh16 = kh16 + 32 * hd;
+    if (row >= 0)
 #pragma unroll
-    for (int u = 0; u < 2; u++)
-      if (kr[u] >= 0)
+      for (int c = 0; c < Z; c++)
+        *(u32x4 *)((_Float16 *)out + ((2 * c + u) * 64 + lane) * 8) = u32x4{w[c][0], w[c][1], w[c][2], w[c][3]};
+  } else {
+    uint16_t *const kd = (uint16_t *)(out + 4 * hd);
 #pragma unroll
-        for (int c = 0; c < Z; c++) *(u32x4 *)(kh16 + ((2 * c + u) * 64 + lane) * 8) = u32x4{kw[u][c][0], kw[u][c][1], kw[u][c][2], kw[u][c][3]};
+    for (int c = 0; c < Z; c++) {
+      u16x2 top = order2(w[c][0]);
+#pragma unroll
+      for (int e = 1; e < 4; e++) top = __builtin_elementwise_max(top, order2(w[c][e]));
+      uint32_t t = max((uint32_t)top[0], (uint32_t)top[1]);
+      t = xlane::bit4(t, [](uint32_t x, uint32_t y) { return max(x, y); });
+      t = xlane::bit5(t, [](uint32_t x, uint32_t y) { return max(x, y); });
+      const _Float16 d = factor_of(t);
+      const float inv = inverse_of(d);
+      uint32_t word = 0;
+#pragma unroll
+      for (int e = 0; e < 8; e++) word |= nibble((float)__builtin_bit_cast(half2, w[c][e / 2])[e & 1], inv) << nibble_of(e);
+      if (row >= 0) {
+        out[word_at(2 * c + u, lane, 2 * Z)] = word;
+        // (position 16u + m is element 4u + m % 4 of group m / 4)
+        if (g == 0) kd[((m >> 2) * Z + c) * 8 + 4 * u + (m & 3)] = __builtin_bit_cast(uint16_t, d);
+      }
+    }
+  }
+}
+
+// New values of a tile, by one wavefront, whose lanes hold pairs of neighbouring values of 8 positions each.
+template <typename T, int Z, bool Q4>
+__device__ __forceinline__ void append_v(const AppendArgs &a, const Rows &rows, const T *v0, uint32_t *out) {
+  constexpr int hd = 32 * Z;
+  const int lane = threadIdx.x & 63, g = lane >> 4, m = lane & 15;
+  int row[8];
+  uint32_t v[8][Z], there = 0;  // of this lane's positions, those that are stored
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    row[e] = rows(position_of(g, e));
+    there |= row[e] >= 0 ? 1u << e : 0u;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; e++)
+#pragma unroll
+    for (int c = 0; c < Z; c++) v[e][c] = pair_at(v0 + (size_t)max(row[e], 0) * a.stride + 32 * c + 2 * m);
+  if constexpr (!Q4) {
+    _Float16 *const values = (_Float16 *)out + 32 * hd;
 #pragma unroll
     for (int c = 0; c < Z; c++)
 #pragma unroll
       for (int x = 0; x < 2; x++) {
-        _Float16 *const p = vh16 + ((2 * c + x) * 64 + lane) * 8;
-        if (vnew == 0xff) {
+        _Float16 *const p = values + ((2 * c + x) * 64 + lane) * 8;
+        if (there == 0xff) {
           u32x4 w;
 #pragma unroll
           for (int e = 0; e < 4; e++) w[e] = __builtin_amdgcn_perm(v[2 * e + 1][c], v[2 * e][c], x ? 0x07060302u : 0x05040100u);
@@ -313,67 +352,55 @@ __device__ __forceinline__ void append_tile(const AppendArgs &a, int b, int tile
         } else {
 #pragma unroll
           for (int e = 0; e < 8; e++)
-            if (vnew >> e & 1) ((uint16_t *)p)[e] = (uint16_t)(v[e][c] >> 16 * x);
+            if (there >> e & 1) ((uint16_t *)p)[e] = (uint16_t)(v[e][c] >> 16 * x);
         }
       }
   } else {
-    constexpr int T2 = 2 * Z;
-    uint16_t *const kd = (uint16_t *)(out + 4 * hd), *const vd = (uint16_t *)(out + 8 * hd + hd / 2);
-    uint32_t *const vw = out + 4 * hd + hd / 2;
+    uint16_t *const vd = (uint16_t *)(out + 8 * hd + hd / 2);
+    uint32_t *const words = out + 4 * hd + hd / 2;
+    uint32_t keep = 0, old[2 * Z];  // nibbles of a word that stay, and the words before
 #pragma unroll
-    for (int u = 0; u < 2; u++) {
+    for (int e = 0; e < 8; e++) keep |= there >> e & 1 ? 0u : 15u << nibble_of(e);
 #pragma unroll
-      for (int c = 0; c < Z; c++) {
-        u16x2 top = order2(kw[u][c][0]);
+    for (int x = 0; x < 2 * Z; x++) old[x] = 0;
+    if (there && keep)
 #pragma unroll
-        for (int e = 1; e < 4; e++) top = __builtin_elementwise_max(top, order2(kw[u][c][e]));
-        uint32_t t = max((uint32_t)top[0], (uint32_t)top[1]);
-        t = xlane::bit4(t, [](uint32_t x, uint32_t y) { return max(x, y); });
-        t = xlane::bit5(t, [](uint32_t x, uint32_t y) { return max(x, y); });
-        const _Float16 d = factor_of(t);
-        const float inv = inverse_of(d);
-        uint32_t w = 0;
-#pragma unroll
-        for (int e = 0; e < 8; e++) w |= nibble((float)__builtin_bit_cast(half2, kw[u][c][e / 2])[e & 1], inv) << nibble_of(e);
-        if (kr[u] >= 0) {
-          out[word_at(2 * c + u, lane, T2)] = w;
-          // (position 16u + m is element 4u + m % 4 of group m / 4)
-          if (g == 0) kd[((m >> 2) * Z + c) * 8 + 4 * u + (m & 3)] = __builtin_bit_cast(uint16_t, d);
-        }
-      }
-    }
-    uint32_t keep = 0;  // nibbles of a word that stay
-#pragma unroll
-    for (int e = 0; e < 8; e++) keep |= vnew >> e & 1 ? 0u : 15u << nibble_of(e);
+      for (int x = 0; x < 2 * Z; x++) old[x] = words[word_at(x, lane, 2 * Z)];
 #pragma unroll
     for (int c = 0; c < Z; c++) {
       uint32_t w[2] = {0, 0};
+      _Float16 d[8];
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
         // (the pair of positions e and e + 1, side by side)
         const u16x2 o = order2(v[e][c]), p = order2(v[e + 1][c]);
-        u16x2 top = max16(u16x2{(uint16_t)max(o[0], o[1]), (uint16_t)max(p[0], p[1])});
+        const u16x2 top = max16(u16x2{(uint16_t)max(o[0], o[1]), (uint16_t)max(p[0], p[1])});
 #pragma unroll
         for (int y = 0; y < 2; y++) {
-          const _Float16 d = factor_of(top[y]);
-          const float inv = inverse_of(d);
+          d[e + y] = factor_of(top[y]);
+          const float inv = inverse_of(d[e + y]);
           const half2 x = __builtin_bit_cast(half2, v[e + y][c]);
           w[0] |= nibble((float)x[0], inv) << nibble_of(e + y), w[1] |= nibble((float)x[1], inv) << nibble_of(e + y);
-          if (m == 0 && vr[e + y] >= 0) vd[(g * Z + c) * 8 + e + y] = __builtin_bit_cast(uint16_t, d);
         }
       }
-      if (vnew)
+      _Float16 *const f = (_Float16 *)vd + (g * Z + c) * 8;
+      if (there == 0xff) {
+        if (m == c) *(half8 *)f = half8{d[0], d[1], d[2], d[3], d[4], d[5], d[6], d[7]};
+      } else if (m < 8 && there >> m & 1) {  // (lane m the one of element m)
+        _Float16 mine = d[0];
 #pragma unroll
-        for (int x = 0; x < 2; x++) {
-          uint32_t *const p = vw + word_at(2 * c + x, lane, T2);
-          *p = keep ? (*p & keep) | (w[x] & ~keep) : w[x];
-        }
+        for (int e = 1; e < 8; e++) mine = m == e ? d[e] : mine;
+        f[m] = mine;
+      }
+      if (there)
+#pragma unroll
+        for (int x = 0; x < 2; x++) words[word_at(2 * c + x, lane, 2 * Z)] = (old[2 * c + x] & keep) | (w[x] & ~keep);
     }
   }
 }
 
-template <typename T, int Z, bool Q4, bool TURN>
-__global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
+template <typename T, int Z, bool Q4, int TURN>
+__global__ __launch_bounds__(256, 4) void append_kernel(AppendArgs a) {
   if (blockIdx.x >= a.tile_blocks) {
     const int row = blockIdx.x - a.tile_blocks, b = row / a.rows, i = row - b * a.rows;
     if (a.count && i >= a.count[b]) return;
@@ -381,15 +408,22 @@ __global__ __launch_bounds__(256) void append_kernel(AppendArgs a) {
     norm_row(a.q, row, n + i, threadIdx.x, 256);
     return;
   }
-  // A wavefront per (sequence, tile, key head), heads first.
-  const unsigned wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), per = (unsigned)a.tiles * a.pages.kv_heads;
-  const int b = wave / per, rest = wave % per, t = rest / a.pages.kv_heads, kh = rest % a.pages.kv_heads;
+  // A wavefront per (sequence, tile, its values or half of its keys, key head), heads first.
+  const unsigned heads = a.pages.kv_heads, per = a.tiles * 3 * heads;
+  const unsigned wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int b = wave / per, rest = wave - b * per, t = rest / (3 * heads), part = rest / heads - 3 * t, kh = rest % heads;
   if (b >= a.batch) return;
   const int n = min(max(a.n[b], 0), a.pages.room), count = a.count ? min(max(a.count[b], 0), a.rows) : a.rows;
   const int end = min(n + count, a.pages.room);
   if (a.n_out && rest == 0 && (threadIdx.x & 63) == 0) a.n_out[b] = end;
-  const int tile = n / TILE + t;
-  if (TILE * tile < end) append_tile<T, Z, Q4, TURN>(a, b, tile, kh, n, end);
+  const int tile = n / TILE + t, j0 = TILE * tile, u = part - 1;
+  if (part ? j0 + 16 * u >= end || j0 + 16 * u + 16 <= n : j0 >= end) return;
+  uint32_t *out = tile_at(a.pages, Q4, b, tile, kh);
+  if (!out) return;
+  const Rows rows{a.path ? a.path + (size_t)b * a.rows : nullptr, j0 - n, end - j0, a.rows};
+  const size_t from = (size_t)b * a.rows * a.stride + (size_t)kh * 32 * Z;
+  if (part) append_k<T, Z, Q4, TURN>(a, rows, (const T *)a.k + from, out, j0, u);
+  else append_v<T, Z, Q4>(a, rows, (const T *)a.v + from, out);
 }
 
 struct ReadArgs {
@@ -472,8 +506,10 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
 
 template <typename T, int Z, bool Q4>
 void append_launch(wh_ctx *ctx, const AppendArgs &a, unsigned blocks) {
-  if (a.turn.k_gain || a.turn.table) wh_launch(ctx, (append_kernel<T, Z, Q4, true>), blocks, 256, 0, a);
-  else wh_launch(ctx, (append_kernel<T, Z, Q4, false>), blocks, 256, 0, a);
+  if (!a.turn.k_gain && !a.turn.table) return wh_launch(ctx, (append_kernel<T, Z, Q4, PLAIN>), blocks, 256, 0, a);
+  if constexpr (Z % 2 == 0)
+    if (a.turn.table && a.turn.rot == 32 * Z && !a.turn.pairs) return wh_launch(ctx, (append_kernel<T, Z, Q4, HALVES>), blocks, 256, 0, a);
+  wh_launch(ctx, (append_kernel<T, Z, Q4, ANY>), blocks, 256, 0, a);
 }
 template <typename T, bool Q4>
 void append_z(wh_ctx *ctx, const AppendArgs &a, unsigned blocks) {
@@ -584,7 +620,7 @@ int launch_page_append(wh_ctx *ctx, const wh_tree *t, const wh_heads *h, const v
   if (n_out == t->n) return wh_fail(ctx, WH_EARG, "page append: n_out cannot be n itself");
   const size_t nodes = (size_t)t->batch * t->rows;
   const int tiles = (t->rows + TILE - 2) / TILE + 1;
-  const size_t waves = (size_t)t->batch * tiles * p->kv_heads, blocks = (waves + 3) / 4 + (q ? nodes : 0);
+  const size_t waves = (size_t)t->batch * tiles * 3 * p->kv_heads, blocks = (waves + 3) / 4 + (q ? nodes : 0);
   if (blocks >= (size_t)1 << 24 || waves >= (size_t)1 << 31) return wh_fail(ctx, WH_EARG, "page append: %zu rows of %d heads in one call", nodes, p->kv_heads);
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "page append: %s", hipGetErrorString(e));
   const int32_t *count = kept ? kept : t->count;
