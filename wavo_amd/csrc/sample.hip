@@ -21,43 +21,114 @@ struct ProbsArgs {
   int rows, vocab;
 };
 
-// One row per workgroup: its maximum and the sum of exp((x - max) / T) in one pass, the probabilities in a second one.
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
 template <typename T>
-__global__ __launch_bounds__(PT) void probs_kernel(ProbsArgs a) {
+struct Piece;
+template <>
+struct Piece<float> {
+  typedef floatx4 any __attribute__((aligned(4)));
+};
+template <>
+struct Piece<_Float16> {
+  typedef half4 any __attribute__((aligned(2)));
+};
+// Values x .. x + 3 of a row of n; `past` for those that are not there.
+template <typename T>
+__device__ __forceinline__ floatx4 four_of(const T *p, int x, int n, float past) {
+  if (x + 4 <= n) {
+    const auto v = *(const typename Piece<T>::any *)(p + x);
+    return floatx4{(float)v[0], (float)v[1], (float)v[2], (float)v[3]};
+  }
+  floatx4 f;
+#pragma unroll
+  for (int e = 0; e < 4; e++) f[e] = x + e < n ? (float)p[x + e] : past;
+  return f;
+}
+
+// The sum (maximum) over a workgroup's WV wavefronts of what each holds for itself.
+template <int WV, class Op>
+__device__ __forceinline__ float over_waves(float v, float *part, Op op, float none) {
+  const int lane = threadIdx.x & 63;
+  if (lane == 0) part[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return xlane::butterfly(lane < WV ? part[lane] : none, op);
+}
+
+// A row per workgroup, its first HELD * 4096 values in registers from their one load to their store (longer rows' others are read
+// three times, from the caches): the maximum, the exponents' sum, the quotients.
+constexpr int HELD = 13;
+template <typename T>
+__global__ __launch_bounds__(PT, 8) void probs_kernel(ProbsArgs a) {
   __shared__ float tops[PT / 64], sums[PT / 64];
   __shared__ int first;
-  const int row = blockIdx.x, b = row / a.rows, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  if (a.count && row - b * a.rows >= a.count[b]) return;
+  constexpr int STEP = 4 * PT;
+  const int row = blockIdx.x, b = row / a.rows, tid = threadIdx.x;
   const T *x = (const T *)a.logits + (size_t)row * a.ld;
   float *y = a.probs + (size_t)row * a.probs_ld;
+  if (a.count && row - b * a.rows >= a.count[b]) return;
   const float t = a.temperature ? a.temperature[b] : 1.0f;
-  float top = -INFINITY;
-  for (int i = tid; i < a.vocab; i += PT) top = fmaxf(top, (float)x[i]);
-  top = xlane::wave_max(top);
-  if (lane == 0) tops[wave] = top;
   if (tid == 0) first = INT_MAX;
-  __syncthreads();
-  top = tops[lane % (PT / 64)];
-  top = xlane::wave_max(top);
+  floatx4 v[HELD];
+  float top = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < HELD; i++) v[i] = i * STEP < a.vocab ? four_of(x, i * STEP + 4 * tid, a.vocab, -INFINITY) : floatx4{-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int i = 0; i < HELD; i++)
+#pragma unroll
+    for (int e = 0; e < 4; e++) top = fmaxf(top, v[i][e]);
+  for (int at = HELD * STEP + 4 * tid; at < a.vocab; at += STEP) {
+    const floatx4 f = four_of(x, at, a.vocab, -INFINITY);
+#pragma unroll
+    for (int e = 0; e < 4; e++) top = fmaxf(top, f[e]);
+  }
+  top = over_waves<PT / 64>(xlane::wave_max(top), tops, xlane::Max{}, -INFINITY);
+  auto store = [&](int at, floatx4 f) {
+    if (at + 4 <= a.vocab) {
+      *(Piece<float>::any *)(y + at) = f;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; e++)
+        if (at + e < a.vocab) y[at + e] = f[e];
+    }
+  };
   if (!(t > 0.0f)) {  // all of it to the first maximum
     int at = INT_MAX;
-    for (int i = tid; i < a.vocab && at == INT_MAX; i += PT)
-      if ((float)x[i] == top && top > -INFINITY) at = i;
+    for (int i = 4 * tid; i < a.vocab && at == INT_MAX; i += STEP) {
+      const floatx4 f = four_of(x, i, a.vocab, -INFINITY);
+#pragma unroll
+      for (int e = 3; e >= 0; e--)
+        if (f[e] == top && top > -INFINITY) at = i + e;
+    }
     if (at != INT_MAX) atomicMin(&first, at);
     __syncthreads();
-    for (int i = tid; i < a.vocab; i += PT) y[i] = i == first ? 1.0f : 0.0f;
+    const int one = first;
+    for (int i = 4 * tid; i < a.vocab; i += STEP)
+      store(i, floatx4{i == one ? 1.0f : 0.0f, i + 1 == one ? 1.0f : 0.0f, i + 2 == one ? 1.0f : 0.0f, i + 3 == one ? 1.0f : 0.0f});
     return;
   }
   const float base = top == -INFINITY ? 0.0f : top, k = fminf(1.44269504088896341f / t, 3.402823466e38f);
-  float sum = 0.0f;
-  for (int i = tid; i < a.vocab; i += PT) sum += __builtin_amdgcn_exp2f(((float)x[i] - base) * k);
-  sum = xlane::wave_sum(sum);
-  if (lane == 0) sums[wave] = sum;
-  __syncthreads();
-  sum = lane < PT / 64 ? sums[lane] : 0.0f;
-  sum = xlane::wave_sum(sum);
+  auto power = [&](floatx4 f) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) f[e] = __builtin_amdgcn_exp2f((f[e] - base) * k);
+    return f;
+  };
+  float sum = 0.0f, more = 0.0f;
+#pragma unroll
+  for (int i = 0; i < HELD; i++) {
+    v[i] = power(v[i]);
+    sum += v[i][0] + v[i][1], more += v[i][2] + v[i][3];
+  }
+  for (int at = HELD * STEP + 4 * tid; at < a.vocab; at += STEP) {
+    const floatx4 f = power(four_of(x, at, a.vocab, -INFINITY));
+    sum += f[0] + f[1], more += f[2] + f[3];
+  }
+  sum = over_waves<PT / 64>(xlane::wave_sum(sum + more), sums, xlane::Add{}, 0.0f);
   const float scale = sum == 0.0f ? 0.0f : 1.0f / sum;
-  for (int i = tid; i < a.vocab; i += PT) y[i] = __builtin_amdgcn_exp2f(((float)x[i] - base) * k) * scale;
+#pragma unroll
+  for (int i = 0; i < HELD; i++)
+    if (i * STEP < a.vocab) store(i * STEP + 4 * tid, v[i] * scale);
+  for (int at = HELD * STEP + 4 * tid; at < a.vocab; at += STEP) store(at, power(four_of(x, at, a.vocab, -INFINITY)) * scale);
 }
 
 struct SampleArgs {
@@ -69,131 +140,204 @@ struct SampleArgs {
   uint32_t *picks;
 };
 
-constexpr int ST = 1024;  // threads of a sequence's workgroup
+constexpr int ST = 1024;      // threads of a sequence's workgroup
+constexpr int PIECES = 1024;  // runs of ids whose sums are kept
+constexpr int BATCH = 6;      // 256 ids each that a wavefront loads at once
 
-// The sum over the workgroup, the same for every thread; `part` is free again after the next barrier.
-__device__ __forceinline__ double block_sum(double v, double *part) {
-  v = xlane::wave_sum(v);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
-  __syncthreads();
-  double s = 0.0;
-#pragma unroll
-  for (int i = 0; i < ST / 64; i++) s += part[i];
-  return s;
+// What is left of a node's probabilities after rejections of its children's tokens, made anew from p and q whenever it is
+// read.  With drafts, w = max(0, w / Z - q) round by round; without, zero at the tokens, which stand in `inverse` as numbers.
+template <bool DRAFTS>
+__device__ __forceinline__ double left_of(float p, float q, int x, const double *inverse, int rounds) {
+  double w = p;
+  for (int r = 0; r < rounds; r++) {
+    if constexpr (DRAFTS) w = fmax(w * inverse[r] - (double)q, 0.0);
+    else w = inverse[r] == (double)x ? 0.0 : w;
+  }
+  return w;
 }
 
-// A sequence's walk by one workgroup.  What is left of a node's probabilities after rejections of its children's tokens is
-// made anew from p and q whenever it is read: with drafts, w = max(0, w / Z - q) round by round; without, zero at the tokens.
+// A sequence's walk by one workgroup.  What its tests need of p and q (a value per node, of its parent's rows) is gathered
+// first, for all nodes side by side; a rejection that is followed by another child costs a pass over the rows for Z, and the
+// draw one more, which leaves the sums of runs of ids behind, so that its place is looked for in one of them.  Everything in
+// 64 bits: random numbers are compared with sums of 1e5 values, whose last bits in f32 would move a place for one of 1e3.
+template <bool DRAFTS>
 __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs a) {
-  __shared__ double part[ST / 64], inverse[TREE_ROWS];
-  __shared__ uint32_t out[TREE_ROWS];
+  __shared__ double part[ST / 64], sums[PIECES], inverse[TREE_ROWS];
+  __shared__ float mine[TREE_ROWS], drafted[TREE_ROWS], numbers[TREE_ROWS];
+  __shared__ uint32_t tokens[TREE_ROWS], out[TREE_ROWS];
+  __shared__ short parents[TREE_ROWS];
   __shared__ int found;
-  const int b = blockIdx.x, tid = threadIdx.x, count = a.count ? min(max(a.count[b], 0), a.rows) : a.rows;
+  constexpr int WV = ST / 64;
+  const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int count = a.count ? min(max(a.count[b], 0), a.rows) : a.rows;
   if (count == 0) return;
   const size_t row0 = (size_t)b * a.rows;
-  const uint32_t *tokens = a.tokens + row0, *mask = a.mask ? a.mask + (size_t)b * a.mask_stride : nullptr;
-  for (int i = tid; i < count; i += ST) out[i] = NONE;
-  if (tid == 0) found = -1;
-  int at = 0, rounds = 0;  // the node, and how many of its children were rejected
-  double total = 1.0;
-  const float *p = a.p + row0 * a.ld, *q = a.q ? a.q + row0 * a.ld : nullptr;
-  // (without drafts: the tokens that are out, in `inverse` as numbers)
-  auto left = [&](int x) {
-    double w = p[x];
-    if (q) {
-      const double y = q[x];
-      for (int r = 0; r < rounds; r++) w = fmax(w * inverse[r] - y, 0.0);
-    } else {
-      for (int r = 0; r < rounds; r++) w = inverse[r] == (double)x ? 0.0 : w;
-    }
-    return w;
-  };
-  __syncthreads();
-  for (int i = 1; i < count; i++) {
-    // i's parent: the highest node below it that it sees.
-    int parent = mask ? -1 : i - 1;
-    if (mask) {
-      const uint32_t *m = mask + (size_t)i * a.words;
+  if (tid < count) {
+    // A node's parent: the highest node below it that it sees.
+    const int i = tid;
+    int parent = i - 1;
+    const float u = a.u[row0 + i];
+    const uint32_t x = i ? a.tokens[row0 + i] : 0u;
+    if (a.mask && i) {
+      const uint32_t *m = a.mask + (size_t)b * a.mask_stride + (size_t)i * a.words;
+      parent = -1;
       for (int w = (i - 1) / 32; w >= 0 && parent < 0; w--) {
         const uint32_t bits = m[w] & (w == i / 32 ? (1u << i % 32) - 1u : 0xffffffffu);
         if (bits) parent = 32 * w + 31 - __clz(bits);
       }
     }
-    if (parent != at || !(total > 0.0)) continue;
-    const uint32_t x = tokens[i];
-    const double mine = x < (uint32_t)a.vocab ? left((int)x) : 0.0, u = a.u[row0 + i];
-    if (x < (uint32_t)a.vocab && u * (q ? (double)q[x] : 1.0) * total < mine) {
-      if (tid == 0) out[at] = x;
-      at = i, rounds = 0, total = 1.0;
-      p = a.p + (row0 + i) * a.ld, q = a.q ? a.q + (row0 + i) * a.ld : nullptr;
+    if (i && x >= (uint32_t)a.vocab) parent = -1;  // (no draft of this vocabulary)
+    const size_t at = (row0 + max(parent, 0)) * a.ld + (x < (uint32_t)a.vocab ? x : 0u);
+    mine[i] = a.p[at];
+    if constexpr (DRAFTS) drafted[i] = a.q[at];
+    numbers[i] = u, tokens[i] = x, parents[i] = (short)(i ? parent : -1), out[i] = NONE;
+  }
+  if (tid == 0) found = -1;
+  __syncthreads();
+
+  int at = 0, rounds = 0;  // the node, and how many of its children were rejected
+  double total = 1.0;
+  const float *p = a.p + row0 * a.ld, *q = DRAFTS ? a.q + row0 * a.ld : nullptr;
+  // The rows of `at`, 256 ids (a wavefront's) at a time: f(piece, ids' weights).  A piece is `per` such blocks, one after the
+  // other by one wavefront, and every wavefront takes every WV-th piece.
+  const int blocks = (a.vocab + 255) / 256, per = (blocks + PIECES - 1) / PIECES, pieces = (blocks + per - 1) / per;
+  auto pass = [&](auto f) {
+    for (int n0 = 0; wave + WV * (n0 / per) < pieces; n0 += BATCH) {
+      floatx4 x[BATCH], y[BATCH];
+      int piece[BATCH], block[BATCH];
+#pragma unroll
+      for (int i = 0; i < BATCH; i++) {
+        piece[i] = wave + WV * ((n0 + i) / per), block[i] = piece[i] * per + (n0 + i) % per;
+        const int id = 256 * block[i] + 4 * lane;
+        if (piece[i] >= pieces || block[i] >= blocks) continue;
+        x[i] = four_of(p, id, a.vocab, 0.0f);
+        if constexpr (DRAFTS) y[i] = rounds ? four_of(q, id, a.vocab, 0.0f) : floatx4{};
+      }
+#pragma unroll
+      for (int i = 0; i < BATCH; i++) {
+        if (piece[i] >= pieces || block[i] >= blocks) continue;
+        double w = 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) w += left_of<DRAFTS>(x[i][e], DRAFTS ? y[i][e] : 0.0f, 256 * block[i] + 4 * lane + e, inverse, rounds);
+        f(piece[i], w);
+      }
+    }
+  };
+  for (int base = 0, from = 1; base < count;) {
+    // The next child of `at`, among 64 nodes at a time.
+    const int i0 = base + lane;
+    const uint64_t any = __ballot(i0 >= from && i0 < count && parents[min(i0, count - 1)] == at);
+    if (!any) {
+      base += 64;
       continue;
     }
-    if (x >= (uint32_t)a.vocab) continue;  // (no draft of this vocabulary)
+    const int i = base + (int)__builtin_ctzll(any);
+    const int x = (int)tokens[i];
+    if (DRAFTS && rounds && total < 0.0) {  // (Z of the rejections so far, wanted only now)
+      double s = 0.0;
+      pass([&](int, double w) { s += w; });
+      s = xlane::wave_sum(s);
+      if (lane == 0) part[wave] = s;
+      __syncthreads();
+      total = 0.0;
+#pragma unroll
+      for (int w = 0; w < WV; w++) total += part[w];
+      __syncthreads();
+    }
+    if (!(total > 0.0)) break;  // nothing is left to accept
+    from = i + 1;
+    const double w = left_of<DRAFTS>(mine[i], DRAFTS ? drafted[i] : 0.0f, x, inverse, rounds);
+    if ((double)numbers[i] * (DRAFTS ? (double)drafted[i] : 1.0) * total < w) {
+      if (tid == 0) out[at] = (uint32_t)x;
+      at = i, rounds = 0, total = 1.0;
+      p = a.p + (row0 + i) * a.ld, q = DRAFTS ? a.q + (row0 + i) * a.ld : nullptr;
+      base = i / 64 * 64;
+      continue;
+    }
     __syncthreads();
-    if (tid == 0) inverse[rounds] = q ? 1.0 / total : (double)x;
+    if (tid == 0) inverse[rounds] = DRAFTS ? 1.0 / total : (double)x;
     __syncthreads();
     rounds++;
-    if (q) {
-      double sum = 0.0;
-      for (int y = tid; y < a.vocab; y += ST) sum += left(y);
-      total = block_sum(sum, part);
-    } else {
-      total -= mine;
-    }
+    total = DRAFTS ? -1.0 : total - w;
   }
-  // The draw: each wavefront sums a run of ids, the one that holds the place looks for it.
-  constexpr int WV = ST / 64;
-  const int wave = tid >> 6, lane = tid & 63, run = ((a.vocab + WV - 1) / WV + 63) / 64 * 64;
+
+  // The draw.
   for (int attempt = 0; attempt < 2; attempt++) {
-    const int begin = min(wave * run, a.vocab), end = min(begin + run, a.vocab);
-    double sum = 0.0;
-    for (int x = begin + lane; x < end; x += 64) sum += left(x);
-    sum = xlane::wave_sum(sum);
     __syncthreads();
-    if (lane == 0) part[wave] = sum;
+    for (int i = tid; i < pieces; i += ST) sums[i] = 0.0;
     __syncthreads();
-    double all = 0.0, before = 0.0;
-    for (int i = 0; i < WV; i++) {
-      if (i == wave) before = all;
-      all += part[i];
+    pass([&](int piece, double w) {
+      w = xlane::wave_sum(w);
+      if (lane == 0) sums[piece] += w;
+    });
+    __syncthreads();
+    // Running sums of 16 pieces a lane, by every wavefront for itself.
+    double s = 0.0;
+    for (int i = 0; i < PIECES / 64; i++) {
+      const int k = PIECES / 64 * lane + i;
+      if (k < pieces) s += sums[k];
     }
+    double c = s;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const double o = __shfl_up(c, d);
+      if (lane >= d) c += o;
+    }
+    const double all = __shfl(c, 63);
     if (!(all > 0.0)) {  // nothing left: from the node's probabilities themselves
       rounds = 0;
       continue;
     }
-    const double place = (double)a.u[row0] * all;
-    // One run holds the place.  (Its own running sums may end a last bit before it: then it is at the run's last id.)
-    if (before <= place && place < before + part[wave]) {
-      int last = -1, hit = -1;
-      for (int x0 = begin; x0 < end && hit < 0; x0 += 64) {
-        const int x = x0 + lane;
-        const double w = x < end ? left(x) : 0.0;
-        double c = w;  // running sums of the 64
-        for (int d = 1; d < 64; d *= 2) {
-          const double o = __shfl_up(c, d);
-          if (lane >= d) c += o;
-        }
-        const uint64_t over = __ballot(w > 0.0 && before + c > place), some = __ballot(w > 0.0);
-        if (some) last = x0 + 63 - __clzll(some);
-        if (over) hit = x0 + (int)__builtin_ctzll(over);
-        before += __shfl(c, 63);
+    const double place = (double)numbers[0] * all;
+    if (wave == 0) {
+      // The first lane, then its first piece, then the first id whose running sum is past the place; where last bits leave none,
+      // the last one of any weight.
+      const uint64_t over = __ballot(s > 0.0 && c > place), some = __ballot(s > 0.0);
+      const int l = over ? (int)__builtin_ctzll(over) : 63 - (int)__clzll(some);
+      double before = __shfl(c - s, l);
+      int piece = -1, last = 0;
+      for (int i = 0; i < PIECES / 64 && piece < 0; i++) {
+        const int k = PIECES / 64 * l + i;
+        if (k >= pieces) break;
+        if (sums[k] > 0.0) last = k;
+        if (sums[k] > 0.0 && before + sums[k] > place) piece = k;
+        else before += sums[k];
       }
-      if (lane == 0) found = hit >= 0 ? hit : last;
+      if (piece < 0) piece = last, before -= sums[last];
+      int hit = -1, tail = -1;
+      for (int k = piece * per; k < min((piece + 1) * per, blocks) && hit < 0; k++) {
+        const int id = 256 * k + 4 * lane;
+        const floatx4 x = four_of(p, id, a.vocab, 0.0f), y = DRAFTS && rounds ? four_of(q, id, a.vocab, 0.0f) : floatx4{};
+        double w[4], r = 0.0;
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = left_of<DRAFTS>(x[e], y[e], id + e, inverse, rounds), r += w[e];
+        double run = r;
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+          const double o = __shfl_up(run, d);
+          if (lane >= d) run += o;
+        }
+        double here = before + (run - r);
+        int own = -1, end = -1;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          here += w[e];
+          if (w[e] > 0.0) end = id + e;
+          if (own < 0 && w[e] > 0.0 && here > place) own = id + e;
+        }
+        const uint64_t hits = __ballot(own >= 0), ends = __ballot(end >= 0);
+        if (hits) hit = __shfl(own, (int)__builtin_ctzll(hits));
+        if (ends) tail = __shfl(end, 63 - (int)__clzll(ends));
+        before += __shfl(run, 63);
+      }
+      if (lane == 0) found = hit >= 0 ? hit : tail;
     }
     __syncthreads();
-    if (found < 0) {  // (a random number that is not below one: the last id of any mass)
-      int most = -1;
-      for (int x = tid; x < a.vocab; x += ST)
-        if (left(x) > 0.0) most = x;
-      atomicMax(&found, most);
-      __syncthreads();
-    }
     if (tid == 0) out[at] = (uint32_t)found;
     break;
   }
   __syncthreads();
-  for (int i = tid; i < count; i += ST) a.picks[row0 + i] = out[i];
+  if (tid < count) a.picks[row0 + tid] = out[tid];
 }
 
 }  // namespace
@@ -222,6 +366,7 @@ int launch_tree_sample(wh_ctx *ctx, const wh_tree *t, const float *probs, const 
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "tree sample: %s", hipGetErrorString(e));
   const SampleArgs a{probs, drafts, u, t->count, t->tokens, t->mask, t->mask_stride, ld, t->rows, (t->rows + 31) / 32, vocab, picks};
   ProfScope prof(ctx, "tree_sample", 0.0, 4.0 * t->batch * vocab * (drafts ? 2 : 1));
-  wh_launch(ctx, sample_kernel, (unsigned)t->batch, ST, 0, a);
+  if (drafts) wh_launch(ctx, sample_kernel<true>, (unsigned)t->batch, ST, 0, a);
+  else wh_launch(ctx, sample_kernel<false>, (unsigned)t->batch, ST, 0, a);
   return wh_launched(ctx, "tree sample");
 }
