@@ -142,18 +142,22 @@ struct SampleArgs {
 
 constexpr int ST = 1024;      // threads of a sequence's workgroup
 constexpr int PIECES = 1024;  // runs of ids whose sums are kept
-constexpr int BATCH = 6;      // 256 ids each that a wavefront loads at once
 
-// What is left of a node's probabilities after rejections of its children's tokens, made anew from p and q whenever it is
-// read.  With drafts, w = max(0, w / Z - q) round by round; without, zero at the tokens, which stand in `inverse` as numbers.
-template <bool DRAFTS>
-__device__ __forceinline__ double left_of(float p, float q, int x, const double *inverse, int rounds) {
-  double w = p;
+// What is left of N ids' probabilities x after rejections of their node's children's tokens, made anew from p and q whenever
+// they are read.  With drafts y, w = max(0, w / Z - q) round by round (gone: 1 / Z); without, zero at the tokens (gone).
+template <bool DRAFTS, int N, class Id>
+__device__ __forceinline__ void left_of(const float (&x)[N], const float (&y)[N], double (&w)[N], const double *gone, int rounds, Id id) {
+#pragma unroll
+  for (int i = 0; i < N; i++) w[i] = x[i];
   for (int r = 0; r < rounds; r++) {
-    if constexpr (DRAFTS) w = fmax(w * inverse[r] - (double)q, 0.0);
-    else w = inverse[r] == (double)x ? 0.0 : w;
+    const double z = gone[r];
+    const int token = (int)z;
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      if constexpr (DRAFTS) w[i] = fmax(w[i] * z - (double)y[i], 0.0);
+      else w[i] = id(i) == token ? 0.0 : w[i];
+    }
   }
-  return w;
 }
 
 // A sequence's walk by one workgroup.  What its tests need of p and q (a value per node, of its parent's rows) is gathered
@@ -162,12 +166,12 @@ __device__ __forceinline__ double left_of(float p, float q, int x, const double 
 // 64 bits: random numbers are compared with sums of 1e5 values, whose last bits in f32 would move a place for one of 1e3.
 template <bool DRAFTS>
 __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs a) {
-  __shared__ double part[ST / 64], sums[PIECES], inverse[TREE_ROWS];
+  __shared__ double part[ST / 64], sums[PIECES], gone[TREE_ROWS];
   __shared__ float mine[TREE_ROWS], drafted[TREE_ROWS], numbers[TREE_ROWS];
   __shared__ uint32_t tokens[TREE_ROWS], out[TREE_ROWS];
   __shared__ short parents[TREE_ROWS];
   __shared__ int found;
-  constexpr int WV = ST / 64;
+  constexpr int WV = ST / 64, BATCH = DRAFTS ? 5 : 7;  // BATCH: blocks of 256 ids that a wavefront loads at once
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int count = a.count ? min(max(a.count[b], 0), a.rows) : a.rows;
   if (count == 0) return;
@@ -203,24 +207,21 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs a) {
   const int blocks = (a.vocab + 255) / 256, per = (blocks + PIECES - 1) / PIECES, pieces = (blocks + per - 1) / per;
   auto pass = [&](auto f) {
     for (int n0 = 0; wave + WV * (n0 / per) < pieces; n0 += BATCH) {
-      floatx4 x[BATCH], y[BATCH];
+      float x[4 * BATCH], y[4 * BATCH];
+      double w[4 * BATCH];
       int piece[BATCH], block[BATCH];
 #pragma unroll
       for (int i = 0; i < BATCH; i++) {
         piece[i] = wave + WV * ((n0 + i) / per), block[i] = piece[i] * per + (n0 + i) % per;
+        if (piece[i] >= pieces) block[i] = blocks;  // (nothing there: zeros)
         const int id = 256 * block[i] + 4 * lane;
-        if (piece[i] >= pieces || block[i] >= blocks) continue;
-        x[i] = four_of(p, id, a.vocab, 0.0f);
-        if constexpr (DRAFTS) y[i] = rounds ? four_of(q, id, a.vocab, 0.0f) : floatx4{};
+        *(floatx4 *)&x[4 * i] = four_of(p, id, a.vocab, 0.0f);
+        if constexpr (DRAFTS) *(floatx4 *)&y[4 * i] = rounds ? four_of(q, id, a.vocab, 0.0f) : floatx4{};
       }
+      left_of<DRAFTS>(x, y, w, gone, rounds, [&](int i) { return 256 * block[i / 4] + 4 * lane + i % 4; });
 #pragma unroll
-      for (int i = 0; i < BATCH; i++) {
-        if (piece[i] >= pieces || block[i] >= blocks) continue;
-        double w = 0.0;
-#pragma unroll
-        for (int e = 0; e < 4; e++) w += left_of<DRAFTS>(x[i][e], DRAFTS ? y[i][e] : 0.0f, 256 * block[i] + 4 * lane + e, inverse, rounds);
-        f(piece[i], w);
-      }
+      for (int i = 0; i < BATCH; i++)
+        if (block[i] < blocks) f(piece[i], (w[4 * i] + w[4 * i + 1]) + (w[4 * i + 2] + w[4 * i + 3]));
     }
   };
   for (int base = 0, from = 1; base < count;) {
@@ -246,7 +247,10 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs a) {
     }
     if (!(total > 0.0)) break;  // nothing is left to accept
     from = i + 1;
-    const double w = left_of<DRAFTS>(mine[i], DRAFTS ? drafted[i] : 0.0f, x, inverse, rounds);
+    const float own[1] = {mine[i]}, draft[1] = {DRAFTS ? drafted[i] : 0.0f};
+    double kept[1];
+    left_of<DRAFTS>(own, draft, kept, gone, rounds, [&](int) { return x; });
+    const double w = kept[0];
     if ((double)numbers[i] * (DRAFTS ? (double)drafted[i] : 1.0) * total < w) {
       if (tid == 0) out[at] = (uint32_t)x;
       at = i, rounds = 0, total = 1.0;
@@ -255,7 +259,7 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs a) {
       continue;
     }
     __syncthreads();
-    if (tid == 0) inverse[rounds] = DRAFTS ? 1.0 / total : (double)x;
+    if (tid == 0) gone[rounds] = DRAFTS ? 1.0 / total : (double)x;
     __syncthreads();
     rounds++;
     total = DRAFTS ? -1.0 : total - w;
@@ -264,7 +268,7 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs a) {
   // The draw.
   for (int attempt = 0; attempt < 2; attempt++) {
     __syncthreads();
-    for (int i = tid; i < pieces; i += ST) sums[i] = 0.0;
+    for (int i = tid; i < PIECES; i += ST) sums[i] = 0.0;
     __syncthreads();
     pass([&](int piece, double w) {
       w = xlane::wave_sum(w);
@@ -273,10 +277,8 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs a) {
     __syncthreads();
     // Running sums of 16 pieces a lane, by every wavefront for itself.
     double s = 0.0;
-    for (int i = 0; i < PIECES / 64; i++) {
-      const int k = PIECES / 64 * lane + i;
-      if (k < pieces) s += sums[k];
-    }
+#pragma unroll
+    for (int i = 0; i < PIECES / 64; i++) s += sums[PIECES / 64 * lane + i];
     double c = s;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -307,10 +309,12 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs a) {
       int hit = -1, tail = -1;
       for (int k = piece * per; k < min((piece + 1) * per, blocks) && hit < 0; k++) {
         const int id = 256 * k + 4 * lane;
-        const floatx4 x = four_of(p, id, a.vocab, 0.0f), y = DRAFTS && rounds ? four_of(q, id, a.vocab, 0.0f) : floatx4{};
-        double w[4], r = 0.0;
-#pragma unroll
-        for (int e = 0; e < 4; e++) w[e] = left_of<DRAFTS>(x[e], y[e], id + e, inverse, rounds), r += w[e];
+        float x[4], y[4];
+        *(floatx4 *)x = four_of(p, id, a.vocab, 0.0f);
+        *(floatx4 *)y = DRAFTS && rounds ? four_of(q, id, a.vocab, 0.0f) : floatx4{};
+        double w[4];
+        left_of<DRAFTS>(x, y, w, gone, rounds, [&](int e) { return id + e; });
+        const double r = (w[0] + w[1]) + (w[2] + w[3]);
         double run = r;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
