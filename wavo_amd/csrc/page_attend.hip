@@ -23,31 +23,98 @@ struct PageAttendArgs {
   size_t mask_stride;
   int batch, rows, words, heads;
   float scale;
-  int kw, splits, per, row_blocks;  // per: tiles of a split
-  // splits > 1: unnormalized outputs [split][batch * rows][heads][hd] and (maximum, sum, factor of the maximum's exponent,
-  // -) [split][batch * rows][heads] of the splits that are used.
+  int kw, row_blocks, qt;  // qt: tiles of 16 rows of a block
+  // even: how many workgroups share all the tiles of a key head evenly (0: each has a block of rows to itself), and the tiles that
+  // one takes at least; their outputs, two parts each: unnormalized [part][row][hd] and (maximum, sum, factor of the
+  // maximum's exponent, -) [part][row].
+  int even, least;
   float *po, *pml;
 };
 
-constexpr int WAVES = 8;    // wavefronts of a workgroup, at most
-constexpr int SPLITS = 64;  // and splits of a cache
-constexpr float LOWEST = -1e30f;  // the maximum of a row that has seen nothing
+constexpr int WAVES = 8;             // wavefronts of a workgroup, at most
+constexpr float LOWEST = -1e30f;     // the maximum of a row that has seen nothing
+constexpr int START = 24;
 constexpr int JOIN_LDS = 128 << 10;  // bytes in which wavefronts' results are joined
 
-// The tiles of a sequence (the cache's, then the nodes'): its workgroups take runs of `per`, so that a short sequence uses fewer
-// of them and they all take about as long.
+// A sequence's tiles: the cache's, then the nodes'.
 struct Share {
-  int n, count, cached, tiles, used;
+  int n, count, cached, tiles;
 };
-__device__ __forceinline__ Share share_of(const PageAttendArgs &a, int b) {
+__device__ __forceinline__ Share share_of(const PageAttendArgs &a, int n, int count) {
   Share s;
-  s.n = min(max(a.n[b], 0), a.pages.room);
-  s.count = a.count ? min(max(a.count[b], 0), a.rows) : a.rows;
+  s.n = min(max(n, 0), a.pages.room);
+  s.count = min(max(count, 0), a.rows);
   s.cached = (s.n + TILE - 1) / TILE;
   s.tiles = s.cached + (a.mask && a.k ? (s.count + TILE - 1) / TILE : 0);
-  s.used = a.splits > 1 ? max((s.tiles + a.per - 1) / a.per, 1) : 1;
   return s;
 }
+__device__ __forceinline__ Share share_of(const PageAttendArgs &a, int b) { return share_of(a, a.n[b], a.count ? a.count[b] : a.rows); }
+
+// All the tiles of a key head in a row: sequence by sequence, block of `rows` rows by block, each at least one.  (Every key
+// head's are shared out alike, so that all of them are in the same pages at about the same time.)  64 sequences at a time are kept in LDS: their lengths and counts, and how many tiles they and those before them have.
+struct EvenLds {
+  int n[64], count[64];
+  uint32_t sum[64];
+};
+struct Even {
+  const PageAttendArgs &a;
+  EvenLds &lds;
+  int rows, b0;             // of the 64, the first
+  uint32_t all, per, before;  // tiles; those of a workgroup; those before the 64
+  __device__ __forceinline__ uint32_t load(int base) {  // (the tiles of the 64)
+    const int lane = threadIdx.x & 63, b = base + lane;
+    int n = 0, count = 0;
+    if (b < a.batch) n = a.n[b], count = a.count ? a.count[b] : a.rows;
+    const Share s = share_of(a, n, count);
+    uint32_t sum = blocks_of(s) * tiles_of(s);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const uint32_t o = __shfl_up(sum, d);
+      if (lane >= d) sum += o;
+    }
+    if (threadIdx.x < 64) lds.n[lane] = n, lds.count[lane] = count, lds.sum[lane] = sum;
+    return __builtin_amdgcn_readlane(sum, 63);
+  }
+  // A block's: as many besides its own as its start and end take the time of.
+  static __device__ __forceinline__ uint32_t tiles_of(const Share &s) { return START + max(s.tiles, 1); }
+  __device__ __forceinline__ uint32_t blocks_of(const Share &s) const {
+    return (s.count * (a.heads / a.pages.kv_heads) + rows - 1) / rows;
+  }
+  // (by every thread of a workgroup)
+  __device__ __forceinline__ Even(const PageAttendArgs &a, EvenLds &lds, int rows) : a(a), lds(lds), rows(rows), b0(0), before(0) {
+    all = load(0);
+    if (a.batch > 64) {
+      for (int base = 64; base < a.batch; base += 64) {
+        __syncthreads();
+        all += load(base);
+      }
+      __syncthreads();
+      load(0);
+    }
+    __syncthreads();
+    all = __builtin_amdgcn_readfirstlane(all);
+    per = max((all + a.even - 1) / a.even, (uint32_t)a.least);
+  }
+  // The next 64 sequences.
+  __device__ __forceinline__ void next() {
+    before += __builtin_amdgcn_readfirstlane(lds.sum[63]), b0 += 64;
+    __syncthreads();
+    load(b0);
+    __syncthreads();
+  }
+  // The sequence of the tile at `place` (< all, and not before the 64), and its first tile's place.
+  __device__ __forceinline__ void find(uint32_t place, int &b, Share &s, uint32_t &first) {
+    for (;; next()) {
+      const uint32_t sum = lds.sum[threadIdx.x & 63];
+      const uint64_t past = __ballot(before + sum > place);
+      if (!past) continue;
+      const int l = __builtin_ctzll(past);
+      b = b0 + l, first = before + (l ? __builtin_amdgcn_readlane(sum, l - 1) : 0u);
+      s = share_of(a, __builtin_amdgcn_readfirstlane(lds.n[l]), __builtin_amdgcn_readfirstlane(lds.count[l]));
+      return;
+    }
+  }
+};
 
 // A tile's share of a lane: words of K and V, and for 4 bits their factors.
 // OWN: of K those of the positions of the lane's own words (halfs for u = 0 and 1), otherwise those of its scores.
@@ -56,7 +123,11 @@ struct Tile;
 template <int Z, bool OWN>
 struct Tile<Z, true, OWN> {
   uint32_t k[2 * Z], v[2 * Z];
-  typename std::conditional<OWN, half2, half8>::type kd[Z];
+  // (halfs as they are loaded, one a register: put together they would be waited for where that is done)
+  struct Pair {
+    uint16_t u[2];
+  };
+  typename std::conditional<OWN, Pair, half8>::type kd[Z];
   half8 vd[Z];
   static __device__ __forceinline__ void words(uint32_t (&w)[2 * Z], const uint32_t *p, int lane) {
     constexpr int T = 2 * Z, whole = T & ~3;
@@ -73,9 +144,9 @@ struct Tile<Z, true, OWN> {
   __device__ __forceinline__ void load_k(const uint32_t *p, int lane, int g) {
     words(k, p, lane);
     if constexpr (OWN) {
-      const _Float16 *d = (const _Float16 *)(p + 128 * Z) + (lane % 16 / 4) * 8 * Z + lane % 4;
+      const uint16_t *d = (const uint16_t *)(p + 128 * Z) + (lane % 16 / 4) * 8 * Z + lane % 4;
 #pragma unroll
-      for (int c = 0; c < Z; c++) kd[c] = half2{d[8 * c], d[8 * c + 4]};
+      for (int c = 0; c < Z; c++) kd[c].u[0] = d[8 * c], kd[c].u[1] = d[8 * c + 4];
     } else {
 #pragma unroll
       for (int c = 0; c < Z; c++) kd[c] = *(const half8 *)(p + 128 * Z + (g * Z + c) * 4);
@@ -129,8 +200,15 @@ struct Tile<Z, false, OWN> {
   }
 };
 
+// A row of queries (of one that is not there: the last one's).
+template <typename T, int Z>
+__device__ __forceinline__ void load_rows(const PageAttendArgs &a, int b, int kh, int row, int g, float (&f)[Z][8]) {
+  const int group = a.heads / a.pages.kv_heads, r = min(row, a.rows * group - 1);
+  load_query<T, Z>((const T *)a.q + ((size_t)b * a.rows + node_of(r, group)) * a.stride + (size_t)(kh * group + head_of(r, group)) * 32 * Z, g, 32 * Z, f);
+}
+
 // A workgroup takes one key head of a sequence, 16 * QT of its rows (the heads / kv_heads query heads of a node are rows next
-// to each other) and one split of its tiles, of which each of its kw wavefronts takes every kw-th.
+// to each other) and a run of its tiles, of which each of its kw wavefronts takes every kw-th.
 //   Scores transposed, S^T = K Q^T: lane 16g + i holds row i's scores of positions position_of(g, e), e < 8.  For 4 bits the
 //   products are those of nibble - 8, exact in f16, chunk by chunk of 32 values, and every chunk's sum is multiplied by its
 //   position's factor in f32: K is taken as it stands.
@@ -146,33 +224,22 @@ struct Tile<Z, false, OWN> {
 //
 // OPEN (4 bits and P16): K and V are multiplied by their factors as they are opened, once for all rows, and rounded to f16 (2^-11 of
 // themselves, as an f16 cache would hold them), so that weights are operands as they stand.
+//
+// attend_part: the tiles from start to end of sequence b's block of rows from r0 on of a key head; into the outputs, or as part `part`.
 template <int Z, int QT, int QP, bool P16, bool Q4>
-__global__ __launch_bounds__(64 * WAVES, QT == 1 && (QP == 1 || Z < 4) ? 4 : 2) void page_attend_kernel(PageAttendArgs a) {
+__device__ __forceinline__ void attend_part(const PageAttendArgs &a, uint8_t *smem, int b, int kh, int r0, const Share &s, int start, int end, int part,
+                                            float (&f)[Z][8]) {
   typedef typename std::conditional<QP == 2, float, _Float16>::type T;
   constexpr int hd = 32 * Z;
   constexpr bool SHARED = QT > 1, OPEN = Q4 && P16;  // SHARED: queries in LDS
-  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
-  const int lane = threadIdx.x & 63, ki = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  int tid = threadIdx.x;
+  asm volatile("" : "+v"(tid));  // (nothing that follows from it is kept in registers from one run to the next)
+  const int lane = tid & 63, ki = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int g = lane >> 4, m = lane & 15;
-  const int split = blockIdx.z, kh = blockIdx.x, b = a.row_blocks == 1 ? blockIdx.y : blockIdx.y / a.row_blocks;
-  const int group = a.heads / a.pages.kv_heads, r0 = 16 * QT * (blockIdx.y - b * a.row_blocks);
+  const int group = a.heads / a.pages.kv_heads, total = s.count * group;
   const size_t row0 = (size_t)b * a.rows;
-  auto query = [&](int row, float (&f)[Z][8]) {  // (of rows that are not there, too: nothing is known of the lengths yet)
-    const int r = min(row, a.rows * group - 1);
-    load_query<T, Z>((const T *)a.q + (row0 + node_of(r, group)) * a.stride + (size_t)(kh * group + head_of(r, group)) * hd, g, hd, f);
-  };
-  float f[Z][8];
-  if constexpr (!SHARED) query(r0 + m, f);
-  const Share s = share_of(a, b);
-  const int total = s.count * group;
-  if constexpr (!SHARED)  // (asked for above, with the lengths, and not where they are first used)
-#pragma unroll
-    for (int c = 0; c < Z; c++)
-#pragma unroll
-      for (int e = 0; e < 8; e++) asm volatile("" : "+v"(f[c][e]));
-  if (split >= s.used || r0 >= total) return;
-  const int end = a.splits > 1 ? min((split + 1) * a.per, s.tiles) : s.tiles, start = split * a.per, cached = min(end, s.cached);
-  const int slot = a.pages.shift - 5;
+  end = min(end, s.tiles);
+  const int cached = min(end, s.cached), slot = a.pages.shift - 5;
   // (nothing writes the table meanwhile: its numbers by scalar loads)
   typedef const __attribute__((address_space(4))) int32_t *Table;
   const Table table = (Table)(uintptr_t)(a.pages.table + (size_t)b * a.pages.table_stride);
@@ -218,7 +285,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 && (QP == 1 || Z < 4) ? 4 : 2) 
   if constexpr (SHARED) {
     for (int t = ki; t < QT; t += a.kw) {
       half8 x[Z][QP];
-      query(r0 + 16 * t + m, f);
+      load_rows<T, Z>(a, b, kh, r0 + 16 * t + m, g, f);
       const float y = taken(r0 + 16 * t + m, x);
       if (g == 0) cfs[16 * t + m] = y;
 #pragma unroll
@@ -226,7 +293,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 && (QP == 1 || Z < 4) ? 4 : 2) 
 #pragma unroll
         for (int part = 0; part < QP; part++) qs[((t * Z + c) * QP + part) * 64 + lane] = x[c][part];
     }
-    __syncthreads();
+    meet();
     if constexpr (QP == 2)
 #pragma unroll
       for (int t = 0; t < QT; t++) cf[t] = cfs[16 * t + m];
@@ -333,7 +400,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 && (QP == 1 || Z < 4) ? 4 : 2) 
     // (matrix instructions of a word among the vector ones that open the next)
     auto open_k = [&](int i) {
       half8 k = w.open(w.k[i]);
-      if constexpr (OPEN) k *= (half8)w.kd[i / 2][i % 2];
+      if constexpr (OPEN) k *= (half8)__builtin_bit_cast(_Float16, w.kd[i / 2].u[i % 2]);
       return k;
     };
     // (and queries asked for when the chunk before them is done)
@@ -536,7 +603,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 && (QP == 1 || Z < 4) ? 4 : 2) 
   int waves = a.kw;
   floatx4 *merge = (floatx4 *)smem;                             // [wave][...][lane]
   float *ml = (float *)(merge + min(waves, FIT) * SLOT);  // [wave][t][maxima, sums][row]
-  if constexpr (SHARED) __syncthreads();
+  if constexpr (SHARED) meet();
   if constexpr (FIT < WAVES)
     for (; waves > FIT; waves /= 2) {
       const int half = waves / 2;
@@ -548,7 +615,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 && (QP == 1 || Z < 4) ? 4 : 2) 
           for (int x = 0; x < 2 * Z; x++) merge[(ki - half) * SLOT + (t * 2 * Z + x) * 64 + lane] = acc[t][x];
         }
       }
-      __syncthreads();
+      meet();
       if (ki < half) {
 #pragma unroll
         for (int t = 0; t < QT; t++) {
@@ -559,7 +626,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 && (QP == 1 || Z < 4) ? 4 : 2) 
           for (int x = 0; x < 2 * Z; x++) acc[t][x] = acc[t][x] * y + merge[ki * SLOT + (t * 2 * Z + x) * 64 + lane] * z;
         }
       }
-      __syncthreads();
+      meet();
     }
   if (ki < waves) {
 #pragma unroll
@@ -573,7 +640,7 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 && (QP == 1 || Z < 4) ? 4 : 2) 
               floatx4{acc[t][2 * c][2 * h], acc[t][2 * c + 1][2 * h], acc[t][2 * c][2 * h + 1], acc[t][2 * c + 1][2 * h + 1]};
     }
   }
-  __syncthreads();
+  meet();
   for (int x = ki; x < QT * Z * 2; x += a.kw) {
     const int t = x / (2 * Z), c = x / 2 % Z, d = 32 * c + 8 * g + 4 * (x % 2), r = r0 + 16 * t + m;
     if (r >= total) continue;
@@ -599,10 +666,10 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 && (QP == 1 || Z < 4) ? 4 : 2) 
     }
     const int i = node_of(r, group), head = kh * group + head_of(r, group);
     const size_t out = ((row0 + i) * a.heads + head) * hd + d;
-    if (s.used > 1) {
-      const size_t part = (size_t)split * a.batch * a.rows * a.heads;
-      if (d == 0) *(floatx4 *)(a.pml + 4 * (part + (row0 + i) * a.heads + head)) = floatx4{top, l, scale, 0.0f};
-      *(floatx4 *)(a.po + part * hd + out) = o;
+    if (part >= 0) {
+      const size_t row = (size_t)part * 16 * QT + 16 * t + m;
+      if (d == 0) *(floatx4 *)(a.pml + 4 * row) = floatx4{top, l, scale, 0.0f};
+      *(floatx4 *)(a.po + row * hd + d) = o;
       continue;
     }
     o *= l == 0.0f ? 0.0f : 1.0f / l;
@@ -611,26 +678,78 @@ __global__ __launch_bounds__(64 * WAVES, QT == 1 && (QP == 1 || Z < 4) ? 4 : 2) 
   }
 }
 
-// The splits of a row's head joined, a lane per four values, 32 lanes a head.
+// EVEN: the workgroups take runs of all the tiles, of the same length, whatever sequences' they are.
+template <int Z, int QT, int QP, bool P16, bool Q4, bool EVEN>
+__global__ __launch_bounds__(64 * WAVES, QT == 1 && (QP == 1 || Z < 4) ? 4 : 2) void page_attend_kernel(PageAttendArgs a) {
+  typedef typename std::conditional<QP == 2, float, _Float16>::type T;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const int g = threadIdx.x >> 4 & 3, m = threadIdx.x & 15, group = a.heads / a.pages.kv_heads;
+  float f[Z][8];
+  if constexpr (EVEN) {
+    __shared__ EvenLds lds;
+    Even even(a, lds, 16 * QT);
+    const uint32_t last = min((blockIdx.y + 1) * even.per, even.all);
+    const int kh = blockIdx.x;
+    for (uint32_t place = blockIdx.y * even.per; place < last;) {
+      int b;
+      Share s;
+      uint32_t first;
+      even.find(place, b, s, first);
+      const uint32_t tiles = Even::tiles_of(s), block = (place - first) / tiles;
+      first += block * tiles;
+      const int r0 = 16 * QT * block, start = max((int)(place - first) - START, 0), end = (int)min(tiles, last - first) - START;
+      place = first + tiles;
+      if (end <= start) continue;
+      if constexpr (QT == 1) load_rows<T, Z>(a, b, kh, r0 + m, g, f);
+      attend_part<Z, QT, QP, P16, Q4>(a, smem, b, kh, r0, s, start, end, start || place > last ? (int)(2 * (kh * a.even + blockIdx.y) + !start) : -1, f);
+      if (place < last) meet();
+    }
+  } else {
+    const int kh = blockIdx.x, b = a.row_blocks == 1 ? blockIdx.y : blockIdx.y / a.row_blocks, r0 = 16 * QT * (blockIdx.y - b * a.row_blocks);
+    if constexpr (QT == 1) load_rows<T, Z>(a, b, kh, r0 + m, g, f);  // (nothing is known of the lengths yet)
+    const Share s = share_of(a, b);
+    if constexpr (QT == 1)  // (asked for above, with the lengths, and not where they are first used)
+#pragma unroll
+      for (int c = 0; c < Z; c++)
+#pragma unroll
+        for (int e = 0; e < 8; e++) asm volatile("" : "+v"(f[c][e]));
+    if (r0 < s.count * group) attend_part<Z, QT, QP, P16, Q4>(a, smem, b, kh, r0, s, 0, s.tiles, -1, f);
+  }
+}
+
+// The parts of a block of rows joined, where it has several: 8 rows a workgroup, four values a thread.
 __global__ __launch_bounds__(256) void page_join_kernel(PageAttendArgs a) {
-  const int hd = a.pages.hd;
-  const size_t unit = (size_t)blockIdx.x * 8 + threadIdx.x / 32, heads = (size_t)a.batch * a.rows * a.heads;
-  const int d = 4 * (threadIdx.x % 32);
-  if (unit >= heads || d >= hd) return;
-  const int row = unit / a.heads, b = row / a.rows, i = row - b * a.rows;
-  const Share s = share_of(a, b);
-  if (i >= s.count || s.used == 1) return;
+  __shared__ EvenLds lds;
+  const int hd = a.pages.hd, group = a.heads / a.pages.kv_heads, rows = 16 * a.qt;
+  Even even(a, lds, rows);
+  const int unit = blockIdx.x, rb = unit % a.row_blocks, kh = unit / a.row_blocks % a.pages.kv_heads, b = unit / a.row_blocks / a.pages.kv_heads;
+  while (b >= even.b0 + 64) even.next();
+  const Share s = share_of(a, lds.n[b - even.b0], lds.count[b - even.b0]);
+  const int blocks = even.blocks_of(s), local = 8 * blockIdx.y + threadIdx.x / 32, d = 4 * (threadIdx.x % 32), r = rows * rb + local;
+  if (rb >= blocks || r >= s.count * group || d >= hd) return;
+  const uint32_t tiles = Even::tiles_of(s), first = even.before + (b > even.b0 ? lds.sum[b - even.b0 - 1] : 0u) + (uint32_t)rb * tiles;
+  const int w0 = (first + START) / even.per, w1 = (first + tiles - 1) / even.per;
+  if (w0 == w1) return;
+  auto at = [&](int w) { return (size_t)(2 * (kh * a.even + w) + (w == w0)) * rows + local; };
   float top = -INFINITY, l = 0.0f;
   floatx4 o{};
-  for (int k = 0; k < s.used; k++) top = fmaxf(top, a.pml[4 * (k * heads + unit)]);
-  for (int k = 0; k < s.used; k++) {
-    const floatx4 x = *(const floatx4 *)(a.pml + 4 * (k * heads + unit));
-    const float w = x[0] == top ? 1.0f : __builtin_amdgcn_exp2f((x[0] - top) * x[2]);
-    l += w * x[1], o += w * *(const floatx4 *)(a.po + (k * heads + unit) * hd + d);
+  for (int w = w0; w <= w1; w += 4) {
+    // (four parts at a time; those past the last: the last, not counted)
+    floatx4 y[4], x[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) y[i] = *(const floatx4 *)(a.pml + 4 * at(min(w + i, w1))), x[i] = *(const floatx4 *)(a.po + at(min(w + i, w1)) * hd + d);
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      if (w + i > w1) break;
+      const float more = fmaxf(top, y[i][0]), u = top == more ? 1.0f : __builtin_amdgcn_exp2f((top - more) * y[i][2]);
+      const float v = y[i][0] == more ? 1.0f : __builtin_amdgcn_exp2f((y[i][0] - more) * y[i][2]);
+      l = l * u + y[i][1] * v, o = o * u + x[i] * v, top = more;
+    }
   }
   o *= l == 0.0f ? 0.0f : 1.0f / l;
-  if (a.out16) *(u32x2_a4 *)((_Float16 *)a.o + unit * hd + d) = u32x2{pack2(o[0], o[1]), pack2(o[2], o[3])};
-  else *(floatx4_a4 *)((float *)a.o + unit * hd + d) = o;
+  const size_t out = (((size_t)b * a.rows + node_of(r, group)) * a.heads + kh * group + head_of(r, group)) * hd + d;
+  if (a.out16) *(u32x2_a4 *)((_Float16 *)a.o + out) = u32x2{pack2(o[0], o[1]), pack2(o[2], o[3])};
+  else *(floatx4_a4 *)((float *)a.o + out) = o;
 }
 
 template <int Z, int QT, int QP, bool P16, bool Q4>
@@ -639,7 +758,8 @@ int attend_launch(wh_ctx *ctx, const PageAttendArgs &a) {
   ProfScope prof(ctx, "page_attend", 4.0 * keys * a.rows * a.heads * a.pages.hd, keys * a.pages.kv_heads * a.pages.hd * (Q4 ? 1.125 : 4.0));
   const size_t join = (size_t)std::min(a.kw, JOIN_LDS / (QT * Z * 2048)) * QT * (Z * 2048 + 128), queries = QT > 1 ? QT * (Z * QP * 1024 + 64) : 0;
   const size_t shm = std::max(join, queries);
-  wh_launch(ctx, (page_attend_kernel<Z, QT, QP, P16, Q4>), dim3(a.pages.kv_heads, a.batch * a.row_blocks, a.splits), 64 * a.kw, shm, a);
+  if (a.even) wh_launch(ctx, (page_attend_kernel<Z, QT, QP, P16, Q4, true>), dim3(a.pages.kv_heads, a.even), 64 * a.kw, shm, a);
+  else wh_launch(ctx, (page_attend_kernel<Z, QT, QP, P16, Q4, false>), dim3(a.pages.kv_heads, a.batch * a.row_blocks), 64 * a.kw, shm, a);
   return wh_launched(ctx, "page attention");
 }
 template <int Z, int QP, bool P16, bool Q4>
@@ -678,37 +798,33 @@ int launch_page_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
   if (((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)o) % 4 || (in16 && stride % 2))
     return wh_fail(ctx, WH_EARG, "page attention: buffers and rows must be 4-byte aligned");
   PageAttendArgs a{q, k, v, stride, pages_of(p), o, out16 != 0, t->n, t->count, t->mask, t->mask_stride, t->batch, t->rows, (t->rows + 31) / 32,
-                   heads, 1.0f / sqrtf((float)p->hd), 1, 1, 1, 1, nullptr, nullptr};
+                   heads, 1.0f / sqrtf((float)p->hd), 1, 1, 1, 0, 0, nullptr, nullptr};
   const int rows = (t->rows * (heads / p->kv_heads) + 15) / 16, most = p->type == WH_Q4_0 ? 4 : 2;  // tiles of 16
   a.row_blocks = (rows + most - 1) / most;
   const int qt = (rows + a.row_blocks - 1) / a.row_blocks;
-  a.row_blocks = (rows + qt - 1) / qt;
+  a.row_blocks = (rows + qt - 1) / qt, a.qt = qt;
   const int tiles = a.pages.room / TILE + (t->mask && k ? (t->rows + TILE - 1) / TILE : 0);
   while (2 * a.kw <= std::min(WAVES, tiles)) a.kw *= 2;
-  const size_t units = (size_t)t->batch * p->kv_heads * a.row_blocks;
+  if (const char *e = getenv("KW")) a.kw = atoi(e);
+  const size_t blocks = (size_t)t->batch * a.row_blocks, units = blocks * p->kv_heads, nodes = (size_t)t->batch * t->rows;
   const size_t cus = ctx->cus > 0 ? ctx->cus : 256;
-  const int least = 4 * a.kw;
-  if (tiles > 2 * least) {
-    const size_t slots = cus * (qt == 1 ? 2 : 1);
-    size_t best = SIZE_MAX;
-    for (int x = 1; x <= std::min(SPLITS, (tiles + least - 1) / least); x++) {
-      const size_t cost = (units * x + slots - 1) / slots * ((tiles + x - 1) / x + least);
-      if (cost < best) best = cost, a.splits = x;
-    }
+  if (tiles > 8 * a.kw && blocks * (tiles + START) < (size_t)1 << 31) {
+    a.even = (int)std::max<size_t>(cus * (qt == 1 ? 2 : 1) / p->kv_heads, 1);
+    a.least = START + a.kw;
+    if (const char *e = getenv("SPL")) a.even = atoi(e) * 64 / p->kv_heads;
+    if (const char *e = getenv("LEAST")) a.least = atoi(e);
   }
-  a.per = (tiles + a.splits - 1) / a.splits;
-  const size_t nodes = (size_t)t->batch * t->rows;
-  if ((size_t)t->batch * a.row_blocks > 65535 || units * a.splits >= (size_t)1 << 22 || nodes * heads >= (size_t)1 << 25)  // (a launch's limits)
+  if (blocks > 65535 || units >= (size_t)1 << 22 || nodes * heads >= (size_t)1 << 25)  // (a launch's limits)
     return wh_fail(ctx, WH_EARG, "page attention: %d heads of %zu nodes in one call", heads, nodes);
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "page attention: %s", hipGetErrorString(e));
-  if (a.splits > 1) {
-    const size_t part = (size_t)a.splits * nodes * heads;
-    if (!(a.po = (float *)wh_scratch(ctx, part * (p->hd + 4) * sizeof(float)))) return WH_EOOM;
-    a.pml = a.po + part * p->hd;
+  if (a.even) {
+    const size_t part_rows = (size_t)2 * a.even * p->kv_heads * 16 * qt;
+    if (!(a.po = (float *)wh_scratch(ctx, part_rows * (p->hd + 4) * sizeof(float)))) return WH_EOOM;
+    a.pml = a.po + part_rows * p->hd;
   }
   if (int rc = p->type == WH_Q4_0 ? attend_types<true>(ctx, a, in16, out16, qt) : attend_types<false>(ctx, a, in16, out16, qt)) return rc;
-  if (a.splits == 1) return WH_OK;
-  ProfScope prof(ctx, "page_attend_join", 0.0, 4.0 * nodes * heads * a.splits * (p->hd + 4));
-  wh_launch(ctx, page_join_kernel, (unsigned)((nodes * heads + 7) / 8), 256, 0, a);
+  if (!a.even) return WH_OK;
+  ProfScope prof(ctx, "page_attend_join", 0.0, 8.0 * a.even * p->kv_heads * 16 * qt * (p->hd + 4));
+  wh_launch(ctx, page_join_kernel, dim3((unsigned)units, 2 * qt), 256, 0, a);
   return wh_launched(ctx, "page attention's join");
 }

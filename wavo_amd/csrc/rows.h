@@ -65,6 +65,13 @@ __device__ __forceinline__ float not_finite(const T *p, int d, int hd) {
   return isfinite(x) ? 0.0f : x;
 }
 
+// A barrier for what is in LDS: loads from memory stay under way.
+__device__ __forceinline__ void meet() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 __device__ __forceinline__ floatx4 mfma(half8 a, half8 b, floatx4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }

@@ -76,13 +76,6 @@ __device__ __forceinline__ u32x2 read_tr(const uint32_t *p) {
                                        (__attribute__((address_space(3))) s16x4 *)(__attribute__((address_space(3))) void *)p));
 }
 
-// A barrier for what is in LDS: loads from memory stay under way.
-__device__ __forceinline__ void meet() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-  __builtin_amdgcn_s_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-}
-
 // Attention over a run of key blocks, for few rows.  A workgroup takes one key head of a sequence, 16 * QT of its rows
 // (the heads / kv_heads query heads of a node are rows next to each other) and one split of its key blocks
 // (64 positions for heads of up to 64 values, 32 for larger ones and of nodes), of which each of its kw wavefronts takes every
