@@ -316,38 +316,57 @@ __device__ __forceinline__ void attend_part(const PageAttendArgs &a, uint8_t *sm
 
   typedef float floatx8 __attribute__((ext_vector_type(8)));
   typedef typename std::conditional<P16, half8, floatx8>::type P;
-  // Scores st of a tile into weights p: exp2 against the running maximum, and their sum.  seen: the lane's positions.
-  auto weights = [&](floatx4 (&st)[2], int t, bool masked, uint32_t seen, P &p) {
+  // Scores st of a tile into weights p: exp2 against the running maxima, and their sums.  seen(t): the lane's positions.  All of
+  // the block's rows together, so that a branch parts them only once.
+  auto weights = [&](floatx4 (&st)[QT][2], bool masked, auto seen, P (&p)[QT]) {
     if (masked)
 #pragma unroll
-      for (int e = 0; e < 8; e++)
-        if (!(seen >> e & 1)) st[e >> 2][e & 3] = -INFINITY;
-    float top = st[0][0];
+      for (int t = 0; t < QT; t++) {
+        const uint32_t s = seen(t);
 #pragma unroll
-    for (int e = 1; e < 8; e++) top = fmaxf(top, st[e >> 2][e & 3]);
-    // The maximum is moved, for all of a row's lanes, where one of them has a score well past it: otherwise they need not meet.
-    const float c = factor(t);
-    float by = fminf(fmaf(-mx[t], c, digits), -LOWEST);
-    if (__any((far ? fmaf(top - mx[t], c, digits) : fmaf(top, c, by)) > digits + SLACK)) {
-      top = xlane::bit4(top, xlane::Max{});
-      top = fmaxf(xlane::bit5(top, xlane::Max{}), mx[t]);
-      const float old = __builtin_amdgcn_exp2f((mx[t] - top) * c);
-      sum[t] *= old;
+        for (int e = 0; e < 8; e++)
+          if (!(s >> e & 1)) st[t][e >> 2][e & 3] = -INFINITY;
+      }
+    float top[QT], by[QT];
+    bool past = false;
 #pragma unroll
-      for (int x = 0; x < 2 * Z; x++) acc[t][x] *= old;
-      mx[t] = top;
-      by = fminf(fmaf(-top, c, digits), -LOWEST);
-      far = far || __any(top != LOWEST && fabsf(by) > FAR);
+    for (int t = 0; t < QT; t++) {
+      top[t] = st[t][0][0];
+#pragma unroll
+      for (int e = 1; e < 8; e++) top[t] = fmaxf(top[t], st[t][e >> 2][e & 3]);
+      by[t] = fminf(fmaf(-mx[t], factor(t), digits), -LOWEST);
+      past |= fmaf(top[t], factor(t), by[t]) > digits + SLACK;
     }
-    if (far) st[0] -= mx[t], st[1] -= mx[t], by = digits;
+    // A maximum is moved, for all of a row's lanes, where one of them has a score well past it: otherwise they need not meet.
+    if (far || __any(past)) {
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      const float p0 = __builtin_amdgcn_exp2f(fmaf(st[e >> 2][e & 3], c, by));
-      const float p1 = __builtin_amdgcn_exp2f(fmaf(st[e >> 2][e + 1 & 3], c, by));
-      sum[t] += p0, sum[t] += p1;
-      if constexpr (P16) weights2<true>(p0, p1, p, p, e);
-      else p[e] = p0, p[e + 1] = p1;
+      for (int t = 0; t < QT; t++) {
+        const float c = factor(t);
+        if (!__any(fmaf(top[t] - mx[t], c, digits) > digits + SLACK)) continue;
+        top[t] = xlane::bit4(top[t], xlane::Max{});
+        top[t] = fmaxf(xlane::bit5(top[t], xlane::Max{}), mx[t]);
+        const float old = __builtin_amdgcn_exp2f((mx[t] - top[t]) * c);
+        sum[t] *= old;
+#pragma unroll
+        for (int x = 0; x < 2 * Z; x++) acc[t][x] *= old;
+        mx[t] = top[t];
+        by[t] = fminf(fmaf(-top[t], c, digits), -LOWEST);
+        far = far || __any(top[t] != LOWEST && fabsf(by[t]) > FAR);
+      }
+      if (far)
+#pragma unroll
+        for (int t = 0; t < QT; t++) st[t][0] -= mx[t], st[t][1] -= mx[t], by[t] = digits;
     }
+#pragma unroll
+    for (int t = 0; t < QT; t++)
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(st[t][e >> 2][e & 3], factor(t), by[t]));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(st[t][e >> 2][e + 1 & 3], factor(t), by[t]));
+        sum[t] += p0, sum[t] += p1;
+        if constexpr (P16) weights2<true>(p0, p1, p[t], p[t], e);
+        else p[t][e] = p0, p[t][e + 1] = p1;
+      }
   };
   // p times a chunk's factors as an operand, and (unless P16) what that leaves of them.
   auto operand = [&](const P &p, const half8 *d, half8 &h, half8 &l) {
@@ -454,11 +473,7 @@ __device__ __forceinline__ void attend_part(const PageAttendArgs &a, uint8_t *sm
     }
     room();
     P p[QT];
-#pragma unroll
-    for (int t = 0; t < QT; t++) {
-      if constexpr (QT > 1) __builtin_amdgcn_sched_barrier(0);
-      weights(st[t], t, left < TILE, seen, p[t]);
-    }
+    weights(st, left < TILE, [&](int) { return seen; }, p);
     auto open_v = [&](int i) {
       half8 v = w.open(w.v[i]);
       if constexpr (OPEN) v *= w.vd[i / 2];
@@ -528,11 +543,10 @@ __device__ __forceinline__ void attend_part(const PageAttendArgs &a, uint8_t *sm
       }
     }
     P p[QT];
-#pragma unroll
-    for (int t = 0; t < QT; t++) {
+    weights(st, true, [&](int t) {
       const uint32_t sees = there & mask_of(t, j0 / 32);
-      weights(st[t], t, true, (sees >> 4 * g & 15) | (sees >> (16 + 4 * g) & 15) << 4, p[t]);
-    }
+      return (sees >> 4 * g & 15) | (sees >> (16 + 4 * g) & 15) << 4;
+    }, p);
 #pragma unroll
     for (int c = 0; c < Z; c++) {
       // Values of nodes that are not there are zeroed, and so are those that are no finite numbers: they must not meet the zero
@@ -805,14 +819,11 @@ int launch_page_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
   a.row_blocks = (rows + qt - 1) / qt, a.qt = qt;
   const int tiles = a.pages.room / TILE + (t->mask && k ? (t->rows + TILE - 1) / TILE : 0);
   while (2 * a.kw <= std::min(WAVES, tiles)) a.kw *= 2;
-  if (const char *e = getenv("KW")) a.kw = atoi(e);
   const size_t blocks = (size_t)t->batch * a.row_blocks, units = blocks * p->kv_heads, nodes = (size_t)t->batch * t->rows;
   const size_t cus = ctx->cus > 0 ? ctx->cus : 256;
   if (tiles > 8 * a.kw && blocks * (tiles + START) < (size_t)1 << 31) {
     a.even = (int)std::max<size_t>(cus * (qt == 1 ? 2 : 1) / p->kv_heads, 1);
     a.least = START + a.kw;
-    if (const char *e = getenv("SPL")) a.even = atoi(e) * 64 / p->kv_heads;
-    if (const char *e = getenv("LEAST")) a.least = atoi(e);
   }
   if (blocks > 65535 || units >= (size_t)1 << 22 || nodes * heads >= (size_t)1 << 25)  // (a launch's limits)
     return wh_fail(ctx, WH_EARG, "page attention: %d heads of %zu nodes in one call", heads, nodes);
