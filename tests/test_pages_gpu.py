@@ -428,9 +428,12 @@ def attend(gpu, cache, x, heads, n, count=None, seen=None, out16=False, nodes=Tr
 
 def check_attend(got, cache, x, heads, n, count=None, seen=None, nodes=True, before=7.0):
     """Softmax over the positions of pages that are there and the seen nodes, row by row, with a worst case of its error: that of
-    caches that are not in pages, and, of p * d in two f16 parts or (f16 rows and outputs) p and p * d rounded to f16: 2^-11
+    caches that are not in pages, and, of p * d in two f16 parts or (f16 rows and outputs) p and V (of 4 bits) rounded to f16: 2^-11
     each of the values' size, and 2^-25 at most where they are subnormal, of weights whose largest is at least 2^10 (less the
-    power of two of V's largest factor, which is below the largest value)."""
+    power of two of V's largest factor, which is below the largest value).
+    Where V of 4 bits is so rounded, K is too: each of its values is off by 2^-11 of itself, or 2^-25, so a score is off by at most
+    D = max_j sum |q| (2^-11 |k| + 2^-25) / sqrt(hd), a weight by a factor between e^-D and e^D beside the sum that is off by the
+    same, and the mean of the values by (e^2D - 1) max|v|; V's 2^-25 stands where p's did."""
     batch, rows = x.shape[:2]
     hd, g, room = cache.hd, cache.kv_heads, cache.cols * cache.page
     p16 = got.dtype == np.float16 and x.dtype == np.float16
@@ -457,6 +460,8 @@ def check_attend(got, cache, x, heads, n, count=None, seen=None, nodes=True, bef
                 tol = attend_tolerance(q, kk, vv, hd) + len(both) * 2.0**-32 * max(1, size)
                 if p16:
                     tol += (2 * EPS16 + EPS16**2 + len(both) * 2.0**-35 * max(1, size)) * size
+                    if cache.type == wa.Q4_0:
+                        tol += np.expm1(2 * np.max(np.abs(q) @ (EPS16 * np.abs(kk) + 2.0**-25).T) / np.sqrt(hd)) * size + 2.0**-25
                 if got.dtype == np.float16:
                     tol = tol + EPS16 * np.abs(want) + 2.0**-25
                 err = np.abs(row - want)
@@ -555,6 +560,82 @@ def test_attend_long_caches_in_splits(gpu, type, in16):
     x[..., :heads * hd] *= 3
     _, seen = trees(rng, batch, rows)
     check_attend(attend(gpu, cache, x, heads, n, [2, 0, 1], seen, in16), cache, x, heads, n, [2, 0, 1], seen)
+
+
+@pytest.mark.parametrize("type", [wa.Q4_0, wa.F16])
+@pytest.mark.parametrize("in16,out16", [(False, False), (True, True), (True, False)])
+@pytest.mark.parametrize("heads,kv_heads,hd,rows", [(2, 1, 64, 33), (3, 3, 32, 20), (2, 1, 96, 30), (2, 2, 128, 64), (6, 2, 128, 5)])
+def test_attend_long_caches_shared_out(gpu, type, in16, out16, heads, kv_heads, hd, rows):
+    """Blocks of all sizes over tables that are shared out: sequences of nothing, of little, of no nodes, pages that are not there."""
+    rng = np.random.default_rng(heads + hd + rows)
+    batch, page, cols = 6, 256, 9
+    cache = Cache(rng, type, page, kv_heads, hd, batch, cols)
+    n, count = [cols * page, 0, 1500, 700, 33, 2000], [rows, rows, (rows + 1) // 2, 0, 1, rows]
+    cache.table[0, [0, 3, 4, 8]] = -1
+    cache.table[5] = cache.pages
+    cache.fill(rng, n)
+    x = rows_of(rng, batch, rows, heads, kv_heads, hd, in16, 2)
+    x[..., :heads * hd] *= 2
+    _, seen = trees(rng, batch, rows)
+    seen[0, rows // 2] = False
+    check_attend(attend(gpu, cache, x, heads, n, count, seen, out16), cache, x, heads, n, count, seen)
+    got = attend(gpu, cache, x, heads, n, count, None, out16, nodes=False)
+    assert np.all(got[5] == 0)
+    check_attend(got, cache, x, heads, n, count, None, nodes=False)
+
+
+@pytest.mark.parametrize("type", [wa.Q4_0, wa.F16])
+@pytest.mark.parametrize("batch,few", [(64, False), (65, False), (150, False), (200, True)])
+def test_attend_many_sequences_shared_out(gpu, type, batch, few):
+    """More sequences than are looked at together; those with something to do few and far between."""
+    rng = np.random.default_rng(batch)
+    rows, heads, g, hd, page, cols = 3, 2, 1, 32, 128, 18
+    cache = Cache(rng, type, page, g, hd, batch, cols, shared=True)
+    n = np.where(rng.random(batch) < 0.7, rng.integers(0, 100, batch), rng.integers(0, cols * page + 1, batch))
+    count = np.where(rng.random(batch) < (0.02 if few else 0.7), rng.integers(1, rows + 1, batch), 0)
+    count[-1] = 2
+    cache.fill(rng, [cols * page])
+    x = rows_of(rng, batch, rows, heads, g, hd, True)
+    _, seen = trees(rng, batch, rows)
+    check_attend(attend(gpu, cache, x, heads, n, count, seen, True), cache, x, heads, n, count, seen)
+    none = attend(gpu, cache, x, heads, n, np.zeros(batch), seen, True)
+    assert np.all(none == 7)
+
+
+def test_attend_recorded_passes_share_the_scratch(gpu):
+    """Two passes whose parts overlap in the scratch, replayed in turn with other lengths, and eager work between."""
+    rng = np.random.default_rng(26)
+    sets = []
+    for type, batch, rows, heads, g, hd in ((wa.Q4_0, 3, 5, 4, 2, 64), (wa.F16, 2, 40, 2, 1, 128)):
+        cache = Cache(rng, type, 256, g, hd, batch, 10)
+        cache.fill(rng, [2560] * batch)
+        pages, n = cache.device(gpu), gpu.upload(np.array([2500] * batch, np.int32))
+        x, mask = gpu.upload(rows_of(rng, batch, rows, heads, g, hd, False)), gpu.upload(bits(trees(rng, batch, rows)[1]))
+        o, t = gpu.buffer(batch * rows * heads * hd), wa.Tree(batch, rows, n, None, None, mask, rows * ((rows + 31) // 32))
+
+        def call(t=t, x=x, pages=pages, o=o, heads=heads, g=g, hd=hd):
+            gpu.page_attend(t, x, x.ptr + 4 * heads * hd, x.ptr + 4 * (heads + g) * hd, (heads + 2 * g) * hd, pages, o, heads)
+
+        sets.append((call, n, batch, o, batch * rows * heads * hd, cache, mask))
+    for s in sets:
+        s[0]()
+    passes = []
+    for s in sets:
+        gpu.record_begin()
+        s[0]()
+        passes.append(gpu.record_end())
+    for turn in range(4):
+        for (call, n, batch, o, size, *_), p in zip(sets, passes):
+            gpu.write(n, np.array([2560 - 640 * turn, 100][:batch] + [7] * (batch - 2), np.int32))
+            call()
+            want = gpu.read(o, (size,))
+            gpu.zero(o)
+            p.replay()
+            if turn % 2:
+                sets[0][0]()
+            assert np.array_equal(gpu.read(o, (size,)), want)
+    for p in passes:
+        p.free()
 
 
 @pytest.mark.parametrize("in16", [False, True])
@@ -826,3 +907,121 @@ def test_sampled_tokens_have_the_targets_distribution(gpu, drafts):
     got = sample(gpu, p, q if drafts else None, tokens, rng.random((batch, rows)).astype(np.float32), vocab, bits(seen))
     share = np.bincount(got[:, 0], minlength=vocab) / batch
     assert np.all(np.abs(share - p[0, 0]) <= 5 * np.sqrt(p[0, 0] * (1 - p[0, 0]) / batch)), share
+
+
+# ------------------------------------------------------------------------------------------- all of them
+
+
+class Sampler:
+    """A decoder of two attention layers whose caches lie in pages: embeddings, [q | k | v] projections, norms and rotation,
+    attention, output projections, logits, their rules and probabilities, verification, and the kept path into the pages."""
+
+    def __init__(self, gpu, type, batch, rows, temperature, heads=4, kv_heads=2, hd=32, vocab=160, page=32, cols=4, layers=2, seed=0):
+        rng = np.random.default_rng(seed)
+        self.gpu, self.batch, self.rows, self.heads, self.kv_heads, self.hd = gpu, batch, rows, heads, kv_heads, hd
+        self.vocab, self.layers, self.room = vocab, layers, page * cols
+        d, dk, m = heads * hd, kv_heads * hd, batch * rows
+        self.d, self.dk, self.stride = d, dk, d + 2 * dk
+        lin = lambda n, k, s: gpu.linear([((s * rng.standard_normal((n, k))).astype(np.float32).tobytes(), wa.F32, k, n)])  # noqa: E731
+        up = lambda a, t: gpu.upload(np.asarray(a, t))  # noqa: E731
+        self.embed, self.none = lin(vocab, d, 1.0), up(np.zeros(d), np.float32)
+        self.qkv = [lin(self.stride, d, 2.0 / np.sqrt(d)) for _ in range(layers)]
+        self.proj = [lin(d, d, 1.0 / np.sqrt(d)) for _ in range(layers)]
+        self.head = lin(vocab, d, 3.0 / np.sqrt(d))
+        gains = [up(1.5 + 0.2 * rng.standard_normal(hd), np.float32) for _ in range(2)]
+        self.table = up(rope_table(self.room, hd), np.float32)
+        self.norms = wa.Heads(heads, kv_heads, hd, gains[0], gains[1], 1e-6, self.table, self.room, hd)
+        pages = batch * cols + 1
+        self.pages = []
+        for _ in range(layers):
+            pool = gpu.upload(rng.integers(0, 2**32, (pages, wa.page_bytes(type, page, kv_heads, hd) // 4), dtype=np.uint32))
+            self.pages.append(wa.Pages(pool, pages, up(rng.permutation(pages)[:batch * cols], np.int32), cols, cols, page, type, kv_heads, hd))
+        self.x, self.raw = gpu.buffer(m * d), [gpu.buffer(m * self.stride) for _ in range(layers)]
+        self.turned, self.o, self.logits, self.probs = gpu.buffer(m * self.stride), gpu.buffer(m * d), gpu.buffer(m * vocab), gpu.buffer(m * vocab)
+        z = lambda *s: up(np.zeros(s), np.int32)  # noqa: E731
+        self.n, self.n1, self.count, self.tokens, self.mask = z(batch), z(batch), z(batch), z(batch, rows), z(batch, rows, (rows + 31) // 32)
+        self.pick, self.path, self.kept, self.next, self.history = z(batch, rows), z(batch, rows), z(batch), z(batch), z(batch, self.room)
+        self.penalty, self.temperature = up([[1.2, 0.1, 0.05]] * batch, np.float32), up([temperature] * batch, np.float32)
+        self.u, self.q = gpu.buffer(m), gpu.buffer(m * vocab)
+        self.draws = temperature > 0
+
+    def tree(self):
+        return wa.Tree(self.batch, self.rows, self.n, self.count, self.tokens, self.mask, self.rows * ((self.rows + 31) // 32))
+
+    def step(self):
+        g, m, t, rules = self.gpu, self.batch * self.rows, self.tree(), wa.Rules(self.penalty, self.history, self.room)
+        for r in range(m):
+            g.embed(self.embed, self.none, self.x.ptr + 4 * r * self.d, self.tokens, r, 0)
+        for l in range(self.layers):
+            g.gemm(self.x, self.qkv[l], self.raw[l], m, wa.BIAS)
+            g.head_norm(t, self.norms, self.raw[l], self.stride, self.turned, self.stride)
+            g.page_attend(t, self.turned, self.turned.ptr + 4 * self.d, self.turned.ptr + 4 * (self.d + self.dk), self.stride, self.pages[l], self.o,
+                          self.heads)
+            g.gemm(self.o, self.proj[l], self.x, m, wa.RESIDUAL, 1.0)
+        g.gemm(self.x, self.head, self.logits, m, wa.BIAS)
+        g.logit_rules(t, rules, self.logits, self.logits, self.vocab, self.vocab)
+        g.logit_probs(t, self.logits, self.probs, self.vocab, self.vocab, self.vocab, self.temperature)
+        g.tree_sample(t, self.probs, self.q if self.draws else None, self.vocab, self.vocab, self.u, self.pick)
+        g.tree_accept(t, self.pick, None, None, 0, 0, None, 0, 0, 0, self.room, 0, self.path, self.kept, self.next, self.n1, self.history, self.room)
+        for l in range(self.layers):
+            k = self.raw[l].ptr + 4 * self.d
+            g.page_append(t, self.norms, None, k, k + 4 * self.dk, self.stride, self.pages[l], self.path, self.kept)
+        g.copy(self.n, self.n1, 4 * self.batch)
+
+    def generate(self, rng, want, drafts=None, record=False):
+        """Texts of `want` tokens, with draft trees of right (from `drafts`) and wrong tokens, or of those drawn from random rows."""
+        g, batch, rows, vocab = self.gpu, self.batch, self.rows, self.vocab
+        g.write(self.n, np.zeros(batch, np.int32))
+        root, text = np.arange(batch) + 20, [[] for _ in range(batch)]
+        steps, recorded = 0, None
+        while min(len(x) for x in text) < want:
+            parents, seen = trees(rng, batch, rows, 4)
+            tokens, count, depth = np.zeros((batch, rows), np.uint32), np.zeros(batch, np.int32), seen.sum(2) - 1
+            q = softmax(3 * rng.standard_normal((batch, rows, vocab)))
+            for b in range(batch):
+                tokens[b, 0], count[b] = root[b], 0 if len(text[b]) >= want else rng.integers((rows + 1) // 2, rows + 1)
+                for i in range(1, rows):
+                    at = len(text[b]) + depth[b, i]
+                    c = np.cumsum(q[b, parents[b, i]].astype(np.float64))
+                    x = min(np.searchsorted(c, rng.random() * c[-1]), vocab - 1)
+                    tokens[b, i] = drafts[b][at] if drafts is not None and at < len(drafts[b]) and rng.random() < 0.6 else x
+            g.write(self.tokens, tokens)
+            g.write(self.count, count)
+            g.write(self.mask, bits(seen))
+            g.write(self.u, rng.random((batch, rows)).astype(np.float32))
+            g.write(self.q, q)
+            if record and steps == 1:
+                g.record_begin()
+                self.step()
+                recorded = g.record_end()
+            if recorded is None:
+                self.step()
+            else:
+                recorded.replay()
+            kept, path, nxt = g.read(self.kept, (batch,), np.int32), g.read(self.path, (batch, rows), np.int32), g.read(self.next, (batch,), np.uint32)
+            for b in range(batch):
+                text[b] += [int(tokens[b, i]) for i in path[b, :kept[b]]]
+                if count[b]:
+                    root[b] = nxt[b]
+            steps += 1
+        assert np.array_equal(g.read(self.n, (batch,), np.int32), [len(x) for x in text])
+        return [x[:want] for x in text], steps
+
+
+@pytest.mark.parametrize("record", [False, True])
+def test_drafted_decoding_over_pages_gives_the_same_tokens(gpu, record):
+    """At temperature zero, over pages of f16: trees of drafts, right and wrong ones, against one token per step.  The two differ by
+    rounding alone (rows of other batch sizes, f32 norms for 64 bits'), so the seed's texts have no ties at that level."""
+    want, _ = Sampler(gpu, wa.F16, 3, 1, 0.0).generate(np.random.default_rng(1), 40)
+    got, steps = Sampler(gpu, wa.F16, 3, 11, 0.0).generate(np.random.default_rng(2), 40, want, record)
+    assert got == want
+    assert steps < 30
+    assert len(set(want[0])) > 10
+
+
+@pytest.mark.parametrize("type", [wa.Q4_0, wa.F16])
+def test_sampled_decoding_over_pages_repeats_itself(gpu, type):
+    """The same random numbers and drafts: the same texts, recorded or not."""
+    texts = [Sampler(gpu, type, 3, 9, 0.8).generate(np.random.default_rng(3), 30, None, record)[0] for record in (False, False, True)]
+    assert texts[0] == texts[1] == texts[2]
+    assert len(set(texts[0][0])) > 10
