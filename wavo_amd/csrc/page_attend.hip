@@ -36,6 +36,11 @@ constexpr float LOWEST = -1e30f;     // the maximum of a row that has seen nothi
 constexpr int START = 24;
 constexpr int JOIN_LDS = 128 << 10;  // bytes in which wavefronts' results are joined
 
+// Whether a compute unit holds two workgroups: where a tile, its queries and outputs fit 128 registers.  (f16 pages of heads of
+// 128, one f16 row a key head, 32 sequences of 1000 to 8191: 112 us alone for 157 with registers spilled; f32 rows over 4 bits 53
+// for 60.)
+constexpr bool two_of(int z, int qt, bool half_rows, bool q4) { return qt == 1 && (q4 ? half_rows || z < 4 : z < 3); }
+
 // A sequence's tiles: the cache's, then the nodes'.
 struct Share {
   int n, count, cached, tiles;
@@ -694,7 +699,7 @@ __device__ __forceinline__ void attend_part(const PageAttendArgs &a, uint8_t *sm
 
 // EVEN: the workgroups take runs of all the tiles, of the same length, whatever sequences' they are.
 template <int Z, int QT, int QP, bool P16, bool Q4, bool EVEN>
-__global__ __launch_bounds__(64 * WAVES, QT == 1 && (QP == 1 || Z < 4) ? 4 : 2) void page_attend_kernel(PageAttendArgs a) {
+__global__ __launch_bounds__(64 * WAVES, two_of(Z, QT, QP == 1, Q4) ? 4 : 2) void page_attend_kernel(PageAttendArgs a) {
   typedef typename std::conditional<QP == 2, float, _Float16>::type T;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int g = threadIdx.x >> 4 & 3, m = threadIdx.x & 15, group = a.heads / a.pages.kv_heads;
@@ -778,7 +783,7 @@ int attend_launch(wh_ctx *ctx, const PageAttendArgs &a) {
 }
 template <int Z, int QP, bool P16, bool Q4>
 int attend_qt(wh_ctx *ctx, const PageAttendArgs &a, int qt) {
-  if constexpr (Q4) {
+  if constexpr (Q4 && P16) {
     if (qt == 4) return attend_launch<Z, 4, QP, P16, Q4>(ctx, a);
     if (qt == 3) return attend_launch<Z, 3, QP, P16, Q4>(ctx, a);
   }
@@ -813,7 +818,10 @@ int launch_page_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
     return wh_fail(ctx, WH_EARG, "page attention: buffers and rows must be 4-byte aligned");
   PageAttendArgs a{q, k, v, stride, pages_of(p), o, out16 != 0, t->n, t->count, t->mask, t->mask_stride, t->batch, t->rows, (t->rows + 31) / 32,
                    heads, 1.0f / sqrtf((float)p->hd), 1, 1, 1, 0, 0, nullptr, nullptr};
-  const int rows = (t->rows * (heads / p->kv_heads) + 15) / 16, most = p->type == WH_Q4_0 ? 4 : 2;  // tiles of 16
+  // Rows in tiles of 16, evenly in blocks of `most` at most.  4 tiles read a nibble once for 64 rows: with 32 query heads over 8 of
+  // 128 and f16 throughout, 100 rows over 28 k positions take 129 us for 139 with 2 (48 for 46 over 7 k).  f32 weights and
+  // outputs leave registers for 2 (225 us for 364), and f16 pages have nothing to open (81 and 83 with 2 and 3).
+  const int rows = (t->rows * (heads / p->kv_heads) + 15) / 16, most = p->type == WH_Q4_0 && in16 && out16 ? 4 : 2;
   a.row_blocks = (rows + most - 1) / most;
   const int qt = (rows + a.row_blocks - 1) / a.row_blocks;
   a.row_blocks = (rows + qt - 1) / qt, a.qt = qt;
@@ -822,7 +830,7 @@ int launch_page_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
   const size_t blocks = (size_t)t->batch * a.row_blocks, units = blocks * p->kv_heads, nodes = (size_t)t->batch * t->rows;
   const size_t cus = ctx->cus > 0 ? ctx->cus : 256;
   if (tiles > 8 * a.kw && blocks * (tiles + START) < (size_t)1 << 31) {
-    a.even = (int)std::max<size_t>(cus * (qt == 1 ? 2 : 1) / p->kv_heads, 1);
+    a.even = (int)std::max<size_t>(cus * (two_of(p->hd / 32, qt, in16, p->type == WH_Q4_0) ? 2 : 1) / p->kv_heads, 1);
     a.least = START + a.kw;
   }
   if (blocks > 65535 || units >= (size_t)1 << 22 || nodes * heads >= (size_t)1 << 25)  // (a launch's limits)
