@@ -503,7 +503,7 @@ size_t wh_page_bytes(int type, int page, int kv_heads, int hd);
  * stores nothing).  Row r's keys and values are at k and v + r * stride values, f32 or (in16) f16.  With q and qo (not with a path) queries
  * are normed and rotated on the way, row r of q (the same stride) to qo + r * qo_stride, f32 or (out16) f16; qo may be q itself (same type
  * and stride) and otherwise overlaps nothing.  n_out[b] (or NULL) = n[b] + the positions that are there, n[b] at least; it is
- * not n.  The tree's mask and tokens are not read.  Nothing but those positions changes; a page belongs to one sequence of a call,
+ * none of n, count and kept.  The tree's mask and tokens are not read.  Nothing but those positions changes; a page belongs to one sequence of a call,
  * where it is stored to. */
 int wh_page_append(wh_ctx *ctx, const wh_tree *t, const wh_heads *heads, const void *q, const void *k, const void *v,
                    size_t stride, int in16, const int32_t *path, const int32_t *kept, const wh_pages *pages, void *qo,
@@ -514,21 +514,23 @@ int wh_page_append(wh_ctx *ctx, const wh_tree *t, const wh_heads *heads, const v
 int wh_page_read(wh_ctx *ctx, const wh_tree *t, const wh_pages *pages, void *k, void *v, size_t stride, int out16);
 
 /* wh_tree_attend over caches in pages: attention of every node over its sequence's positions j < n[b] in the pages and the
- * nodes that it sees, whose k and v (rows as there, already normed and rotated) are taken as f16.  Keys and values of 4 bits are taken as they stand,
- * without a rounding to f16 in between.  f32 queries are taken in two f16 parts and, for f32 outputs, so are the softmax weights times V's
- * factors, which leaves 2^-22 of them; with f16 rows and outputs both products are rounded to f16 (2^-11 each; the weights' sum stays
- * f32).  Masked keys and values may hold anything, and so may the rows past count[b], which are read; a row that sees a key or
- * value that is no finite number may get NaN.  o overlaps none of the inputs.  heads % kv_heads == 0, heads <= 1024, stride <= 2^23;
- * pointers 4-byte aligned (stride even for f16).  A workgroup takes 16 or 32 rows of a key head: batch times such blocks
- * <= 65535, that times kv_heads and the splits of a long cache < 2^22, and batch * rows * heads < 2^25.  Splits are planned from
- * the tables' size, whatever part of them is in use. */
+ * nodes that it sees, whose k and v (rows as there, already normed and rotated) are taken as f16.  f32 queries are taken in two f16
+ * parts, which leaves 2^-22 of them, and for f32 outputs so are the softmax weights (times V's factors, where it is of 4 bits), and
+ * keys and values of 4 bits as they stand.  With f16 rows and outputs weights are rounded to f16, and so are keys and values of 4
+ * bits (2^-11 of each, as a cache of f16 would hold them; the weights' sum stays f32).  Masked keys and values may hold anything, and so may
+ * the rows past count[b], which are read; a row that sees a key or value that is no finite number may get NaN.  o overlaps none of the
+ * inputs.  heads % kv_heads == 0, heads <= 1024, stride <= 2^23; pointers 4-byte aligned (stride even for f16).  The rows * heads /
+ * kv_heads rows of a sequence's key head are taken in blocks of 64 at most (of 32, but for f16 rows and outputs over 4 bits): batch
+ * times such blocks <= 65535, that times kv_heads < 2^22, and batch * rows * heads < 2^25.  Where a table holds more than 2048 positions, its nodes
+ * counted in, the tiles of all sequences are shared out evenly among the workgroups, from the lengths of their time, and a second
+ * launch joins the parts, in the context's scratch: such a call is made once before it is recorded. */
 int wh_page_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void *k, const void *v, size_t stride, int in16,
                    const wh_pages *pages, void *o, int out16, int heads);
 
 /* Probabilities of the rows of logits [batch * rows] (row r at r * ld values, f32 or (f16) f16, vocab values each; wh_logit_rules'
  * out): probs[r * probs_ld + x] = exp((l_x - max) / T) / their sum, in f32, T = temperature[b] (NULL: 1).  T <= 0 (or NaN): 1 for
  * the first maximum, 0 for the others.  A row with nothing left (minus infinity everywhere) gets zeros, one with NaN or plus infinity gets
- * NaN.  Rows past count[b] are not written, nor is anything past vocab; probs overlaps no input. */
+ * NaN.  Rows past count[b] are not written, nor is anything past vocab; probs overlaps no input.  batch * rows < 2^22. */
 int wh_logit_probs(wh_ctx *ctx, const wh_tree *t, const void *logits, size_t ld, int f16, int vocab, const float *temperature,
                    float *probs, size_t probs_ld);
 
@@ -543,7 +545,7 @@ int wh_logit_probs(wh_ctx *ctx, const wh_tree *t, const void *logits, size_t ld,
  * probs, where w has come to nothing).  All of it in 64 bits.  picks [batch * rows]: for the nodes on the walk the token after
  * them, 0xffffffff for the others and where probs has nothing: wh_tree_accept takes that walk and keeps it.  Rows of probs and drafts hold finite
  * numbers, none below zero; those off the walk may hold anything.  Tokens past vocab are passed over.  picks overlaps no input.
- * count[b] rows of picks are written. */
+ * count[b] rows of picks are written.  batch < 2^22. */
 int wh_tree_sample(wh_ctx *ctx, const wh_tree *t, const float *probs, const float *drafts, int vocab, size_t ld, const float *u,
                    uint32_t *picks);
 

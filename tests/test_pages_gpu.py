@@ -779,6 +779,14 @@ def test_probs_of_odd_rows(gpu):
     assert np.all(probs(gpu, l[:1], 1, 1, vocab, [0.0])[0] == 0)  # nothing left, greedily
 
 
+def test_probs_of_temperatures_without_end(gpu):
+    """All that is left alike, and nothing of what is not."""
+    l = np.float32(np.random.default_rng(2).standard_normal((3, 4100)))
+    l[:, 100:] = -np.inf
+    got = probs(gpu, l, 3, 1, 4100, [np.inf, 3e38, 1e30])
+    assert np.all(np.abs(got[:, :100] - 0.01) <= 0.01 * 2.0**-20) and np.all(got[:, 100:] == 0)
+
+
 # ------------------------------------------------------------------------------------------- verification
 
 

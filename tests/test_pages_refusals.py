@@ -129,6 +129,8 @@ int main() {
   append("odd f16 rows", "aligned", A { a.in16 = 1, a.stride = 513; });
   append("in place of another type", "place", A { a.y = (void *)a.x, a.in16 = 1; });
   append("lengths out in place", "n_out", A { a.n_out = (int32_t *)a.t.n; });
+  append("lengths out over counts", "n_out", A { a.n_out = at<int32_t>(16384), a.t.count = a.n_out; });
+  append("lengths out over what was kept", "n_out", A { a.kept = a.n_out; });
   append("rows past a launch", "one call", A { a.t.batch = 1 << 14, a.t.rows = 256, a.t.mask_stride = 0, a.h.heads = a.h.kv_heads = a.p.kv_heads = 1024, a.stride = 1024 * 64, a.y_stride = 1024 * 64; });
 
   read("no tree", "tree", A { a.tree = false; });
@@ -137,6 +139,7 @@ int main() {
   read("no values", "needed", A { a.v = nullptr; });
   read("rows too close", "apart", A { a.stride = 127; });
   read("odd f16 rows", "aligned", A { a.out16 = 1, a.stride = 129; });
+  read("rows past a launch", "one call", A { a.t.batch = 32768, a.t.rows = 128, a.t.mask_stride = 0, a.p.kv_heads = 410, a.stride = 410 * 64; });
   read("misaligned rows", "aligned", A { a.v = at<void>(M + 1); });
 
   attend("no tree", "tree", A { a.tree = false; });
@@ -165,6 +168,7 @@ int main() {
   probs("misaligned logits", "misaligned", A { a.logits = at<void>(4098); });
   probs("misaligned f16 logits", "misaligned", A { a.in16 = 1, a.logits = at<void>(4097); });
   probs("misaligned temperatures", "misaligned", A { a.temperature = at<float>(4098); });
+  probs("rows past a launch", "one call", A { a.t.batch = 1 << 22, a.t.rows = 1; });
 
   sample("no tree", "tree", A { a.tree = false; });
   sample("no probabilities", "needed", A { a.probs = nullptr; });
@@ -174,6 +178,7 @@ int main() {
   sample("no ids", "needed", A { a.vocab = 0; });
   sample("rows too close", "needed", A { a.ld = 999; });
   sample("misaligned drafts", "misaligned", A { a.drafts = at<float>(4098); });
+  sample("sequences past a launch", "one call", A { a.t.batch = 1 << 22, a.t.rows = 1; });
   sample("misaligned random numbers", "misaligned", A { a.u = at<float>(4097); });
   printf("%d calls, %d not refused\n", calls, bad);
   return bad != 0;

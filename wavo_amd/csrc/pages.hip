@@ -46,7 +46,7 @@ __device__ __forceinline__ void store4(void *y, size_t at, int out16, floatx4 f)
   else *(floatx4_a4 *)((float *)y + at) = f;
 }
 
-// The sum over a head's lanes, 1 << n of them next to each other.
+// The sum over a head's lanes: per of them next to each other, a power of two, 32 at most.
 __device__ __forceinline__ float head_sum(float v, int per) {
   if (per > 1) v += xlane::dpp<xlane::XOR1>(v);
   if (per > 2) v += xlane::dpp<xlane::XOR2>(v);
@@ -65,8 +65,10 @@ __device__ __forceinline__ int depth_of(const uint32_t *mask, int i) {
 
 constexpr int NORM_THREADS = 256;
 
-// A row's heads, `per` lanes each: lane i holds 4 values of the head from `first` and 4 from `second` on, which the
-// rotation turns against each other.  first of the workgroup's `part` of the row's heads.
+// A row's heads, `per` lanes each, by a workgroup: lane i holds 4 values of the head from `first` and 4 from `second` on, which
+// the rotation turns against each other, so that a head is read and written once, in pieces of 8 or 16 bytes, and its squares meet
+// in a few lane exchanges.  Bound by HBM: 8192 rows of 48 f16 heads of 128 take 45 us, 4.5 TB/s.  (One token: 5 us, a launch and
+// three reads that wait for each other.)
 __device__ __forceinline__ void norm_row(const NormArgs &a, size_t row, int position, int tid, int threads) {
   const int per = a.per, at = tid / per, lane = tid % per, half = a.turn.rot / 2, hd = a.hd;
   const bool there = 8 * lane < hd;
@@ -399,6 +401,11 @@ __device__ __forceinline__ void append_v(const AppendArgs &a, const Rows &rows, 
   }
 }
 
+// Tiles, and behind them the queries' rows.  A tile's words are put together in registers and written whole wherever all of their positions are
+// new; keys of 16 positions and values of 32 go to wavefronts of their own, since one wavefront for a whole tile had its reads wait
+// for each other three times over (16 tokens of 8 heads of 128 into 4 bits: 30 us, 8.3 now; 8192 rows: 132, 58 now).  Those
+// 8192 rows, f16 with 32 query heads on the way, move 170 MB, 2.9 TB/s; the queries' part alone takes 30 of the 58, the keys' and values' 25: the 64-bit
+// norm and rotation (half the rate of f32) and the nibbles, some 20 instructions a value.
 template <typename T, int Z, bool Q4, int TURN>
 __global__ __launch_bounds__(256, 4) void append_kernel(AppendArgs a) {
   if (blockIdx.x >= a.tile_blocks) {
@@ -434,7 +441,8 @@ struct ReadArgs {
   size_t stride;
 };
 
-// Keys and values out of a tile, in the order of its words.
+// Keys and values out of a tile, in the order of its words: a wavefront reads a tile of a head whole and stores pieces of rows.  8192 rows of 8
+// heads of 128 out of 4 bits into f16: 16 us, 2.6 TB/s, bound by the stores' pieces of 8 and 4 bytes.
 template <int Z, bool Q4>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
   const unsigned wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), per = (unsigned)a.tiles * a.pages.kv_heads;
@@ -617,7 +625,8 @@ int launch_page_append(wh_ctx *ctx, const wh_tree *t, const wh_heads *h, const v
     return wh_fail(ctx, WH_EARG, "page append: buffers and rows must be 4-byte aligned");
   if (q == qo && q && (!in16 != !out16 || stride != qo_stride))
     return wh_fail(ctx, WH_EARG, "page append: queries in their own place keep type and stride");
-  if (n_out == t->n) return wh_fail(ctx, WH_EARG, "page append: n_out cannot be n itself");
+  if (n_out && (n_out == t->n || n_out == t->count || n_out == kept))
+    return wh_fail(ctx, WH_EARG, "page append: n_out cannot be n or the numbers of rows");
   const size_t nodes = (size_t)t->batch * t->rows;
   const int tiles = (t->rows + TILE - 2) / TILE + 1;
   const size_t waves = (size_t)t->batch * tiles * 3 * p->kv_heads, blocks = (waves + 3) / 4 + (q ? nodes : 0);
@@ -642,12 +651,12 @@ int launch_page_read(wh_ctx *ctx, const wh_tree *t, const wh_pages *p, void *k, 
     return wh_fail(ctx, WH_EARG, "page read: rows of %d values %zu apart", p->kv_heads * p->hd, stride);
   if (((uintptr_t)k | (uintptr_t)v) % 4 || (out16 && stride % 2)) return wh_fail(ctx, WH_EARG, "page read: buffers and rows must be 4-byte aligned");
   const int tiles = (t->rows + TILE - 2) / TILE + 1;
-  const size_t waves = (size_t)t->batch * tiles * p->kv_heads;
-  if (waves / 4 >= (size_t)1 << 24) return wh_fail(ctx, WH_EARG, "page read: %d rows of %d sequences in one call", t->rows, t->batch);
+  const size_t waves = (size_t)t->batch * tiles * p->kv_heads, blocks = (waves + 3) / 4;
+  if (blocks >= (size_t)1 << 24) return wh_fail(ctx, WH_EARG, "page read: %d rows of %d sequences in one call", t->rows, t->batch);
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "page read: %s", hipGetErrorString(e));
   const ReadArgs a{pages_of(p), t->n, t->count, t->batch, t->rows, tiles, out16 != 0, k, v, stride};
   ProfScope prof(ctx, "page_read", 0.0, (double)t->batch * t->rows * p->kv_heads * p->hd * 2 * (out16 ? 2 : 4));
-  if (p->type == WH_Q4_0) read_z<true>(ctx, a, (unsigned)((waves + 3) / 4));
-  else read_z<false>(ctx, a, (unsigned)((waves + 3) / 4));
+  if (p->type == WH_Q4_0) read_z<true>(ctx, a, blocks);
+  else read_z<false>(ctx, a, blocks);
   return wh_launched(ctx, "page read");
 }

@@ -56,7 +56,10 @@ __device__ __forceinline__ float over_waves(float v, float *part, Op op, float n
 }
 
 // A row per workgroup, its first HELD * 4096 values in registers from their one load to their store (longer rows' others are read
-// three times, from the caches): the maximum, the exponents' sum, the quotients.
+// three times, from the caches): the maximum, the exponents' sum, the quotients.  Sums in f32, of few terms a thread.
+// Many rows are bound by HBM: two workgroups a compute unit, one's loads beside the other's stores (about 290 rows of 51866 f32
+// logits: 30 us, 4 TB/s).  One row (8.7 us) is bound by one compute unit's loads and stores of 200 KB each; in three passes over
+// the row it took 21, the 290 57.
 constexpr int HELD = 13;
 template <typename T>
 __global__ __launch_bounds__(PT, 8) void probs_kernel(ProbsArgs a) {
@@ -107,7 +110,8 @@ __global__ __launch_bounds__(PT, 8) void probs_kernel(ProbsArgs a) {
       store(i, floatx4{i == one ? 1.0f : 0.0f, i + 1 == one ? 1.0f : 0.0f, i + 2 == one ? 1.0f : 0.0f, i + 3 == one ? 1.0f : 0.0f});
     return;
   }
-  const float base = top == -INFINITY ? 0.0f : top, k = fminf(1.44269504088896341f / t, 3.402823466e38f);
+  // (k is finite and no zero, so that what is left of minus infinity is nothing at any temperature)
+  const float base = top == -INFINITY ? 0.0f : top, k = fminf(fmaxf(1.44269504088896341f / t, 1.17549435e-38f), 3.402823466e38f);
   auto power = [&](floatx4 f) {
 #pragma unroll
     for (int e = 0; e < 4; e++) f[e] = __builtin_amdgcn_exp2f((f[e] - base) * k);
@@ -164,6 +168,9 @@ __device__ __forceinline__ void left_of(const float (&x)[N], const float (&y)[N]
 // first, for all nodes side by side; a rejection that is followed by another child costs a pass over the rows for Z, and the
 // draw one more, which leaves the sums of runs of ids behind, so that its place is looked for in one of them.  Everything in
 // 64 bits: random numbers are compared with sums of 1e5 values, whose last bits in f32 would move a place for one of 1e3.
+// The floor of the bytes (13 MB for 32 trees of 24 nodes over 51866 ids with drafts: 3 us) is far: a walk is a chain of passes, each of one
+// compute unit's reads of two rows from the caches, 64-bit sums, and a meeting of 16 wavefronts.  Those trees take 33 us, a
+// chain of 8 nodes without drafts 15; with p and q looked up node by node and the draw's place by a second pass 104 and 29.
 template <bool DRAFTS>
 __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs a) {
   __shared__ double part[ST / 64], sums[PIECES], gone[TREE_ROWS];
@@ -354,6 +361,7 @@ int launch_logit_probs(wh_ctx *ctx, const wh_tree *t, const void *logits, size_t
   if (((uintptr_t)temperature | (uintptr_t)probs) % 4 || (uintptr_t)logits % (f16 ? 2 : 4))
     return wh_fail(ctx, WH_EARG, "logit probabilities: misaligned arrays");
   const size_t nodes = (size_t)t->batch * t->rows;
+  if (nodes * PT >= (size_t)1 << 32) return wh_fail(ctx, WH_EARG, "logit probabilities: %zu rows in one call", nodes);
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "logit probabilities: %s", hipGetErrorString(e));
   const ProbsArgs a{logits, ld, probs, probs_ld, temperature, t->count, t->rows, vocab};
   ProfScope prof(ctx, "logit_probs", 0.0, (double)nodes * vocab * (f16 ? 6 : 8));
@@ -367,6 +375,7 @@ int launch_tree_sample(wh_ctx *ctx, const wh_tree *t, const float *probs, const 
   if (!probs || !u || !picks || (t->rows > 1 && !t->tokens) || vocab <= 0 || vocab > 1 << 28 || ld < (size_t)vocab)
     return wh_fail(ctx, WH_EARG, "tree sample: probabilities of %d ids (%zu apart), random numbers, picks, and the nodes' tokens are needed", vocab, ld);
   if (((uintptr_t)probs | (uintptr_t)drafts | (uintptr_t)u | (uintptr_t)picks) % 4) return wh_fail(ctx, WH_EARG, "tree sample: misaligned arrays");
+  if ((size_t)t->batch * ST >= (size_t)1 << 32) return wh_fail(ctx, WH_EARG, "tree sample: %d sequences in one call", t->batch);
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "tree sample: %s", hipGetErrorString(e));
   const SampleArgs a{probs, drafts, u, t->count, t->tokens, t->mask, t->mask_stride, ld, t->rows, (t->rows + 31) / 32, vocab, picks};
   ProfScope prof(ctx, "tree_sample", 0.0, 4.0 * t->batch * vocab * (drafts ? 2 : 1));
