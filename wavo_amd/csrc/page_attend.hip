@@ -33,13 +33,17 @@ struct PageAttendArgs {
 
 constexpr int WAVES = 8;             // wavefronts of a workgroup, at most
 constexpr float LOWEST = -1e30f;     // the maximum of a row that has seen nothing
-constexpr int START = 24;
 constexpr int JOIN_LDS = 128 << 10;  // bytes in which wavefronts' results are joined
 
 // Whether a compute unit holds two workgroups: where a tile, its queries and outputs fit 128 registers.  (f16 pages of heads of
 // 128, one f16 row a key head, 32 sequences of 1000 to 8191: 112 us alone for 157 with registers spilled; f32 rows over 4 bits 53
 // for 60.)
 constexpr bool two_of(int z, int qt, bool half_rows, bool q4) { return qt == 1 && (q4 ? half_rows || z < 4 : z < 3); }
+
+// What a block of rows costs a workgroup before its first tile and behind its last (its reads that wait for each other, the
+// wavefronts' results joined), as tiles of its time.  One row a key head, 32 sequences of 1000 to 8191: 43.0, 42.2, 41.2 and 42.2 us
+// with 0, 8, 24 and 48 (over f16 pages 115, 111, 113 and 119); 100 rows, 8 sequences of 1000 to 8000: 45, 44, 41 and 38.
+constexpr __host__ __device__ int start_of(int qt) { return qt == 1 ? 24 : 48; }
 
 // A sequence's tiles: the cache's, then the nodes'.
 struct Share {
@@ -56,7 +60,8 @@ __device__ __forceinline__ Share share_of(const PageAttendArgs &a, int n, int co
 __device__ __forceinline__ Share share_of(const PageAttendArgs &a, int b) { return share_of(a, a.n[b], a.count ? a.count[b] : a.rows); }
 
 // All the tiles of a key head in a row: sequence by sequence, block of `rows` rows by block, each at least one.  (Every key
-// head's are shared out alike, so that all of them are in the same pages at about the same time.)  64 sequences at a time are kept in LDS: their lengths and counts, and how many tiles they and those before them have.
+// head's are shared out alike, so that all of them are in the same pages at about the same time.)  64 sequences at a time are
+// kept in LDS: their lengths and counts, and how many tiles they and those before them have.
 struct EvenLds {
   int n[64], count[64];
   uint32_t sum[64];
@@ -81,7 +86,7 @@ struct Even {
     return __builtin_amdgcn_readlane(sum, 63);
   }
   // A block's: as many besides its own as its start and end take the time of.
-  static __device__ __forceinline__ uint32_t tiles_of(const Share &s) { return START + max(s.tiles, 1); }
+  __device__ __forceinline__ uint32_t tiles_of(const Share &s) const { return start_of(rows / 16) + max(s.tiles, 1); }
   __device__ __forceinline__ uint32_t blocks_of(const Share &s) const {
     return (s.count * (a.heads / a.pages.kv_heads) + rows - 1) / rows;
   }
@@ -229,6 +234,13 @@ __device__ __forceinline__ void load_rows(const PageAttendArgs &a, int b, int kh
 //
 // OPEN (4 bits and P16): K and V are multiplied by their factors as they are opened, once for all rows, and rounded to f16 (2^-11 of
 // themselves, as an f16 cache would hold them), so that weights are operands as they stand.
+//
+// What bounds it.  16 rows over f16 pages: HBM (64 sequences of 4000 positions, 8 key heads of 128: 183 us, 5.7 TB/s).  16 rows
+// over 4 bits, a quarter of the bytes: the vector instructions that open them, beside the starts and ends of blocks (the same
+// 64 sequences: 68 us, 4.2 TB/s; 32 of 1000 to 8191 40 and 4 for the join, 3.9 TB/s; f32 rows, whose weights are split, 86).
+// More rows: vector instructions, 429 for 64 rows of 32 positions, 208 of them for nibbles, 8 a weight and row tile, which keep the vector
+// units busy 79% of the time and the matrix cores 33% (100 rows over 8 caches of 24 to 33 k positions, 8 key heads of 128: 129 to 140
+// us, 500 TFLOP/s).
 //
 // attend_part: the tiles from start to end of sequence b's block of rows from r0 on of a key head; into the outputs, or as part `part`.
 template <int Z, int QT, int QP, bool P16, bool Q4>
@@ -714,9 +726,9 @@ __global__ __launch_bounds__(64 * WAVES, two_of(Z, QT, QP == 1, Q4) ? 4 : 2) voi
       Share s;
       uint32_t first;
       even.find(place, b, s, first);
-      const uint32_t tiles = Even::tiles_of(s), block = (place - first) / tiles;
+      const uint32_t tiles = even.tiles_of(s), block = (place - first) / tiles;
       first += block * tiles;
-      const int r0 = 16 * QT * block, start = max((int)(place - first) - START, 0), end = (int)min(tiles, last - first) - START;
+      const int r0 = 16 * QT * block, start = max((int)(place - first) - start_of(QT), 0), end = (int)min(tiles, last - first) - start_of(QT);
       place = first + tiles;
       if (end <= start) continue;
       if constexpr (QT == 1) load_rows<T, Z>(a, b, kh, r0 + m, g, f);
@@ -746,8 +758,8 @@ __global__ __launch_bounds__(256) void page_join_kernel(PageAttendArgs a) {
   const Share s = share_of(a, lds.n[b - even.b0], lds.count[b - even.b0]);
   const int blocks = even.blocks_of(s), local = 8 * blockIdx.y + threadIdx.x / 32, d = 4 * (threadIdx.x % 32), r = rows * rb + local;
   if (rb >= blocks || r >= s.count * group || d >= hd) return;
-  const uint32_t tiles = Even::tiles_of(s), first = even.before + (b > even.b0 ? lds.sum[b - even.b0 - 1] : 0u) + (uint32_t)rb * tiles;
-  const int w0 = (first + START) / even.per, w1 = (first + tiles - 1) / even.per;
+  const uint32_t tiles = even.tiles_of(s), first = even.before + (b > even.b0 ? lds.sum[b - even.b0 - 1] : 0u) + (uint32_t)rb * tiles;
+  const int w0 = (first + start_of(a.qt)) / even.per, w1 = (first + tiles - 1) / even.per;
   if (w0 == w1) return;
   auto at = [&](int w) { return (size_t)(2 * (kh * a.even + w) + (w == w0)) * rows + local; };
   float top = -INFINITY, l = 0.0f;
@@ -829,9 +841,9 @@ int launch_page_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
   while (2 * a.kw <= std::min(WAVES, tiles)) a.kw *= 2;
   const size_t blocks = (size_t)t->batch * a.row_blocks, units = blocks * p->kv_heads, nodes = (size_t)t->batch * t->rows;
   const size_t cus = ctx->cus > 0 ? ctx->cus : 256;
-  if (tiles > 8 * a.kw && blocks * (tiles + START) < (size_t)1 << 31) {
+  if (tiles > 8 * a.kw && blocks * (tiles + start_of(qt)) < (size_t)1 << 31) {
     a.even = (int)std::max<size_t>(cus * (two_of(p->hd / 32, qt, in16, p->type == WH_Q4_0) ? 2 : 1) / p->kv_heads, 1);
-    a.least = START + a.kw;
+    a.least = start_of(qt) + a.kw;
   }
   if (blocks > 65535 || units >= (size_t)1 << 22 || nodes * heads >= (size_t)1 << 25)  // (a launch's limits)
     return wh_fail(ctx, WH_EARG, "page attention: %d heads of %zu nodes in one call", heads, nodes);
