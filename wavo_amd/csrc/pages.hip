@@ -433,6 +433,19 @@ __global__ __launch_bounds__(256, 4) void append_kernel(AppendArgs a) {
   else append_v<T, Z, Q4>(a, rows, (const T *)a.v + from, out);
 }
 
+// One step of turning four lanes' four words: words i and i + D, of which lane and partner (D apart) exchange one each.
+template <int D>
+__device__ __forceinline__ void swap_pairs(uint32_t (&w)[4], int m) {
+  const bool high = m & D;
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    if (i & D) continue;
+    const uint32_t got = xlane::dpp<D == 1 ? xlane::XOR1 : xlane::XOR2>((int)(high ? w[i] : w[i + D]));
+    if (high) w[i] = got;
+    else w[i + D] = got;
+  }
+}
+
 struct ReadArgs {
   Pages pages;
   const int32_t *n, *count;
@@ -476,7 +489,12 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
           for (int e = 0; e < 8; e++) f[e / 4][e % 4] = (float)h[e];
         }
       }
-      store4(a.k, to + 32 * c, a.out16, f[0]), store4(a.k, to + 32 * c + 4, a.out16, f[1]);
+      if (a.out16) {
+        typedef u32x4 any __attribute__((aligned(4)));
+        *(any *)((_Float16 *)a.k + to + 32 * c) = u32x4{pack2(f[0][0], f[0][1]), pack2(f[0][2], f[0][3]), pack2(f[1][0], f[1][1]), pack2(f[1][2], f[1][3])};
+      } else {
+        store4(a.k, to + 32 * c, 0, f[0]), store4(a.k, to + 32 * c + 4, 0, f[1]);
+      }
     }
   }
 #pragma unroll
@@ -497,16 +515,24 @@ __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
         }
       }
     }
+    if (a.out16) {
+      // Four lanes' pairs of four positions turned, so that lane m has 8 values of position 16i + 4g + m % 4.
 #pragma unroll
-    for (int e = 0; e < 8; e++) {
-      const int j = j0 + position_of(g, e);
-      if (j < n || j >= end) continue;
-      const size_t to = (row0 + (j - n)) * a.stride + (size_t)kh * hd + 32 * c + 2 * m;
-      if (a.out16) {
-        *(uint32_t *)((_Float16 *)a.v + to) = pack2(f[0][e], f[1][e]);
-      } else {
+      for (int i = 0; i < 2; i++) {
+        uint32_t w[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) w[e] = pack2(f[0][4 * i + e], f[1][4 * i + e]);
+        swap_pairs<1>(w, m), swap_pairs<2>(w, m);
+        const int j = j0 + position_of(g, 4 * i + m % 4);
+        typedef u32x4 any __attribute__((aligned(4)));
+        if (j >= n && j < end) *(any *)((_Float16 *)a.v + (row0 + (j - n)) * a.stride + (size_t)kh * hd + 32 * c + m / 4 * 8) = u32x4{w[0], w[1], w[2], w[3]};
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; e++) {
+        const int j = j0 + position_of(g, e);
         typedef floatx2 any __attribute__((aligned(4)));
-        *(any *)((float *)a.v + to) = floatx2{f[0][e], f[1][e]};
+        if (j >= n && j < end) *(any *)((float *)a.v + (row0 + (j - n)) * a.stride + (size_t)kh * hd + 32 * c + 2 * m) = floatx2{f[0][e], f[1][e]};
       }
     }
   }
