@@ -515,12 +515,12 @@ int wh_page_read(wh_ctx *ctx, const wh_tree *t, const wh_pages *pages, void *k, 
 
 /* wh_tree_attend over caches in pages: attention of every node over its sequence's positions j < n[b] in the pages and the
  * nodes that it sees, whose k and v (rows as there, already normed and rotated) are taken as f16.  f32 queries are taken in two f16
- * parts, which leaves 2^-22 of them, and for f32 outputs so are the softmax weights (times V's factors, where it is of 4 bits), and
- * keys and values of 4 bits as they stand.  With f16 rows and outputs weights are rounded to f16, and so are keys and values of 4
- * bits (2^-11 of each, as a cache of f16 would hold them; the weights' sum stays f32).  Masked keys and values may hold anything, and so may
+ * parts, which leaves 2^-22 of them, and for f32 outputs so are the softmax weights (times V's factors, where it is of 4 bits); keys
+ * of 4 bits are taken as they stand.  With f16 rows and outputs weights are rounded to f16, and so are values of 4 bits (2^-11 of
+ * each, as a cache of f16 would hold them; the weights' sum stays f32).  Masked keys and values may hold anything, and so may
  * the rows past count[b], which are read; a row that sees a key or value that is no finite number may get NaN.  o overlaps none of the
  * inputs.  heads % kv_heads == 0, heads <= 1024, stride <= 2^23; pointers 4-byte aligned (stride even for f16).  The rows * heads /
- * kv_heads rows of a sequence's key head are taken in blocks of 64 at most (of 32, but for f16 rows and outputs over 4 bits): batch
+ * kv_heads rows of a sequence's key head are taken in blocks of 48 at most (of 32, but for f16 rows and outputs over 4 bits): batch
  * times such blocks <= 65535, that times kv_heads < 2^22, and batch * rows * heads < 2^25.  Where a table holds more than 2048 positions, its nodes
  * counted in, the tiles of all sequences are shared out evenly among the workgroups, from the lengths of their time, and a second
  * launch joins the parts, in the context's scratch: such a call is made once before it is recorded. */

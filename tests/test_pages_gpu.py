@@ -430,10 +430,7 @@ def check_attend(got, cache, x, heads, n, count=None, seen=None, nodes=True, bef
     """Softmax over the positions of pages that are there and the seen nodes, row by row, with a worst case of its error: that of
     caches that are not in pages, and, of p * d in two f16 parts or (f16 rows and outputs) p and V (of 4 bits) rounded to f16: 2^-11
     each of the values' size, and 2^-25 at most where they are subnormal, of weights whose largest is at least 2^10 (less the
-    power of two of V's largest factor, which is below the largest value).
-    Where V of 4 bits is so rounded, K is too: each of its values is off by 2^-11 of itself, or 2^-25, so a score is off by at most
-    D = max_j sum |q| (2^-11 |k| + 2^-25) / sqrt(hd), a weight by a factor between e^-D and e^D beside the sum that is off by the
-    same, and the mean of the values by (e^2D - 1) max|v|; V's 2^-25 stands where p's did."""
+    power of two of V's largest factor, which is below the largest value)."""
     batch, rows = x.shape[:2]
     hd, g, room = cache.hd, cache.kv_heads, cache.cols * cache.page
     p16 = got.dtype == np.float16 and x.dtype == np.float16
@@ -460,8 +457,6 @@ def check_attend(got, cache, x, heads, n, count=None, seen=None, nodes=True, bef
                 tol = attend_tolerance(q, kk, vv, hd) + len(both) * 2.0**-32 * max(1, size)
                 if p16:
                     tol += (2 * EPS16 + EPS16**2 + len(both) * 2.0**-35 * max(1, size)) * size
-                    if cache.type == wa.Q4_0:
-                        tol += np.expm1(2 * np.max(np.abs(q) @ (EPS16 * np.abs(kk) + 2.0**-25).T) / np.sqrt(hd)) * size + 2.0**-25
                 if got.dtype == np.float16:
                     tol = tol + EPS16 * np.abs(want) + 2.0**-25
                 err = np.abs(row - want)

@@ -127,18 +127,13 @@ struct Even {
 };
 
 // A tile's share of a lane: words of K and V, and for 4 bits their factors.
-// OWN: of K those of the positions of the lane's own words (halfs for u = 0 and 1), otherwise those of its scores.
-template <int Z, bool Q4, bool OWN>
+// (the positions of its scores and weights).
+template <int Z, bool Q4>
 struct Tile;
-template <int Z, bool OWN>
-struct Tile<Z, true, OWN> {
+template <int Z>
+struct Tile<Z, true> {
   uint32_t k[2 * Z], v[2 * Z];
-  // (halfs as they are loaded, one a register: put together they would be waited for where that is done)
-  struct Pair {
-    uint16_t u[2];
-  };
-  typename std::conditional<OWN, Pair, half8>::type kd[Z];
-  half8 vd[Z];
+  half8 kd[Z], vd[Z];
   static __device__ __forceinline__ void words(uint32_t (&w)[2 * Z], const uint32_t *p, int lane) {
     constexpr int T = 2 * Z, whole = T & ~3;
 #pragma unroll
@@ -153,14 +148,8 @@ struct Tile<Z, true, OWN> {
   }
   __device__ __forceinline__ void load_k(const uint32_t *p, int lane, int g) {
     words(k, p, lane);
-    if constexpr (OWN) {
-      const uint16_t *d = (const uint16_t *)(p + 128 * Z) + (lane % 16 / 4) * 8 * Z + lane % 4;
 #pragma unroll
-      for (int c = 0; c < Z; c++) kd[c].u[0] = d[8 * c], kd[c].u[1] = d[8 * c + 4];
-    } else {
-#pragma unroll
-      for (int c = 0; c < Z; c++) kd[c] = *(const half8 *)(p + 128 * Z + (g * Z + c) * 4);
-    }
+    for (int c = 0; c < Z; c++) kd[c] = *(const half8 *)(p + 128 * Z + (g * Z + c) * 4);
   }
   __device__ __forceinline__ void load_v(const uint32_t *p, int lane, int g) {
     words(v, p + 144 * Z, lane);
@@ -190,8 +179,8 @@ struct Tile<Z, true, OWN> {
         if (!(there >> e & 1)) vd[c][e] = (_Float16)0;
   }
 };
-template <int Z, bool OWN>
-struct Tile<Z, false, OWN> {
+template <int Z>
+struct Tile<Z, false> {
   u32x4 k[2 * Z], v[2 * Z];
   __device__ __forceinline__ void load_k(const uint32_t *p, int lane, int) {
 #pragma unroll
@@ -222,25 +211,25 @@ __device__ __forceinline__ void load_rows(const PageAttendArgs &a, int b, int kh
 //   Scores transposed, S^T = K Q^T: lane 16g + i holds row i's scores of positions position_of(g, e), e < 8.  For 4 bits the
 //   products are those of nibble - 8, exact in f16, chunk by chunk of 32 values, and every chunk's sum is multiplied by its
 //   position's factor in f32: K is taken as it stands.
-//   Outputs transposed, O^T = V^T P^T, with V's factors in the weights: a chunk's 32 values of V share one factor, so the
-//   operand of P for that chunk is p * d.
+//   Outputs transposed, O^T = V^T P^T, with V's factors in the weights (but for OPEN): a chunk's 32 values of V share one
+//   factor, so the operand of P for that chunk is p * d.
 // The next tile's K is asked for as soon as this one's scores are done, and its V after this one's outputs; its page two tiles
 // ahead.
 //
 // Precision: f32 queries are scaled by a power of two per row and split into two f16 parts, as are the weights (p * d) for
 // f32 outputs: two products each, with an error of 2^-22.  Weights are exp2(s - max + 10 - E): the second part is no
-// subnormal, and E, zero until a factor of V reaches 2, keeps p * d within f16.  P16 (f16 outputs): p and p * d are rounded to
-// f16, off by 2^-11 of themselves each, beside the output's own rounding; the weights' sum stays f32.
+// subnormal, and E, zero until a factor of V reaches 2, keeps p * d within f16.  P16 (f16 outputs): p is rounded to f16,
+// off by 2^-11 of itself, beside the output's own rounding; the weights' sum stays f32.
 //
-// OPEN (4 bits and P16): K and V are multiplied by their factors as they are opened, once for all rows, and rounded to f16 (2^-11 of
-// themselves, as an f16 cache would hold them), so that weights are operands as they stand.
+// OPEN (4 bits and P16): V is multiplied by its factors as it is opened, once for all rows, and rounded to f16 (2^-11 of itself, as
+// an f16 cache would hold it), so that weights are operands as they stand.  K is not: so opened it took 142 us for the 162 of
+// the 100 rows below, and made the outputs' error against 64 bits 4e-4 for 2.6e-4 (of which their own rounding is 2.1e-4).
 //
 // What bounds it.  16 rows over f16 pages: HBM (64 sequences of 4000 positions, 8 key heads of 128: 183 us, 5.7 TB/s).  16 rows
-// over 4 bits, a quarter of the bytes: the vector instructions that open them, beside the starts and ends of blocks (the same
-// 64 sequences: 68 us, 4.2 TB/s; 32 of 1000 to 8191 40 and 4 for the join, 3.9 TB/s; f32 rows, whose weights are split, 86).
-// More rows: vector instructions, 429 for 64 rows of 32 positions, 208 of them for nibbles, 8 a weight and row tile, which keep the vector
-// units busy 79% of the time and the matrix cores 33% (100 rows over 8 caches of 24 to 33 k positions, 8 key heads of 128: 129 to 140
-// us, 500 TFLOP/s).
+// over 4 bits, a quarter of the bytes: the vector instructions that open them, beside the starts and ends of blocks (32 sequences
+// of 1000 to 8191: 43 us and 4 for the join, 3.6 TB/s).  More rows: vector instructions, some 150 for the nibbles of 32 positions
+// and 15 a row tile for every one of its 8 weights, beside matrix instructions for a third of the time (100 rows over 8 caches of 24 to 33 k positions, 8
+// key heads of 128: 145 to 165 us, 450 TFLOP/s).
 //
 // attend_part: the tiles from start to end of sequence b's block of rows from r0 on of a key head; into the outputs, or as part `part`.
 template <int Z, int QT, int QP, bool P16, bool Q4>
@@ -269,7 +258,7 @@ __device__ __forceinline__ void attend_part(const PageAttendArgs &a, uint8_t *sm
   auto at = [&](int tile, int id) {
     return (const uint32_t *)a.pages.pool + (size_t)id * a.pages.page_words + (size_t)((kh << slot) + (tile & ((1 << slot) - 1))) * tile_words(Q4, hd);
   };
-  Tile<Z, Q4, OPEN> w;
+  Tile<Z, Q4> w;
   int blk = start + ki, next = cached, next_id = -1;
   if (blk < cached) {
     int id = id_of(blk);
@@ -434,13 +423,8 @@ __device__ __forceinline__ void attend_part(const PageAttendArgs &a, uint8_t *sm
 #pragma unroll
     for (int t = 0; t < QT; t++) st[t][0] = st[t][1] = floatx4{};
     // (matrix instructions of a word among the vector ones that open the next)
-    auto open_k = [&](int i) {
-      half8 k = w.open(w.k[i]);
-      if constexpr (OPEN) k *= (half8)__builtin_bit_cast(_Float16, w.kd[i / 2].u[i % 2]);
-      return k;
-    };
     // (and queries asked for when the chunk before them is done)
-    half8 k = open_k(0), x[QT][QP];
+    half8 k = w.open(w.k[0]), x[QT][QP];
 #pragma unroll
     for (int t = 0; t < QT; t++)
 #pragma unroll
@@ -450,14 +434,13 @@ __device__ __forceinline__ void attend_part(const PageAttendArgs &a, uint8_t *sm
     for (int i = 0; i < 2 * Z; i++) {
       const int c = i / 2, u = i % 2;
       half8 after = k;
-      if (i + 1 < 2 * Z) after = open_k(i + 1);
+      floatx4 y[QT];
+      if (i + 1 < 2 * Z) after = w.open(w.k[i + 1]);
 #pragma unroll
       for (int t = 0; t < QT; t++) {
-        if constexpr (Q4 && !OPEN) {
-          floatx4 y = mfma(k, x[t][0], floatx4{});
-          if constexpr (QP == 2) y = mfma(k, x[t][QP - 1], y);
-#pragma unroll
-          for (int r = 0; r < 4; r++) st[t][u][r] = fmaf(y[r], (float)w.kd[c][4 * u + r], st[t][u][r]);
+        if constexpr (Q4) {
+          y[t] = mfma(k, x[t][0], floatx4{});
+          if constexpr (QP == 2) y[t] = mfma(k, x[t][QP - 1], y[t]);
         } else {
 #pragma unroll
           for (int part = 0; part < QP; part++) st[t][u] = mfma(k, x[t][part], st[t][u]);
@@ -466,13 +449,18 @@ __device__ __forceinline__ void attend_part(const PageAttendArgs &a, uint8_t *sm
 #pragma unroll
           for (int part = 0; part < QP; part++) x[t][part] = query_of(t, c + 1, part);
       }
+      if constexpr (Q4)
+#pragma unroll
+        for (int t = 0; t < QT; t++)
+#pragma unroll
+          for (int r = 0; r < 4; r++) st[t][u][r] = fmaf(y[t][r], (float)w.kd[c][4 * u + r], st[t][u][r]);
       k = after;
       if constexpr (QT > 1 && OPEN) {
 #pragma unroll
         for (int t = 0; t < QT; t++) {
           __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
           if (u == 1 && c + 1 < Z) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-          __builtin_amdgcn_sched_group_barrier(0x002, (13 + QT - 1) / QT, 0);
+          __builtin_amdgcn_sched_group_barrier(0x002, (9 + QT - 1) / QT, 0);
         }
         __builtin_amdgcn_sched_barrier(0);
       }
@@ -796,7 +784,6 @@ int attend_launch(wh_ctx *ctx, const PageAttendArgs &a) {
 template <int Z, int QP, bool P16, bool Q4>
 int attend_qt(wh_ctx *ctx, const PageAttendArgs &a, int qt) {
   if constexpr (Q4 && P16) {
-    if (qt == 4) return attend_launch<Z, 4, QP, P16, Q4>(ctx, a);
     if (qt == 3) return attend_launch<Z, 3, QP, P16, Q4>(ctx, a);
   }
   return qt == 1 ? attend_launch<Z, 1, QP, P16, Q4>(ctx, a) : attend_launch<Z, 2, QP, P16, Q4>(ctx, a);
@@ -830,10 +817,10 @@ int launch_page_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
     return wh_fail(ctx, WH_EARG, "page attention: buffers and rows must be 4-byte aligned");
   PageAttendArgs a{q, k, v, stride, pages_of(p), o, out16 != 0, t->n, t->count, t->mask, t->mask_stride, t->batch, t->rows, (t->rows + 31) / 32,
                    heads, 1.0f / sqrtf((float)p->hd), 1, 1, 1, 0, 0, nullptr, nullptr};
-  // Rows in tiles of 16, evenly in blocks of `most` at most.  4 tiles read a nibble once for 64 rows: with 32 query heads over 8 of
-  // 128 and f16 throughout, 100 rows over 28 k positions take 129 us for 139 with 2 (48 for 46 over 7 k).  f32 weights and
-  // outputs leave registers for 2 (225 us for 364), and f16 pages have nothing to open (81 and 83 with 2 and 3).
-  const int rows = (t->rows * (heads / p->kv_heads) + 15) / 16, most = p->type == WH_Q4_0 && in16 && out16 ? 4 : 2;
+  // Rows in tiles of 16, evenly in blocks of `most` at most.  3 tiles open a nibble once for 48 rows: with 32 query heads over 8 of
+  // 128 and f16 throughout, 100 rows over 28 k positions take 162 us for 169 with 2 (42 for 40 over 5 k), and 4 spill registers
+  // (192).  f32 weights and outputs leave registers for 2, and f16 pages have nothing to open (81 and 83 us with 2 and 3).
+  const int rows = (t->rows * (heads / p->kv_heads) + 15) / 16, most = p->type == WH_Q4_0 && in16 && out16 ? 3 : 2;
   a.row_blocks = (rows + most - 1) / most;
   const int qt = (rows + a.row_blocks - 1) / a.row_blocks;
   a.row_blocks = (rows + qt - 1) / qt, a.qt = qt;
