@@ -227,9 +227,9 @@ __device__ __forceinline__ void load_rows(const PageAttendArgs &a, int b, int kh
 //
 // What bounds it.  16 rows over f16 pages: HBM (64 sequences of 4000 positions, 8 key heads of 128: 183 us, 5.7 TB/s).  16 rows
 // over 4 bits, a quarter of the bytes: the vector instructions that open them, beside the starts and ends of blocks (32 sequences
-// of 1000 to 8191: 43 us and 4 for the join, 3.6 TB/s).  More rows: vector instructions, some 150 for the nibbles of 32 positions
-// and 15 a row tile for every one of its 8 weights, beside matrix instructions for a third of the time (100 rows over 8 caches of 24 to 33 k positions, 8
-// key heads of 128: 145 to 165 us, 450 TFLOP/s).
+// of 1000 to 8191: 43 us and 4 for the join, 3.6 TB/s).  More rows: vector instructions, 365 for 48 rows of 32 positions,
+// of which some 180 open nibbles: 74% of the time, and matrix instructions 28% (100 rows over 8 caches of 24 to 33 k positions, 8 key
+// heads of 128: 145 to 165 us, 450 TFLOP/s).
 //
 // attend_part: the tiles from start to end of sequence b's block of rows from r0 on of a key head; into the outputs, or as part `part`.
 template <int Z, int QT, int QP, bool P16, bool Q4>
