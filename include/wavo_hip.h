@@ -484,7 +484,7 @@ int wh_head_norm(wh_ctx *ctx, const wh_tree *t, const wh_heads *heads, const voi
  * are NaN where one of them is no finite number), in tiles of 32 positions (wavo_amd/csrc/pages.h).  Position j of sequence b
  * lies in page table[b * table_stride + j / page] of the pool (table_stride 0: one table for all), in device memory and read when the queued work
  * runs.  Pages whose number is not in 0 .. pages - 1 are not there: their positions are not seen, not stored, and read as zeros.
- * A sequence has table_cols * page positions at most (<= 2^24).  pool: pages * wh_page_bytes() bytes, 16-byte aligned.  What
+ * Values that 4 bits stand for are within f16, as all that is stored here is.  A sequence has table_cols * page positions at most (<= 2^24).  pool: pages * wh_page_bytes() bytes, 16-byte aligned.  What
  * lies in positions that were never stored does not matter. */
 typedef struct wh_pages {
   void *pool;

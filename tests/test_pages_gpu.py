@@ -652,6 +652,27 @@ def test_attend_factors_of_any_size(gpu, in16, scale):
 
 
 @pytest.mark.parametrize("type", [wa.Q4_0, wa.F16])
+@pytest.mark.parametrize("scale", [1e-4, 100.0, 8188.0])
+def test_attend_values_of_any_size_in_f16(gpu, type, scale):
+    """f16 rows and outputs: values up to f16's largest (8188 times -8 in 4 bits) among ordinary ones, keys as they were."""
+    rng = np.random.default_rng(27)
+    batch, rows, heads, g, hd, page, cols = 2, 20, 2, 2, 64, 32, 12
+    cache = Cache(rng, type, page, g, hd, batch, cols)
+    n = [cols * page, 100]
+    cache.fill(rng, n)
+    for b, j in ((0, 5), (0, 300), (0, 383), (1, 40), (1, 99)):
+        pg, tile, p = cache.place(b, j)
+        half_words = cache.pool[pg, :, tile].view(np.float16)
+        if type == wa.Q4_0:
+            half_words[:, 2 * (8 * hd + hd // 2) + cache.factor[p]] = scale * rng.uniform(0.3, 1, (g, hd // 32))
+        else:
+            half_words[:, cache.at[1][0][p] + 32 * hd] = 8 * scale * rng.uniform(-1, 1, (g, hd))
+    x = rows_of(rng, batch, rows, heads, g, hd, True)
+    _, seen = trees(rng, batch, rows)
+    check_attend(attend(gpu, cache, x, heads, n, None, seen, True), cache, x, heads, n, None, seen)
+
+
+@pytest.mark.parametrize("type", [wa.Q4_0, wa.F16])
 @pytest.mark.parametrize("size", [1e-6, 300.0, 3e4])
 def test_attend_scores_far_apart(gpu, type, size):
     rng = np.random.default_rng(24)
@@ -910,6 +931,99 @@ def test_sampled_tokens_have_the_targets_distribution(gpu, drafts):
     got = sample(gpu, p, q if drafts else None, tokens, rng.random((batch, rows)).astype(np.float32), vocab, bits(seen))
     share = np.bincount(got[:, 0], minlength=vocab) / batch
     assert np.all(np.abs(share - p[0, 0]) <= 5 * np.sqrt(p[0, 0] * (1 - p[0, 0]) / batch)), share
+
+
+# ------------------------------------------------------------------------------------------- calls beside each other
+
+
+def long_call(gpu, cache, rng, rows=3, heads=4):
+    """page_attend over a table that is shared out, as a call of its own and its output."""
+    batch, g, hd = len(cache.table), cache.kv_heads, cache.hd
+    x, mask = gpu.upload(rows_of(rng, batch, rows, heads, g, hd, True)), gpu.upload(bits(trees(rng, batch, rows)[1]))
+    n, o, pages = gpu.upload(np.array([2400, 1700][:batch], np.int32)), gpu.buffer(batch * rows * heads * hd // 2), cache.device(gpu)
+    t = wa.Tree(batch, rows, n, None, None, mask, rows * ((rows + 31) // 32))
+    call = lambda: gpu.page_attend(t, x, x.ptr + 2 * heads * hd, x.ptr + 2 * (heads + g) * hd, (heads + 2 * g) * hd, pages, o, heads, True, True)  # noqa: E731
+    return call, lambda: gpu.read(o, (batch, rows, heads * hd), np.float16)
+
+
+def test_two_contexts_at_once(gpu):
+    """Calls queued on two contexts in turn, each with parts of its own: what each gives by itself."""
+    rng = np.random.default_rng(30)
+    caches = [Cache(rng, type, 128, 2, 64, 2, 20) for type in (wa.Q4_0, wa.F16)]
+    for c in caches:
+        c.fill(rng, [2560, 2560])
+    other = wa.Gpu(0)
+    try:
+        sides = [long_call(g, c, np.random.default_rng(31)) for g, c in zip((gpu, other), caches)]
+        want = []
+        for call, result in sides:
+            call()
+            want.append(result())
+        for _ in range(20):
+            for call, _result in sides:
+                call()
+        for (_call, result), w in zip(sides, want):
+            assert np.array_equal(result(), w)
+    finally:
+        del sides
+        other.close()
+
+
+def test_recording_does_not_grow_the_scratch():
+    """A call that needs parts, recorded on a context that has never made it: refused, and the context goes on."""
+    rng = np.random.default_rng(32)
+    cache = Cache(rng, wa.Q4_0, 256, 2, 64, 1, 10)
+    cache.fill(rng, [2560])
+    fresh = wa.Gpu(0)
+    try:
+        call, result = long_call(fresh, cache, rng)
+        fresh.record_begin()
+        with pytest.raises(wa.WavoError, match="record"):
+            call()
+        fresh.record_end().free()
+        call()
+        want = result()
+        fresh.record_begin()
+        call()
+        p = fresh.record_end()
+        p.replay()
+        assert np.array_equal(result(), want) and np.abs(want).max() > 0
+        p.free()
+    finally:
+        fresh.close()
+
+
+@pytest.mark.parametrize("type", [wa.Q4_0, wa.F16])
+def test_pools_past_4_gib(gpu, type):
+    """Pages at a pool's far end: the words, rows and outputs of the same tokens in a pool of two."""
+    rng = np.random.default_rng(33)
+    heads, g, hd, page, rows = 4, 2, 128, 256, 300
+    size = wa.page_bytes(type, page, g, hd)
+    many = (5 << 30) // size
+    x = gpu.upload(rows_of(rng, 1, rows, heads, g, hd, True))
+    n, n1 = gpu.upload(np.array([0], np.int32)), gpu.upload(np.array([rows], np.int32))
+    h, stride = wa.Heads(heads, g, hd), (heads + 2 * g) * hd
+    got = []
+    for pages, table in ((2, [1, 0]), (many, [many - 1, many - 2])):
+        pool, tb = gpu.buffer(pages * size // 4), gpu.upload(np.array(table, np.int32))
+        p = wa.Pages(pool, pages, tb, 2, 2, page, type, g, hd)
+        gpu.page_append(wa.Tree(1, rows, n), h, None, x.ptr + 2 * heads * hd, x.ptr + 2 * (heads + g) * hd, stride, p, in16=True)
+        k, v, o = (gpu.buffer(rows * w * hd) for w in (g, g, heads))
+        gpu.page_read(wa.Tree(1, rows, n), p, k, v, g * hd)
+        gpu.page_attend(wa.Tree(1, rows, n1), x, None, None, stride, p, o, heads, in16=True)
+        got.append([gpu.read(a, (rows, w * hd)) for a, w in ((k, g), (v, g), (o, heads))])
+        del pool, p
+    assert all(np.array_equal(a, b) and np.abs(a).max() > 0 for a, b in zip(*got))
+
+
+def test_sample_large_vocabularies(gpu):
+    """More ids than single runs of sums hold."""
+    rng = np.random.default_rng(34)
+    for vocab, draft in ((300007, True), (524289, False)):
+        p, q, tokens, parents, mask, u = drafted(rng, 3, 4, vocab, vocab)
+        got = sample(gpu, p, q if draft else None, tokens, u, vocab, mask)
+        for b in range(3):
+            assert np.array_equal(got[b], walk(p[b], q[b] if draft else None, tokens[b], parents[b], u[b], vocab))
 
 
 # ------------------------------------------------------------------------------------------- all of them
