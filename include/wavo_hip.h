@@ -482,10 +482,11 @@ int wh_head_norm(wh_ctx *ctx, const wh_tree *t, const wh_heads *heads, const voi
  * 128), as f16 (WH_F16) or in 4 bits (WH_Q4_0: per position and 32 values of a head one f16 factor d = m / -8, m the one of
  * largest magnitude, the positive one of two, and x as floor(x / d + 8.5) in 0 .. 15, which stands for (that - 8) * d; the 32
  * are NaN where one of them is no finite number), in tiles of 32 positions (wavo_amd/csrc/pages.h).  Position j of sequence b
- * lies in page table[b * table_stride + j / page] of the pool (table_stride 0: one table for all), in device memory and read when the queued work
- * runs.  Pages whose number is not in 0 .. pages - 1 are not there: their positions are not seen, not stored, and read as zeros.
- * Values that 4 bits stand for are within f16, as all that is stored here is.  A sequence has table_cols * page positions at most (<= 2^24).  pool: pages * wh_page_bytes() bytes, 16-byte aligned.  What
- * lies in positions that were never stored does not matter. */
+ * lies in page table[b * table_stride + j / page] of the pool (table_stride 0: one table for all), in device memory and read
+ * when the queued work runs.  Pages whose number is not in 0 .. pages - 1 are not there: their positions are not seen, not
+ * stored, and read as zeros.  Values that 4 bits stand for are within f16, as all that is stored here is.  A sequence has
+ * table_cols * page positions at most (<= 2^24).  pool: pages * wh_page_bytes() bytes, 16-byte aligned.  What lies in
+ * positions that were never stored does not matter. */
 typedef struct wh_pages {
   void *pool;
   int pages;
@@ -497,14 +498,14 @@ typedef struct wh_pages {
 /* Bytes of a page; 0 where its type or sizes are not supported. */
 size_t wh_page_bytes(int type, int page, int kv_heads, int hd);
 
-/* Appends keys and values to the pages: position n[b] + i gets those of row i of sequence b, i < count[b] (kept[b], where kept is
- * given), keys normed and rotated as that position's (heads->k_gain and table; in 64 bits), then rounded to f32, f16 and the pages' type; or, with path
- * [batch][rows], those of row path[b][i] (wh_tree_accept's path and kept: the accepted nodes; an entry outside 0 .. rows - 1
- * stores nothing).  Row r's keys and values are at k and v + r * stride values, f32 or (in16) f16.  With q and qo (not with a path) queries
- * are normed and rotated on the way, row r of q (the same stride) to qo + r * qo_stride, f32 or (out16) f16; qo may be q itself (same type
- * and stride) and otherwise overlaps nothing.  n_out[b] (or NULL) = n[b] + the positions that are there, n[b] at least; it is
- * none of n, count and kept.  The tree's mask and tokens are not read.  Nothing but those positions changes; a page belongs to one sequence of a call,
- * where it is stored to. */
+/* Appends keys and values to the pages: position n[b] + i gets those of row i of sequence b, i < count[b] (kept[b], where kept
+ * is given), keys normed and rotated as that position's (heads->k_gain and table; in 64 bits), then rounded to f32, f16 and
+ * the pages' type; or, with path [batch][rows], those of row path[b][i] (wh_tree_accept's path and kept: the accepted nodes;
+ * an entry outside 0 .. rows - 1 stores nothing).  Row r's keys and values are at k and v + r * stride values, f32 or (in16)
+ * f16.  With q and qo (not with a path) queries are normed and rotated on the way, row r of q (the same stride) to qo + r *
+ * qo_stride, f32 or (out16) f16; qo may be q itself (same type and stride) and otherwise overlaps nothing.  n_out[b] (or NULL)
+ * = n[b] + the positions that are there, n[b] at least; it is none of n, count and kept.  The tree's mask and tokens are not
+ * read.  Nothing but those positions changes; a page belongs to one sequence of a call, where it is stored to. */
 int wh_page_append(wh_ctx *ctx, const wh_tree *t, const wh_heads *heads, const void *q, const void *k, const void *v,
                    size_t stride, int in16, const int32_t *path, const int32_t *kept, const wh_pages *pages, void *qo,
                    size_t qo_stride, int out16, int32_t *n_out);
@@ -514,38 +515,41 @@ int wh_page_append(wh_ctx *ctx, const wh_tree *t, const wh_heads *heads, const v
 int wh_page_read(wh_ctx *ctx, const wh_tree *t, const wh_pages *pages, void *k, void *v, size_t stride, int out16);
 
 /* wh_tree_attend over caches in pages: attention of every node over its sequence's positions j < n[b] in the pages and the
- * nodes that it sees, whose k and v (rows as there, already normed and rotated) are taken as f16.  f32 queries are taken in two f16
- * parts, which leaves 2^-22 of them, and for f32 outputs so are the softmax weights (times V's factors, where it is of 4 bits); keys
- * of 4 bits are taken as they stand.  With f16 rows and outputs weights are rounded to f16, and so are values of 4 bits (2^-11 of
- * each, as a cache of f16 would hold them; the weights' sum stays f32).  Masked keys and values may hold anything, and so may
- * the rows past count[b], which are read; a row that sees a key or value that is no finite number may get NaN.  o overlaps none of the
- * inputs.  heads % kv_heads == 0, heads <= 1024, stride <= 2^23; pointers 4-byte aligned (stride even for f16).  The rows * heads /
- * kv_heads rows of a sequence's key head are taken in blocks of 48 at most (of 32, but for f16 rows and outputs over 4 bits): batch
- * times such blocks <= 65535, that times kv_heads < 2^22, and batch * rows * heads < 2^25.  Where a table holds more than 2048 positions, its nodes
- * counted in, the tiles of all sequences are shared out evenly among the workgroups, from the lengths of their time, and a second
- * launch joins the parts, in the context's scratch: such a call is made once before it is recorded. */
+ * nodes that it sees, whose k and v (rows as there, already normed and rotated) are taken as f16.  f32 queries are taken in
+ * two f16 parts, which leaves 2^-22 of them, and for f32 outputs so are the softmax weights (times V's factors, where it is of
+ * 4 bits); keys of 4 bits are taken as they stand.  With f16 rows and outputs weights are rounded to f16, and so are values of
+ * 4 bits (2^-11 of each, as a cache of f16 would hold them; the weights' sum stays f32).  Masked keys and values may hold
+ * anything, and so may the rows past count[b], which are read; a row that sees a key or value that is no finite number may get
+ * NaN.  o overlaps none of the inputs.  heads % kv_heads == 0, heads <= 1024, stride <= 2^23; pointers 4-byte aligned (stride
+ * even for f16).  The rows * heads / kv_heads rows of a sequence's key head are taken in blocks of 48 at most (of 32, but for
+ * f16 rows and outputs over 4 bits): batch times such blocks <= 65535, that times kv_heads < 2^22, and batch * rows * heads <
+ * 2^25.  Where a table holds more than 2048 positions, its nodes counted in, the tiles of all sequences are shared out evenly
+ * among the workgroups, from the lengths of their time, and a second launch joins the parts, in the context's scratch: such a
+ * call is made once before it is recorded. */
 int wh_page_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void *k, const void *v, size_t stride, int in16,
                    const wh_pages *pages, void *o, int out16, int heads);
 
-/* Probabilities of the rows of logits [batch * rows] (row r at r * ld values, f32 or (f16) f16, vocab values each; wh_logit_rules'
- * out): probs[r * probs_ld + x] = exp((l_x - max) / T) / their sum, in f32, T = temperature[b] (NULL: 1).  T <= 0 (or NaN): 1 for
- * the first maximum, 0 for the others.  A row with nothing left (minus infinity everywhere) gets zeros, one with NaN or plus infinity gets
- * NaN.  Rows past count[b] are not written, nor is anything past vocab; probs overlaps no input.  batch * rows < 2^22. */
+/* Probabilities of the rows of logits [batch * rows] (row r at r * ld values, f32 or (f16) f16, vocab values each;
+ * wh_logit_rules' out): probs[r * probs_ld + x] = exp((l_x - max) / T) / their sum, in f32, T = temperature[b] (NULL: 1).  T
+ * <= 0 (or NaN): 1 for the first maximum, 0 for the others.  A row with nothing left (minus infinity everywhere) gets zeros,
+ * one with NaN or plus infinity gets NaN.  Rows past count[b] are not written, nor is anything past vocab; probs overlaps no
+ * input.  batch * rows < 2^22. */
 int wh_logit_probs(wh_ctx *ctx, const wh_tree *t, const void *logits, size_t ld, int f16, int vocab, const float *temperature,
                    float *probs, size_t probs_ld);
 
-/* Verifies drafted tokens against the target's probabilities, so that the tokens that come out are distributed as if drawn from
- * those one by one.  probs: the target's, row b * rows + i (ld apart) for the token after node i; drafts (the same layout): those
- * that node i's children were drawn from, independently, or NULL: the children are given (a known text, the likeliest ones).
- * u [batch][rows]: random numbers in [0, 1).  From the root on, with w = probs of the node and Z = 1, its children in turn (i's
- * parent is the highest node below it that it sees; without a mask, i - 1):
- *   the child with token x is accepted if u[b][child] * drafts[x] * Z < w[x] (NULL: u[b][child] * Z < w[x]), and the walk goes on there;
+/* Verifies drafted tokens against the target's probabilities, so that the tokens that come out are distributed as if drawn
+ * from those one by one.  probs: the target's, row b * rows + i (ld apart) for the token after node i; drafts (the same
+ * layout): those that node i's children were drawn from, independently, or NULL: the children are given (a known text, the
+ * likeliest ones).  u [batch][rows]: random numbers in [0, 1).  From the root on, with w = probs of the node and Z = 1, its
+ * children in turn (i's parent is the highest node below it that it sees; without a mask, i - 1):
+ *   the child with token x is accepted if u[b][child] * drafts[x] * Z < w[x] (NULL: u[b][child] * Z < w[x]), and the walk goes
+ *   on there;
  *   otherwise w = max(0, w / Z - drafts) and Z = the sum of w (NULL: Z = Z - w[x] and w[x] = 0), while Z > 0.
- * Where none is accepted the next token is drawn from w: the first id whose running sum is above u[b][0] times the sum of w (from
- * probs, where w has come to nothing).  All of it in 64 bits.  picks [batch * rows]: for the nodes on the walk the token after
- * them, 0xffffffff for the others and where probs has nothing: wh_tree_accept takes that walk and keeps it.  Rows of probs and drafts hold finite
- * numbers, none below zero; those off the walk may hold anything.  Tokens past vocab are passed over.  picks overlaps no input.
- * count[b] rows of picks are written.  batch < 2^22. */
+ * Where none is accepted the next token is drawn from w: the first id whose running sum is above u[b][0] times the sum of w
+ * (from probs, where w has come to nothing).  All of it in 64 bits.  picks [batch * rows]: for the nodes on the walk the token
+ * after them, 0xffffffff for the others and where probs has nothing: wh_tree_accept takes that walk and keeps it.  Rows of
+ * probs and drafts hold finite numbers, none below zero; those off the walk may hold anything.  Tokens past vocab are passed
+ * over.  picks overlaps no input.  count[b] rows of picks are written.  batch < 2^22. */
 int wh_tree_sample(wh_ctx *ctx, const wh_tree *t, const float *probs, const float *drafts, int vocab, size_t ld, const float *u,
                    uint32_t *picks);
 

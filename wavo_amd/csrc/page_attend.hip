@@ -126,8 +126,7 @@ struct Even {
   }
 };
 
-// A tile's share of a lane: words of K and V, and for 4 bits their factors.
-// (the positions of its scores and weights).
+// A tile's share of a lane: words of K and V, and for 4 bits the factors of the positions of its scores and weights.
 template <int Z, bool Q4>
 struct Tile;
 template <int Z>

@@ -401,11 +401,12 @@ __device__ __forceinline__ void append_v(const AppendArgs &a, const Rows &rows, 
   }
 }
 
-// Tiles, and behind them the queries' rows.  A tile's words are put together in registers and written whole wherever all of their positions are
-// new; keys of 16 positions and values of 32 go to wavefronts of their own, since one wavefront for a whole tile had its reads wait
-// for each other three times over (16 tokens of 8 heads of 128 into 4 bits: 30 us, 8.3 now; 8192 rows: 132, 58 now).  Those
-// 8192 rows, f16 with 32 query heads on the way, move 170 MB, 2.9 TB/s; the queries' part alone takes 30 of the 58, the keys' and values' 25: the 64-bit
-// norm and rotation (half the rate of f32) and the nibbles, some 20 instructions a value.
+// Tiles, and behind them the queries' rows.  A tile's words are put together in registers and written whole wherever all of
+// their positions are new; keys of 16 positions and values of 32 go to wavefronts of their own, since one wavefront for a whole
+// tile had its reads wait for each other three times over (16 tokens of 8 heads of 128 into 4 bits: 30 us, 8.3 now; 8192 rows:
+// 132, 58 now).  Those 8192 rows, f16 with 32 query heads on the way, move 170 MB, 2.9 TB/s; the queries' part alone takes 30
+// of the 58, the keys' and values' 25: the 64-bit norm and rotation (half the rate of f32) and the nibbles, some 20
+// instructions a value.
 template <typename T, int Z, bool Q4, int TURN>
 __global__ __launch_bounds__(256, 4) void append_kernel(AppendArgs a) {
   if (blockIdx.x >= a.tile_blocks) {
@@ -454,8 +455,9 @@ struct ReadArgs {
   size_t stride;
 };
 
-// Keys and values out of a tile, in the order of its words: a wavefront reads a tile of a head whole and stores pieces of rows.  8192 rows of 8
-// heads of 128 out of 4 bits into f16: 16 us, 2.6 TB/s, bound by the stores' pieces of 8 and 4 bytes.
+// Keys and values out of a tile, in the order of its words: a wavefront reads a tile of a head whole and stores 16 bytes of a
+// row a lane (f16; values are turned for it).  8192 rows of 8 heads of 128 out of 4 bits into f16: 15 us, 2.9 TB/s (16.4 with values
+// stored pair by pair); the launch, a tile's chain of length, page and words, and one wave of workgroups.
 template <int Z, bool Q4>
 __global__ __launch_bounds__(256) void read_kernel(ReadArgs a) {
   const unsigned wave = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), per = (unsigned)a.tiles * a.pages.kv_heads;

@@ -166,11 +166,12 @@ __device__ __forceinline__ void left_of(const float (&x)[N], const float (&y)[N]
 
 // A sequence's walk by one workgroup.  What its tests need of p and q (a value per node, of its parent's rows) is gathered
 // first, for all nodes side by side; a rejection that is followed by another child costs a pass over the rows for Z, and the
-// draw one more, which leaves the sums of runs of ids behind, so that its place is looked for in one of them.  Everything in
-// 64 bits: random numbers are compared with sums of 1e5 values, whose last bits in f32 would move a place for one of 1e3.
-// The floor of the bytes (13 MB for 32 trees of 24 nodes over 51866 ids with drafts: 3 us) is far: a walk is a chain of passes, each of one
-// compute unit's reads of two rows from the caches, 64-bit sums, and a meeting of 16 wavefronts.  Those trees take 33 us, a
-// chain of 8 nodes without drafts 15; with p and q looked up node by node and the draw's place by a second pass 104 and 29.
+// draw one more, which leaves the sums of runs of ids behind, so that its place is looked for in one of them.  Everything in 64
+// bits: random numbers are compared with sums of 1e5 values, whose last bits in f32 would move a place for one of 1e3.  The
+// floor of the bytes (13 MB for 32 trees of 24 nodes over 51866 ids with drafts: 3 us) is far: a walk is a chain of passes,
+// each of one compute unit's reads of two rows from the caches, 64-bit sums, and a meeting of 16 wavefronts.  Those trees take
+// 33 us, a chain of 8 nodes without drafts 15; with p and q looked up node by node and the draw's place by a second pass 104
+// and 29.
 template <bool DRAFTS>
 __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs a) {
   __shared__ double part[ST / 64], sums[PIECES], gone[TREE_ROWS];
