@@ -546,7 +546,9 @@ int wh_logit_probs(wh_ctx *ctx, const wh_tree *t, const void *logits, size_t ld,
  *   on there;
  *   otherwise w = max(0, w / Z - drafts) and Z = the sum of w (NULL: Z = Z - w[x] and w[x] = 0), while Z > 0.
  * Where none is accepted the next token is drawn from w: the first id whose running sum is above u[b][0] times the sum of w
- * (from probs, where w has come to nothing).  All of it in 64 bits.  picks [batch * rows]: for the nodes on the walk the token
+ * (from probs, where w has come to nothing).  Where that id is a child's token after all (as sums are rounded, none of the
+ * children may be accepted though they are all that is wanted), the walk goes on at the first such child, and u[b][0] is
+ * from then on what is left of it within that id's share: (u * sum - the sum before the id) / its w.  All of it in 64 bits.  picks [batch * rows]: for the nodes on the walk the token
  * after them, 0xffffffff for the others and where probs has nothing: wh_tree_accept takes that walk and keeps it.  Rows of
  * probs and drafts hold finite numbers, none below zero; those off the walk may hold anything.  Tokens past vocab are passed
  * over.  picks overlaps no input.  count[b] rows of picks are written.  batch < 2^22. */

@@ -1,0 +1,128 @@
+"""Ends of the range of sampled decoding over caches in pages: draws that fall on a drafted token, rows without a number at any
+temperature, values next to f32's ends, outputs between the rows of inputs, scores far from zero, prompts, tables with gaps.
+The plain forms and their tolerances are those of test_pages_gpu, with eps = 2^-24 (half a step of f32) and 2^-11 (of f16)."""
+
+import numpy as np
+import pytest
+
+import wavo_amd as wa
+from test_pages_gpu import NONE, Cache, attend, norm_tolerance, probs, rope_table, rows_of, sample, softmax, turned
+from test_tree_gpu import EPS, EPS16, attend_tolerance, bits, trees
+
+pytestmark = pytest.mark.gpu
+
+# ------------------------------------------------------------------------------------------- draws of a child's token
+
+
+def walk(p, q, tokens, parent, u, vocab):
+    """One sequence, in 64 bits: picks, the nodes of the walk, and how often a draw fell on a child's token."""
+    picks, path, number, falls = np.full(len(tokens), NONE, np.uint32), [0], float(u[0]), 0
+    at, start, w, total = 0, 1, p[0].astype(np.float64), 1.0
+    while True:
+        for i in range(start, len(tokens)):
+            if parent[i] != at or not total > 0 or tokens[i] >= vocab:
+                continue
+            x = tokens[i]
+            if float(u[i]) * (1.0 if q is None else float(q[at, x])) * total < w[x]:
+                picks[at] = x
+                path.append(i)
+                at, w, total = i, p[i].astype(np.float64), 1.0
+            elif q is None:
+                total -= w[x]
+                w[x] = 0
+            else:
+                w = np.maximum(w / total - q[at].astype(np.float64), 0)
+                total = w.sum()
+        if not w.sum() > 0:
+            w = p[at].astype(np.float64)
+        c = np.cumsum(w)
+        place = number * c[-1]
+        over = np.flatnonzero((c > place) & (w > 0))
+        if not len(over):
+            return picks, path, falls
+        picks[at] = x = over[0]
+        child = [i for i in range(at + 1, len(tokens)) if parent[i] == at and tokens[i] == x]
+        if not child:
+            return picks, path, falls
+        falls += 1
+        number = (place - (c[x] - w[x])) / w[x]
+        at, start, w, total = child[0], child[0] + 1, p[child[0]].astype(np.float64), 1.0
+        path.append(at)
+
+
+def full_tree(levels, spread=3):
+    """Parents and who sees whom where every node but the last level's has `spread` children."""
+    parents = [0]
+    first, end = 0, 1
+    for _ in range(levels):
+        parents += [i for i in range(first, end) for _ in range(spread)]
+        first, end = end, len(parents)
+    seen = np.eye(len(parents), dtype=bool)
+    for i in range(1, len(parents)):
+        seen[i] |= seen[parents[i]]
+    return np.array(parents), seen
+
+
+@pytest.mark.parametrize("kind", ["rejected", "untested", "drafts"])
+def test_draws_of_a_childs_token_go_on_there(gpu, kind):
+    """Children that are all that is wanted and of which none is accepted, as sums are rounded: the draw takes one of them all the
+    same, and the walk that wh_tree_accept takes does not end in a node without a pick."""
+    rng = np.random.default_rng({"rejected": 1, "untested": 2, "drafts": 3}[kind])
+    vocab, want = 3, 24
+    parents, seen = full_tree(3)
+    rows = len(parents)
+    found = []
+    for _ in range(20000):
+        x = rng.standard_normal((rows, vocab))
+        if kind == "untested":  # (the last child's share is less than the others' roundings)
+            x[:, 2] -= rng.uniform(15, 18)
+        p, q = softmax(x), None
+        tokens = np.zeros(rows, np.uint32)
+        for i in range(1, rows, 3):
+            tokens[i:i + 3] = np.arange(3) if kind == "untested" else rng.permutation(3)
+        u = rng.random(rows).astype(np.float32)
+        u[rng.random(rows) < 0.8] = np.float32(1 - 2.0**-24)
+        u[0] = rng.random() if kind != "untested" else np.float32(1 - 2.0**-24)
+        if kind == "drafts":  # (rows that do not sum to 1: most rejections leave nothing)
+            q, p = softmax(rng.standard_normal((rows, vocab))), p * np.float32(2.0**-6)
+        if walk(p, q, tokens, parents, u, vocab)[2]:
+            found.append((p, q, tokens, u))
+        if len(found) == want:
+            break
+    assert len(found) >= 8
+    p, tokens, u = (np.stack([f[i] for f in found]) for i in (0, 2, 3))
+    q = np.stack([f[1] for f in found]) if kind == "drafts" else None
+    batch = len(found)
+    mask = bits(np.broadcast_to(seen, (batch, rows, rows)))
+    got = sample(gpu, p, q, tokens, u, vocab, mask)
+    paths = []
+    for b in range(batch):
+        picks, path, _ = walk(p[b], None if q is None else q[b], tokens[b], parents, u[b], vocab)
+        assert np.array_equal(got[b], picks), f"sequence {b}"
+        paths.append(path)
+    up = lambda a: gpu.upload(np.ascontiguousarray(a))  # noqa: E731
+    keep = [up(np.zeros(batch, np.int32)), up(tokens), up(mask), up(got)]
+    path, kept, nxt, n_out = (up(np.full(s, -9, np.int32)) for s in ((batch, rows), batch, batch, batch))
+    gpu.tree_accept(wa.Tree(batch, rows, keep[0], None, keep[1], keep[2], mask[0].size), keep[3], None, None, 0, 0, None, 0, 0, 0, 100, 0, path,
+                    kept, nxt, n_out)
+    assert np.all(gpu.read(nxt, (batch,), np.uint32) < vocab)
+    path, kept = gpu.read(path, (batch, rows), np.int32), gpu.read(kept, (batch,), np.int32)
+    assert [path[b, :kept[b]].tolist() for b in range(batch)] == paths
+
+
+def test_tokens_after_such_a_draw_have_the_targets_distribution(gpu):
+    """20000 roots whose children are hardly ever accepted: what is drawn after the child that the first draw fell on."""
+    rng = np.random.default_rng(4)
+    batch, rows, vocab = 20000, 3, 4
+    p, q = np.zeros((batch, rows, vocab), np.float32), np.full((batch, rows, vocab), 0.25, np.float32)
+    p[:, 0] = np.float32([0.4, 0.3, 0.2, 0.1]) * np.float32(2.0**-10)
+    p[:, 1:] = np.float32([0.1, 0.4, 0.2, 0.3])
+    tokens = np.broadcast_to(np.uint32([0, 0, 1]), (batch, rows))
+    seen = np.eye(rows, dtype=bool)[None].repeat(batch, 0)
+    seen[:, :, 0] = True
+    got = sample(gpu, p, q, tokens, rng.random((batch, rows)).astype(np.float32), vocab, bits(seen))
+    for node in (1, 2):
+        there = got[got[:, 0] == node - 1, node]
+        assert len(there) > 4000
+        share, want = np.bincount(there, minlength=vocab)[:vocab] / len(there), p[0, 1]
+        assert np.all(np.abs(share - want) <= 5 * np.sqrt(want * (1 - want) / len(there))), share

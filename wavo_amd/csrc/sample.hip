@@ -179,6 +179,7 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs a) {
   __shared__ uint32_t tokens[TREE_ROWS], out[TREE_ROWS];
   __shared__ short parents[TREE_ROWS];
   __shared__ int found;
+  __shared__ double left[2];
   constexpr int WV = ST / 64, BATCH = DRAFTS ? 5 : 7;  // BATCH: blocks of 256 ids that a wavefront loads at once
   const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int count = a.count ? min(max(a.count[b], 0), a.rows) : a.rows;
@@ -208,8 +209,12 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs a) {
   __syncthreads();
 
   int at = 0, rounds = 0;  // the node, and how many of its children were rejected
-  double total = 1.0;
+  double total = 1.0, number = numbers[0];  // Z, and the draw's random number
   const float *p = a.p + row0 * a.ld, *q = DRAFTS ? a.q + row0 * a.ld : nullptr;
+  auto enter = [&](int node) {
+    at = node, rounds = 0, total = 1.0;
+    p = a.p + (row0 + node) * a.ld, q = DRAFTS ? a.q + (row0 + node) * a.ld : nullptr;
+  };
   // The rows of `at`, 256 ids (a wavefront's) at a time: f(piece, ids' weights).  A piece is `per` such blocks, one after the
   // other by one wavefront, and every wavefront takes every WV-th piece.
   const int blocks = (a.vocab + 255) / 256, per = (blocks + PIECES - 1) / PIECES, pieces = (blocks + per - 1) / per;
@@ -232,121 +237,145 @@ __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs a) {
         if (block[i] < blocks) f(piece[i], (w[4 * i] + w[4 * i + 1]) + (w[4 * i + 2] + w[4 * i + 3]));
     }
   };
-  for (int base = 0, from = 1; base < count;) {
-    // The next child of `at`, among 64 nodes at a time.
-    const int i0 = base + lane;
-    const uint64_t any = __ballot(i0 >= from && i0 < count && parents[min(i0, count - 1)] == at);
-    if (!any) {
-      base += 64;
-      continue;
+  // From `at` on, among the nodes from `from` on.
+  int base = 0, from = 1;
+  auto walk = [&] {
+    while (base < count) {
+      // The next child of `at`, among 64 nodes at a time.
+      const int i0 = base + lane;
+      const uint64_t any = __ballot(i0 >= from && i0 < count && parents[min(i0, count - 1)] == at);
+      if (!any) {
+        base += 64;
+        continue;
+      }
+      const int i = base + (int)__builtin_ctzll(any);
+      const int x = (int)tokens[i];
+      if (DRAFTS && rounds && total < 0.0) {  // (Z of the rejections so far, wanted only now)
+        double s = 0.0;
+        pass([&](int, double w) { s += w; });
+        s = xlane::wave_sum(s);
+        if (lane == 0) part[wave] = s;
+        __syncthreads();
+        total = 0.0;
+#pragma unroll
+        for (int w = 0; w < WV; w++) total += part[w];
+        __syncthreads();
+      }
+      if (!(total > 0.0)) break;  // nothing is left to accept
+      from = i + 1;
+      const float own[1] = {mine[i]}, draft[1] = {DRAFTS ? drafted[i] : 0.0f};
+      double kept[1];
+      left_of<DRAFTS>(own, draft, kept, gone, rounds, [&](int) { return x; });
+      const double w = kept[0];
+      if ((double)numbers[i] * (DRAFTS ? (double)drafted[i] : 1.0) * total < w) {
+        if (tid == 0) out[at] = (uint32_t)x;
+        enter(i);
+        base = i / 64 * 64;
+        continue;
+      }
+      __syncthreads();
+      if (tid == 0) gone[rounds] = DRAFTS ? 1.0 / total : (double)x;
+      __syncthreads();
+      rounds++;
+      total = DRAFTS ? -1.0 : total - w;
     }
-    const int i = base + (int)__builtin_ctzll(any);
-    const int x = (int)tokens[i];
-    if (DRAFTS && rounds && total < 0.0) {  // (Z of the rejections so far, wanted only now)
+  };
+  // The id drawn at `at`, or -1.  How far the place is into the id's weight, and that, stay behind as `left`.
+  auto draw = [&] {
+    for (int attempt = 0; attempt < 2; attempt++) {
+      __syncthreads();
+      for (int i = tid; i < PIECES; i += ST) sums[i] = 0.0;
+      __syncthreads();
+      pass([&](int piece, double w) {
+        w = xlane::wave_sum(w);
+        if (lane == 0) sums[piece] += w;
+      });
+      __syncthreads();
+      // Running sums of 16 pieces a lane, by every wavefront for itself.
       double s = 0.0;
-      pass([&](int, double w) { s += w; });
-      s = xlane::wave_sum(s);
-      if (lane == 0) part[wave] = s;
-      __syncthreads();
-      total = 0.0;
 #pragma unroll
-      for (int w = 0; w < WV; w++) total += part[w];
-      __syncthreads();
-    }
-    if (!(total > 0.0)) break;  // nothing is left to accept
-    from = i + 1;
-    const float own[1] = {mine[i]}, draft[1] = {DRAFTS ? drafted[i] : 0.0f};
-    double kept[1];
-    left_of<DRAFTS>(own, draft, kept, gone, rounds, [&](int) { return x; });
-    const double w = kept[0];
-    if ((double)numbers[i] * (DRAFTS ? (double)drafted[i] : 1.0) * total < w) {
-      if (tid == 0) out[at] = (uint32_t)x;
-      at = i, rounds = 0, total = 1.0;
-      p = a.p + (row0 + i) * a.ld, q = DRAFTS ? a.q + (row0 + i) * a.ld : nullptr;
-      base = i / 64 * 64;
-      continue;
-    }
-    __syncthreads();
-    if (tid == 0) gone[rounds] = DRAFTS ? 1.0 / total : (double)x;
-    __syncthreads();
-    rounds++;
-    total = DRAFTS ? -1.0 : total - w;
-  }
-
-  // The draw.
-  for (int attempt = 0; attempt < 2; attempt++) {
-    __syncthreads();
-    for (int i = tid; i < PIECES; i += ST) sums[i] = 0.0;
-    __syncthreads();
-    pass([&](int piece, double w) {
-      w = xlane::wave_sum(w);
-      if (lane == 0) sums[piece] += w;
-    });
-    __syncthreads();
-    // Running sums of 16 pieces a lane, by every wavefront for itself.
-    double s = 0.0;
+      for (int i = 0; i < PIECES / 64; i++) s += sums[PIECES / 64 * lane + i];
+      double c = s;
 #pragma unroll
-    for (int i = 0; i < PIECES / 64; i++) s += sums[PIECES / 64 * lane + i];
-    double c = s;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const double o = __shfl_up(c, d);
-      if (lane >= d) c += o;
-    }
-    const double all = __shfl(c, 63);
-    if (!(all > 0.0)) {  // nothing left: from the node's probabilities themselves
-      rounds = 0;
-      continue;
-    }
-    const double place = (double)numbers[0] * all;
-    if (wave == 0) {
-      // The first lane, then its first piece, then the first id whose running sum is past the place; where last bits leave none,
-      // the last one of any weight.
-      const uint64_t over = __ballot(s > 0.0 && c > place), some = __ballot(s > 0.0);
-      const int l = over ? (int)__builtin_ctzll(over) : 63 - (int)__clzll(some);
-      double before = __shfl(c - s, l);
-      int piece = -1, last = 0;
-      for (int i = 0; i < PIECES / 64 && piece < 0; i++) {
-        const int k = PIECES / 64 * l + i;
-        if (k >= pieces) break;
-        if (sums[k] > 0.0) last = k;
-        if (sums[k] > 0.0 && before + sums[k] > place) piece = k;
-        else before += sums[k];
+      for (int d = 1; d < 64; d *= 2) {
+        const double o = __shfl_up(c, d);
+        if (lane >= d) c += o;
       }
-      if (piece < 0) piece = last, before -= sums[last];
-      int hit = -1, tail = -1;
-      for (int k = piece * per; k < min((piece + 1) * per, blocks) && hit < 0; k++) {
-        const int id = 256 * k + 4 * lane;
-        float x[4], y[4];
-        *(floatx4 *)x = four_of(p, id, a.vocab, 0.0f);
-        *(floatx4 *)y = DRAFTS && rounds ? four_of(q, id, a.vocab, 0.0f) : floatx4{};
-        double w[4];
-        left_of<DRAFTS>(x, y, w, gone, rounds, [&](int e) { return id + e; });
-        const double r = (w[0] + w[1]) + (w[2] + w[3]);
-        double run = r;
-#pragma unroll
-        for (int d = 1; d < 64; d *= 2) {
-          const double o = __shfl_up(run, d);
-          if (lane >= d) run += o;
-        }
-        double here = before + (run - r);
-        int own = -1, end = -1;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          here += w[e];
-          if (w[e] > 0.0) end = id + e;
-          if (own < 0 && w[e] > 0.0 && here > place) own = id + e;
-        }
-        const uint64_t hits = __ballot(own >= 0), ends = __ballot(end >= 0);
-        if (hits) hit = __shfl(own, (int)__builtin_ctzll(hits));
-        if (ends) tail = __shfl(end, 63 - (int)__clzll(ends));
-        before += __shfl(run, 63);
+      const double all = __shfl(c, 63);
+      if (!(all > 0.0)) {  // nothing left: from the node's probabilities themselves
+        rounds = 0;
+        continue;
       }
-      if (lane == 0) found = hit >= 0 ? hit : tail;
+      const double place = number * all;
+      if (wave == 0) {
+        // The first lane, then its first piece, then the first id whose running sum is past the place; where last bits leave none,
+        // the last one of any weight.
+        const uint64_t over = __ballot(s > 0.0 && c > place), some = __ballot(s > 0.0);
+        const int l = over ? (int)__builtin_ctzll(over) : 63 - (int)__clzll(some);
+        double before = __shfl(c - s, l);
+        int piece = -1, last = 0;
+        for (int i = 0; i < PIECES / 64 && piece < 0; i++) {
+          const int k = PIECES / 64 * l + i;
+          if (k >= pieces) break;
+          if (sums[k] > 0.0) last = k;
+          if (sums[k] > 0.0 && before + sums[k] > place) piece = k;
+          else before += sums[k];
+        }
+        if (piece < 0) piece = last, before -= sums[last];
+        int hit = -1, tail = -1;
+        double past = 1.0, weight = 1.0;
+        for (int k = piece * per; k < min((piece + 1) * per, blocks) && hit < 0; k++) {
+          const int id = 256 * k + 4 * lane;
+          float x[4], y[4];
+          *(floatx4 *)x = four_of(p, id, a.vocab, 0.0f);
+          *(floatx4 *)y = DRAFTS && rounds ? four_of(q, id, a.vocab, 0.0f) : floatx4{};
+          double w[4];
+          left_of<DRAFTS>(x, y, w, gone, rounds, [&](int e) { return id + e; });
+          const double r = (w[0] + w[1]) + (w[2] + w[3]);
+          double run = r;
+#pragma unroll
+          for (int d = 1; d < 64; d *= 2) {
+            const double o = __shfl_up(run, d);
+            if (lane >= d) run += o;
+          }
+          double here = before + (run - r), below = 0.0, share = 1.0;
+          int own = -1, end = -1;
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            if (w[e] > 0.0) end = id + e;
+            if (own < 0 && w[e] > 0.0 && here + w[e] > place) own = id + e, below = here, share = w[e];
+            here += w[e];
+          }
+          const uint64_t hits = __ballot(own >= 0), ends = __ballot(end >= 0);
+          if (hits) {
+            const int x = (int)__builtin_ctzll(hits);
+            hit = __shfl(own, x), past = place - __shfl(below, x), weight = __shfl(share, x);
+          }
+          if (ends) tail = __shfl(end, 63 - (int)__clzll(ends));
+          before += __shfl(run, 63);
+        }
+        if (lane == 0) found = hit >= 0 ? hit : tail, left[0] = past, left[1] = weight;
+      }
+      __syncthreads();
+      return found;
     }
-    __syncthreads();
-    if (tid == 0) out[at] = (uint32_t)found;
-    break;
+    return -1;
+  };
+  // A draw that falls on the token of a child, though none was accepted, goes on there: wh_tree_accept will.
+  for (;;) {
+    walk();
+    const int id = draw();
+    if (tid == 0) out[at] = (uint32_t)id;
+    int next = -1;
+    for (int i0 = at / 64 * 64; id >= 0 && i0 < count && next < 0; i0 += 64) {
+      const int i = min(i0 + lane, count - 1);
+      const uint64_t any = __ballot(i > at && parents[i] == at && tokens[i] == (uint32_t)id);
+      if (any) next = i0 + (int)__builtin_ctzll(any);
+    }
+    if (next < 0) break;
+    number = fmin(fmax(left[0] / left[1], 0.0), 0x1.fffffffffffffp-1);
+    enter(next);
+    base = next / 64 * 64, from = next + 1;
   }
   __syncthreads();
   if (tid < count) a.picks[row0 + tid] = out[tid];
