@@ -57,10 +57,13 @@ __device__ __forceinline__ float over_waves(float v, float *part, Op op, float n
 
 // A row per workgroup, its first HELD * 4096 values in registers from their one load to their store (longer rows' others are read
 // three times, from the caches): the maximum, the exponents' sum, the quotients.  Sums in f32, of few terms a thread.
-// Many rows are bound by HBM: two workgroups a compute unit, one's loads beside the other's stores (about 290 rows of 51866 f32
-// logits: 30 us, 4 TB/s).  One row (8.7 us) is bound by one compute unit's loads and stores of 200 KB each; in three passes over
-// the row it took 21, the 290 57.
-constexpr int HELD = 13;
+// HELD: as many pieces as 64 registers take without a spill, which is what two workgroups a compute unit leave a thread.  12 spill
+// some and 13 more; with 11, 12 and 13 one row of 20000 f32 logits takes 5.5, 5.9 and 6.4 us, 384 rows 13, 14 and 16; of 51866
+// (of which 11 read the last 6810 again) 7.8, 8.1 and 8.3, and 29, 30 and 35; of 131071 126, 126 and 129.  8 are better where they hold
+// the whole row (12 us for 384 rows of 20000), and worse past that (133 of 131071).
+// Many rows are bound by HBM: two workgroups a compute unit, one's loads beside the other's stores (384 rows of 51866: 159 MB in 29 us, some of them from the chip's cache).
+// One row is bound by one compute unit's loads and stores of 200 KB each; in three passes over the row it took 21 us.
+constexpr int HELD = 11;
 template <typename T>
 __global__ __launch_bounds__(PT, 8) void probs_kernel(ProbsArgs a) {
   __shared__ float tops[PT / 64], sums[PT / 64];
