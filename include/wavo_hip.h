@@ -531,8 +531,8 @@ int wh_page_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void *k, 
 
 /* Probabilities of the rows of logits [batch * rows] (row r at r * ld values, f32 or (f16) f16, vocab values each;
  * wh_logit_rules' out): probs[r * probs_ld + x] = exp((l_x - max) / T) / their sum, in f32, T = temperature[b] (NULL: 1).  T
- * <= 0 (or NaN): 1 for the first maximum, 0 for the others.  A row with nothing left (minus infinity everywhere) gets zeros,
- * one with NaN or plus infinity gets NaN.  Rows past count[b] are not written, nor is anything past vocab; probs overlaps no
+ * <= 0 (or NaN): 1 for the first maximum, 0 for the others.  At any T a row with nothing left (minus infinity everywhere) gets
+ * zeros, one with NaN or plus infinity gets NaN.  Rows past count[b] are not written, nor is anything past vocab; probs overlaps no
  * input.  batch * rows < 2^22. */
 int wh_logit_probs(wh_ctx *ctx, const wh_tree *t, const void *logits, size_t ld, int f16, int vocab, const float *temperature,
                    float *probs, size_t probs_ld);

@@ -126,3 +126,29 @@ def test_tokens_after_such_a_draw_have_the_targets_distribution(gpu):
         assert len(there) > 4000
         share, want = np.bincount(there, minlength=vocab)[:vocab] / len(there), p[0, 1]
         assert np.all(np.abs(share - want) <= 5 * np.sqrt(want * (1 - want) / len(there))), share
+
+
+# ------------------------------------------------------------------------------------------- probabilities
+
+
+@pytest.mark.parametrize("half", [False, True])
+@pytest.mark.parametrize("vocab", [37, 5000, 70001])
+def test_probs_without_a_number_at_any_temperature(gpu, half, vocab):
+    """NaN and plus infinity, wherever they stand, are not taken for a row's maximum at a temperature of zero, either."""
+    l = np.random.default_rng(vocab).standard_normal((10, vocab)).astype(np.float16 if half else np.float32)
+    l[0, 0] = l[1, vocab - 1] = l[2, vocab // 2] = np.nan
+    l[3, 5] = l[4, vocab - 1] = np.inf
+    l[5] = np.nan
+    l[6] = -np.inf
+    l[7] = -np.inf
+    l[7, vocab // 3] = np.nan
+    l[8] = -np.inf
+    l[8, vocab - 2] = -60000
+    for t in (0.0, -1.0, np.nan, 1.0):
+        got = probs(gpu, l, 10, 1, vocab, [t] * 10)
+        for r in (0, 1, 2, 3, 4, 5, 7):
+            assert np.all(np.isnan(got[r])), f"row {r} at {t}"
+        assert np.all(got[6] == 0)
+        assert got[8, vocab - 2] == 1 and got[8].sum() == 1
+        if t != 1:
+            assert got[9, l[9].argmax()] == 1 and got[9].sum() == 1

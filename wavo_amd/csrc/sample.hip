@@ -98,19 +98,19 @@ __global__ __launch_bounds__(PT, 8) void probs_kernel(ProbsArgs a) {
         if (at + e < a.vocab) y[at + e] = f[e];
     }
   };
-  if (!(t > 0.0f)) {  // all of it to the first maximum
+  if (!(t > 0.0f)) {  // all of it to the first maximum; NaN, if there is any or plus infinity (whose place is -1)
     int at = INT_MAX;
-    for (int i = 4 * tid; i < a.vocab && at == INT_MAX; i += STEP) {
+    for (int i = 4 * tid; i < a.vocab; i += STEP) {
       const floatx4 f = four_of(x, i, a.vocab, -INFINITY);
 #pragma unroll
-      for (int e = 3; e >= 0; e--)
-        if (f[e] == top && top > -INFINITY) at = i + e;
+      for (int e = 0; e < 4; e++) at = min(at, !(f[e] < INFINITY) ? -1 : f[e] == top && top > -INFINITY ? i + e : INT_MAX);
     }
     if (at != INT_MAX) atomicMin(&first, at);
     __syncthreads();
     const int one = first;
+    const float none = one < 0 ? NAN : 0.0f;
     for (int i = 4 * tid; i < a.vocab; i += STEP)
-      store(i, floatx4{i == one ? 1.0f : 0.0f, i + 1 == one ? 1.0f : 0.0f, i + 2 == one ? 1.0f : 0.0f, i + 3 == one ? 1.0f : 0.0f});
+      store(i, floatx4{i == one ? 1.0f : none, i + 1 == one ? 1.0f : none, i + 2 == one ? 1.0f : none, i + 3 == one ? 1.0f : none});
     return;
   }
   // (k is finite and no zero, so that what is left of minus infinity is nothing at any temperature)
