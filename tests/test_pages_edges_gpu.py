@@ -152,3 +152,28 @@ def test_probs_without_a_number_at_any_temperature(gpu, half, vocab):
         assert got[8, vocab - 2] == 1 and got[8].sum() == 1
         if t != 1:
             assert got[9, l[9].argmax()] == 1 and got[9].sum() == 1
+
+
+@pytest.mark.parametrize("vocab", [100, 70001])
+def test_probs_of_the_largest_values(gpu, vocab):
+    """Logits up to f32's ends over the largest temperatures: the exponents' difference is wider than f32, and its factor less than
+    f32's smallest normal number (which leaves 2^-22 of it at 1.44 / 3.4e38)."""
+    rng = np.random.default_rng(vocab)
+    most = np.finfo(np.float32).max
+    l = rng.standard_normal((4, vocab)).astype(np.float32)
+    l[0, ::3] = -most
+    l[1] = most * rng.choice([-1, -0.5, 0, 0.25, 1], vocab).astype(np.float32)
+    l[2] = l[1] * np.float32(0.3)
+    l[3, 1::2] = -np.inf
+    l[3, ::4] = -most
+    for t in (np.inf, most, np.float32(2e38), np.float32(1e38), np.float32(1e37)):
+        got = probs(gpu, l, 4, 1, vocab, [t] * 4)
+        x = l.astype(np.float64)
+        with np.errstate(invalid="ignore"):
+            z = np.where(np.isneginf(x), -np.inf, (x - x.max(1, keepdims=True)) / np.float64(t))
+        want = np.exp(z)
+        want /= want.sum(1, keepdims=True)
+        size = np.abs(np.where(np.isfinite(z), z, 0)) * 1.4427
+        rel = (size + (want * size).sum(1, keepdims=True)) * (3 * EPS + 2.0**-22) + 2.0**-21 + (vocab / 1024 + 30) * EPS + 2.0**-20 * (t == np.inf)
+        err = np.abs(got - want)
+        assert np.all(err <= want * rel + 1e-37), f"temperature {t}: {np.max(err / (want * rel + 1e-37)):.3g} of what is allowed"

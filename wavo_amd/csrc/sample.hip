@@ -113,11 +113,12 @@ __global__ __launch_bounds__(PT, 8) void probs_kernel(ProbsArgs a) {
       store(i, floatx4{i == one ? 1.0f : none, i + 1 == one ? 1.0f : none, i + 2 == one ? 1.0f : none, i + 3 == one ? 1.0f : none});
     return;
   }
-  // (k is finite and no zero, so that what is left of minus infinity is nothing at any temperature)
-  const float base = top == -INFINITY ? 0.0f : top, k = fminf(fmaxf(1.44269504088896341f / t, 1.17549435e-38f), 3.402823466e38f);
+  // Half the difference, which is within f32 for any two values; and its factor, finite and no zero, so that what is left of minus
+  // infinity is nothing at any temperature, and what is left of numbers at an infinite one all of them (2^-21 off, at f32's ends).
+  const float base = top == -INFINITY ? 0.0f : -0.5f * top, k = fminf(fmaxf(2.88539008177792681f / t, 0x1p-149f), 3.402823466e38f);
   auto power = [&](floatx4 f) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) f[e] = __builtin_amdgcn_exp2f((f[e] - base) * k);
+    for (int e = 0; e < 4; e++) f[e] = __builtin_amdgcn_exp2f(fmaf(f[e], 0.5f, base) * k);
     return f;
   };
   float sum = 0.0f, more = 0.0f;
