@@ -625,14 +625,13 @@ int launch_head_norm(wh_ctx *ctx, const wh_tree *t, const wh_heads *h, const voi
     return wh_fail(ctx, WH_EARG, "head norm: buffers and rows must be 4-byte aligned");
   const bool same = x == y;
   if (same && (!in16 != !out16 || stride != y_stride)) return wh_fail(ctx, WH_EARG, "head norm: rows in their own place keep type and stride");
-  const size_t nodes = (size_t)t->batch * t->rows, x_bytes = ((nodes - 1) * stride + least) * (in16 ? 2 : 4),
-               y_bytes = ((nodes - 1) * y_stride + least) * (out16 ? 2 : 4);
-  if (!same && (uintptr_t)x < (uintptr_t)y + y_bytes && (uintptr_t)y < (uintptr_t)x + x_bytes && nodes > 0)
+  const size_t nodes = (size_t)t->batch * t->rows, in = in16 ? 2 : 4, out = out16 ? 2 : 4;
+  if (!same && rows_meet(x, least * in, stride * in, y, least * out, y_stride * out, nodes))
     return wh_fail(ctx, WH_EARG, "head norm: the output overlaps the rows");
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "head norm: %s", hipGetErrorString(e));
   const NormArgs a{turn_of(h), x, stride, y, y_stride, t->n, t->count, t->mask, t->mask_stride, t->rows, (t->rows + 31) / 32, h->heads,
                    h->heads + h->kv_heads, h->heads + (same ? 1 : 2) * h->kv_heads, h->hd, lanes_of(h->hd), in16 != 0, out16 != 0};
-  ProfScope prof(ctx, "head_norm", 10.0 * nodes * a.turned * h->hd, (double)nodes * a.all * h->hd * ((in16 ? 2 : 4) + (out16 ? 2 : 4)));
+  ProfScope prof(ctx, "head_norm", 10.0 * nodes * a.turned * h->hd, (double)nodes * a.all * h->hd * (in + out));
   wh_launch(ctx, norm_kernel, (unsigned)nodes, NORM_THREADS, 0, a);
   return wh_launched(ctx, "head norm");
 }

@@ -93,6 +93,24 @@ void *wh_scratch(wh_ctx *ctx, size_t bytes) {
   return ctx->scratch;
 }
 
+bool rows_meet(const void *pa, size_t a_len, size_t a_step, const void *pb, size_t b_len, size_t b_step, size_t rows) {
+  if (!rows || !a_len || !b_len) return false;
+  uintptr_t a = (uintptr_t)pa, b = (uintptr_t)pb;
+  if (b < a) std::swap(a, b), std::swap(a_len, b_len), std::swap(a_step, b_step);
+  if (b >= a + (rows - 1) * a_step + a_len) return false;
+  if (a_step == b_step) {  // every row of b is at the same place of its row of a, and of the next one
+    const size_t row = (b - a) / a_step, at = (b - a) % a_step;
+    return at < a_len || (at + b_len > a_step && row + 1 < rows);
+  }
+  for (size_t i = 0, j = 0; i < rows && j < rows;) {
+    const uintptr_t x = a + i * a_step, y = b + j * b_step;
+    if (x + a_len <= y) i++;
+    else if (y + b_len <= x) j++;
+    else return true;
+  }
+  return false;
+}
+
 size_t wh_type_bytes(int type, size_t n) {
   switch (type) {
     case WH_F32: return n * 4;
