@@ -177,3 +177,36 @@ def test_probs_of_the_largest_values(gpu, vocab):
         rel = (size + (want * size).sum(1, keepdims=True)) * (3 * EPS + 2.0**-22) + 2.0**-21 + (vocab / 1024 + 30) * EPS + 2.0**-20 * (t == np.inf)
         err = np.abs(got - want)
         assert np.all(err <= want * rel + 1e-37), f"temperature {t}: {np.max(err / (want * rel + 1e-37)):.3g} of what is allowed"
+
+
+# ------------------------------------------------------------------------------------------- norms
+
+
+def test_rows_between_each_other(gpu):
+    """Outputs whose rows lie in the gaps of their inputs' overlap nothing: the results of buffers of their own."""
+    rng = np.random.default_rng(6)
+    rows, heads, g, hd = 9, 4, 2, 64
+    d = (heads + 2 * g) * hd
+    x = rows_of(rng, 1, rows, heads, g, hd, False)[0]
+    n, table = gpu.upload(np.array([3], np.int32)), gpu.upload(rope_table(20, hd))
+    h, t = wa.Heads(heads, g, hd, table=table, positions=20, rot=hd), wa.Tree(1, rows, n)
+    alone, xb = gpu.buffer(rows * d), gpu.upload(x)
+    gpu.head_norm(t, h, xb, d, alone, d)
+    want = gpu.read(alone, (rows, d))
+    both = gpu.upload(np.concatenate([x, np.full((rows, 2 * d), 7, np.float32)], 1))
+    gpu.head_norm(t, h, both, 3 * d, both.ptr + 4 * d, 3 * d)
+    got = gpu.read(both, (rows, 3, d))
+    assert np.array_equal(got[:, 0], x) and np.array_equal(got[:, 1], want) and np.all(got[:, 2] == 7)
+    # Queries into the rows of another stride: their own rows' gaps, every second one left.
+    cache = Cache(rng, wa.F16, 32, g, hd, 1, 1)
+    both = gpu.upload(np.concatenate([x, np.full((rows, d), 7, np.float32)], 1))
+    q = both.ptr
+    gpu.page_append(t, h, q, q + 4 * heads * hd, q + 4 * (heads + g) * hd, 2 * d, cache.device(gpu), qo=q + 4 * d, qo_stride=2 * d)
+    got = gpu.read(both, (rows, 2, d))
+    assert np.array_equal(got[:, 0], x) and np.array_equal(got[:, 1, :heads * hd], want[:, :heads * hd]) and np.all(got[:, 1, heads * hd:] == 7)
+    # Keys and values side by side.
+    kv = gpu.upload(np.full((rows, 2 * g * hd + 2), 7, np.float32))
+    gpu.page_read(t, wa.Pages(cache.pool_buffer, cache.pages, cache.table_buffer, 1, 1, 32, wa.F16, g, hd), kv, kv.ptr + 4 * g * hd, 2 * g * hd + 2)
+    got = gpu.read(kv, (rows, 2 * g * hd + 2))
+    assert np.array_equal(got[:, :g * hd], want[:, heads * hd:(heads + g) * hd].astype(np.float16))
+    assert np.array_equal(got[:, g * hd:2 * g * hd], x[:, (heads + g) * hd:].astype(np.float16)) and np.all(got[:, 2 * g * hd:] == 7)
