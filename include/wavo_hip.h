@@ -504,14 +504,14 @@ size_t wh_page_bytes(int type, int page, int kv_heads, int hd);
  * an entry outside 0 .. rows - 1 stores nothing).  Row r's keys and values are at k and v + r * stride values, f32 or (in16)
  * f16.  With q and qo (not with a path) queries are normed and rotated on the way, row r of q (the same stride) to qo + r *
  * qo_stride, f32 or (out16) f16; qo may be q itself (same type and stride) and otherwise overlaps nothing.  n_out[b] (or NULL)
- * = n[b] + the positions that are there, n[b] at least; it is none of n, count and kept.  The tree's mask and tokens are not
+ * = n[b] + the positions that are there, n[b] at least; it overlaps none of n, count, kept and path.  The tree's mask and tokens are not
  * read.  Nothing but those positions changes; a page belongs to one sequence of a call, where it is stored to. */
 int wh_page_append(wh_ctx *ctx, const wh_tree *t, const wh_heads *heads, const void *q, const void *k, const void *v,
                    size_t stride, int in16, const int32_t *path, const int32_t *kept, const wh_pages *pages, void *qo,
                    size_t qo_stride, int out16, int32_t *n_out);
 
 /* Keys and values out of the pages: position n[b] + i of sequence b to row b * rows + i of k and v (kv_heads * hd values each,
- * stride apart, f32 or (out16) f16), i < count[b]; zeros where no page is there. */
+ * stride apart, f32 or (out16) f16), i < count[b]; zeros where no page is there.  Rows of k and v do not overlap. */
 int wh_page_read(wh_ctx *ctx, const wh_tree *t, const wh_pages *pages, void *k, void *v, size_t stride, int out16);
 
 /* wh_tree_attend over caches in pages: attention of every node over its sequence's positions j < n[b] in the pages and the

@@ -143,7 +143,7 @@ void linear_stage_free(wh_ctx *ctx);
 int gemm_noalloc_init(wh_ctx *ctx);
 
 // Whether two sets of `rows` rows share a byte: of a_len bytes each a_step apart, and of b_len bytes b_step apart (rows in
-// the gaps of others share none).
+// the gaps of others share none; a step of 0: one row).
 bool rows_meet(const void *a, size_t a_len, size_t a_step, const void *b, size_t b_len, size_t b_step, size_t rows);
 // At least `bytes` of device scratch (256-byte aligned), or nullptr with ctx->error set.  Growing
 // it drains the stream first; a caller that must not allocate reserves the size up front.

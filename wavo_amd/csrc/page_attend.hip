@@ -833,6 +833,9 @@ int launch_page_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
   }
   if (blocks > 65535 || units >= (size_t)1 << 22 || nodes * heads >= (size_t)1 << 25)  // (a launch's limits)
     return wh_fail(ctx, WH_EARG, "page attention: %d heads of %zu nodes in one call", heads, nodes);
+  const size_t in = in16 ? 2 : 4, out = (size_t)heads * p->hd * (out16 ? 2 : 4);
+  auto over = [&](const void *x, int of) { return x && rows_meet(o, out, out, x, (size_t)of * p->hd * in, stride * in, nodes); };
+  if (over(q, heads) || over(k, p->kv_heads) || over(v, p->kv_heads)) return wh_fail(ctx, WH_EARG, "page attention: the output overlaps the rows");
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "page attention: %s", hipGetErrorString(e));
   if (a.even) {
     const size_t part_rows = (size_t)2 * a.even * p->kv_heads * 16 * qt;

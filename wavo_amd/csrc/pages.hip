@@ -652,12 +652,17 @@ int launch_page_append(wh_ctx *ctx, const wh_tree *t, const wh_heads *h, const v
     return wh_fail(ctx, WH_EARG, "page append: buffers and rows must be 4-byte aligned");
   if (q == qo && q && (!in16 != !out16 || stride != qo_stride))
     return wh_fail(ctx, WH_EARG, "page append: queries in their own place keep type and stride");
-  if (n_out && (n_out == t->n || n_out == t->count || n_out == kept))
-    return wh_fail(ctx, WH_EARG, "page append: n_out cannot be n or the numbers of rows");
   const size_t nodes = (size_t)t->batch * t->rows;
   const int tiles = (t->rows + TILE - 2) / TILE + 1;
   const size_t waves = (size_t)t->batch * tiles * 3 * p->kv_heads, blocks = (waves + 3) / 4 + (q ? nodes : 0);
   if (blocks >= (size_t)1 << 24 || waves >= (size_t)1 << 31) return wh_fail(ctx, WH_EARG, "page append: %zu rows of %d heads in one call", nodes, p->kv_heads);
+  const size_t in = in16 ? 2 : 4, out = out16 ? 2 : 4;
+  auto over = [&](const void *x, size_t values) { return rows_meet(qo, qleast * out, qo_stride * out, x, values * in, stride * in, nodes); };
+  if (q && ((q != qo && over(q, qleast)) || over(k, least) || over(v, least)))
+    return wh_fail(ctx, WH_EARG, "page append: the queries' output overlaps the rows");
+  auto counts = [&](const int32_t *x, size_t n) { return x && rows_meet(n_out, 4 * (size_t)t->batch, 4 * (size_t)t->batch, x, 4 * n, 4 * n, 1); };
+  if (n_out && (counts(t->n, t->batch) || counts(t->count, t->batch) || counts(kept, t->batch) || counts(path, nodes)))
+    return wh_fail(ctx, WH_EARG, "page append: n_out cannot be n, the numbers of rows or the paths");
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "page append: %s", hipGetErrorString(e));
   const int32_t *count = kept ? kept : t->count;
   const Turn turn = turn_of(h);
@@ -680,6 +685,9 @@ int launch_page_read(wh_ctx *ctx, const wh_tree *t, const wh_pages *p, void *k, 
   const int tiles = (t->rows + TILE - 2) / TILE + 1;
   const size_t waves = (size_t)t->batch * tiles * p->kv_heads, blocks = (waves + 3) / 4;
   if (blocks >= (size_t)1 << 24) return wh_fail(ctx, WH_EARG, "page read: %d rows of %d sequences in one call", t->rows, t->batch);
+  const size_t out = out16 ? 2 : 4, values = (size_t)p->kv_heads * p->hd * out;
+  if (rows_meet(k, values, stride * out, v, values, stride * out, (size_t)t->batch * t->rows))
+    return wh_fail(ctx, WH_EARG, "page read: the rows of k and v overlap");
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "page read: %s", hipGetErrorString(e));
   const ReadArgs a{pages_of(p), t->n, t->count, t->batch, t->rows, tiles, out16 != 0, k, v, stride};
   ProfScope prof(ctx, "page_read", 0.0, (double)t->batch * t->rows * p->kv_heads * p->hd * 2 * (out16 ? 2 : 4));

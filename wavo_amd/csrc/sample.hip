@@ -396,9 +396,12 @@ int launch_logit_probs(wh_ctx *ctx, const wh_tree *t, const void *logits, size_t
     return wh_fail(ctx, WH_EARG, "logit probabilities: misaligned arrays");
   const size_t nodes = (size_t)t->batch * t->rows;
   if (nodes * PT >= (size_t)1 << 32) return wh_fail(ctx, WH_EARG, "logit probabilities: %zu rows in one call", nodes);
+  const size_t in = f16 ? 2 : 4;
+  if (rows_meet(logits, vocab * in, ld * in, probs, 4 * (size_t)vocab, 4 * probs_ld, nodes))
+    return wh_fail(ctx, WH_EARG, "logit probabilities: they overlap the logits");
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "logit probabilities: %s", hipGetErrorString(e));
   const ProbsArgs a{logits, ld, probs, probs_ld, temperature, t->count, t->rows, vocab};
-  ProfScope prof(ctx, "logit_probs", 0.0, (double)nodes * vocab * (f16 ? 6 : 8));
+  ProfScope prof(ctx, "logit_probs", 0.0, (double)nodes * vocab * (in + 4));
   if (f16) wh_launch(ctx, probs_kernel<_Float16>, (unsigned)nodes, PT, 0, a);
   else wh_launch(ctx, probs_kernel<float>, (unsigned)nodes, PT, 0, a);
   return wh_launched(ctx, "logit probabilities");
@@ -410,6 +413,10 @@ int launch_tree_sample(wh_ctx *ctx, const wh_tree *t, const float *probs, const 
     return wh_fail(ctx, WH_EARG, "tree sample: probabilities of %d ids (%zu apart), random numbers, picks, and the nodes' tokens are needed", vocab, ld);
   if (((uintptr_t)probs | (uintptr_t)drafts | (uintptr_t)u | (uintptr_t)picks) % 4) return wh_fail(ctx, WH_EARG, "tree sample: misaligned arrays");
   if ((size_t)t->batch * ST >= (size_t)1 << 32) return wh_fail(ctx, WH_EARG, "tree sample: %d sequences in one call", t->batch);
+  const size_t nodes = (size_t)t->batch * t->rows;
+  auto over = [&](const void *x, size_t values, size_t step) { return x && rows_meet(x, 4 * values, 4 * step, picks, 4 * nodes, 0, nodes); };
+  if (over(probs, vocab, ld) || over(drafts, vocab, ld) || over(u, 1, 1) || over(t->tokens, 1, 1))
+    return wh_fail(ctx, WH_EARG, "tree sample: the picks overlap what is read");
   if (hipError_t e = hipSetDevice(ctx->device)) return wh_fail(ctx, WH_EGPU, "tree sample: %s", hipGetErrorString(e));
   const SampleArgs a{probs, drafts, u, t->count, t->tokens, t->mask, t->mask_stride, ld, t->rows, (t->rows + 31) / 32, vocab, picks};
   ProfScope prof(ctx, "tree_sample", 0.0, 4.0 * t->batch * vocab * (drafts ? 2 : 1));
