@@ -182,6 +182,33 @@ def test_probs_of_the_largest_values(gpu, vocab):
 # ------------------------------------------------------------------------------------------- norms
 
 
+@pytest.mark.parametrize("hd", [8, 40, 64, 128, 256])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_head_norm_of_values_whose_squares_leave_f32(gpu, hd, in_place):
+    """Heads of the largest and of the smallest numbers among ordinary ones: their norm is of f32's range, and so is the result."""
+    rng = np.random.default_rng(hd)
+    heads, g, rows = 6, 2, 5
+    x = rows_of(rng, 1, rows, heads, g, hd, False)
+    hx = x[0].reshape(rows, heads + 2 * g, hd)
+    hx[0, 1] *= np.float32(1e25)
+    hx[0, 7] *= np.float32(1e-25)
+    hx[1, :6] *= np.float32(2.0)**rng.integers(-120, 120, 6).astype(np.float32)[:, None]
+    hx[2, 0] = rng.choice([-1, 1], hd) * np.finfo(np.float32).max
+    hx[2, 6] = rng.integers(-100, 100, hd) * np.float32(2.0**-149)
+    hx[2, 7] = np.float32(2.0**-149)
+    hx[3, 2, 1:] *= np.float32(1e-30)  # (one large value)
+    for eps in (0.0, 1e-6, 1e-38):
+        gain, table = (1 + 0.3 * rng.standard_normal(hd)).astype(np.float32), rope_table(20, hd)
+        keep = [gpu.upload(a) for a in (gain, table, np.array([7], np.int32), x)]
+        y = keep[3] if in_place else gpu.buffer(x.size)
+        gpu.head_norm(wa.Tree(1, rows, keep[2]), wa.Heads(heads, g, hd, keep[0], keep[0], eps, keep[1], 20, hd), keep[3], x.shape[-1], y, x.shape[-1])
+        got = gpu.read(y, hx.shape)
+        want = turned(hx[:, :heads + g], gain, eps, table, hd, False, 7 + np.arange(rows))
+        err = np.abs(got[:, :heads + g] - want)
+        assert np.all(err <= norm_tolerance(hx[:, :heads + g], gain, hd)), f"eps {eps}: {err.max()}"
+        assert np.array_equal(got[:, heads + g:], hx[:, heads + g:])
+
+
 def test_rows_between_each_other(gpu):
     """Outputs whose rows lie in the gaps of their inputs' overlap nothing: the results of buffers of their own."""
     rng = np.random.default_rng(6)

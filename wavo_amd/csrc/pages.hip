@@ -67,9 +67,11 @@ constexpr int NORM_THREADS = 256;
 
 // A row's heads, `per` lanes each, by a workgroup: lane i holds 4 values of the head from `first` and 4 from `second` on, which
 // the rotation turns against each other, so that a head is read and written once, in pieces of 8 or 16 bytes, and its squares meet
-// in a few lane exchanges.  Bound by HBM: 8192 rows of 48 f16 heads of 128 take 45 us, 4.5 TB/s.  (One token: 5 us, a launch and
-// three reads that wait for each other.)
-__device__ __forceinline__ void norm_row(const NormArgs &a, size_t row, int position, int tid, int threads) {
+// in a few lane exchanges.  Bound by HBM: 8192 rows of 48 f16 heads of 128 take 42 us, 4.8 TB/s, f32 ones 78.  (One token: 4 us, a
+// launch and three reads that wait for each other.)  H: f16 rows, whose squares never leave f32.  f32 rows' may, and the branch for
+// those makes the next head's loads wait for this one's sums (100 us for 93 where 8192 rows are appended), so they are asked for first.
+template <bool H>
+__device__ __forceinline__ void norm_heads(const NormArgs &a, size_t row, int position, int tid, int threads) {
   const int per = a.per, at = tid / per, lane = tid % per, half = a.turn.rot / 2, hd = a.hd;
   const bool there = 8 * lane < hd;
   int first = 8 * lane, second = first + 4;  // neighbours
@@ -83,17 +85,34 @@ __device__ __forceinline__ void norm_row(const NormArgs &a, size_t row, int posi
 #pragma unroll
     for (int e = 0; e < 4; e++) c[e] = t[i + e], s[e] = t[half + i + e];
   }
-  for (int head = at; head < a.all; head += threads / per) {
-    const size_t from = row * a.stride + (size_t)head * hd, to = row * a.y_stride + (size_t)head * hd;
-    floatx4 u = load4(a.x, from + first, a.in16), w = load4(a.x, from + second, a.in16);
+  auto load = [&](int head, floatx4 &u, floatx4 &w) {
+    const size_t from = row * a.stride + (size_t)head * hd;
+    u = load4(a.x, from + first, H), w = load4(a.x, from + second, H);
+  };
+  floatx4 next_u{}, next_w{};
+  if (!H && at < a.all) load(at, next_u, next_w);
+  for (int head = at, next; head < a.all; head = next) {
+    next = head + threads / per;
+    const size_t to = row * a.y_stride + (size_t)head * hd;
+    floatx4 u = next_u, w = next_w;
+    if (H) load(head, u, w);
+    else if (next < a.all) load(next, next_u, next_w);
     const float *gain = head < a.heads ? a.turn.q_gain : a.turn.k_gain;
     if (head < a.turned) {
       if (gain) {
-        float sum = 0.0f;
+        auto mean = [&](float eps) {
+          float sum = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; e++) sum = fmaf(u[e], u[e], fmaf(w[e], w[e], sum));
-        sum = head_sum(there ? sum : 0.0f, per);
-        const float r = 1.0f / sqrtf(sum / hd + a.turn.eps);
+          for (int e = 0; e < 4; e++) sum = fmaf(u[e], u[e], fmaf(w[e], w[e], sum));
+          return head_sum(there ? sum : 0.0f, per) / hd + eps;
+        };
+        float square = mean(a.turn.eps);
+        if (!H && !(square >= 0x1p-100f && square < INFINITY)) {  // (squares past f32 on either side: of the values, scaled)
+          const float scale = square < 1.0f ? 0x1p96f : 0x1p-96f;
+          u *= scale, w *= scale;
+          square = mean(a.turn.eps * scale * scale);
+        }
+        const float r = 1.0f / sqrtf(square);
         u *= r * raw4(gain + first), w *= r * raw4(gain + second);
       }
       if (turns) {
@@ -112,6 +131,11 @@ __device__ __forceinline__ void norm_row(const NormArgs &a, size_t row, int posi
     }
     if (there) store4(a.y, to + first, a.out16, u), store4(a.y, to + second, a.out16, w);
   }
+}
+
+__device__ __forceinline__ void norm_row(const NormArgs &a, size_t row, int position, int tid, int threads) {
+  if (a.in16) norm_heads<true>(a, row, position, tid, threads);
+  else norm_heads<false>(a, row, position, tid, threads);
 }
 
 __global__ __launch_bounds__(NORM_THREADS) void norm_kernel(NormArgs a) {
