@@ -35,10 +35,13 @@ constexpr int WAVES = 8;             // wavefronts of a workgroup, at most
 constexpr float LOWEST = -1e30f;     // the maximum of a row that has seen nothing
 constexpr int JOIN_LDS = 128 << 10;  // bytes in which wavefronts' results are joined
 
-// Whether a compute unit holds two workgroups: where a tile, its queries and outputs fit 128 registers.  (f16 pages of heads of
-// 128, one f16 row a key head, 32 sequences of 1000 to 8191: 112 us alone for 157 with registers spilled; f32 rows over 4 bits 53
-// for 60.)
-constexpr bool two_of(int z, int qt, bool half_rows, bool q4) { return qt == 1 && (q4 ? half_rows || z < 4 : z < 3); }
+// Whether a compute unit holds two workgroups, of 128 registers a thread, or one of 256.  Where tiles are shared out, two do better
+// while a tile, its queries and outputs fit (f16 rows of 96 over 4 bits, 32 sequences of 1000 to 8191: 37 us for 39 alone), and
+// worse where they spill (f16 rows of 128 over 4 bits spill 18 registers: 60 us for 47 alone, with f32 outputs 25: 67 for 55; f32
+// rows of 96 18: 51 for 46; f16 pages of heads of 128: 157 for 112).  Without shares a block's start and end are
+// hidden by the other workgroup's, which is worth some spilled registers over 4 bits (64 sequences of 100 to 1500, 16 key heads: f16
+// rows of 128 spill 4, 38 us for 41 alone; f32 rows of 96 4, 38 for 44).
+constexpr bool two_of(int z, int qt, bool half_rows, bool q4, bool even) { return qt == 1 && z < (q4 ? 3 + half_rows + !even : 3); }
 
 // What a block of rows costs a workgroup before its first tile and behind its last (its reads that wait for each other, the
 // wavefronts' results joined), as tiles of its time.  One row a key head, 32 sequences of 1000 to 8191: 43.0, 42.2, 41.2 and 42.2 us
@@ -698,7 +701,7 @@ __device__ __forceinline__ void attend_part(const PageAttendArgs &a, uint8_t *sm
 
 // EVEN: the workgroups take runs of all the tiles, of the same length, whatever sequences' they are.
 template <int Z, int QT, int QP, bool P16, bool Q4, bool EVEN>
-__global__ __launch_bounds__(64 * WAVES, two_of(Z, QT, QP == 1, Q4) ? 4 : 2) void page_attend_kernel(PageAttendArgs a) {
+__global__ __launch_bounds__(64 * WAVES, two_of(Z, QT, QP == 1, Q4, EVEN) ? 4 : 2) void page_attend_kernel(PageAttendArgs a) {
   typedef typename std::conditional<QP == 2, float, _Float16>::type T;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
   const int g = threadIdx.x >> 4 & 3, m = threadIdx.x & 15, group = a.heads / a.pages.kv_heads;
@@ -828,7 +831,7 @@ int launch_page_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
   const size_t blocks = (size_t)t->batch * a.row_blocks, units = blocks * p->kv_heads, nodes = (size_t)t->batch * t->rows;
   const size_t cus = ctx->cus > 0 ? ctx->cus : 256;
   if (tiles > 8 * a.kw && blocks * (tiles + start_of(qt)) < (size_t)1 << 31) {
-    a.even = (int)std::max<size_t>(cus * (two_of(p->hd / 32, qt, in16, p->type == WH_Q4_0) ? 2 : 1) / p->kv_heads, 1);
+    a.even = (int)std::max<size_t>(cus * (two_of(p->hd / 32, qt, in16, p->type == WH_Q4_0, true) ? 2 : 1) / p->kv_heads, 1);
     a.least = start_of(qt) + a.kw;
   }
   if (blocks > 65535 || units >= (size_t)1 << 22 || nodes * heads >= (size_t)1 << 25)  // (a launch's limits)
