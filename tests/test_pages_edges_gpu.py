@@ -128,6 +128,24 @@ def test_tokens_after_such_a_draw_have_the_targets_distribution(gpu):
         assert np.all(np.abs(share - want) <= 5 * np.sqrt(want * (1 - want) / len(there))), share
 
 
+@pytest.mark.parametrize("drafts", [True, False])
+def test_second_tokens_have_the_targets_distribution(gpu, drafts):
+    """20000 trees of two levels: the tokens after accepted children, within 5 standard deviations."""
+    rng = np.random.default_rng(5)
+    batch, vocab = 20000, 6
+    parents, seen = full_tree(2)
+    rows = len(parents)
+    p = np.broadcast_to(np.float32([0.05, 0.3, 0.1, 0.25, 0.1, 0.2]), (batch, rows, vocab)).copy()
+    p[:, 1:] = np.float32([0.2, 0.05, 0.25, 0.1, 0.3, 0.1])
+    q = np.broadcast_to(np.float32([0.3, 0.05, 0.1, 0.05, 0.4, 0.1]), (batch, rows, vocab)).copy()
+    tokens = rng.choice(vocab, (batch, rows), p=q[0, 0].astype(np.float64) / q[0, 0].sum(dtype=np.float64)).astype(np.uint32)
+    got = sample(gpu, p, q if drafts else None, tokens, rng.random((batch, rows)).astype(np.float32), vocab, bits(seen[None].repeat(batch, 0)))
+    second = got[:, 1:4][got[:, 1:4] != NONE]
+    assert len(second) > 5000 and (got[:, 4:] != NONE).any(1).sum() > 1000
+    share, want = np.bincount(second, minlength=vocab) / len(second), p[0, 1]
+    assert np.all(np.abs(share - want) <= 5 * np.sqrt(want * (1 - want) / len(second))), share
+
+
 # ------------------------------------------------------------------------------------------- probabilities
 
 
@@ -237,3 +255,118 @@ def test_rows_between_each_other(gpu):
     got = gpu.read(kv, (rows, 2 * g * hd + 2))
     assert np.array_equal(got[:, :g * hd], want[:, heads * hd:(heads + g) * hd].astype(np.float16))
     assert np.array_equal(got[:, g * hd:2 * g * hd], x[:, (heads + g) * hd:].astype(np.float16)) and np.all(got[:, 2 * g * hd:] == 7)
+
+
+# ------------------------------------------------------------------------------------------- attention
+
+
+def check_rows(got, cache, x, heads, n, seen, exact_scores=False, nodes=True):
+    """All rows of a sequence's head at once, with the worst case of their error as test_pages_gpu.check_attend has it.  exact_scores:
+    scores are sums of whole numbers below 2^24, without a rounding: what is left of the exponents' are three of those (of at most
+    2^4 digits), and the exponential's and the weights' 2^-20."""
+    batch, rows = x.shape[:2]
+    hd, g = cache.hd, cache.kv_heads
+    p16 = got.dtype == np.float16 and x.dtype == np.float16
+    for b in range(batch):
+        kept = [z for z in (cache.load(b, j) for j in range(n[b])) if z is not None]
+        kv = x[b, :, heads * hd:(heads + 2 * g) * hd].astype(np.float16).astype(np.float64).reshape(rows, 2, g, hd)
+        both = np.concatenate([np.stack(kept) if kept else np.zeros((0, 2, g, hd)), kv])
+        sees = np.concatenate([np.ones((rows, len(kept)), bool), seen[b] if nodes else np.zeros((rows, rows), bool)], 1)
+        for h in range(heads):
+            q = x[b, :, h * hd:(h + 1) * hd].astype(np.float64)
+            kk, vv = both[:, 0, h // (heads // g)], both[:, 1, h // (heads // g)]
+            s = np.where(sees, q @ kk.T / np.sqrt(hd), -np.inf)
+            with np.errstate(invalid="ignore"):
+                p = np.exp(s - s.max(1, keepdims=True))
+                want = np.where(sees.any(1)[:, None], p @ vv / p.sum(1, keepdims=True), 0)
+            size = np.abs(vv).max()
+            if exact_scores:
+                d = 2.0**4 * 3 * EPS + 2.0**-20
+                tol = np.full((rows, 1), (2 * d + 2 * len(both) * EPS) * size)
+            else:
+                tol = np.array([[attend_tolerance(y, kk, vv, hd)] for y in q])
+            tol = tol + len(both) * 2.0**-32 * max(1, size)
+            if p16:
+                tol = tol + (2 * EPS16 + EPS16**2 + len(both) * 2.0**-35 * max(1, size)) * size
+            if got.dtype == np.float16:
+                tol = tol + EPS16 * np.abs(want) + 2.0**-25
+            err = np.abs(got[b, :, h * hd:(h + 1) * hd].astype(np.float64) - want)
+            assert np.all(err <= tol), f"sequence {b} head {h}: {err.max():.3e}, {np.max(err / tol):.2f} of what is allowed"
+
+
+@pytest.mark.parametrize("type", [wa.Q4_0, wa.F16])
+@pytest.mark.parametrize("in16,out16", [(False, False), (True, True), (True, False), (False, True)])
+@pytest.mark.parametrize("heads,rows,page,cols", [(2, 4, 32, 10), (4, 13, 32, 10), (4, 13, 256, 9), (1, 3, 256, 10)])
+def test_attend_scores_far_from_zero(gpu, type, in16, out16, heads, rows, page, cols):
+    """Scores of some 1e6 whose differences decide: whole numbers, so that they are exact, above and below zero, in few and many row
+    tiles, and over tables that are shared out and joined."""
+    rng = np.random.default_rng(heads + rows + page)
+    batch, g, hd = 2, 1, 64
+    cache = Cache(rng, type, page, g, hd, batch, cols)
+    n = [cols * page, cols * page - 77]
+    cache.fill(rng, n)
+    for b in range(batch):
+        for j in range(n[b]):
+            pg, tile, p = cache.place(b, j)
+            w = cache.pool[pg, :, tile]
+            key = np.zeros(hd)
+            key[0], key[1] = (28, 24)[int(j % 97 == 5)], 4 * rng.integers(-8, 8)
+            if type == wa.F16:
+                w.view(np.float16)[:, cache.at[0][0][p]] = key
+                continue
+            w.view(np.float16)[:, 2 * 4 * hd + cache.factor[p]] = 4
+            word, shift = (y[p] for y in cache.at[0])
+            for i in range(hd):
+                w[0, word[i]] = (w[0, word[i]] & ~np.uint32(15 << shift[i])) | np.uint32(int(key[i]) // 4 + 8) << np.uint32(shift[i])
+    x = rows_of(rng, batch, rows, heads, g, hd, in16)
+    x[..., :(heads + g) * hd] = 0
+    x[..., :heads * hd:hd] = 61440 * rng.choice([-1, 1], (batch, rows, heads))
+    x[..., 1:heads * hd:hd] = rng.integers(-2, 3, (batch, rows, heads))
+    x[..., heads * hd] = 28
+    x[..., heads * hd + 1] = 4 * rng.integers(-8, 8, (batch, rows))
+    _, seen = trees(rng, batch, rows)
+    got = attend(gpu, cache, x, heads, n, None, seen, out16)
+    check_rows(got, cache, x, heads, n, seen, True)
+
+
+@pytest.mark.parametrize("type", [wa.Q4_0, wa.F16])
+@pytest.mark.parametrize("in16", [False, True])
+def test_attend_prompts(gpu, type, in16):
+    """The most rows there are, each seeing itself and those before it, with and without positions in pages before them."""
+    rng = np.random.default_rng(7)
+    batch, rows, heads, g, hd = 2, 1024, 4, 2, 64
+    cache = Cache(rng, type, 64, g, hd, batch, 2)
+    n = [0, 77]
+    cache.fill(rng, n)
+    x = rows_of(rng, batch, rows, heads, g, hd, in16)
+    x[..., :heads * hd] *= 2
+    seen = np.tril(np.ones((rows, rows), bool))[None].repeat(batch, 0)
+    check_rows(attend(gpu, cache, x, heads, n, None, seen, in16), cache, x, heads, n, seen)
+
+
+@pytest.mark.parametrize("type", [wa.Q4_0, wa.F16])
+@pytest.mark.parametrize("cols", [3, 70])
+def test_tables_wider_than_their_columns(gpu, type, cols):
+    """Tables inside wider rows: what stands beside them are pages of nobody."""
+    rng = np.random.default_rng(cols)
+    batch, rows, heads, g, hd, page = 3, 4, 2, 1, 32, 32
+    cache = Cache(rng, type, page, g, hd, batch, cols)
+    n = [cols * page - 4, 40, 7]
+    cache.fill(rng, n)
+    x = rows_of(rng, batch, rows, heads, g, hd, True)
+    _, seen = trees(rng, batch, rows)
+    xb, mb, nb = gpu.upload(x), gpu.upload(bits(seen)), gpu.upload(np.array(n, np.int32))
+    t = wa.Tree(batch, rows, nb, None, None, mb, rows)
+    got = []
+    for more in (0, 5):
+        pages = cache.device(gpu)
+        wide = np.concatenate([cache.table, np.tile(cache.table[:1, :1], (batch, more))], 1).astype(np.int32)
+        tb, o, k, v = gpu.upload(wide), gpu.buffer(batch * rows * heads * hd), gpu.buffer(batch * rows * g * hd), gpu.buffer(batch * rows * g * hd)
+        pages = wa.Pages(cache.pool_buffer, cache.pages, tb, cols, cols + more, page, type, g, hd)
+        at = xb.ptr + 2 * heads * hd
+        gpu.page_attend(t, xb, at, at + 2 * g * hd, x.shape[-1], pages, o, heads, in16=True)
+        gpu.page_append(t, wa.Heads(heads, g, hd), None, at, at + 2 * g * hd, x.shape[-1], pages, in16=True)
+        gpu.page_read(t, pages, k, v, g * hd)
+        got.append([gpu.read(o, (batch, rows, heads * hd)), cache.read_back(gpu), gpu.read(k, (batch, rows, g * hd)), gpu.read(v, (batch, rows, g * hd))])
+    assert all(np.array_equal(a, b, equal_nan=True) for a, b in zip(*got))
+    check_rows(got[0][0], cache, x, heads, n, seen)
