@@ -522,10 +522,10 @@ int wh_page_read(wh_ctx *ctx, const wh_tree *t, const wh_pages *pages, void *k, 
  * anything, and so may the rows past count[b], which are read; a row that sees a key or value that is no finite number may get
  * NaN.  o overlaps none of the inputs.  heads % kv_heads == 0, heads <= 1024, stride <= 2^23; pointers 4-byte aligned (stride
  * even for f16).  The rows * heads / kv_heads rows of a sequence's key head are taken in blocks of 48 at most (of 32, but for
- * f16 rows and outputs over 4 bits): batch times such blocks <= 65535, that times kv_heads < 2^22, and batch * rows * heads <
- * 2^25.  Where a table holds more than 2048 positions, its nodes counted in, the tiles of all sequences are shared out evenly
- * among the workgroups, from the lengths of their time, and a second launch joins the parts, in the context's scratch: such a
- * call is made once before it is recorded. */
+ * f16 rows and outputs over 4 bits or over tables that are shared out): batch times such blocks <= 65535, that times
+ * kv_heads < 2^22, and batch * rows * heads < 2^25.  Where a table holds more than 2048 positions, its nodes counted in, the
+ * tiles of all sequences are shared out evenly among the workgroups, from the lengths of their time, and a second launch joins
+ * the parts, in the context's scratch: such a call is made once before it is recorded. */
 int wh_page_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void *k, const void *v, size_t stride, int in16,
                    const wh_pages *pages, void *o, int out16, int heads);
 

@@ -785,7 +785,7 @@ int attend_launch(wh_ctx *ctx, const PageAttendArgs &a) {
 }
 template <int Z, int QP, bool P16, bool Q4>
 int attend_qt(wh_ctx *ctx, const PageAttendArgs &a, int qt) {
-  if constexpr (Q4 && P16) {
+  if constexpr (P16) {
     if (qt == 3) return attend_launch<Z, 3, QP, P16, Q4>(ctx, a);
   }
   return qt == 1 ? attend_launch<Z, 1, QP, P16, Q4>(ctx, a) : attend_launch<Z, 2, QP, P16, Q4>(ctx, a);
@@ -819,18 +819,21 @@ int launch_page_attend(wh_ctx *ctx, const wh_tree *t, const void *q, const void 
     return wh_fail(ctx, WH_EARG, "page attention: buffers and rows must be 4-byte aligned");
   PageAttendArgs a{q, k, v, stride, pages_of(p), o, out16 != 0, t->n, t->count, t->mask, t->mask_stride, t->batch, t->rows, (t->rows + 31) / 32,
                    heads, 1.0f / sqrtf((float)p->hd), 1, 1, 1, 0, 0, nullptr, nullptr};
-  // Rows in tiles of 16, evenly in blocks of `most` at most.  3 tiles open a nibble once for 48 rows: with 32 query heads over 8 of
-  // 128 and f16 throughout, 100 rows over 28 k positions take 162 us for 169 with 2 (42 for 40 over 5 k), and 4 spill registers
-  // (192).  f32 weights and outputs leave registers for 2, and f16 pages have nothing to open (81 and 83 us with 2 and 3).
-  const int rows = (t->rows * (heads / p->kv_heads) + 15) / 16, most = p->type == WH_Q4_0 && in16 && out16 ? 3 : 2;
+  const int tiles = a.pages.room / TILE + (t->mask && k ? (t->rows + TILE - 1) / TILE : 0);
+  while (2 * a.kw <= std::min(WAVES, tiles)) a.kw *= 2;
+  const bool shared = tiles > 8 * a.kw;
+  // Rows in tiles of 16, evenly in blocks of `most` at most.  3 tiles read a tile of the cache, and open its nibbles, once for 48
+  // rows: with 32 query heads over 8 of 128 and f16 throughout, 100 rows over 28 k positions take 160 us for 165 with 2, 296 for 384
+  // over f16 pages (heads of 64: 102 for 107, 147 for 189), over 5 k 47 for 46, and 58 for 63.  f16 pages that are not shared out do
+  // better with more workgroups (8 times 48 rows over 200 to 1500, 8 key heads: 20 us for 16 with 2).  4 spill registers (192; 3 spill
+  // 8 or 9 in heads of 128), and f32 weights and outputs leave registers for 2.
+  const int rows = (t->rows * (heads / p->kv_heads) + 15) / 16, most = in16 && out16 && (shared || p->type == WH_Q4_0) ? 3 : 2;
   a.row_blocks = (rows + most - 1) / most;
   const int qt = (rows + a.row_blocks - 1) / a.row_blocks;
   a.row_blocks = (rows + qt - 1) / qt, a.qt = qt;
-  const int tiles = a.pages.room / TILE + (t->mask && k ? (t->rows + TILE - 1) / TILE : 0);
-  while (2 * a.kw <= std::min(WAVES, tiles)) a.kw *= 2;
   const size_t blocks = (size_t)t->batch * a.row_blocks, units = blocks * p->kv_heads, nodes = (size_t)t->batch * t->rows;
   const size_t cus = ctx->cus > 0 ? ctx->cus : 256;
-  if (tiles > 8 * a.kw && blocks * (tiles + start_of(qt)) < (size_t)1 << 31) {
+  if (shared && blocks * (tiles + start_of(qt)) < (size_t)1 << 31) {
     a.even = (int)std::max<size_t>(cus * (two_of(p->hd / 32, qt, in16, p->type == WH_Q4_0, true) ? 2 : 1) / p->kv_heads, 1);
     a.least = start_of(qt) + a.kw;
   }
