@@ -485,8 +485,8 @@ int wh_head_norm(wh_ctx *ctx, const wh_tree *t, const wh_heads *heads, const voi
  * lies in page table[b * table_stride + j / page] of the pool (table_stride 0: one table for all), in device memory and read
  * when the queued work runs.  Pages whose number is not in 0 .. pages - 1 are not there: their positions are not seen, not
  * stored, and read as zeros.  Values that 4 bits stand for are within f16, as all that is stored here is.  A sequence has
- * table_cols * page positions at most (<= 2^24).  pool: pages * wh_page_bytes() bytes, 16-byte aligned.  What lies in
- * positions that were never stored does not matter. */
+ * table_cols * page positions at most (<= 2^24), within which every n[b] is taken.  pool: pages * wh_page_bytes() bytes, 16-byte
+ * aligned.  What lies in positions from a sequence's length on does not matter. */
 typedef struct wh_pages {
   void *pool;
   int pages;
@@ -504,8 +504,11 @@ size_t wh_page_bytes(int type, int page, int kv_heads, int hd);
  * an entry outside 0 .. rows - 1 stores nothing).  Row r's keys and values are at k and v + r * stride values, f32 or (in16)
  * f16.  With q and qo (not with a path) queries are normed and rotated on the way, row r of q (the same stride) to qo + r *
  * qo_stride, f32 or (out16) f16; qo may be q itself (same type and stride) and otherwise overlaps nothing.  n_out[b] (or NULL)
- * = n[b] + the positions that are there, n[b] at least; it overlaps none of n, count, kept and path.  The tree's mask and tokens are not
- * read.  Nothing but those positions changes; a page belongs to one sequence of a call, where it is stored to. */
+ * = n[b] + the number of its rows, or the table's positions, where that is more; it overlaps none of n, count, kept and path.
+ * Rows are counted whatever became of them: a position whose page is not there is not seen later either, but one whose path
+ * entry stored nothing keeps what stood in its page, and attention over n_out[b] positions reads that.  The tree's mask and
+ * tokens are not read.  Nothing but the rows' positions changes; a page belongs to one sequence of a call, where it is stored
+ * to. */
 int wh_page_append(wh_ctx *ctx, const wh_tree *t, const wh_heads *heads, const void *q, const void *k, const void *v,
                    size_t stride, int in16, const int32_t *path, const int32_t *kept, const wh_pages *pages, void *qo,
                    size_t qo_stride, int out16, int32_t *n_out);

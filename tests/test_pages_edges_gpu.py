@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import wavo_amd as wa
-from test_pages_gpu import NONE, Cache, attend, norm_tolerance, probs, rope_table, rows_of, sample, softmax, turned
+from test_pages_gpu import NONE, Cache, append, attend, expect, norm_tolerance, probs, rope_table, rows_of, same_words, sample, softmax, turned
 from test_tree_gpu import EPS, EPS16, attend_tolerance, bits, trees
 
 pytestmark = pytest.mark.gpu
@@ -255,6 +255,29 @@ def test_rows_between_each_other(gpu):
     got = gpu.read(kv, (rows, 2 * g * hd + 2))
     assert np.array_equal(got[:, :g * hd], want[:, heads * hd:(heads + g) * hd].astype(np.float16))
     assert np.array_equal(got[:, g * hd:2 * g * hd], x[:, (heads + g) * hd:].astype(np.float16)) and np.all(got[:, 2 * g * hd:] == 7)
+
+
+@pytest.mark.parametrize("type", [wa.Q4_0, wa.F16])
+def test_lengths_out_count_rows_whatever_became_of_them(gpu, type):
+    """Missing pages, path entries of no row, lengths outside the table: n_out counts rows up to the table's positions, and a
+    position that nothing was stored to keeps its words."""
+    rng = np.random.default_rng(8)
+    batch, rows, g, hd = 5, 12, 1, 32
+    cache = Cache(rng, type, 32, g, hd, batch, 2)
+    cache.table[0, 0] = -1
+    n, count = [3, 30, 70, -4, 60], [12, 5, 12, 3, 12]
+    path = np.tile(np.arange(rows, dtype=np.int32), (batch, 1))
+    path[1, 2], path[3, 0] = -1, rows
+    before = cache.pool.copy()
+    x = rows_of(rng, batch, rows, 1, g, hd, True)
+    _, n_out = append(gpu, cache, x, 1, n, None, path, count, q=False)
+    assert n_out.tolist() == [15, 35, 64, 3, 64] == expect(cache, x, 1, n, count, path)
+    same_words(cache, cache.read_back(gpu))
+    after = Cache.__new__(Cache)
+    after.__dict__.update(cache.__dict__)
+    after.pool = before
+    for b, j in ((1, 32), (3, 0)):
+        assert np.array_equal(cache.load(b, j), after.load(b, j), equal_nan=True)
 
 
 # ------------------------------------------------------------------------------------------- attention
