@@ -44,8 +44,9 @@ constexpr int JOIN_LDS = 128 << 10;  // bytes in which wavefronts' results are j
 constexpr bool two_of(int z, int qt, bool half_rows, bool q4, bool even) { return qt == 1 && z < (q4 ? 3 + half_rows + !even : 3); }
 
 // What a block of rows costs a workgroup before its first tile and behind its last (its reads that wait for each other, the
-// wavefronts' results joined), as tiles of its time.  One row a key head, 32 sequences of 1000 to 8191: 43.0, 42.2, 41.2 and 42.2 us
-// with 0, 8, 24 and 48 (over f16 pages 115, 111, 113 and 119); 100 rows, 8 sequences of 1000 to 8000: 45, 44, 41 and 38.
+// wavefronts' results joined), as tiles of its time.  One row a key head, 32 sequences of 1000 to 8191: 50, 44, 41 and 42 us
+// with 0, 8, 24 and 48 (over f16 pages 112, 110, 112 and 117); 100 rows, 8 sequences of 1000 to 8000: 53, 50, 44 and 50 with 0, 8, 48
+// and 96.
 constexpr __host__ __device__ int start_of(int qt) { return qt == 1 ? 24 : 48; }
 
 // A sequence's tiles: the cache's, then the nodes'.
@@ -227,11 +228,11 @@ __device__ __forceinline__ void load_rows(const PageAttendArgs &a, int b, int kh
 // an f16 cache would hold it), so that weights are operands as they stand.  K is not: so opened it took 142 us for the 162 of
 // the 100 rows below, and made the outputs' error against 64 bits 4e-4 for 2.6e-4 (of which their own rounding is 2.1e-4).
 //
-// What bounds it.  16 rows over f16 pages: HBM (64 sequences of 4000 positions, 8 key heads of 128: 183 us, 5.7 TB/s).  16 rows
-// over 4 bits, a quarter of the bytes: the vector instructions that open them, beside the starts and ends of blocks (32 sequences
-// of 1000 to 8191: 43 us and 4 for the join, 3.6 TB/s).  More rows: vector instructions, 365 for 48 rows of 32 positions,
-// of which some 180 open nibbles: 74% of the time, and matrix instructions 28% (100 rows over 8 caches of 24 to 33 k positions, 8 key
-// heads of 128: 145 to 165 us, 450 TFLOP/s).
+// What bounds it.  16 rows over f16 pages: HBM (64 sequences of 4000 positions, 8 key heads of 128: 179 us, 5.9 TB/s).  16 rows
+// over 4 bits, a quarter of the bytes: the vector instructions that open them (60 % of the time), beside the starts and ends of blocks
+// (32 sequences of 1000 to 8191: 41 us and 4 for the join, 3.7 TB/s).  More rows: vector instructions, 365 for 48 rows of 32
+// positions, of which some 180 open nibbles: 74% of the time, and matrix instructions 28% (100 rows over 8 caches of 24 to 33 k
+// positions, 8 key heads of 128: 148 us and 5 for the join, 460 TFLOP/s, some 40 more on a card that comes from idling).
 //
 // attend_part: the tiles from start to end of sequence b's block of rows from r0 on of a key head; into the outputs, or as part `part`.
 template <int Z, int QT, int QP, bool P16, bool Q4>

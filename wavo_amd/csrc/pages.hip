@@ -427,10 +427,10 @@ __device__ __forceinline__ void append_v(const AppendArgs &a, const Rows &rows, 
 
 // Tiles, and behind them the queries' rows.  A tile's words are put together in registers and written whole wherever all of
 // their positions are new; keys of 16 positions and values of 32 go to wavefronts of their own, since one wavefront for a whole
-// tile had its reads wait for each other three times over (16 tokens of 8 heads of 128 into 4 bits: 30 us, 8.3 now; 8192 rows:
-// 132, 58 now).  Those 8192 rows, f16 with 32 query heads on the way, move 170 MB, 2.9 TB/s; the queries' part alone takes 30
-// of the 58, the keys' and values' 25: the 64-bit norm and rotation (half the rate of f32) and the nibbles, some 20
-// instructions a value.
+// tile had its reads wait for each other three times over (16 tokens of 8 heads of 128 into 4 bits: 30 us, 8.4 now; 8192 rows:
+// 132, 51 now).  Those 8192 rows, f16 with 32 query heads on the way, move 170 MB, 3.3 TB/s; without the queries they take 21 us (18
+// into f16 pages) for 43 MB: vector instructions, 12 a value of K and 18 of V for factors and nibbles, and 11 of K, at half the
+// rate, for the norm and rotation in 64 bits.
 template <typename T, int Z, bool Q4, int TURN>
 __global__ __launch_bounds__(256, 4) void append_kernel(AppendArgs a) {
   if (blockIdx.x >= a.tile_blocks) {

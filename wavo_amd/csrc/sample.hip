@@ -174,8 +174,11 @@ __device__ __forceinline__ void left_of(const float (&x)[N], const float (&y)[N]
 // bits: random numbers are compared with sums of 1e5 values, whose last bits in f32 would move a place for one of 1e3.  The
 // floor of the bytes (13 MB for 32 trees of 24 nodes over 51866 ids with drafts: 3 us) is far: a walk is a chain of passes,
 // each of one compute unit's reads of two rows from the caches, 64-bit sums, and a meeting of 16 wavefronts.  Those trees take
-// 33 us, a chain of 8 nodes without drafts 15; with p and q looked up node by node and the draw's place by a second pass 104
-// and 29.
+// 31 to 41 us, by the tokens that were drawn, a chain of 8 nodes without drafts 14; with p and q looked up node by node and the
+// draw's place by a second pass 104 and 29.
+// Sums and products are rounded: of children that are all that is wanted none may be accepted, or Z be nothing before the last is
+// looked at.  Then the draw falls on a child's token, and the walk goes on there (once for some 1e8 verifications), with the part of
+// the random number that the draw did not use.
 template <bool DRAFTS>
 __global__ __launch_bounds__(ST) void sample_kernel(SampleArgs a) {
   __shared__ double part[ST / 64], sums[PIECES], gone[TREE_ROWS];
